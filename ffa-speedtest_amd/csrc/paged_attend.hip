@@ -1,0 +1,741 @@
+// Exact attention of L query tokens per sequence over the paged quantized caches, and the same for groups of
+// sequences that share leading pages.
+//
+// Row (b, i, h) is query token i of sequence b at head h.  It sees the keys t < lim = len_b - qlen_b + i + 1 and
+//   out = sum_t p_t v_t / sum_t p_t,   p_t = 2^(s_t - m),   s_t = scale log2(e) q . k_t,   m >= max s_t - 8,
+// one pass over the pages with a running m; k = code * scale + zero + residual (2-bit), level * scale + residual
+// (nvfp4, nf4) in fp32, rounded once to the fp16 matrix operand.  Partial results (m, sum p, sum p v) of page ranges
+// are fp32 and joined by q's row afterwards; a call whose rows each have one range writes the output directly.
+//
+// The pools' order is the order of the matrix operands: with S^T = K Q^T (16x16x32 f16), the A operand of tile tau
+// (tokens 4 m + tau, m = 0..15) is what lane (kc, m) loads, and the four tiles' results in lane (g, n) are the 16
+// consecutive tokens 16 g .. 16 g + 15 of query row n: with O^T = V^T P^T those are the B operand, V^T's blocks the A
+// operand, and each lane's results belong to its own row n again, whose m and sum it holds.  No value of S, P or O
+// changes lanes.
+#include "decode_common.h"
+#include "ffa_mi355x.h"
+
+extern "C" int ffa_set_error_internal(int code, const char *msg);
+
+namespace ffa {
+
+enum { kFmtQ2 = 0, kFmtNvfp4 = 1, kFmtNf4 = 2 };
+constexpr float kNoMax = -1e30f;  // m of a row that has seen no key: below every score, and 2^(x - m) stays defined
+constexpr float kStale = 8.f;     // log2 units a row's m may lag its maximum: p <= 2^8 fits the fp16 operand as well
+
+struct AttendParams {
+  const void *q;
+  const uint8_t *k;
+  const uint8_t *ks;
+  const uint8_t *kz;
+  const uint8_t *kr;
+  const uint8_t *v;
+  const int32_t *bt;
+  const int32_t *seq_lens, *q_lens;
+  const int32_t *group_start, *group_pages, *seq_group;
+  void *out;
+  float *part_ml, *part_o;  // [rows][nslots][2], [rows][nslots][128]
+  int bt_stride, num_pages, ngroups;
+  int B, T, L, HQ, HKV, G;
+  int q_bf16, out_bf16;
+  float scale2;
+  int nslots;  // 0: one page range per row, written to out
+  int slot0, ppw, shared;
+  int shared_slots, shared_ppw, own_slots, own_ppw;  // for the join
+};
+
+// QLoRA NF4 levels (the published 16 normal-float values)
+__constant__ float kAttendNF4[16] = {
+    -1.0f, -0.6961928009986877f, -0.5229921340942383f, -0.39491748809814453f, -0.28444138169288635f,
+    -0.18477343022823334f, -0.09105003625154495f, 0.0f, 0.07958029955625534f, 0.16093020141124725f,
+    0.24611230194568634f, 0.33791524171829224f, 0.44070982933044434f, 0.5626170039176941f,
+    0.7229568362236023f, 1.0f};
+
+__device__ __forceinline__ int seq_len_of(const AttendParams &p, int b) {
+  return p.seq_lens ? min(max(p.seq_lens[b], 0), p.T) : p.T;
+}
+// pages of sequence b that its group shares (0 without groups)
+__device__ __forceinline__ int shared_pages_of(const AttendParams &p, int b) {
+  if (p.ngroups == 0) return 0;
+  const int g = p.seq_group[b];
+  return (unsigned)g < (unsigned)p.ngroups ? min(max(p.group_pages[g], 0), p.bt_stride) : 0;
+}
+// keys that query token i of sequence b sees: positions below this
+__device__ __forceinline__ int row_limit(const AttendParams &p, int b, int i) {
+  const int len = seq_len_of(p, b);
+  const int ql = p.q_lens ? min(max(p.q_lens[b], 0), p.L) : p.L;
+  return i < ql ? max(len - ql + i + 1, 0) : 0;
+}
+
+// The rows and pages of a workgroup: sequences b0 .. b0 + n - 1 (a group's, over the shared pages; or one, over its
+// own), pages [p0, p1) of the block-table row of b0.
+struct AttendSet {
+  int b0, n, p0, p1;
+};
+__device__ __forceinline__ AttendSet attend_set(const AttendParams &p, int z) {
+  AttendSet s;
+  if (p.shared) {
+    s.b0 = min(max(p.group_start[z], 0), p.B);
+    s.n = max(min(p.group_start[z + 1], p.B) - s.b0, 0);
+    s.p0 = 0;
+    s.p1 = min(max(p.group_pages[z], 0), p.bt_stride);
+  } else {
+    s.b0 = z;
+    s.n = 1;
+    s.p0 = shared_pages_of(p, z);
+    s.p1 = (seq_len_of(p, z) + kPage - 1) / kPage;
+  }
+  return s;
+}
+
+// ---------------------------------------------------------------------------
+// K of one (page, KV head): what lane (kc, m) loads, and its operands
+// ---------------------------------------------------------------------------
+template <int FMT, int RES>
+struct KRaw {
+  uint4 code[FMT == kFmtQ2 ? 2 : 4];
+  uint4 res[RES == kResNone ? 1 : 8];
+  uint16_t s[4], z[FMT == kFmtQ2 ? 4 : 1];
+};
+
+template <int FMT, int RES>
+__device__ __forceinline__ void load_k(const AttendParams &p, size_t blk, int lane, KRaw<FMT, RES> &r) {
+  const int kc = lane >> 4, m = lane & 15;
+  if constexpr (FMT == kFmtQ2) {
+    const uint4 *c = (const uint4 *)(p.k + blk * 2048);
+    r.code[0] = c[lane];
+    r.code[1] = c[64 + lane];
+    const uint16_t *s = (const uint16_t *)(p.ks + blk * 512), *z = (const uint16_t *)(p.kz + blk * 512);
+#pragma unroll
+    for (int tau = 0; tau < 4; ++tau) {
+      const int at = (((tau >> 1) * 4 + kc) * 4 + (m >> 2)) * 8 + 4 * (tau & 1) + (m & 3);
+      r.s[tau] = s[at];
+      r.z[tau] = z[at];
+    }
+  } else {
+    const uint4 *c = (const uint4 *)(p.k + blk * 4096);
+#pragma unroll
+    for (int tau = 0; tau < 4; ++tau) {
+      r.code[tau] = c[64 * tau + lane];
+      if constexpr (FMT == kFmtNvfp4) r.s[tau] = ((const uint16_t *)(p.ks + blk * 512))[(4 * m + tau) * 4 + kc];
+      else r.s[tau] = ((const uint16_t *)(p.ks + blk * 256))[(4 * m + tau) * 2 + (kc >> 1)];
+    }
+  }
+  if constexpr (RES != kResNone) {
+    const uint4 *c = (const uint4 *)(p.kr + blk * 8192);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r.res[i] = c[64 * i + lane];
+  }
+}
+
+template <bool E4M3, bool HI>
+__device__ __forceinline__ f32x2 fp8_pair(uint32_t w) {
+  if constexpr (E4M3) return __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w, 1.0f, HI);
+  else return __builtin_amdgcn_cvt_scalef32_pk_f32_bf8(w, 1.0f, HI);
+}
+
+// Operands e = 0..3 of tile tau: channels 32 kc + 8 e + (0..7) of token 4 m + tau.  fp32 arithmetic, one rounding.
+template <int FMT, int RES>
+__device__ __forceinline__ void k_operands(const KRaw<FMT, RES> &r, int tau, const float2 *nf4, f16x8 *op) {
+  float s, z = 0.f, s1 = 0.f;
+  if constexpr (FMT == kFmtNvfp4) {
+    const f32x2 w = fp8_pair<true, false>(r.s[tau]);
+    s = w[0];
+    s1 = w[1];
+  } else {
+    s = f16_bits_to_f32(r.s[tau]);
+    if constexpr (FMT == kFmtQ2) z = f16_bits_to_f32(r.z[tau]);
+  }
+  uint32_t cw[4];  // q2: two words of 16 codes; 4-bit: a word of 8 codes for each e
+  if constexpr (FMT == kFmtQ2) {
+    const uint4 c = r.code[tau >> 1];
+    cw[0] = tau & 1 ? c.z : c.x;
+    cw[1] = tau & 1 ? c.w : c.y;
+  } else {
+    const uint4 c = r.code[tau];
+    cw[0] = c.x;
+    cw[1] = c.y;
+    cw[2] = c.z;
+    cw[3] = c.w;
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    float k[8];
+    f32x2 res[4];
+    if constexpr (RES != kResNone) {
+      const uint4 rw = r.res[2 * tau + (e >> 1)];
+      const uint32_t lo = e & 1 ? rw.z : rw.x, hi = e & 1 ? rw.w : rw.y;
+      res[0] = fp8_pair<RES == kResE4M3, false>(lo);
+      res[1] = fp8_pair<RES == kResE4M3, true>(lo);
+      res[2] = fp8_pair<RES == kResE4M3, false>(hi);
+      res[3] = fp8_pair<RES == kResE4M3, true>(hi);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) res[i] = f32x2{0.f, 0.f};
+    }
+    if constexpr (FMT == kFmtQ2) {
+      // a 2-bit code as a nibble is the e2m1 value c / 2: the conversion with scale 2 gives codes 4 i, 4 i + 2 of
+      // byte i, and of the word shifted by one code 4 i + 1, 4 i + 3
+      const uint32_t a = cw[e >> 1] & 0x33333333u, b = (cw[e >> 1] >> 2) & 0x33333333u;
+      f32x2 a0, a1, b0, b1;
+      if (e & 1) {
+        a0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(a, 2.0f, 2);
+        a1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(a, 2.0f, 3);
+        b0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(b, 2.0f, 2);
+        b1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(b, 2.0f, 3);
+      } else {
+        a0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(a, 2.0f, 0);
+        a1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(a, 2.0f, 1);
+        b0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(b, 2.0f, 0);
+        b1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(b, 2.0f, 1);
+      }
+      const float c[8] = {a0[0], b0[0], a0[1], b0[1], a1[0], b1[0], a1[1], b1[1]};
+#pragma unroll
+      for (int i = 0; i < 8; ++i) k[i] = __builtin_fmaf(c[i], s, z) + res[i >> 1][i & 1];
+    } else if constexpr (FMT == kFmtNvfp4) {
+      const float se = e < 2 ? s : s1;
+      const f32x2 c[4] = {__builtin_amdgcn_cvt_scalef32_pk_f32_fp4(cw[e], 1.0f, 0),
+                          __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(cw[e], 1.0f, 1),
+                          __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(cw[e], 1.0f, 2),
+                          __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(cw[e], 1.0f, 3)};
+#pragma unroll
+      for (int i = 0; i < 8; ++i) k[i] = __builtin_fmaf(c[i >> 1][i & 1], se, res[i >> 1][i & 1]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 c = nf4[(cw[e] >> (8 * i)) & 0xffu];
+        k[2 * i] = __builtin_fmaf(c.x, s, res[i][0]);
+        k[2 * i + 1] = __builtin_fmaf(c.y, s, res[i][1]);
+      }
+    }
+    const u32x4 w = {pk_f16_bits(k[0], k[1]), pk_f16_bits(k[2], k[3]), pk_f16_bits(k[4], k[5]), pk_f16_bits(k[6], k[7])};
+    op[e] = __builtin_bit_cast(f16x8, w);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// q of one row tile as the B operands, each row divided by a power of two that brings its largest element into
+// [1, 2): every bf16 row fits fp16 that way (elements below 2^-14 of the row's largest lose bits that its scores,
+// rounded at 2^-24 of the sum, do not hold).  cs: the row's factor back to log2-scaled scores.
+// ---------------------------------------------------------------------------
+__device__ __forceinline__ void load_q(const AttendParams &p, size_t row, bool ok, int kc, f16x8 *op, float &cs) {
+  float x[32];
+  const uint4 *src = (const uint4 *)((const uint16_t *)p.q + row * kD + 32 * kc);
+  float top = 0.f;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const uint4 w = ok ? src[e] : make_uint4(0, 0, 0, 0);
+    const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[8 * e + 2 * i] = p.q_bf16 ? __uint_as_float(ww[i] << 16) : f16_bits_to_f32(ww[i] & 0xffffu);
+      x[8 * e + 2 * i + 1] = p.q_bf16 ? __uint_as_float(ww[i] & 0xffff0000u) : f16_bits_to_f32(ww[i] >> 16);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x[8 * e + i]));
+  }
+  top = xor_max(top, 16);
+  top = xor_max(top, 32);
+  int ex = (int)((__float_as_uint(top) >> 23) & 0xffu);  // 0: all zero or tiny; 255: an infinity
+  ex = ex == 255 ? 127 : min(max(ex, 1), 253);
+  const float f = __uint_as_float((uint32_t)(254 - ex) << 23);
+  cs = p.scale2 * __uint_as_float((uint32_t)ex << 23);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    u32x4 w;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = pk_f16_bits(x[8 * e + 2 * i] * f, x[8 * e + 2 * i + 1] * f);
+    op[e] = __builtin_bit_cast(f16x8, w);
+  }
+}
+
+// whether a half of the 8 fp16 values is an infinity or NaN: bit 15 or 31 of the result
+__device__ __forceinline__ uint32_t not_finite8(f16x8 v) {
+  const u32x4 w = __builtin_bit_cast(u32x4, v);
+  uint32_t r = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r |= (w[i] & 0x7c007c00u) + 0x04000400u;
+  return r & 0x80008000u;
+}
+
+// ---------------------------------------------------------------------------
+// The softmax step of one row tile over one page: scores to P operands, m and l of lane (g, n)'s row n
+// (l: the lane's own tokens only, summed over g at the end).  MASK: tokens at or past lim (relative to the page) do
+// not count.  Returns the factor that the row's O so far is to be multiplied by (1 where m stands).
+// ---------------------------------------------------------------------------
+template <bool MASK>
+__device__ __forceinline__ bool softmax_step(f32x4 *S, float cs, int nvis, int g, float &m, float &l, float &alpha,
+                                             f16x8 *P) {
+  float x[16];
+  float top = kNoMax;
+#pragma unroll
+  for (int tau = 0; tau < 4; ++tau)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int k = 4 * i + tau;
+      x[k] = S[tau][i] * cs;
+      if (!MASK || 16 * g + k < nvis) top = fmaxf(top, x[k]);
+    }
+  // the largest m may lag by kStale: most pages need no exchange between the row's four lanes and leave O as it is
+  const bool moved = __ballot(top > m + kStale) != 0;
+  alpha = 1.f;
+  if (moved) {
+    top = xor_max(top, 16);
+    top = xor_max(top, 32);
+    const float mn = fmaxf(m, top);
+    alpha = exp2_hw(m - mn);
+    m = mn;
+    l *= alpha;
+  }
+  float sum = 0.f;
+#pragma unroll
+  for (int k = 0; k < 16; ++k) {
+    x[k] = (!MASK || 16 * g + k < nvis) ? exp2_hw(x[k] - m) : 0.f;
+    sum += x[k];
+  }
+  l += sum;
+#pragma unroll
+  for (int kap = 0; kap < 2; ++kap) {
+    u32x4 w;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = pk_f16_bits(x[8 * kap + 2 * i], x[8 * kap + 2 * i + 1]);
+    P[kap] = __builtin_bit_cast(f16x8, w);
+  }
+  return moved;
+}
+
+__device__ __forceinline__ f32x4 mfma16(f16x8 a, f16x8 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+
+// a partial (or, without slots, the output) of 8 columns of one row
+__device__ __forceinline__ void store_row8(const AttendParams &p, size_t row, int slot, int c0, const float *o, float m,
+                                           float l, bool sees) {
+  if (p.nslots == 0) {
+    const float inv = sees ? 1.f / l : 0.f;
+    float y[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) y[e] = sees ? o[e] * inv : 0.f;
+    uint4 w;
+    if (p.out_bf16) w = make_uint4(pk_bf16_bits(y[0], y[1]), pk_bf16_bits(y[2], y[3]), pk_bf16_bits(y[4], y[5]), pk_bf16_bits(y[6], y[7]));
+    else w = make_uint4(pk_f16_bits(y[0], y[1]), pk_f16_bits(y[2], y[3]), pk_f16_bits(y[4], y[5]), pk_f16_bits(y[6], y[7]));
+    *(uint4 *)((uint16_t *)p.out + row * kD + c0) = w;
+    return;
+  }
+  const size_t at = row * p.nslots + slot;
+  float4 *dst = (float4 *)(p.part_o + at * kD + c0);
+  dst[0] = make_float4(o[0], o[1], o[2], o[3]);
+  dst[1] = make_float4(o[4], o[5], o[6], o[7]);
+  if (c0 == 0) *(float2 *)(p.part_ml + 2 * at) = make_float2(m, l);
+}
+
+// ---------------------------------------------------------------------------
+// Few rows (up to 16 NT of a KV head and set per workgroup): each wave takes every fourth page of the range with all
+// rows, its operands straight from memory; the waves' results are joined in LDS.
+// ---------------------------------------------------------------------------
+template <int FMT, int RES, int VT, int NT>
+__global__ __launch_bounds__(256) void paged_attend_kernel(const AttendParams p) {
+  typedef VTraits<VT> VTr;
+  const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int g = lane >> 4, n = lane & 15;
+  const int split = blockIdx.x, hkv = blockIdx.y % p.HKV, rb = blockIdx.y / p.HKV;
+  const AttendSet set = attend_set(p, blockIdx.z);
+  const int LG = p.L * p.G, R = set.n * LG, r0 = rb * 16 * NT;
+  if (r0 >= R) return;
+  const int pa = set.p0 + split * p.ppw, pe = min(pa + p.ppw, set.p1);
+  if (pa >= pe && p.nslots != 0) return;
+
+  __shared__ float s_m[4][16 * NT], s_l[4][16 * NT];
+  __shared__ __attribute__((aligned(16))) float s_o[4][16][kD + 4];
+  __shared__ float2 s_nf4[FMT == kFmtNf4 ? 256 : 1];
+  if constexpr (FMT == kFmtNf4) {
+    s_nf4[threadIdx.x] = make_float2(kAttendNF4[threadIdx.x & 15], kAttendNF4[threadIdx.x >> 4]);
+    __syncthreads();
+  }
+
+  f16x8 Q[NT][4];
+  float cs[NT], m[NT], l[NT];
+  int lim[NT];
+  int lo = 0x7fffffff, hi = 0;
+  f32x4 O[NT][8];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    const int r = r0 + 16 * t + n;
+    const bool ok = r < R;
+    const int bi = ok ? r / LG : 0, j = ok ? r - bi * LG : 0, i = j / p.G;
+    const size_t row = ((size_t)(set.b0 + bi) * p.L + i) * p.HQ + hkv * p.G + (j - i * p.G);
+    load_q(p, row, ok, g, Q[t], cs[t]);
+    lim[t] = ok ? row_limit(p, set.b0 + bi, i) : 0x7fffffff;  // rows past the last are computed, and not stored
+    lo = min(lo, lim[t]);
+    hi = max(hi, ok ? lim[t] : 0);
+    m[t] = kNoMax;
+    l[t] = 0.f;
+#pragma unroll
+    for (int u = 0; u < 8; ++u) O[t][u] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+#pragma unroll
+  for (int s = 1; s < 16; s <<= 1) {
+    lo = min(lo, __shfl_xor(lo, s));
+    hi = max(hi, __shfl_xor(hi, s));
+  }
+  lo = __builtin_amdgcn_readfirstlane(lo);
+  hi = __builtin_amdgcn_readfirstlane(hi);
+  const int32_t *bt = p.bt + (size_t)set.b0 * p.bt_stride;
+
+  for (int pg = pa + wv; pg < pe; pg += 4) {
+    const int t0 = pg * kPage;
+    if (t0 >= hi) break;  // no row sees this page or a later one
+    int id = bt[pg];
+    id = __builtin_amdgcn_readfirstlane((unsigned)id < (unsigned)p.num_pages ? id : 0);
+    const size_t blk = (size_t)id * p.HKV + hkv;
+    KRaw<FMT, RES> kr;
+    load_k<FMT, RES>(p, blk, lane, kr);
+    u32x4 V[16];
+    const u32x4 *vp = (const u32x4 *)(p.v + blk * (kD * kPage * 2));
+#pragma unroll
+    for (int i = 0; i < 16; ++i) V[i] = vp[64 * i + lane];
+
+    f32x4 S[NT][4];
+#pragma unroll
+    for (int tau = 0; tau < 4; ++tau) {
+      f16x8 K[4];
+      k_operands<FMT, RES>(kr, tau, s_nf4, K);
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        f32x4 a = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) a = mfma16(K[e], Q[t][e], a);
+        S[t][tau] = a;
+      }
+    }
+    const bool full = lo >= t0 + kPage;  // every row sees the whole page
+    f16x8 P[NT][2];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      float alpha;
+      const bool moved = full ? softmax_step<false>(S[t], cs[t], 64, g, m[t], l[t], alpha, P[t])
+                              : softmax_step<true>(S[t], cs[t], lim[t] - t0, g, m[t], l[t], alpha, P[t]);
+      if (moved)
+#pragma unroll
+        for (int u = 0; u < 8; ++u) O[t][u] *= alpha;
+    }
+    bool apart = false;  // rows that do not see an infinity or NaN of V would get 0 * inf
+    if (!full) {
+      u32x4 keep[2];
+      partial_page_masks(g, hi - t0, keep);  // slots that no row sees are not data
+      uint32_t bad = 0;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        V[i] &= keep[i & 1];
+        bad |= not_finite8(VTr::operand(V[i]));
+      }
+      apart = lo < min(hi, t0 + kPage) && __ballot(bad != 0) != 0;
+    }
+    if (!apart) {
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+#pragma unroll
+        for (int kap = 0; kap < 2; ++kap) {
+          const f16x8 a = VTr::operand(V[2 * u + kap]);
+#pragma unroll
+          for (int t = 0; t < NT; ++t) O[t][u] = mfma16(a, P[t][kap], O[t][u]);
+        }
+    } else {
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+        for (int r = 0; r < 16; ++r) {  // row by row, with the tokens that the row sees
+          const int nv = __shfl(lim[t], r) - t0;
+          if (nv <= 0) continue;
+          u32x4 keep[2];
+          partial_page_masks(g, nv, keep);
+#pragma unroll
+          for (int u = 0; u < 8; ++u) {
+            f32x4 a = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int kap = 0; kap < 2; ++kap) a = mfma16(VTr::operand(V[2 * u + kap] & keep[kap]), P[t][kap], a);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) O[t][u][e] += n == r ? a[e] : 0.f;
+          }
+        }
+    }
+  }
+
+  // join the four waves
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    l[t] = xor_sum(l[t], 16);
+    l[t] = xor_sum(l[t], 32);
+    if (g == 0) {
+      s_m[wv][16 * t + n] = m[t];
+      s_l[wv][16 * t + n] = l[t];
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    float M = kNoMax;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) M = fmaxf(M, s_m[w][16 * t + n]);
+    const float f = exp2_hw(m[t] - M);
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
+      *(f32x4 *)&s_o[wv][n][16 * u + 4 * g] = O[t][u] * f;
+    __syncthreads();
+    const int rr = threadIdx.x >> 4, c0 = 8 * (threadIdx.x & 15);
+    const int r = r0 + 16 * t + rr;
+    if (r < R) {
+      float mm = kNoMax, ll = 0.f, o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int w = 0; w < 4; ++w) mm = fmaxf(mm, s_m[w][16 * t + rr]);
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        ll += s_l[w][16 * t + rr] * exp2_hw(s_m[w][16 * t + rr] - mm);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[e] += s_o[w][rr][c0 + e];
+      }
+      const int bi = r / LG, j = r - bi * LG, i = j / p.G, b = set.b0 + bi;
+      const size_t row = ((size_t)b * p.L + i) * p.HQ + hkv * p.G + (j - i * p.G);
+      store_row8(p, row, p.slot0 + split, c0, o, mm, ll, row_limit(p, b, i) > 0);
+    }
+    __syncthreads();
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Join of the partials: one workgroup per row; wave w adds the slots w, w + 4, ...
+// ---------------------------------------------------------------------------
+__global__ __launch_bounds__(256) void paged_attend_join_kernel(const AttendParams p) {
+  const int h = blockIdx.x % p.HQ, i = (blockIdx.x / p.HQ) % p.L, b = blockIdx.x / (p.HQ * p.L);
+  const size_t row = blockIdx.x;
+  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
+  (void)h;
+  __shared__ float s_m[4], s_l[4];
+  __shared__ float s_o[4][kD];
+  const bool sees = row_limit(p, b, i) > 0;
+  const int sp = shared_pages_of(p, b), own = max((seq_len_of(p, b) + kPage - 1) / kPage - sp, 0);
+  const int na = p.shared_slots ? min((sp + p.shared_ppw - 1) / p.shared_ppw, p.shared_slots) : 0;
+  const int nb = min((own + p.own_ppw - 1) / p.own_ppw, p.own_slots);
+  const float2 *ml = (const float2 *)p.part_ml + row * p.nslots;
+  const float *po = p.part_o + row * p.nslots * kD;
+  float m = kNoMax, l = 0.f;
+  float2 o = make_float2(0.f, 0.f);
+  for (int s = wv; s < na + nb && sees; s += 4) {
+    const int slot = s < na ? s : p.shared_slots + s - na;
+    const float2 x = ml[slot];
+    const float2 y = *(const float2 *)(po + (size_t)slot * kD + 2 * lane);
+    const float mn = fmaxf(m, x.x), fo = exp2_hw(m - mn), fn = exp2_hw(x.x - mn);
+    m = mn;
+    l = l * fo + x.y * fn;
+    o.x = o.x * fo + y.x * fn;
+    o.y = o.y * fo + y.y * fn;
+  }
+  if (lane == 0) {
+    s_m[wv] = m;
+    s_l[wv] = l;
+  }
+  *(float2 *)&s_o[wv][2 * lane] = o;
+  __syncthreads();
+  if (wv == 0) {
+    const float M = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
+    float L = 0.f, x = 0.f, y = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float f = exp2_hw(s_m[w] - M);
+      L += s_l[w] * f;
+      x += s_o[w][2 * lane] * f;
+      y += s_o[w][2 * lane + 1] * f;
+    }
+    const float inv = 1.f / L;
+    x = sees ? x * inv : 0.f;
+    y = sees ? y * inv : 0.f;
+    ((uint32_t *)p.out)[row * (kD / 2) + lane] = p.out_bf16 ? pk_bf16_bits(x, y) : pk_f16_bits(x, y);
+  }
+}
+
+// Launch plan of a call: page ranges of the shared and of the own pages
+struct AttendPlan {
+  int shared_slots, shared_ppw, own_slots, own_ppw, nslots;
+  int shared_nt, shared_blocks, own_nt, own_blocks;
+  int own_pages;
+};
+
+static int tiles_for(long rows) { return rows <= 16 ? 1 : (rows <= 32 ? 2 : 4); }
+
+static AttendPlan attend_plan(const ffa_paged_attend_args *a, int cus) {
+  AttendPlan pl = {};
+  const int G = a->HQ / a->HKV;
+  const long want = 4l * (cus > 0 ? cus : 256);  // workgroups that fill the chip
+  const long LG = (long)a->L * G;
+  auto ranges = [&](long units, int pages, int &ppw, int &slots) {
+    // units: pages over all sets, heads and row blocks; a workgroup of at least 4 pages, one per wave
+    long w = (units + want - 1) / want;
+    w = (w + 3) / 4 * 4;
+    ppw = (int)(w < 4 ? 4 : (w > pages ? (pages < 4 ? 4 : pages) : w));
+    slots = (pages + ppw - 1) / ppw;
+  };
+  int min_shared = 0;
+  if (a->ngroups > 0) {
+    long units = 0, rows = 0;
+    int pages = 0;
+    min_shared = a->group_pages_host[0];
+    for (int g = 0; g < a->ngroups; ++g) {
+      const long n = a->group_start_host[g + 1] - a->group_start_host[g];
+      const int gp = a->group_pages_host[g];
+      if (gp > 0 && n * LG > rows) rows = n * LG;
+      if (gp > pages) pages = gp;
+      if (gp < min_shared) min_shared = gp;
+    }
+    if (pages > 0) {
+      pl.shared_nt = tiles_for(rows);
+      pl.shared_blocks = (int)((rows + 16 * pl.shared_nt - 1) / (16 * pl.shared_nt));
+      for (int g = 0; g < a->ngroups; ++g) {
+        const long n = a->group_start_host[g + 1] - a->group_start_host[g];
+        units += (long)a->group_pages_host[g] * a->HKV * ((n * LG + 16 * pl.shared_nt - 1) / (16 * pl.shared_nt));
+      }
+      ranges(units, pages, pl.shared_ppw, pl.shared_slots);
+    }
+  }
+  pl.own_pages = (a->T + kPage - 1) / kPage - min_shared;
+  if (pl.own_pages < 0) pl.own_pages = 0;
+  pl.own_nt = tiles_for(LG);
+  pl.own_blocks = (int)((LG + 16 * pl.own_nt - 1) / (16 * pl.own_nt));
+  pl.own_ppw = 4;
+  if (pl.own_pages > 0) ranges((long)pl.own_pages * a->HKV * pl.own_blocks * a->B, pl.own_pages, pl.own_ppw, pl.own_slots);
+  pl.nslots = pl.shared_slots + pl.own_slots;
+  if (pl.shared_slots == 0 && pl.own_slots <= 1) {  // one range: no partials
+    pl.own_slots = 1;
+    pl.nslots = 0;
+  }
+  return pl;
+}
+
+template <int FMT, int RES, int VT>
+static void launch_attend(const AttendParams &p, int nt, dim3 grid, hipStream_t st) {
+  if (nt == 1) hipLaunchKernelGGL((paged_attend_kernel<FMT, RES, VT, 1>), grid, dim3(256), 0, st, p);
+  else if (nt == 2) hipLaunchKernelGGL((paged_attend_kernel<FMT, RES, VT, 2>), grid, dim3(256), 0, st, p);
+  else hipLaunchKernelGGL((paged_attend_kernel<FMT, RES, VT, 4>), grid, dim3(256), 0, st, p);
+}
+
+template <int FMT>
+static void launch_attend_fmt(const AttendParams &p, int res, int vdt, int nt, dim3 grid, hipStream_t st) {
+#define FFA_CASE(RR, RC)                                                                \
+  if (res == RC) {                                                                      \
+    if (vdt == FFA_DT_BF16) launch_attend<FMT, RR, kVBF16>(p, nt, grid, st);            \
+    else launch_attend<FMT, RR, kVF16>(p, nt, grid, st);                                \
+  }
+  FFA_CASE(kResE4M3, FFA_DT_FP8_E4M3)
+  FFA_CASE(kResE5M2, FFA_DT_FP8_E5M2)
+  FFA_CASE(kResNone, FFA_DT_NONE)
+#undef FFA_CASE
+}
+
+static int attend_check(const ffa_paged_attend_args *a) {
+#define FFA_BAD(msg) return ffa_set_error_internal(FFA_E_INVALID, msg)
+#define FFA_NO(msg) return ffa_set_error_internal(FFA_E_UNSUPPORTED, msg)
+  if (!a) FFA_BAD("null args");
+  if (a->B <= 0 || a->T <= 0 || a->L <= 0 || a->HQ <= 0 || a->HKV <= 0) FFA_BAD("bad dims");
+  if (a->HQ % a->HKV) FFA_BAD("HQ must be a multiple of HKV");
+  if (a->B > 65535) FFA_NO("B is a grid dimension");
+  if (a->T > 1 << 30) FFA_NO("T above 2^30 tokens");
+  if (!(a->q_dtype == FFA_DT_F16 || a->q_dtype == FFA_DT_BF16)) FFA_BAD("q must be fp16 or bf16");
+  if (!(a->v_dtype == FFA_DT_F16 || a->v_dtype == FFA_DT_BF16)) FFA_BAD("v dtype");
+  if (a->format < FFA_PAGES_Q2 || a->format > FFA_PAGES_NF4) FFA_BAD("page format");
+  if (!(a->res_dtype == FFA_DT_FP8_E4M3 || a->res_dtype == FFA_DT_FP8_E5M2 || a->res_dtype == FFA_DT_NONE))
+    FFA_BAD("residual dtype must be fp8 or none");
+  if (a->bt_stride <= 0 || a->num_pages <= 0) FFA_BAD("empty block table or pool");
+  if ((long)a->bt_stride * kPage < a->T) FFA_BAD("block table has fewer than ceil(T/64) columns");
+  if (!a->q || !a->k || !a->k_scale || !a->v || !a->block_table || !a->out) FFA_BAD("null pointer");
+  if (a->format == FFA_PAGES_Q2 && !a->k_zero) FFA_BAD("2-bit pages need k_zero");
+  if (a->res_dtype != FFA_DT_NONE && !a->k_residual) FFA_BAD("null residual");
+  if ((long)a->B * a->L * a->HQ > 0x7fffffffl) FFA_NO("more than 2^31 - 1 query rows");
+  if (a->ngroups < 0 || a->ngroups > a->B) FFA_BAD("ngroups must be within [0, B]");
+  if (a->ngroups > 0) {
+    if (!a->group_start || !a->group_pages || !a->seq_group || !a->group_start_host || !a->group_pages_host)
+      FFA_BAD("groups need their arrays");
+    if (a->group_start_host[0] != 0 || a->group_start_host[a->ngroups] != a->B) FFA_BAD("groups must cover the batch");
+    for (int g = 0; g < a->ngroups; ++g) {
+      if (a->group_start_host[g + 1] <= a->group_start_host[g]) FFA_BAD("a group without sequences");
+      if (a->group_pages_host[g] < 0 || a->group_pages_host[g] > a->bt_stride) FFA_BAD("shared pages exceed the block table");
+    }
+  }
+  const uintptr_t al = (uintptr_t)a->q | (uintptr_t)a->k | (uintptr_t)a->v | (uintptr_t)a->out |
+                       (uintptr_t)a->k_residual | (uintptr_t)a->k_scale | (uintptr_t)a->k_zero;
+  if (al & 15) FFA_BAD("q, out and the pools must be multiples of 16 bytes");
+  return FFA_OK;
+}
+
+}  // namespace ffa
+
+extern "C" size_t ffa_paged_attend_scratch(const ffa_paged_attend_args *a) {
+  using namespace ffa;
+  if (attend_check(a) != FFA_OK) return 0;
+  return (size_t)a->B * a->L * a->HQ * attend_plan(a, device_cus()).nslots * (kD + 2) * sizeof(float);
+}
+
+extern "C" int ffa_paged_attend(const ffa_paged_attend_args *a, void *stream) {
+  using namespace ffa;
+  const int bad = attend_check(a);
+  if (bad != FFA_OK) return bad;
+  const AttendPlan pl = attend_plan(a, device_cus());
+  const size_t rows = (size_t)a->B * a->L * a->HQ;
+  if (a->scratch_bytes < rows * pl.nslots * (kD + 2) * sizeof(float) || (pl.nslots && !a->scratch))
+    FFA_BAD("scratch below ffa_paged_attend_scratch()");
+  if ((uintptr_t)a->scratch & 15) FFA_BAD("scratch must be a multiple of 16 bytes");
+  if ((long)pl.own_blocks * a->HKV > 65535 || (long)pl.shared_blocks * a->HKV > 65535) FFA_NO("more than 65535 row blocks");
+  AttendParams p = {};
+  p.q = a->q;
+  p.k = a->k;
+  p.ks = (const uint8_t *)a->k_scale;
+  p.kz = (const uint8_t *)a->k_zero;
+  p.kr = a->k_residual;
+  p.v = (const uint8_t *)a->v;
+  p.bt = a->block_table;
+  p.seq_lens = a->seq_lens;
+  p.q_lens = a->q_lens;
+  p.group_start = a->group_start;
+  p.group_pages = a->group_pages;
+  p.seq_group = a->seq_group;
+  p.out = a->out;
+  p.part_o = (float *)a->scratch;
+  p.part_ml = p.part_o + rows * pl.nslots * kD;
+  p.bt_stride = a->bt_stride;
+  p.num_pages = a->num_pages;
+  p.ngroups = a->ngroups;
+  p.B = a->B;
+  p.T = a->T;
+  p.L = a->L;
+  p.HQ = a->HQ;
+  p.HKV = a->HKV;
+  p.G = a->HQ / a->HKV;
+  p.q_bf16 = p.out_bf16 = a->q_dtype == FFA_DT_BF16;
+  p.scale2 = a->scale * kLog2e;
+  p.nslots = pl.nslots;
+  p.shared_slots = pl.shared_slots;
+  p.shared_ppw = pl.shared_ppw;
+  p.own_slots = pl.own_slots;
+  p.own_ppw = pl.own_ppw;
+  const hipStream_t st = (hipStream_t)stream;
+  auto launch = [&](int nt, dim3 grid) {
+    if (a->format == FFA_PAGES_Q2) launch_attend_fmt<kFmtQ2>(p, a->res_dtype, a->v_dtype, nt, grid, st);
+    else if (a->format == FFA_PAGES_NVFP4) launch_attend_fmt<kFmtNvfp4>(p, a->res_dtype, a->v_dtype, nt, grid, st);
+    else launch_attend_fmt<kFmtNf4>(p, a->res_dtype, a->v_dtype, nt, grid, st);
+  };
+  if (pl.shared_slots > 0) {
+    p.shared = 1;
+    p.slot0 = 0;
+    p.ppw = pl.shared_ppw;
+    launch(pl.shared_nt, dim3((unsigned)pl.shared_slots, (unsigned)(a->HKV * pl.shared_blocks), (unsigned)a->ngroups));
+  }
+  if (pl.own_slots > 0) {
+    p.shared = 0;
+    p.slot0 = pl.shared_slots;
+    p.ppw = pl.own_ppw;
+    launch(pl.own_nt, dim3((unsigned)pl.own_slots, (unsigned)(a->HKV * pl.own_blocks), (unsigned)a->B));
+  }
+  if (pl.nslots > 0)
+    hipLaunchKernelGGL(paged_attend_join_kernel, dim3((unsigned)rows), dim3(256), 0, st, p);
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? FFA_OK : ffa_set_error_internal(FFA_E_LAUNCH, hipGetErrorString(e));
+}
+#undef FFA_BAD
+#undef FFA_NO

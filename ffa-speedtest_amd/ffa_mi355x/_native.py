@@ -18,6 +18,7 @@ DT_F16, DT_BF16, DT_F32, DT_FP8_E4M3, DT_FP8_E5M2, DT_NONE = range(6)
 LAYOUT_CONTIG, LAYOUT_PAGED = 0, 1
 SCALE_CHANNEL, SCALE_G32 = 0, 1
 KFMT_FP8_E4M3, KFMT_FP8_E5M2, KFMT_NVFP4, KFMT_NF4 = range(4)
+PAGES_Q2, PAGES_NVFP4, PAGES_NF4 = range(3)
 KSCALE_NONE, KSCALE_TOKEN, KSCALE_BLOCK, KSCALE_CHANNEL, KSCALE_G16, KSCALE_G64 = range(6)
 
 EXPORTS = (
@@ -48,6 +49,8 @@ EXPORTS = (
     "ffa_nf4_g64_append",
     "ffa_nvfp4_g16_append_cast",
     "ffa_nf4_g64_append_cast",
+    "ffa_paged_attend_scratch",
+    "ffa_paged_attend",
     "ffa_last_error",
     "ffa_version",
 )
@@ -155,6 +158,41 @@ class KfmtArgs(ctypes.Structure):
     ]
 
 
+class AttendArgs(ctypes.Structure):
+    _fields_ = [
+        ("q", ctypes.c_void_p),
+        ("q_dtype", ctypes.c_int),
+        ("format", ctypes.c_int),
+        ("k", ctypes.c_void_p),
+        ("k_scale", ctypes.c_void_p),
+        ("k_zero", ctypes.c_void_p),
+        ("k_residual", ctypes.c_void_p),
+        ("res_dtype", ctypes.c_int),
+        ("v", ctypes.c_void_p),
+        ("v_dtype", ctypes.c_int),
+        ("block_table", ctypes.c_void_p),
+        ("bt_stride", ctypes.c_int),
+        ("num_pages", ctypes.c_int),
+        ("seq_lens", ctypes.c_void_p),
+        ("q_lens", ctypes.c_void_p),
+        ("B", ctypes.c_int),
+        ("T", ctypes.c_int),
+        ("L", ctypes.c_int),
+        ("HQ", ctypes.c_int),
+        ("HKV", ctypes.c_int),
+        ("scale", ctypes.c_float),
+        ("ngroups", ctypes.c_int),
+        ("group_start", ctypes.c_void_p),
+        ("group_pages", ctypes.c_void_p),
+        ("seq_group", ctypes.c_void_p),
+        ("group_start_host", ctypes.c_void_p),
+        ("group_pages_host", ctypes.c_void_p),
+        ("out", ctypes.c_void_p),
+        ("scratch", ctypes.c_void_p),
+        ("scratch_bytes", ctypes.c_size_t),
+    ]
+
+
 _lib = None
 _lock = threading.Lock()
 
@@ -227,6 +265,10 @@ def lib() -> ctypes.CDLL:
         for name in ("ffa_nvfp4_g16_append_cast", "ffa_nf4_g64_append_cast"):
             getattr(L, name).argtypes = [vp, ci, ci, ci, ci, vp, vp, ci, ci, vp, vp, vp, ci, vp, ci, vp, ci, vp]
             getattr(L, name).restype = ci
+        L.ffa_paged_attend_scratch.argtypes = [ctypes.POINTER(AttendArgs)]
+        L.ffa_paged_attend_scratch.restype = ctypes.c_size_t
+        L.ffa_paged_attend.argtypes = [ctypes.POINTER(AttendArgs), vp]
+        L.ffa_paged_attend.restype = ci
         _lib = L
         return _lib
 

@@ -118,6 +118,10 @@ class PagedQ2Cache:
     def nbytes_per_page(self) -> int:
         return sum(t[0].numel() * t.element_size() for t in (self.k_q, self.k_scale, self.k_zero, self.k_res, self.v))
 
+    def pools(self) -> list[torch.Tensor]:
+        """The pools, one page of each per page id."""
+        return [self.k_q, self.k_scale, self.k_zero, self.k_res, self.v]
+
     # ------------------------------------------------------------------ writes
     def append(self, k: torch.Tensor, v: torch.Tensor | None, pos: torch.Tensor, block_table: torch.Tensor):
         """g32-quantize k [B, Tn, HKV, 128] and write it (and v) at positions pos[b] + n."""
@@ -203,3 +207,11 @@ class PagedQ2Cache:
             layout=N.LAYOUT_PAGED, scale_mode=N.SCALE_G32, T=T, HKV=self.HKV, scale=scale, BS=BS, SBS=SBS,
             delta=delta, use_res=use_fp8_residual, precomputed_threshold=precomputed_threshold,
             block_table=block_table, seq_lens=seq_lens, workspace=workspace, stage=stage, v_mean=v_mean)
+
+    # ------------------------------------------------------------------ exact attention
+    def attend(self, q, block_table, seq_lens=None, **kw) -> torch.Tensor:
+        """Exact causal attention of the newest L tokens' q [B, L, HQ, 128] (fp16 or bf16) over the cache, without
+        pruning: T, q_lens, scale, use_fp8_residual, shared (SharedPrefix), out as in attend.run_attend."""
+        from .attend import run_attend
+
+        return run_attend("q2", q, self.k_q, self.k_scale, self.k_zero, self.k_res, self.v, block_table, seq_lens, **kw)

@@ -101,6 +101,10 @@ class PagedKfmtCache:
     def nbytes_per_page(self) -> int:
         return sum(t[0].numel() * t.element_size() for t in (self.k, self.k_scale, self.k_res, self.v))
 
+    def pools(self) -> list[torch.Tensor]:
+        """The pools, one page of each per page id."""
+        return [self.k, self.k_scale, self.k_res, self.v]
+
     def append(self, k: torch.Tensor, v: torch.Tensor | None, pos: torch.Tensor, block_table: torch.Tensor):
         """Quantize k [B, Tn, HKV, 128] and write it (and v) at positions pos[b] + n."""
         B, Tn, HKV, D = k.shape
@@ -124,3 +128,10 @@ class PagedKfmtCache:
 
     def decode(self, q, block_table, seq_lens=None, **kw) -> DecodeWorkspace:
         return decode_pools(self.fmt, q, self.k, self.k_scale, self.v, self.k_res, block_table, seq_lens, **kw)
+
+    def attend(self, q, block_table, seq_lens=None, **kw) -> torch.Tensor:
+        """Exact causal attention of the newest L tokens' q [B, L, HQ, 128] (fp16 or bf16) over the cache, without
+        pruning: T, q_lens, scale, use_fp8_residual, shared (SharedPrefix), out as in attend.run_attend."""
+        from .attend import run_attend
+
+        return run_attend(self.fmt, q, self.k, self.k_scale, None, self.k_res, self.v, block_table, seq_lens, **kw)

@@ -39,6 +39,10 @@
  *                             K-proj + RoPE + g32 quantize into the paged cache
  *                             (incremental quantisation is a TODO in the reference,
  *                              ffa-q2fp8/OPTIMIZATION_NOTES.md:23-26)
+ *   ffa_paged_attend          no reference counterpart: exact attention of L query tokens per
+ *                             sequence over the paged caches, shared leading pages read once
+ *                             per group of sequences (the reference attends to dequantized
+ *                             keys with a library call, ffa-fp8fp8/e2e/modeling_llama.py:322-337)
  *   ffa_kproj_rope            F.linear + apply_rope of every reference producer, e.g.
  *                             ffa-fp8fp8/fused_kproj_rope_fp8fp8.py:80-88,
  *                             ffa-nvfp4fp8/fused_kproj_rope_nvfp4fp8.py:131-139,
@@ -433,6 +437,58 @@ typedef struct ffa_kfmt_decode_args {
 } ffa_kfmt_decode_args;
 
 int ffa_kfmt_decode(const ffa_kfmt_decode_args *args, void *stream);
+
+/*
+ * Exact attention of L query tokens per sequence over a paged cache (no pruning):
+ *   out[b, i, h] = sum_t softmax_t(scale * q[b, i, h] . k_t) v_t over the keys t < len_b - qlen_b + i + 1
+ * (query token i of sequence b sits at position len_b - qlen_b + i, causal), with
+ *   k = code * scale + zero + residual (2-bit pages), level * scale + residual (nvfp4, nf4 pages).
+ * Rows that see no key (i >= qlen_b, an empty sequence, more query tokens than keys) are zeros.
+ * q and out [B, L, HQ, 128] in fp16 or bf16; k is rounded to fp16 once, V of a bf16 pool likewise
+ * (|v| <= 65504), products of fp16 operands are summed in fp32, and so are the softmax statistics.
+ *
+ * Groups (ngroups > 0): sequences group_start[g] .. group_start[g + 1] - 1 share the pages of the
+ * first group_pages[g] columns of their block-table rows (the first sequence's row is read), which
+ * are then read once for all of them.  The result is that of the call without groups.  The arrays
+ * are given on the device and again in host memory (read during the call, for the launch plan).
+ *
+ * Scratch (caller-owned, ffa_paged_attend_scratch() bytes; 0 when no page range is split): fp32
+ * partials of the page ranges.  Calls that share scratch must be ordered on one stream.  Block-table
+ * entries outside [0, num_pages) read page 0.
+ */
+enum { FFA_PAGES_Q2 = 0, FFA_PAGES_NVFP4 = 1, FFA_PAGES_NF4 = 2 };
+typedef struct ffa_paged_attend_args {
+  const void *q; /* [B, L, HQ, 128] */
+  int q_dtype;   /* F16 or BF16, also out's */
+  int format;    /* FFA_PAGES_* */
+  const uint8_t *k;
+  const void *k_scale;
+  const void *k_zero;        /* 2-bit pages only, else NULL */
+  const uint8_t *k_residual; /* may be NULL when res_dtype == FFA_DT_NONE */
+  int res_dtype;
+  const void *v;
+  int v_dtype; /* F16 or BF16 */
+  const int32_t *block_table; /* [B, bt_stride], bt_stride >= ceil(T/64) */
+  int bt_stride;
+  int num_pages;
+  const int32_t *seq_lens; /* [B] or NULL (every sequence has T tokens); clamped to [0, T] */
+  const int32_t *q_lens;   /* [B] or NULL (L query tokens each); clamped to [0, L] */
+  int B, T, L, HQ, HKV;
+  float scale;
+  int ngroups;
+  const int32_t *group_start; /* device, [ngroups + 1] */
+  const int32_t *group_pages; /* device, [ngroups] */
+  const int32_t *seq_group;   /* device, [B]: the group of each sequence */
+  const int32_t *group_start_host;
+  const int32_t *group_pages_host;
+  void *out; /* [B, L, HQ, 128] */
+  void *scratch;
+  size_t scratch_bytes;
+} ffa_paged_attend_args;
+
+/* Bytes of scratch that a call with these arguments needs (scratch and scratch_bytes are not read). */
+size_t ffa_paged_attend_scratch(const ffa_paged_attend_args *args);
+int ffa_paged_attend(const ffa_paged_attend_args *args, void *stream);
 
 const char *ffa_last_error(void);
 const char *ffa_version(void);
