@@ -100,7 +100,11 @@ def check_append_fits(pos: torch.Tensor, Tn: int, block_table: torch.Tensor, num
         raise ValueError("append positions exceed the block table")
     used = table[:, : last // PAGE + 1]
     if int(used.min().item()) < 0 or int(used.max().item()) >= num_pages:
-        raise ValueError("block table references pages outside the pool")
+        # rows of a ragged batch hold no pages past their own last position (PagePool leaves -1 there)
+        used, pos = torch.as_tensor(used).cpu(), pos.reshape(-1, 1).cpu()
+        used = used[torch.arange(used.shape[1]) <= (pos + (Tn - 1)) // PAGE]
+        if int(used.min()) < 0 or int(used.max()) >= num_pages:
+            raise ValueError("block table references pages outside the pool")
 
 
 class PagedQ2Cache:
