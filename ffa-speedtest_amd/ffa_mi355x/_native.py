@@ -51,6 +51,13 @@ EXPORTS = (
     "ffa_nf4_g64_append_cast",
     "ffa_paged_attend_scratch",
     "ffa_paged_attend",
+    "ffa_pages_copy",
+    "ffa_pages_alloc_scratch",
+    "ffa_pages_fork",
+    "ffa_pages_extend",
+    "ffa_pages_count",
+    "ffa_pages_compact_scratch",
+    "ffa_pages_compact",
     "ffa_last_error",
     "ffa_version",
 )
@@ -193,6 +200,16 @@ class AttendArgs(ctypes.Structure):
     ]
 
 
+class Pages(ctypes.Structure):
+    _fields_ = [
+        ("pools", ctypes.c_void_p),
+        ("page_bytes", ctypes.c_void_p),
+        ("npools", ctypes.c_int),
+        ("num_pages", ctypes.c_int),
+        ("refs", ctypes.c_void_p),
+    ]
+
+
 _lib = None
 _lock = threading.Lock()
 
@@ -269,6 +286,17 @@ def lib() -> ctypes.CDLL:
         L.ffa_paged_attend_scratch.restype = ctypes.c_size_t
         L.ffa_paged_attend.argtypes = [ctypes.POINTER(AttendArgs), vp]
         L.ffa_paged_attend.restype = ci
+        pg, cz = ctypes.POINTER(Pages), ctypes.c_size_t
+        L.ffa_pages_copy.argtypes = [pg, vp, vp, ci, vp]
+        L.ffa_pages_alloc_scratch.argtypes = [ci, ci]
+        L.ffa_pages_fork.argtypes = [pg, vp, ci, ci, vp, vp, ci, vp, vp, vp, vp]
+        L.ffa_pages_extend.argtypes = [pg, vp, ci, ci, vp, ci, vp, vp, vp]
+        L.ffa_pages_count.argtypes = [pg, vp, ci, ci, vp, ci, vp, vp, vp]
+        L.ffa_pages_compact_scratch.argtypes = [ci]
+        L.ffa_pages_compact.argtypes = [pg, vp, vp, ci, vp, vp]
+        for name in ("copy", "fork", "extend", "count", "compact"):
+            getattr(L, "ffa_pages_" + name).restype = ci
+        L.ffa_pages_alloc_scratch.restype = L.ffa_pages_compact_scratch.restype = cz
         _lib = L
         return _lib
 

@@ -43,6 +43,9 @@
  *                             sequence over the paged caches, shared leading pages read once
  *                             per group of sequences (the reference attends to dequantized
  *                             keys with a library call, ffa-fp8fp8/e2e/modeling_llama.py:322-337)
+ *   ffa_pages_*               no reference counterpart: copying, forking, extending, freeing and
+ *                             compacting the pages of the paged caches (the reference grows one
+ *                             contiguous cache by torch.cat, ffa-fp8fp8/e2e/fp8fp8_cache.py:84-89)
  *   ffa_kproj_rope            F.linear + apply_rope of every reference producer, e.g.
  *                             ffa-fp8fp8/fused_kproj_rope_fp8fp8.py:80-88,
  *                             ffa-nvfp4fp8/fused_kproj_rope_nvfp4fp8.py:131-139,
@@ -489,6 +492,57 @@ typedef struct ffa_paged_attend_args {
 /* Bytes of scratch that a call with these arguments needs (scratch and scratch_bytes are not read). */
 size_t ffa_paged_attend_scratch(const ffa_paged_attend_args *args);
 int ffa_paged_attend(const ffa_paged_attend_args *args, void *stream);
+
+/*
+ * Management of the pages of one or several caches (layers) that share page ids.  refs [num_pages]
+ * counts the block-table rows that hold each page; a page is free while its count is 0.  New pages
+ * are the lowest free ids, in (row, column) order: results depend on counts and tables alone.  Block
+ * tables are [rows, bt_stride] int32, seq_lens [rows]; a row's pages are its first ceil(len / 64)
+ * columns.  Page contents are copied whole, in every pool of the list.  Nothing synchronises: errors
+ * of the device data set bits in *errors (kept until the caller clears it) and in the call's own word
+ * (scratch[0], call_errors): 1 not enough free pages, 2 a row that cannot be served (a parent outside
+ * the batch, a length outside its row, a partial page that is free or outside the pool), 4 a page id
+ * outside the pool or a page that was free where a held one is needed.
+ */
+typedef struct ffa_pages {
+  void *const *pools;       /* host array of npools device pointers, multiples of 16 bytes */
+  const size_t *page_bytes; /* host array: bytes of one page in each pool, multiples of 16 */
+  int npools;
+  int num_pages;
+  int32_t *refs; /* device, [num_pages] */
+} ffa_pages;
+
+/* Copy page src[i] to page dst[i] for i < n in every pool (counts stay).  Pairs whose ids are outside the
+ * pool are left out; the destinations must be distinct and none of them a source. */
+int ffa_pages_copy(const ffa_pages *pages, const int32_t *src, const int32_t *dst, int n, void *stream);
+
+/* int32 words of scratch of ffa_pages_fork (tokens = 0) and ffa_pages_extend. */
+size_t ffa_pages_alloc_scratch(int rows, int tokens);
+
+/* Fork: child c continues sequence parents[c]: its row holds the parent's whole pages (counted once
+ * more) and, where the length ends inside a page, a new page with that page's contents; columns past
+ * them are -1.  child_table [children, bt_stride].  When the pages do not suffice or a row cannot be
+ * served, every child's row is -1 and nothing else changes; scratch[1] is the number of new pages. */
+int ffa_pages_fork(const ffa_pages *pages, const int32_t *block_table, int bt_stride, int B, const int32_t *seq_lens,
+                   const int32_t *parents, int children, int32_t *child_table, int32_t *scratch, int32_t *errors,
+                   void *stream);
+
+/* Extend: new pages in block_table for the next `tokens` tokens of every row (columns ceil(len / 64) ..
+ * ceil((len + tokens) / 64) - 1); all rows or, on an error, none. */
+int ffa_pages_extend(const ffa_pages *pages, int32_t *block_table, int bt_stride, int rows, const int32_t *seq_lens,
+                     int tokens, int32_t *scratch, int32_t *errors, void *stream);
+
+/* Add step (1: hold, -1: free) to the counts of the rows' pages, once for each time that a row holds
+ * one; a count of 0 stays 0 (and is an error).  call_errors: one word, cleared by the caller. */
+int ffa_pages_count(const ffa_pages *pages, const int32_t *block_table, int bt_stride, int rows,
+                    const int32_t *seq_lens, int step, int32_t *call_errors, int32_t *errors, void *stream);
+
+/* Compact: with n pages held, the i-th held page from id n on moves to the i-th free page below n
+ * (contents and count), and entries of the tables that name a moved page name its new id.  scratch:
+ * ffa_pages_compact_scratch() int32 words; afterwards scratch[0] pages have moved and scratch[1] = n. */
+size_t ffa_pages_compact_scratch(int num_pages);
+int ffa_pages_compact(const ffa_pages *pages, int32_t *const *tables, const size_t *table_entries, int ntables,
+                      int32_t *scratch, void *stream);
 
 const char *ffa_last_error(void);
 const char *ffa_version(void);
