@@ -134,37 +134,16 @@ __device__ __forceinline__ f32x2 fp8_pair(uint32_t w) {
   else return __builtin_amdgcn_cvt_scalef32_pk_f32_bf8(w, 1.0f, HI);
 }
 
-// Operands e = 0..3 of tile tau: channels 32 kc + 8 e + (0..7) of token 4 m + tau.  fp32 arithmetic, one rounding.
+// Two operands: channels 32 kc + 16 h + (0..7) and + (8..15) of a token, in fp32 arithmetic with one rounding.
+// q2: c0 holds the 16 codes; 4-bit: c0 and c1 8 codes each.  s: the scale of these channels, z the zero point (q2).
 template <int FMT, int RES>
-__device__ __forceinline__ void k_operands(const KRaw<FMT, RES> &r, int tau, const float2 *nf4, f16x8 *op) {
-  float s, z = 0.f, s1 = 0.f;
-  if constexpr (FMT == kFmtNvfp4) {
-    const f32x2 w = fp8_pair<true, false>(r.s[tau]);
-    s = w[0];
-    s1 = w[1];
-  } else {
-    s = f16_bits_to_f32(r.s[tau]);
-    if constexpr (FMT == kFmtQ2) z = f16_bits_to_f32(r.z[tau]);
-  }
-  uint32_t cw[4];  // q2: two words of 16 codes; 4-bit: a word of 8 codes for each e
-  if constexpr (FMT == kFmtQ2) {
-    const uint4 c = r.code[tau >> 1];
-    cw[0] = tau & 1 ? c.z : c.x;
-    cw[1] = tau & 1 ? c.w : c.y;
-  } else {
-    const uint4 c = r.code[tau];
-    cw[0] = c.x;
-    cw[1] = c.y;
-    cw[2] = c.z;
-    cw[3] = c.w;
-  }
+__device__ __forceinline__ void k_half(uint32_t c0, uint32_t c1, float s, float z, uint4 rw, const float2 *nf4, f16x8 *op) {
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
+  for (int e = 0; e < 2; ++e) {
     float k[8];
     f32x2 res[4];
     if constexpr (RES != kResNone) {
-      const uint4 rw = r.res[2 * tau + (e >> 1)];
-      const uint32_t lo = e & 1 ? rw.z : rw.x, hi = e & 1 ? rw.w : rw.y;
+      const uint32_t lo = e ? rw.z : rw.x, hi = e ? rw.w : rw.y;
       res[0] = fp8_pair<RES == kResE4M3, false>(lo);
       res[1] = fp8_pair<RES == kResE4M3, true>(lo);
       res[2] = fp8_pair<RES == kResE4M3, false>(hi);
@@ -176,9 +155,9 @@ __device__ __forceinline__ void k_operands(const KRaw<FMT, RES> &r, int tau, con
     if constexpr (FMT == kFmtQ2) {
       // a 2-bit code as a nibble is the e2m1 value c / 2: the conversion with scale 2 gives codes 4 i, 4 i + 2 of
       // byte i, and of the word shifted by one code 4 i + 1, 4 i + 3
-      const uint32_t a = cw[e >> 1] & 0x33333333u, b = (cw[e >> 1] >> 2) & 0x33333333u;
+      const uint32_t a = c0 & 0x33333333u, b = (c0 >> 2) & 0x33333333u;
       f32x2 a0, a1, b0, b1;
-      if (e & 1) {
+      if (e) {
         a0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(a, 2.0f, 2);
         a1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(a, 2.0f, 3);
         b0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(b, 2.0f, 2);
@@ -193,23 +172,50 @@ __device__ __forceinline__ void k_operands(const KRaw<FMT, RES> &r, int tau, con
 #pragma unroll
       for (int i = 0; i < 8; ++i) k[i] = __builtin_fmaf(c[i], s, z) + res[i >> 1][i & 1];
     } else if constexpr (FMT == kFmtNvfp4) {
-      const float se = e < 2 ? s : s1;
-      const f32x2 c[4] = {__builtin_amdgcn_cvt_scalef32_pk_f32_fp4(cw[e], 1.0f, 0),
-                          __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(cw[e], 1.0f, 1),
-                          __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(cw[e], 1.0f, 2),
-                          __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(cw[e], 1.0f, 3)};
+      const uint32_t w = e ? c1 : c0;
+      const f32x2 c[4] = {__builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 0),
+                          __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 1),
+                          __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 2),
+                          __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 3)};
 #pragma unroll
-      for (int i = 0; i < 8; ++i) k[i] = __builtin_fmaf(c[i >> 1][i & 1], se, res[i >> 1][i & 1]);
+      for (int i = 0; i < 8; ++i) k[i] = __builtin_fmaf(c[i >> 1][i & 1], s, res[i >> 1][i & 1]);
     } else {
+      const uint32_t w = e ? c1 : c0;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float2 c = nf4[(cw[e] >> (8 * i)) & 0xffu];
+        const float2 c = nf4[(w >> (8 * i)) & 0xffu];
         k[2 * i] = __builtin_fmaf(c.x, s, res[i][0]);
         k[2 * i + 1] = __builtin_fmaf(c.y, s, res[i][1]);
       }
     }
     const u32x4 w = {pk_f16_bits(k[0], k[1]), pk_f16_bits(k[2], k[3]), pk_f16_bits(k[4], k[5]), pk_f16_bits(k[6], k[7])};
     op[e] = __builtin_bit_cast(f16x8, w);
+  }
+}
+
+// Operands e = 0..3 of tile tau: channels 32 kc + 8 e + (0..7) of token 4 m + tau
+template <int FMT, int RES>
+__device__ __forceinline__ void k_operands(const KRaw<FMT, RES> &r, int tau, const float2 *nf4, f16x8 *op) {
+  float s[2], z = 0.f;
+  if constexpr (FMT == kFmtNvfp4) {
+    const f32x2 w = fp8_pair<true, false>(r.s[tau]);
+    s[0] = w[0];
+    s[1] = w[1];
+  } else {
+    s[0] = s[1] = f16_bits_to_f32(r.s[tau]);
+    if constexpr (FMT == kFmtQ2) z = f16_bits_to_f32(r.z[tau]);
+  }
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    uint32_t c0, c1 = 0;
+    if constexpr (FMT == kFmtQ2) {
+      const uint4 c = r.code[tau >> 1];
+      c0 = h ? (tau & 1 ? c.w : c.y) : (tau & 1 ? c.z : c.x);
+    } else {
+      c0 = h ? r.code[tau].z : r.code[tau].x;
+      c1 = h ? r.code[tau].w : r.code[tau].y;
+    }
+    k_half<FMT, RES>(c0, c1, s[h], z, r.res[RES == kResNone ? 0 : 2 * tau + h], nf4, op + 2 * h);
   }
 }
 
@@ -238,8 +244,10 @@ __device__ __forceinline__ void load_q(const AttendParams &p, size_t row, bool o
   top = xor_max(top, 32);
   int ex = (int)((__float_as_uint(top) >> 23) & 0xffu);  // 0: all zero or tiny; 255: an infinity
   ex = ex == 255 ? 127 : min(max(ex, 1), 253);
-  const float f = __uint_as_float((uint32_t)(254 - ex) << 23);
+  float f = __uint_as_float((uint32_t)(254 - ex) << 23);
   cs = p.scale2 * __uint_as_float((uint32_t)ex << 23);
+  if (cs < 0.f) f = -f;  // a negative scale: into q, so that the largest product is the largest score
+  cs = fmaxf(fabsf(cs), 1e-37f);  // above 0: a hidden key's product of -inf stays -inf
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
     u32x4 w;
@@ -249,13 +257,32 @@ __device__ __forceinline__ void load_q(const AttendParams &p, size_t row, bool o
   }
 }
 
-// whether a half of the 8 fp16 values is an infinity or NaN: bit 15 or 31 of the result
-__device__ __forceinline__ uint32_t not_finite8(f16x8 v) {
-  const u32x4 w = __builtin_bit_cast(u32x4, v);
-  uint32_t r = 0;
+// V words (8 tokens of a column) with infinities and NaN taken out; `bad` becomes non-zero where there were any.
+// A product with them would give 0 * inf to the rows that do not see them; add_not_finite puts them back.
+__device__ __forceinline__ u32x4 finite8(u32x4 w, uint32_t &bad) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) r |= (w[i] & 0x7c007c00u) + 0x04000400u;
-  return r & 0x80008000u;
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t x = ((w[i] & 0x7c007c00u) + 0x04000400u) & 0x80008000u;  // top bit of a half: all exponent bits set
+    bad |= x;
+    w[i] &= ~((x >> 15) * 0xffffu);
+  }
+  return w;
+}
+
+// infinities and NaN of V at tokens that the lane's row sees, into its columns 16 u + 4 g + (0..3): whatever the
+// weight (above zero), they make the result what they are
+template <int VT>
+__device__ __forceinline__ void add_not_finite(const uint8_t *v, int g, int nvis, f32x4 *o) {
+#pragma unroll 1
+  for (int t = 0; t < nvis && t < kPage; ++t)
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t w = ((const uint16_t *)v)[vt_off(16 * u + 4 * g + e, t)];
+        const float x = VT == kVBF16 ? round_to(bf16_bits_to_f32(w), 0) : f16_bits_to_f32(w);
+        if (!(fabsf(x) < INFINITY)) o[u][e] += x;
+      }
 }
 
 // ---------------------------------------------------------------------------
@@ -267,15 +294,16 @@ template <bool MASK>
 __device__ __forceinline__ bool softmax_step(f32x4 *S, float cs, int nvis, int g, float &m, float &l, float &alpha,
                                              f16x8 *P) {
   float x[16];
-  float top = kNoMax;
+  float top = -INFINITY;
 #pragma unroll
   for (int tau = 0; tau < 4; ++tau)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int k = 4 * i + tau;
-      x[k] = S[tau][i] * cs;
+      x[k] = S[tau][i];
       if (!MASK || 16 * g + k < nvis) top = fmaxf(top, x[k]);
     }
+  top *= cs;
   // the largest m may lag by kStale: most pages need no exchange between the row's four lanes and leave O as it is
   const bool moved = __ballot(top > m + kStale) != 0;
   alpha = 1.f;
@@ -290,7 +318,7 @@ __device__ __forceinline__ bool softmax_step(f32x4 *S, float cs, int nvis, int g
   float sum = 0.f;
 #pragma unroll
   for (int k = 0; k < 16; ++k) {
-    x[k] = (!MASK || 16 * g + k < nvis) ? exp2_hw(x[k] - m) : 0.f;
+    x[k] = (!MASK || 16 * g + k < nvis) ? exp2_hw(__builtin_fmaf(x[k], cs, -m)) : 0.f;
     sum += x[k];
   }
   l += sum;
@@ -419,45 +447,25 @@ __global__ __launch_bounds__(256) void paged_attend_kernel(const AttendParams p)
 #pragma unroll
         for (int u = 0; u < 8; ++u) O[t][u] *= alpha;
     }
-    bool apart = false;  // rows that do not see an infinity or NaN of V would get 0 * inf
+    uint32_t bad = 0;
     if (!full) {
       u32x4 keep[2];
       partial_page_masks(g, hi - t0, keep);  // slots that no row sees are not data
-      uint32_t bad = 0;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        V[i] &= keep[i & 1];
-        bad |= not_finite8(VTr::operand(V[i]));
+      for (int i = 0; i < 16; ++i)
+        V[i] = finite8(__builtin_bit_cast(u32x4, VTr::operand(V[i] & keep[i & 1])), bad);
+    }
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
+#pragma unroll
+      for (int kap = 0; kap < 2; ++kap) {
+        const f16x8 a = full ? VTr::operand(V[2 * u + kap]) : __builtin_bit_cast(f16x8, V[2 * u + kap]);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) O[t][u] = mfma16(a, P[t][kap], O[t][u]);
       }
-      apart = lo < min(hi, t0 + kPage) && __ballot(bad != 0) != 0;
-    }
-    if (!apart) {
+    if (__ballot(bad != 0) != 0)
 #pragma unroll
-      for (int u = 0; u < 8; ++u)
-#pragma unroll
-        for (int kap = 0; kap < 2; ++kap) {
-          const f16x8 a = VTr::operand(V[2 * u + kap]);
-#pragma unroll
-          for (int t = 0; t < NT; ++t) O[t][u] = mfma16(a, P[t][kap], O[t][u]);
-        }
-    } else {
-#pragma unroll
-      for (int t = 0; t < NT; ++t)
-        for (int r = 0; r < 16; ++r) {  // row by row, with the tokens that the row sees
-          const int nv = __shfl(lim[t], r) - t0;
-          if (nv <= 0) continue;
-          u32x4 keep[2];
-          partial_page_masks(g, nv, keep);
-#pragma unroll
-          for (int u = 0; u < 8; ++u) {
-            f32x4 a = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int kap = 0; kap < 2; ++kap) a = mfma16(VTr::operand(V[2 * u + kap] & keep[kap]), P[t][kap], a);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) O[t][u][e] += n == r ? a[e] : 0.f;
-          }
-        }
-    }
+      for (int t = 0; t < NT; ++t) add_not_finite<VT>(p.v + blk * (kD * kPage * 2), g, lim[t] - t0, O[t]);
   }
 
   // join the four waves
@@ -498,6 +506,277 @@ __global__ __launch_bounds__(256) void paged_attend_kernel(const AttendParams p)
       store_row8(p, row, p.slot0 + split, c0, o, mm, ll, row_limit(p, b, i) > 0);
     }
     __syncthreads();
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Many rows: 16 NT rows to each of the W waves.  The workgroup dequantizes a page once, as operands in LDS (K: wave w
+// takes 8 / W of the eight (tile, half of the channels) units; V comes as it lies in the pool), and every wave reads
+// them for its rows.  Two pages are in flight: while a wave exponentiates page j and multiplies it with V, it computes
+// the scores of page j + 1, dequantizes its share of page j + 2 and has page j + 3's bytes under way, so that matrix
+// and vector instructions have independent work at any time, with one barrier a page.
+// ---------------------------------------------------------------------------
+template <int FMT>
+struct KUnit {  // one unit's bytes of lane (kc, m): token 4 m + tau, channels 32 kc + 16 h + (0..15)
+  uint32_t c0, c1;
+  uint16_t s, z;
+  uint4 res;
+};
+template <int FMT, int RES>
+__device__ __forceinline__ void load_unit(const AttendParams &p, size_t blk, int unit, int lane, KUnit<FMT> &r) {
+  const int kc = lane >> 4, m = lane & 15, tau = unit >> 1, h = unit & 1;
+  if constexpr (FMT == kFmtQ2) {
+    r.c0 = *(const uint32_t *)(p.k + blk * 2048 + (((tau >> 1) * 64 + lane) * 2 + (tau & 1)) * 8 + 4 * h);
+    const int at = (((tau >> 1) * 4 + kc) * 4 + (m >> 2)) * 8 + 4 * (tau & 1) + (m & 3);
+    r.s = ((const uint16_t *)(p.ks + blk * 512))[at];
+    r.z = ((const uint16_t *)(p.kz + blk * 512))[at];
+  } else {
+    const uint2 c = *(const uint2 *)(p.k + blk * 4096 + (tau * 64 + lane) * 16 + 8 * h);
+    r.c0 = c.x;
+    r.c1 = c.y;
+    if constexpr (FMT == kFmtNvfp4) r.s = (p.ks + blk * 512)[(4 * m + tau) * 8 + 2 * kc + h];
+    else r.s = ((const uint16_t *)(p.ks + blk * 256))[(4 * m + tau) * 2 + (kc >> 1)];
+  }
+  if constexpr (RES != kResNone) r.res = ((const uint4 *)(p.kr + blk * 8192))[64 * unit + lane];
+}
+template <int FMT, int RES>
+__device__ __forceinline__ void unit_to_lds(const KUnit<FMT> &r, int unit, int lane, const float2 *nf4, u32x4 *dst) {
+  const float s = FMT == kFmtNvfp4 ? fp8_pair<true, false>(r.s)[0] : f16_bits_to_f32(r.s);
+  const float z = FMT == kFmtQ2 ? f16_bits_to_f32(r.z) : 0.f;
+  f16x8 op[2];
+  k_half<FMT, RES>(r.c0, r.c1, s, z, r.res, nf4, op);
+  dst[(2 * unit) * 64 + lane] = __builtin_bit_cast(u32x4, op[0]);
+  dst[(2 * unit + 1) * 64 + lane] = __builtin_bit_cast(u32x4, op[1]);
+}
+
+template <int FMT, int RES, int VT, int NT, int W>
+__global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2))) void paged_attend_wide_kernel(
+    const AttendParams p) {
+  constexpr int kUnits = 8 / W, kVPieces = 16 / W;  // of a page, per wave
+  const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int g = lane >> 4, n = lane & 15;
+  const int nb = gridDim.x / p.HKV;  // the last rows, which see the most keys of a causal chunk, first
+  const int hkv = blockIdx.x % p.HKV, rb = nb - 1 - blockIdx.x / p.HKV, split = blockIdx.y;
+  const AttendSet set = attend_set(p, blockIdx.z);
+  const int LG = p.L * p.G, R = set.n * LG, r0 = (rb * W + wv) * 16 * NT;
+  if (rb * W * 16 * NT >= R) return;
+  const int pa = set.p0 + split * p.ppw;
+  int pe = min(pa + p.ppw, set.p1);
+  if (pa >= pe && p.nslots != 0) return;
+
+  __shared__ u32x4 s_k[2][16 * 64], s_v[2][16 * 64];
+  __shared__ float2 s_nf4[FMT == kFmtNf4 ? 256 : 1];
+  __shared__ int s_hi[W], s_lo[W], s_bad;
+
+  f16x8 Q[NT][4];
+  float cs[NT], m[NT];
+  int lim[NT], lo = 0x7fffffff, hi = 0;
+  f32x4 O[NT][8], Ls[NT];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    const int r = r0 + 16 * t + n;
+    const bool ok = r < R;
+    const int bi = ok ? r / LG : 0, j = ok ? r - bi * LG : 0, i = j / p.G;
+    const size_t row = ((size_t)(set.b0 + bi) * p.L + i) * p.HQ + hkv * p.G + (j - i * p.G);
+    load_q(p, row, ok, g, Q[t], cs[t]);
+    lim[t] = ok ? row_limit(p, set.b0 + bi, i) : 0x7fffffff;
+    lo = min(lo, lim[t]);
+    hi = max(hi, ok ? lim[t] : 0);
+    m[t] = kNoMax;
+    Ls[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int u = 0; u < 8; ++u) O[t][u] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+#pragma unroll
+  for (int s = 1; s < 16; s <<= 1) {
+    lo = min(lo, __shfl_xor(lo, s));
+    hi = max(hi, __shfl_xor(hi, s));
+  }
+  if (lane == 0) {
+    s_lo[wv] = lo;
+    s_hi[wv] = hi;
+  }
+  if constexpr (FMT == kFmtNf4)
+    if (threadIdx.x < 256) s_nf4[threadIdx.x] = make_float2(kAttendNF4[threadIdx.x & 15], kAttendNF4[threadIdx.x >> 4]);
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < W; ++w) {
+    lo = min(lo, s_lo[w]);
+    hi = max(hi, s_hi[w]);
+  }
+  lo = __builtin_amdgcn_readfirstlane(lo);  // every row of the workgroup sees the keys below lo, none those from hi on
+  hi = __builtin_amdgcn_readfirstlane(hi);
+  pe = min(pe, (hi + kPage - 1) / kPage);
+
+  const int32_t *bt = p.bt + (size_t)set.b0 * p.bt_stride;
+  auto block_of = [&](int pg) {  // pages past the range repeat its last one: loaded, never used
+    int id = bt[min(pg, pe - 1)];
+    id = __builtin_amdgcn_readfirstlane((unsigned)id < (unsigned)p.num_pages ? id : 0);
+    return (size_t)id * p.HKV + hkv;
+  };
+  KUnit<FMT> raw[kUnits];
+  auto load_raw = [&](size_t blk) {
+#pragma unroll
+    for (int i = 0; i < kUnits; ++i) load_unit<FMT, RES>(p, blk, wv * kUnits + i, lane, raw[i]);
+  };
+  auto raw_to_lds = [&](int buf) {
+#pragma unroll
+    for (int i = 0; i < kUnits; ++i) unit_to_lds<FMT, RES>(raw[i], wv * kUnits + i, lane, s_nf4, s_k[buf]);
+  };
+  // V: straight into LDS, or through registers where bf16 becomes the fp16 operand
+  auto load_v = [&](size_t blk, int buf) {
+    const u32x4 *src = (const u32x4 *)(p.v + blk * (kD * kPage * 2));
+#pragma unroll
+    for (int i = 0; i < kVPieces; ++i) {
+      const int at = (wv * kVPieces + i) * 64;
+      if constexpr (VT == kVF16)
+        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)(src + at + lane),
+                                         (__attribute__((address_space(3))) void *)(&s_v[buf][at]), 16, 0, 0);
+      else
+        s_v[buf][at + lane] = __builtin_bit_cast(u32x4, VTraits<VT>::operand(src[at + lane]));
+    }
+  };
+  f32x4 S[NT][4];
+  auto scores = [&](int buf, f32x4 (*X)[4]) {
+#pragma unroll
+    for (int tau = 0; tau < 4; ++tau) {
+      f16x8 K[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) K[e] = __builtin_bit_cast(f16x8, s_k[buf][(4 * tau + e) * 64 + lane]);
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        f32x4 a = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) a = mfma16(K[e], Q[t][e], a);
+        X[t][tau] = a;
+      }
+    }
+  };
+  const f16x8 one = {1, 1, 1, 1, 1, 1, 1, 1};
+  auto weights = [&](int t, f16x8 *P) {  // of S[t], against m[t]; their sum by a product with ones
+    float x[16];
+#pragma unroll
+    for (int tau = 0; tau < 4; ++tau)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[4 * i + tau] = exp2_hw(__builtin_fmaf(S[t][tau][i], cs[t], -m[t]));
+#pragma unroll
+    for (int kap = 0; kap < 2; ++kap) {
+      u32x4 w;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = pk_f16_bits(x[8 * kap + 2 * i], x[8 * kap + 2 * i + 1]);
+      P[kap] = __builtin_bit_cast(f16x8, w);
+      Ls[t] = mfma16(one, P[kap], Ls[t]);
+    }
+  };
+
+  auto page_barrier = [&]() {  // loads into LDS are counted with the others, and no barrier waits for those
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+  };
+  if (pa < pe) {
+    size_t b0 = block_of(pa), b1 = block_of(pa + 1), b2 = block_of(pa + 2);
+    load_v(b0, 0);
+    load_raw(b0);
+    raw_to_lds(0);
+    load_raw(b1);
+    raw_to_lds(1);
+    load_raw(b2);
+    page_barrier();
+    scores(0, S);
+    __syncthreads();
+    for (int pg = pa, cur = 0; pg < pe; ++pg, cur ^= 1) {
+      const size_t b3 = block_of(pg + 3);
+      load_v(b1, cur ^ 1);
+      raw_to_lds(cur);
+      load_raw(b3);
+      const int t0 = pg * kPage;
+      const bool full = lo >= t0 + kPage;
+      if (!full) {  // the last pages of a sequence or chunk
+        if (threadIdx.x == 0) s_bad = 0;
+        u32x4 keep[2];
+        uint32_t bad = 0;
+        partial_page_masks(g, hi - t0, keep);  // slots that no row sees are not data
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kVPieces; ++i) {
+          const int at = (wv * kVPieces + i) * 64 + lane;
+          s_v[cur][at] = finite8(s_v[cur][at] & keep[(wv * kVPieces + i) & 1], bad);
+        }
+        if (bad) s_bad = 1;
+        __syncthreads();
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int tau = 0; tau < 4; ++tau)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (t0 + 16 * g + 4 * i + tau >= lim[t]) S[t][tau][i] = -INFINITY;
+      }
+      float top[NT];
+      bool lag = false;
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        float x = S[t][0][0];
+#pragma unroll
+        for (int k = 1; k < 16; ++k) x = fmaxf(x, S[t][k >> 2][k & 3]);
+        top[t] = x * cs[t];
+        lag |= top[t] > m[t] + kStale;
+      }
+      if (__ballot(lag) != 0) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          const float mn = fmaxf(m[t], xor_max(xor_max(top[t], 16), 32));
+          const float alpha = exp2_hw(m[t] - mn);
+          m[t] = mn;
+          Ls[t] *= alpha;
+#pragma unroll
+          for (int u = 0; u < 8; ++u) O[t][u] *= alpha;
+        }
+      }
+      f16x8 P[NT][2];
+#pragma unroll
+      for (int t = 0; t < NT; ++t) weights(t, P[t]);
+      scores(cur ^ 1, S);
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+#pragma unroll
+        for (int kap = 0; kap < 2; ++kap) {
+          const f16x8 a = __builtin_bit_cast(f16x8, s_v[cur][(2 * u + kap) * 64 + lane]);
+#pragma unroll
+          for (int t = 0; t < NT; ++t) O[t][u] = mfma16(a, P[t][kap], O[t][u]);
+        }
+      if (!full && s_bad)
+#pragma unroll
+        for (int t = 0; t < NT; ++t) add_not_finite<VT>(p.v + b0 * (kD * kPage * 2), g, lim[t] - t0, O[t]);
+      b0 = b1;
+      b1 = b2;
+      b2 = b3;
+      page_barrier();
+    }
+  }
+
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    const int r = r0 + 16 * t + n;
+    if (r >= R) continue;
+    const int bi = r / LG, j = r - bi * LG, i = j / p.G;
+    const size_t row = ((size_t)(set.b0 + bi) * p.L + i) * p.HQ + hkv * p.G + (j - i * p.G);
+    const float l = Ls[t][0];
+    if (p.nslots == 0) {
+      const float inv = lim[t] > 0 ? 1.f / l : 0.f;
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const f32x4 y = lim[t] > 0 ? O[t][u] * inv : f32x4{0.f, 0.f, 0.f, 0.f};
+        const uint2 w = p.out_bf16 ? make_uint2(pk_bf16_bits(y[0], y[1]), pk_bf16_bits(y[2], y[3]))
+                                   : make_uint2(pk_f16_bits(y[0], y[1]), pk_f16_bits(y[2], y[3]));
+        *(uint2 *)((uint16_t *)p.out + row * kD + 16 * u + 4 * g) = w;
+      }
+    } else {
+      const size_t at = row * p.nslots + p.slot0 + split;
+#pragma unroll
+      for (int u = 0; u < 8; ++u) *(f32x4 *)(p.part_o + at * kD + 16 * u + 4 * g) = O[t][u];
+      if (g == 0) *(float2 *)(p.part_ml + 2 * at) = make_float2(m[t], l);
+    }
   }
 }
 
@@ -555,19 +834,25 @@ __global__ __launch_bounds__(256) void paged_attend_join_kernel(const AttendPara
 // Launch plan of a call: page ranges of the shared and of the own pages
 struct AttendPlan {
   int shared_slots, shared_ppw, own_slots, own_ppw, nslots;
-  int shared_nt, shared_blocks, own_nt, own_blocks;
+  int shared_kind, shared_blocks, own_kind, own_blocks;
   int own_pages;
 };
 
-static int tiles_for(long rows) { return rows <= 16 ? 1 : (rows <= 32 ? 2 : 4); }
+// the kernel for so many rows of a KV head and set, and the rows of its workgroup
+enum { kRows16 = 0, kRows32, kRows64, kRows128, kRows256 };
+static int kind_for(long rows) {
+  return rows <= 16 ? kRows16 : (rows <= 32 ? kRows32 : (rows <= 64 ? kRows64 : (rows <= 128 ? kRows128 : kRows256)));
+}
+static long kind_rows(int kind) { return 16l << kind; }
 
 static AttendPlan attend_plan(const ffa_paged_attend_args *a, int cus) {
   AttendPlan pl = {};
   const int G = a->HQ / a->HKV;
-  const long want = 4l * (cus > 0 ? cus : 256);  // workgroups that fill the chip
+  if (cus <= 0) cus = 256;
   const long LG = (long)a->L * G;
-  auto ranges = [&](long units, int pages, int &ppw, int &slots) {
+  auto ranges = [&](long units, int pages, int kind, int &ppw, int &slots) {
     // units: pages over all sets, heads and row blocks; a workgroup of at least 4 pages, one per wave
+    const long want = (kind == kRows256 ? 1l : (kind == kRows128 ? 2l : 4l)) * cus;  // workgroups that fill the chip
     long w = (units + want - 1) / want;
     w = (w + 3) / 4 * 4;
     ppw = (int)(w < 4 ? 4 : (w > pages ? (pages < 4 ? 4 : pages) : w));
@@ -586,21 +871,23 @@ static AttendPlan attend_plan(const ffa_paged_attend_args *a, int cus) {
       if (gp < min_shared) min_shared = gp;
     }
     if (pages > 0) {
-      pl.shared_nt = tiles_for(rows);
-      pl.shared_blocks = (int)((rows + 16 * pl.shared_nt - 1) / (16 * pl.shared_nt));
+      pl.shared_kind = kind_for(rows);
+      const long kr = kind_rows(pl.shared_kind);
+      pl.shared_blocks = (int)((rows + kr - 1) / kr);
       for (int g = 0; g < a->ngroups; ++g) {
         const long n = a->group_start_host[g + 1] - a->group_start_host[g];
-        units += (long)a->group_pages_host[g] * a->HKV * ((n * LG + 16 * pl.shared_nt - 1) / (16 * pl.shared_nt));
+        units += (long)a->group_pages_host[g] * a->HKV * ((n * LG + kr - 1) / kr);
       }
-      ranges(units, pages, pl.shared_ppw, pl.shared_slots);
+      ranges(units, pages, pl.shared_kind, pl.shared_ppw, pl.shared_slots);
     }
   }
   pl.own_pages = (a->T + kPage - 1) / kPage - min_shared;
   if (pl.own_pages < 0) pl.own_pages = 0;
-  pl.own_nt = tiles_for(LG);
-  pl.own_blocks = (int)((LG + 16 * pl.own_nt - 1) / (16 * pl.own_nt));
+  pl.own_kind = kind_for(LG);
+  pl.own_blocks = (int)((LG + kind_rows(pl.own_kind) - 1) / kind_rows(pl.own_kind));
   pl.own_ppw = 4;
-  if (pl.own_pages > 0) ranges((long)pl.own_pages * a->HKV * pl.own_blocks * a->B, pl.own_pages, pl.own_ppw, pl.own_slots);
+  if (pl.own_pages > 0) 
+    ranges((long)pl.own_pages * a->HKV * pl.own_blocks * a->B, pl.own_pages, pl.own_kind, pl.own_ppw, pl.own_slots);
   pl.nslots = pl.shared_slots + pl.own_slots;
   if (pl.shared_slots == 0 && pl.own_slots <= 1) {  // one range: no partials
     pl.own_slots = 1;
@@ -610,18 +897,25 @@ static AttendPlan attend_plan(const ffa_paged_attend_args *a, int cus) {
 }
 
 template <int FMT, int RES, int VT>
-static void launch_attend(const AttendParams &p, int nt, dim3 grid, hipStream_t st) {
-  if (nt == 1) hipLaunchKernelGGL((paged_attend_kernel<FMT, RES, VT, 1>), grid, dim3(256), 0, st, p);
-  else if (nt == 2) hipLaunchKernelGGL((paged_attend_kernel<FMT, RES, VT, 2>), grid, dim3(256), 0, st, p);
-  else hipLaunchKernelGGL((paged_attend_kernel<FMT, RES, VT, 4>), grid, dim3(256), 0, st, p);
+static void launch_attend(const AttendParams &p, int kind, int slots, int blocks, int sets, hipStream_t st) {
+  const dim3 few((unsigned)slots, (unsigned)(p.HKV * blocks), (unsigned)sets);
+  const dim3 wide((unsigned)(p.HKV * blocks), (unsigned)slots, (unsigned)sets);
+  switch (kind) {
+    case kRows16: hipLaunchKernelGGL((paged_attend_kernel<FMT, RES, VT, 1>), few, dim3(256), 0, st, p); break;
+    case kRows32: hipLaunchKernelGGL((paged_attend_kernel<FMT, RES, VT, 2>), few, dim3(256), 0, st, p); break;
+    case kRows64: hipLaunchKernelGGL((paged_attend_kernel<FMT, RES, VT, 4>), few, dim3(256), 0, st, p); break;
+    case kRows128: hipLaunchKernelGGL((paged_attend_wide_kernel<FMT, RES, VT, 2, 4>), wide, dim3(256), 0, st, p); break;
+    default: hipLaunchKernelGGL((paged_attend_wide_kernel<FMT, RES, VT, 2, 8>), wide, dim3(512), 0, st, p);
+  }
 }
 
 template <int FMT>
-static void launch_attend_fmt(const AttendParams &p, int res, int vdt, int nt, dim3 grid, hipStream_t st) {
+static void launch_attend_fmt(const AttendParams &p, int res, int vdt, int kind, int slots, int blocks, int sets,
+                              hipStream_t st) {
 #define FFA_CASE(RR, RC)                                                                \
   if (res == RC) {                                                                      \
-    if (vdt == FFA_DT_BF16) launch_attend<FMT, RR, kVBF16>(p, nt, grid, st);            \
-    else launch_attend<FMT, RR, kVF16>(p, nt, grid, st);                                \
+    if (vdt == FFA_DT_BF16) launch_attend<FMT, RR, kVBF16>(p, kind, slots, blocks, sets, st);            \
+    else launch_attend<FMT, RR, kVF16>(p, kind, slots, blocks, sets, st);                                \
   }
   FFA_CASE(kResE4M3, FFA_DT_FP8_E4M3)
   FFA_CASE(kResE5M2, FFA_DT_FP8_E5M2)
@@ -715,22 +1009,22 @@ extern "C" int ffa_paged_attend(const ffa_paged_attend_args *a, void *stream) {
   p.own_slots = pl.own_slots;
   p.own_ppw = pl.own_ppw;
   const hipStream_t st = (hipStream_t)stream;
-  auto launch = [&](int nt, dim3 grid) {
-    if (a->format == FFA_PAGES_Q2) launch_attend_fmt<kFmtQ2>(p, a->res_dtype, a->v_dtype, nt, grid, st);
-    else if (a->format == FFA_PAGES_NVFP4) launch_attend_fmt<kFmtNvfp4>(p, a->res_dtype, a->v_dtype, nt, grid, st);
-    else launch_attend_fmt<kFmtNf4>(p, a->res_dtype, a->v_dtype, nt, grid, st);
+  auto launch = [&](int kind, int slots, int blocks, int sets) {
+    if (a->format == FFA_PAGES_Q2) launch_attend_fmt<kFmtQ2>(p, a->res_dtype, a->v_dtype, kind, slots, blocks, sets, st);
+    else if (a->format == FFA_PAGES_NVFP4) launch_attend_fmt<kFmtNvfp4>(p, a->res_dtype, a->v_dtype, kind, slots, blocks, sets, st);
+    else launch_attend_fmt<kFmtNf4>(p, a->res_dtype, a->v_dtype, kind, slots, blocks, sets, st);
   };
   if (pl.shared_slots > 0) {
     p.shared = 1;
     p.slot0 = 0;
     p.ppw = pl.shared_ppw;
-    launch(pl.shared_nt, dim3((unsigned)pl.shared_slots, (unsigned)(a->HKV * pl.shared_blocks), (unsigned)a->ngroups));
+    launch(pl.shared_kind, pl.shared_slots, pl.shared_blocks, a->ngroups);
   }
   if (pl.own_slots > 0) {
     p.shared = 0;
     p.slot0 = pl.shared_slots;
     p.ppw = pl.own_ppw;
-    launch(pl.own_nt, dim3((unsigned)pl.own_slots, (unsigned)(a->HKV * pl.own_blocks), (unsigned)a->B));
+    launch(pl.own_kind, pl.own_slots, pl.own_blocks, a->B);
   }
   if (pl.nslots > 0)
     hipLaunchKernelGGL(paged_attend_join_kernel, dim3((unsigned)rows), dim3(256), 0, st, p);
