@@ -39,9 +39,10 @@ struct AttendParams {
   int B, T, L, HQ, HKV, G;
   int q_bf16, out_bf16;
   float scale2;
-  int nslots;  // 0: one page range per row, written to out
-  int slot0, ppw, shared;
-  int shared_slots, shared_ppw, own_slots, own_ppw;  // for the join
+  int nslots;  // partials per row, 0: one page range per row, written to out
+  // sets of a launch: z < nshared are groups over their shared pages, then (from b = 0) sequences over their own
+  int nshared;
+  int shared_slots, shared_ppw, own_slots, own_ppw;
 };
 
 // QLoRA NF4 levels (the published 16 normal-float values)
@@ -68,29 +69,43 @@ __device__ __forceinline__ int row_limit(const AttendParams &p, int b, int i) {
 }
 
 // The rows and pages of a workgroup: sequences b0 .. b0 + n - 1 (a group's, over the shared pages; or one, over its
-// own), pages [p0, p1) of the block-table row of b0.
+// own), pages [p0, p1) of the block-table row of b0; the slot of the partials.
 struct AttendSet {
-  int b0, n, p0, p1;
+  int b0, n, p0, p1, slot;
 };
-__device__ __forceinline__ AttendSet attend_set(const AttendParams &p, int z) {
+// the range `split` of set z, and the slot of its partials
+__device__ __forceinline__ AttendSet attend_set(const AttendParams &p, int z, int split) {
   AttendSet s;
-  if (p.shared) {
+  int ppw;
+  if (z < p.nshared) {
     s.b0 = min(max(p.group_start[z], 0), p.B);
     s.n = max(min(p.group_start[z + 1], p.B) - s.b0, 0);
     s.p0 = 0;
     s.p1 = min(max(p.group_pages[z], 0), p.bt_stride);
+    ppw = p.shared_ppw;
+    s.slot = split;
   } else {
-    s.b0 = z;
+    s.b0 = z - p.nshared;
     s.n = 1;
-    s.p0 = shared_pages_of(p, z);
-    s.p1 = (seq_len_of(p, z) + kPage - 1) / kPage;
+    s.p0 = shared_pages_of(p, s.b0);
+    s.p1 = (seq_len_of(p, s.b0) + kPage - 1) / kPage;
+    ppw = p.own_ppw;
+    s.slot = p.shared_slots + split;
   }
+  s.p0 += split * ppw;
+  s.p1 = min(s.p0 + ppw, s.p1);
   return s;
 }
 
 // ---------------------------------------------------------------------------
 // K of one (page, KV head): what lane (kc, m) loads, and its operands
 // ---------------------------------------------------------------------------
+// 16 bytes of a page that one workgroup reads once (non-temporal: 16 x 8K-64K tokens 394 -> 354 us)
+__device__ __forceinline__ uint4 load_once(const uint4 *p) {
+  const u32x4 w = __builtin_nontemporal_load((const u32x4 *)p);
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
 template <int FMT, int RES>
 struct KRaw {
   uint4 code[FMT == kFmtQ2 ? 2 : 4];
@@ -124,7 +139,7 @@ __device__ __forceinline__ void load_k(const AttendParams &p, size_t blk, int la
   if constexpr (RES != kResNone) {
     const uint4 *c = (const uint4 *)(p.kr + blk * 8192);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) r.res[i] = c[64 * i + lane];
+    for (int i = 0; i < 8; ++i) r.res[i] = load_once(c + 64 * i + lane);
   }
 }
 
@@ -362,15 +377,15 @@ __device__ __forceinline__ void store_row8(const AttendParams &p, size_t row, in
 // rows, its operands straight from memory; the waves' results are joined in LDS.
 // ---------------------------------------------------------------------------
 template <int FMT, int RES, int VT, int NT>
-__global__ __launch_bounds__(256) void paged_attend_kernel(const AttendParams p) {
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NT <= 2 ? 2 : 1))) void paged_attend_kernel(const AttendParams p) {
   typedef VTraits<VT> VTr;
   const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, n = lane & 15;
   const int split = blockIdx.x, hkv = blockIdx.y % p.HKV, rb = blockIdx.y / p.HKV;
-  const AttendSet set = attend_set(p, blockIdx.z);
+  const AttendSet set = attend_set(p, blockIdx.z, split);
   const int LG = p.L * p.G, R = set.n * LG, r0 = rb * 16 * NT;
   if (r0 >= R) return;
-  const int pa = set.p0 + split * p.ppw, pe = min(pa + p.ppw, set.p1);
+  const int pa = set.p0, pe = set.p1;
   if (pa >= pe && p.nslots != 0) return;
 
   __shared__ float s_m[4][16 * NT], s_l[4][16 * NT];
@@ -421,7 +436,7 @@ __global__ __launch_bounds__(256) void paged_attend_kernel(const AttendParams p)
     u32x4 V[16];
     const u32x4 *vp = (const u32x4 *)(p.v + blk * (kD * kPage * 2));
 #pragma unroll
-    for (int i = 0; i < 16; ++i) V[i] = vp[64 * i + lane];
+    for (int i = 0; i < 16; ++i) V[i] = __builtin_nontemporal_load(vp + 64 * i + lane);
 
     f32x4 S[NT][4];
 #pragma unroll
@@ -503,7 +518,7 @@ __global__ __launch_bounds__(256) void paged_attend_kernel(const AttendParams p)
       }
       const int bi = r / LG, j = r - bi * LG, i = j / p.G, b = set.b0 + bi;
       const size_t row = ((size_t)b * p.L + i) * p.HQ + hkv * p.G + (j - i * p.G);
-      store_row8(p, row, p.slot0 + split, c0, o, mm, ll, row_limit(p, b, i) > 0);
+      store_row8(p, row, set.slot, c0, o, mm, ll, row_limit(p, b, i) > 0);
     }
     __syncthreads();
   }
@@ -557,16 +572,61 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2))) voi
   const int g = lane >> 4, n = lane & 15;
   const int nb = gridDim.x / p.HKV;  // the last rows, which see the most keys of a causal chunk, first
   const int hkv = blockIdx.x % p.HKV, rb = nb - 1 - blockIdx.x / p.HKV, split = blockIdx.y;
-  const AttendSet set = attend_set(p, blockIdx.z);
+  const AttendSet set = attend_set(p, blockIdx.z, split);
   const int LG = p.L * p.G, R = set.n * LG, r0 = (rb * W + wv) * 16 * NT;
   if (rb * W * 16 * NT >= R) return;
-  const int pa = set.p0 + split * p.ppw;
-  int pe = min(pa + p.ppw, set.p1);
+  const int pa = set.p0;
+  int pe = set.p1;
   if (pa >= pe && p.nslots != 0) return;
 
   __shared__ u32x4 s_k[2][16 * 64], s_v[2][16 * 64];
   __shared__ float2 s_nf4[FMT == kFmtNf4 ? 256 : 1];
   __shared__ int s_hi[W], s_lo[W], s_bad;
+
+  const int last = max(set.p1 - 1, pa);  // in the table also where the range is empty
+  const int32_t *bt = p.bt + (size_t)set.b0 * p.bt_stride;
+  auto block_of = [&](int pg) {  // pages past the range repeat its last one: loaded, never used
+    int id = bt[min(pg, last)];
+    id = __builtin_amdgcn_readfirstlane((unsigned)id < (unsigned)p.num_pages ? id : 0);
+    return (size_t)id * p.HKV + hkv;
+  };
+  KUnit<FMT> raw[kUnits];
+  auto load_raw = [&](size_t blk, KUnit<FMT> *r) {
+#pragma unroll
+    for (int i = 0; i < kUnits; ++i) load_unit<FMT, RES>(p, blk, wv * kUnits + i, lane, r[i]);
+  };
+  auto raw_to_lds = [&](int buf, const KUnit<FMT> *r) {
+#pragma unroll
+    for (int i = 0; i < kUnits; ++i) unit_to_lds<FMT, RES>(r[i], wv * kUnits + i, lane, s_nf4, s_k[buf]);
+  };
+  // V: straight into LDS; a bf16 pool's, which becomes the fp16 operand, through registers a page earlier
+  u32x4 vraw[VT == kVF16 ? 1 : kVPieces];
+  auto fetch_v = [&](size_t blk) {
+    if constexpr (VT != kVF16) {
+      const u32x4 *src = (const u32x4 *)(p.v + blk * (kD * kPage * 2));
+#pragma unroll
+      for (int i = 0; i < kVPieces; ++i) vraw[i] = src[(wv * kVPieces + i) * 64 + lane];
+    }
+  };
+  auto store_v = [&](size_t blk, int buf) {
+    const u32x4 *src = (const u32x4 *)(p.v + blk * (kD * kPage * 2));
+#pragma unroll
+    for (int i = 0; i < kVPieces; ++i) {
+      const int at = (wv * kVPieces + i) * 64;
+      if constexpr (VT == kVF16)
+        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)(src + at + lane),
+                                         (__attribute__((address_space(3))) void *)(&s_v[buf][at]), 16, 0, 0);
+      else
+        s_v[buf][at + lane] = __builtin_bit_cast(u32x4, VTraits<VT>::operand(vraw[i]));
+    }
+  };
+  // the first pages' bytes are under way while q and the rows' limits are read
+  size_t b0 = block_of(pa), b1 = block_of(pa + 1), b2 = block_of(pa + 2);
+  KUnit<FMT> raw0[kUnits];
+  load_raw(b0, raw0);
+  load_raw(b1, raw);
+  fetch_v(b0);
+  if constexpr (VT == kVF16) store_v(b0, 0);
 
   f16x8 Q[NT][4];
   float cs[NT], m[NT];
@@ -608,34 +668,6 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2))) voi
   hi = __builtin_amdgcn_readfirstlane(hi);
   pe = min(pe, (hi + kPage - 1) / kPage);
 
-  const int32_t *bt = p.bt + (size_t)set.b0 * p.bt_stride;
-  auto block_of = [&](int pg) {  // pages past the range repeat its last one: loaded, never used
-    int id = bt[min(pg, pe - 1)];
-    id = __builtin_amdgcn_readfirstlane((unsigned)id < (unsigned)p.num_pages ? id : 0);
-    return (size_t)id * p.HKV + hkv;
-  };
-  KUnit<FMT> raw[kUnits];
-  auto load_raw = [&](size_t blk) {
-#pragma unroll
-    for (int i = 0; i < kUnits; ++i) load_unit<FMT, RES>(p, blk, wv * kUnits + i, lane, raw[i]);
-  };
-  auto raw_to_lds = [&](int buf) {
-#pragma unroll
-    for (int i = 0; i < kUnits; ++i) unit_to_lds<FMT, RES>(raw[i], wv * kUnits + i, lane, s_nf4, s_k[buf]);
-  };
-  // V: straight into LDS, or through registers where bf16 becomes the fp16 operand
-  auto load_v = [&](size_t blk, int buf) {
-    const u32x4 *src = (const u32x4 *)(p.v + blk * (kD * kPage * 2));
-#pragma unroll
-    for (int i = 0; i < kVPieces; ++i) {
-      const int at = (wv * kVPieces + i) * 64;
-      if constexpr (VT == kVF16)
-        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)(src + at + lane),
-                                         (__attribute__((address_space(3))) void *)(&s_v[buf][at]), 16, 0, 0);
-      else
-        s_v[buf][at + lane] = __builtin_bit_cast(u32x4, VTraits<VT>::operand(src[at + lane]));
-    }
-  };
   f32x4 S[NT][4];
   auto scores = [&](int buf, f32x4 (*X)[4]) {
 #pragma unroll
@@ -674,21 +706,20 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2))) voi
     __syncthreads();
   };
   if (pa < pe) {
-    size_t b0 = block_of(pa), b1 = block_of(pa + 1), b2 = block_of(pa + 2);
-    load_v(b0, 0);
-    load_raw(b0);
-    raw_to_lds(0);
-    load_raw(b1);
-    raw_to_lds(1);
-    load_raw(b2);
+    if constexpr (VT != kVF16) store_v(b0, 0);
+    fetch_v(b1);
+    raw_to_lds(0, raw0);
+    raw_to_lds(1, raw);
+    load_raw(b2, raw);
     page_barrier();
     scores(0, S);
     __syncthreads();
     for (int pg = pa, cur = 0; pg < pe; ++pg, cur ^= 1) {
       const size_t b3 = block_of(pg + 3);
-      load_v(b1, cur ^ 1);
-      raw_to_lds(cur);
-      load_raw(b3);
+      store_v(b1, cur ^ 1);
+      fetch_v(b2);
+      raw_to_lds(cur, raw);
+      load_raw(b3, raw);
       const int t0 = pg * kPage;
       const bool full = lo >= t0 + kPage;
       if (!full) {  // the last pages of a sequence or chunk
@@ -772,7 +803,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2))) voi
         *(uint2 *)((uint16_t *)p.out + row * kD + 16 * u + 4 * g) = w;
       }
     } else {
-      const size_t at = row * p.nslots + p.slot0 + split;
+      const size_t at = row * p.nslots + set.slot;
 #pragma unroll
       for (int u = 0; u < 8; ++u) *(f32x4 *)(p.part_o + at * kD + 16 * u + 4 * g) = O[t][u];
       if (g == 0) *(float2 *)(p.part_ml + 2 * at) = make_float2(m[t], l);
@@ -784,10 +815,9 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2))) voi
 // Join of the partials: one workgroup per row; wave w adds the slots w, w + 4, ...
 // ---------------------------------------------------------------------------
 __global__ __launch_bounds__(256) void paged_attend_join_kernel(const AttendParams p) {
-  const int h = blockIdx.x % p.HQ, i = (blockIdx.x / p.HQ) % p.L, b = blockIdx.x / (p.HQ * p.L);
+  const int i = (blockIdx.x / p.HQ) % p.L, b = blockIdx.x / (p.HQ * p.L);
   const size_t row = blockIdx.x;
   const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
-  (void)h;
   __shared__ float s_m[4], s_l[4];
   __shared__ float s_o[4][kD];
   const bool sees = row_limit(p, b, i) > 0;
@@ -798,15 +828,32 @@ __global__ __launch_bounds__(256) void paged_attend_join_kernel(const AttendPara
   const float *po = p.part_o + row * p.nslots * kD;
   float m = kNoMax, l = 0.f;
   float2 o = make_float2(0.f, 0.f);
-  for (int s = wv; s < na + nb && sees; s += 4) {
-    const int slot = s < na ? s : p.shared_slots + s - na;
-    const float2 x = ml[slot];
-    const float2 y = *(const float2 *)(po + (size_t)slot * kD + 2 * lane);
-    const float mn = fmaxf(m, x.x), fo = exp2_hw(m - mn), fn = exp2_hw(x.x - mn);
+  const int slots = sees ? na + nb : 0;
+  for (int s0 = wv; s0 < slots; s0 += 16) {  // four slots' loads at a time
+    float2 x[4], y[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int s = min(s0 + 4 * i, slots - 1), slot = s < na ? s : p.shared_slots + s - na;
+      x[i] = ml[slot];
+      y[i] = *(const float2 *)(po + (size_t)slot * kD + 2 * lane);
+    }
+    float mn = m;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) mn = fmaxf(mn, x[i].x);
+    const float fo = exp2_hw(m - mn);
     m = mn;
-    l = l * fo + x.y * fn;
-    o.x = o.x * fo + y.x * fn;
-    o.y = o.y * fo + y.y * fn;
+    l *= fo;
+    o.x *= fo;
+    o.y *= fo;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float f = s0 + 4 * i < slots ? exp2_hw(x[i].x - mn) : 0.f;
+      if (f != 0.f) {  // a slot read again, or far below the maximum, adds nothing
+        l += x[i].y * f;
+        o.x += y[i].x * f;
+        o.y += y[i].y * f;
+      }
+    }
   }
   if (lane == 0) {
     s_m[wv] = m;
@@ -852,7 +899,7 @@ static AttendPlan attend_plan(const ffa_paged_attend_args *a, int cus) {
   const long LG = (long)a->L * G;
   auto ranges = [&](long units, int pages, int kind, int &ppw, int &slots) {
     // units: pages over all sets, heads and row blocks; a workgroup of at least 4 pages, one per wave
-    const long want = (kind == kRows256 ? 1l : (kind == kRows128 ? 2l : 4l)) * cus;  // workgroups that fill the chip
+    const long want = (kind == kRows256 ? 1l : 2l) * cus;  // workgroups that fill the chip
     long w = (units + want - 1) / want;
     w = (w + 3) / 4 * 4;
     ppw = (int)(w < 4 ? 4 : (w > pages ? (pages < 4 ? 4 : pages) : w));
@@ -903,7 +950,7 @@ static void launch_attend(const AttendParams &p, int kind, int slots, int blocks
   switch (kind) {
     case kRows16: hipLaunchKernelGGL((paged_attend_kernel<FMT, RES, VT, 1>), few, dim3(256), 0, st, p); break;
     case kRows32: hipLaunchKernelGGL((paged_attend_kernel<FMT, RES, VT, 2>), few, dim3(256), 0, st, p); break;
-    case kRows64: hipLaunchKernelGGL((paged_attend_kernel<FMT, RES, VT, 4>), few, dim3(256), 0, st, p); break;
+    case kRows64: hipLaunchKernelGGL((paged_attend_wide_kernel<FMT, RES, VT, 1, 4>), wide, dim3(256), 0, st, p); break;
     case kRows128: hipLaunchKernelGGL((paged_attend_wide_kernel<FMT, RES, VT, 2, 4>), wide, dim3(256), 0, st, p); break;
     default: hipLaunchKernelGGL((paged_attend_wide_kernel<FMT, RES, VT, 2, 8>), wide, dim3(512), 0, st, p);
   }
@@ -1014,17 +1061,17 @@ extern "C" int ffa_paged_attend(const ffa_paged_attend_args *a, void *stream) {
     else if (a->format == FFA_PAGES_NVFP4) launch_attend_fmt<kFmtNvfp4>(p, a->res_dtype, a->v_dtype, kind, slots, blocks, sets, st);
     else launch_attend_fmt<kFmtNf4>(p, a->res_dtype, a->v_dtype, kind, slots, blocks, sets, st);
   };
-  if (pl.shared_slots > 0) {
-    p.shared = 1;
-    p.slot0 = 0;
-    p.ppw = pl.shared_ppw;
-    launch(pl.shared_kind, pl.shared_slots, pl.shared_blocks, a->ngroups);
-  }
-  if (pl.own_slots > 0) {
-    p.shared = 0;
-    p.slot0 = pl.shared_slots;
-    p.ppw = pl.own_ppw;
-    launch(pl.own_kind, pl.own_slots, pl.own_blocks, a->B);
+  if (pl.shared_slots > 0 && pl.own_slots > 0 && pl.shared_kind == pl.own_kind && a->ngroups + a->B <= 65535) {  // one launch
+    p.nshared = a->ngroups;
+    launch(pl.own_kind, pl.shared_slots > pl.own_slots ? pl.shared_slots : pl.own_slots,
+           pl.shared_blocks > pl.own_blocks ? pl.shared_blocks : pl.own_blocks, a->ngroups + a->B);
+  } else {
+    if (pl.shared_slots > 0) {
+      p.nshared = a->ngroups;
+      launch(pl.shared_kind, pl.shared_slots, pl.shared_blocks, a->ngroups);
+    }
+    p.nshared = 0;
+    if (pl.own_slots > 0) launch(pl.own_kind, pl.own_slots, pl.own_blocks, a->B);
   }
   if (pl.nslots > 0)
     hipLaunchKernelGGL(paged_attend_join_kernel, dim3((unsigned)rows), dim3(256), 0, st, p);

@@ -42,16 +42,15 @@ __device__ __forceinline__ void copy_piece(const PoolSet &s, uint32_t c, int src
   const uint32_t n = min((uint32_t)bytes - off, kPiece);
   const uint8_t *from = s.ptr[lo] + (size_t)src * bytes + off;
   uint8_t *to = s.ptr[lo] + (size_t)dst * bytes + off;
-  uint4 w[4];
+  const uint32_t at = 16 * threadIdx.x;
+  if (n == kPiece) {
+    uint4 w[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint32_t at = 16 * (threadIdx.x + 256 * i);
-    if (at < n) w[i] = *(const uint4 *)(from + at);
-  }
+    for (int i = 0; i < 4; ++i) w[i] = *(const uint4 *)(from + at + 4096 * i);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint32_t at = 16 * (threadIdx.x + 256 * i);
-    if (at < n) *(uint4 *)(to + at) = w[i];
+    for (int i = 0; i < 4; ++i) *(uint4 *)(to + at + 4096 * i) = w[i];
+  } else {
+    for (uint32_t x = at; x < n; x += 4096) *(uint4 *)(to + x) = *(const uint4 *)(from + x);
   }
 }
 
@@ -220,13 +219,12 @@ __global__ __launch_bounds__(256) void pages_count_kernel(int32_t *refs, int P, 
     } else if (step > 0) {
       atomicAdd(&refs[id], 1);
     } else {
-      int old = refs[id];  // a page that is free already stays free
-      while (old > 0) {
-        const int seen = atomicCAS(&refs[id], old, old - 1);
-        if (seen == old) break;
-        old = seen;
+      // a page that is free already stays free: the step is taken back (no step that finds a count above 0 can follow
+      // one that did not, so the result does not depend on their order)
+      if (atomicSub(&refs[id], 1) <= 0) {
+        atomicAdd(&refs[id], 1);
+        bad = true;
       }
-      bad |= old <= 0;
     }
   }
   if (bad) {

@@ -148,7 +148,7 @@ class PagePool:
 
     def _count(self, block_table, seq_lens, step, check, what):
         table, lens = self._rows(block_table, seq_lens)
-        call = torch.zeros(1, dtype=torch.int32, device=self.device)
+        call = torch.zeros(1, dtype=torch.int32, device=self.device) if check else self.errors
         with _on(self.device):
             rc = N.lib().ffa_pages_count(ctypes.byref(self._pg), table.data_ptr(), table.shape[1], table.shape[0],
                                          lens.data_ptr(), step, call.data_ptr(), self.errors.data_ptr(), self._stream())
