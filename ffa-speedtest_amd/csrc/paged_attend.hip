@@ -1,815 +1,9 @@
-// Exact attention of L query tokens per sequence over the paged quantized caches, and the same for groups of
-// sequences that share leading pages.
-//
-// Row (b, i, h) is query token i of sequence b at head h.  It sees the keys t < lim = len_b - qlen_b + i + 1 and
-//   out = sum_t p_t v_t / sum_t p_t,   p_t = 2^(s_t - m),   s_t = scale log2(e) q . k_t,   m >= max s_t - 8,
-// one pass over the pages with a running m; k = code * scale + zero + residual (2-bit), level * scale + residual
-// (nvfp4, nf4) in fp32, rounded once to the fp16 matrix operand.  Partial results (m, sum p, sum p v) of page ranges
-// are fp32 and joined by q's row afterwards; a call whose rows each have one range writes the output directly.
-//
-// The pools' order is the order of the matrix operands: with S^T = K Q^T (16x16x32 f16), the A operand of tile tau
-// (tokens 4 m + tau, m = 0..15) is what lane (kc, m) loads, and the four tiles' results in lane (g, n) are the 16
-// consecutive tokens 16 g .. 16 g + 15 of query row n: with O^T = V^T P^T those are the B operand, V^T's blocks the A
-// operand, and each lane's results belong to its own row n again, whose m and sum it holds.  No value of S, P or O
-// changes lanes.
-#include "decode_common.h"
-#include "ffa_mi355x.h"
+// Exact attention over the paged caches (paged_attend.h): the join of the partials, the launch plan and the C entry.
+#include "paged_attend.h"
 
 extern "C" int ffa_set_error_internal(int code, const char *msg);
 
 namespace ffa {
-
-enum { kFmtQ2 = 0, kFmtNvfp4 = 1, kFmtNf4 = 2 };
-constexpr float kNoMax = -1e30f;  // m of a row that has seen no key: below every score, and 2^(x - m) stays defined
-constexpr float kStale = 8.f;     // log2 units a row's m may lag its maximum: p <= 2^8 fits the fp16 operand as well
-
-struct AttendParams {
-  const void *q;
-  const uint8_t *k;
-  const uint8_t *ks;
-  const uint8_t *kz;
-  const uint8_t *kr;
-  const uint8_t *v;
-  const int32_t *bt;
-  const int32_t *seq_lens, *q_lens;
-  const int32_t *group_start, *group_pages, *seq_group;
-  void *out;
-  float *part_ml, *part_o;  // [rows][nslots][2], [rows][nslots][128]
-  int bt_stride, num_pages, ngroups;
-  int B, T, L, HQ, HKV, G;
-  int q_bf16, out_bf16;
-  float scale2;
-  int nslots;  // partials per row, 0: one page range per row, written to out
-  // sets of a launch: z < nshared are groups over their shared pages, then (from b = 0) sequences over their own
-  int nshared;
-  int shared_slots, shared_ppw, own_slots, own_ppw;
-};
-
-// QLoRA NF4 levels (the published 16 normal-float values)
-__constant__ float kAttendNF4[16] = {
-    -1.0f, -0.6961928009986877f, -0.5229921340942383f, -0.39491748809814453f, -0.28444138169288635f,
-    -0.18477343022823334f, -0.09105003625154495f, 0.0f, 0.07958029955625534f, 0.16093020141124725f,
-    0.24611230194568634f, 0.33791524171829224f, 0.44070982933044434f, 0.5626170039176941f,
-    0.7229568362236023f, 1.0f};
-
-__device__ __forceinline__ int seq_len_of(const AttendParams &p, int b) {
-  return p.seq_lens ? min(max(p.seq_lens[b], 0), p.T) : p.T;
-}
-// pages of sequence b that its group shares (0 without groups)
-__device__ __forceinline__ int shared_pages_of(const AttendParams &p, int b) {
-  if (p.ngroups == 0) return 0;
-  const int g = p.seq_group[b];
-  return (unsigned)g < (unsigned)p.ngroups ? min(max(p.group_pages[g], 0), p.bt_stride) : 0;
-}
-// keys that query token i of sequence b sees: positions below this
-__device__ __forceinline__ int row_limit(const AttendParams &p, int b, int i) {
-  const int len = seq_len_of(p, b);
-  const int ql = p.q_lens ? min(max(p.q_lens[b], 0), p.L) : p.L;
-  return i < ql ? max(len - ql + i + 1, 0) : 0;
-}
-
-// The rows and pages of a workgroup: sequences b0 .. b0 + n - 1 (a group's, over the shared pages; or one, over its
-// own), pages [p0, p1) of the block-table row of b0; the slot of the partials.
-struct AttendSet {
-  int b0, n, p0, p1, slot;
-};
-// the range `split` of set z, and the slot of its partials
-__device__ __forceinline__ AttendSet attend_set(const AttendParams &p, int z, int split) {
-  AttendSet s;
-  int ppw;
-  if (z < p.nshared) {
-    s.b0 = min(max(p.group_start[z], 0), p.B);
-    s.n = max(min(p.group_start[z + 1], p.B) - s.b0, 0);
-    s.p0 = 0;
-    s.p1 = min(max(p.group_pages[z], 0), p.bt_stride);
-    ppw = p.shared_ppw;
-    s.slot = split;
-  } else {
-    s.b0 = z - p.nshared;
-    s.n = 1;
-    s.p0 = shared_pages_of(p, s.b0);
-    s.p1 = (seq_len_of(p, s.b0) + kPage - 1) / kPage;
-    ppw = p.own_ppw;
-    s.slot = p.shared_slots + split;
-  }
-  s.p0 += split * ppw;
-  s.p1 = min(s.p0 + ppw, s.p1);
-  return s;
-}
-
-// ---------------------------------------------------------------------------
-// K of one (page, KV head): what lane (kc, m) loads, and its operands
-// ---------------------------------------------------------------------------
-// 16 bytes of a page that one workgroup reads once (non-temporal: 16 x 8K-64K tokens 394 -> 354 us)
-__device__ __forceinline__ uint4 load_once(const uint4 *p) {
-  const u32x4 w = __builtin_nontemporal_load((const u32x4 *)p);
-  return make_uint4(w[0], w[1], w[2], w[3]);
-}
-
-template <int FMT, int RES>
-struct KRaw {
-  uint4 code[FMT == kFmtQ2 ? 2 : 4];
-  uint4 res[RES == kResNone ? 1 : 8];
-  uint16_t s[4], z[FMT == kFmtQ2 ? 4 : 1];
-};
-
-template <int FMT, int RES>
-__device__ __forceinline__ void load_k(const AttendParams &p, size_t blk, int lane, KRaw<FMT, RES> &r) {
-  const int kc = lane >> 4, m = lane & 15;
-  if constexpr (FMT == kFmtQ2) {
-    const uint4 *c = (const uint4 *)(p.k + blk * 2048);
-    r.code[0] = c[lane];
-    r.code[1] = c[64 + lane];
-    const uint16_t *s = (const uint16_t *)(p.ks + blk * 512), *z = (const uint16_t *)(p.kz + blk * 512);
-#pragma unroll
-    for (int tau = 0; tau < 4; ++tau) {
-      const int at = (((tau >> 1) * 4 + kc) * 4 + (m >> 2)) * 8 + 4 * (tau & 1) + (m & 3);
-      r.s[tau] = s[at];
-      r.z[tau] = z[at];
-    }
-  } else {
-    const uint4 *c = (const uint4 *)(p.k + blk * 4096);
-#pragma unroll
-    for (int tau = 0; tau < 4; ++tau) {
-      r.code[tau] = c[64 * tau + lane];
-      if constexpr (FMT == kFmtNvfp4) r.s[tau] = ((const uint16_t *)(p.ks + blk * 512))[(4 * m + tau) * 4 + kc];
-      else r.s[tau] = ((const uint16_t *)(p.ks + blk * 256))[(4 * m + tau) * 2 + (kc >> 1)];
-    }
-  }
-  if constexpr (RES != kResNone) {
-    const uint4 *c = (const uint4 *)(p.kr + blk * 8192);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) r.res[i] = load_once(c + 64 * i + lane);
-  }
-}
-
-template <bool E4M3, bool HI>
-__device__ __forceinline__ f32x2 fp8_pair(uint32_t w) {
-  if constexpr (E4M3) return __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w, 1.0f, HI);
-  else return __builtin_amdgcn_cvt_scalef32_pk_f32_bf8(w, 1.0f, HI);
-}
-
-// Two operands: channels 32 kc + 16 h + (0..7) and + (8..15) of a token, in fp32 arithmetic with one rounding.
-// q2: c0 holds the 16 codes; 4-bit: c0 and c1 8 codes each.  s: the scale of these channels, z the zero point (q2).
-template <int FMT, int RES>
-__device__ __forceinline__ void k_half(uint32_t c0, uint32_t c1, float s, float z, uint4 rw, const float2 *nf4, f16x8 *op) {
-#pragma unroll
-  for (int e = 0; e < 2; ++e) {
-    float k[8];
-    f32x2 res[4];
-    if constexpr (RES != kResNone) {
-      const uint32_t lo = e ? rw.z : rw.x, hi = e ? rw.w : rw.y;
-      res[0] = fp8_pair<RES == kResE4M3, false>(lo);
-      res[1] = fp8_pair<RES == kResE4M3, true>(lo);
-      res[2] = fp8_pair<RES == kResE4M3, false>(hi);
-      res[3] = fp8_pair<RES == kResE4M3, true>(hi);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) res[i] = f32x2{0.f, 0.f};
-    }
-    if constexpr (FMT == kFmtQ2) {
-      // a 2-bit code as a nibble is the e2m1 value c / 2: the conversion with scale 2 gives codes 4 i, 4 i + 2 of
-      // byte i, and of the word shifted by one code 4 i + 1, 4 i + 3
-      const uint32_t a = c0 & 0x33333333u, b = (c0 >> 2) & 0x33333333u;
-      f32x2 a0, a1, b0, b1;
-      if (e) {
-        a0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(a, 2.0f, 2);
-        a1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(a, 2.0f, 3);
-        b0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(b, 2.0f, 2);
-        b1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(b, 2.0f, 3);
-      } else {
-        a0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(a, 2.0f, 0);
-        a1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(a, 2.0f, 1);
-        b0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(b, 2.0f, 0);
-        b1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(b, 2.0f, 1);
-      }
-      const float c[8] = {a0[0], b0[0], a0[1], b0[1], a1[0], b1[0], a1[1], b1[1]};
-#pragma unroll
-      for (int i = 0; i < 8; ++i) k[i] = __builtin_fmaf(c[i], s, z) + res[i >> 1][i & 1];
-    } else if constexpr (FMT == kFmtNvfp4) {
-      const uint32_t w = e ? c1 : c0;
-      const f32x2 c[4] = {__builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 0),
-                          __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 1),
-                          __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 2),
-                          __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 3)};
-#pragma unroll
-      for (int i = 0; i < 8; ++i) k[i] = __builtin_fmaf(c[i >> 1][i & 1], s, res[i >> 1][i & 1]);
-    } else {
-      const uint32_t w = e ? c1 : c0;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float2 c = nf4[(w >> (8 * i)) & 0xffu];
-        k[2 * i] = __builtin_fmaf(c.x, s, res[i][0]);
-        k[2 * i + 1] = __builtin_fmaf(c.y, s, res[i][1]);
-      }
-    }
-    const u32x4 w = {pk_f16_bits(k[0], k[1]), pk_f16_bits(k[2], k[3]), pk_f16_bits(k[4], k[5]), pk_f16_bits(k[6], k[7])};
-    op[e] = __builtin_bit_cast(f16x8, w);
-  }
-}
-
-// Operands e = 0..3 of tile tau: channels 32 kc + 8 e + (0..7) of token 4 m + tau
-template <int FMT, int RES>
-__device__ __forceinline__ void k_operands(const KRaw<FMT, RES> &r, int tau, const float2 *nf4, f16x8 *op) {
-  float s[2], z = 0.f;
-  if constexpr (FMT == kFmtNvfp4) {
-    const f32x2 w = fp8_pair<true, false>(r.s[tau]);
-    s[0] = w[0];
-    s[1] = w[1];
-  } else {
-    s[0] = s[1] = f16_bits_to_f32(r.s[tau]);
-    if constexpr (FMT == kFmtQ2) z = f16_bits_to_f32(r.z[tau]);
-  }
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    uint32_t c0, c1 = 0;
-    if constexpr (FMT == kFmtQ2) {
-      const uint4 c = r.code[tau >> 1];
-      c0 = h ? (tau & 1 ? c.w : c.y) : (tau & 1 ? c.z : c.x);
-    } else {
-      c0 = h ? r.code[tau].z : r.code[tau].x;
-      c1 = h ? r.code[tau].w : r.code[tau].y;
-    }
-    k_half<FMT, RES>(c0, c1, s[h], z, r.res[RES == kResNone ? 0 : 2 * tau + h], nf4, op + 2 * h);
-  }
-}
-
-// ---------------------------------------------------------------------------
-// q of one row tile as the B operands, each row divided by a power of two that brings its largest element into
-// [1, 2): every bf16 row fits fp16 that way (elements below 2^-14 of the row's largest lose bits that its scores,
-// rounded at 2^-24 of the sum, do not hold).  cs: the row's factor back to log2-scaled scores.
-// ---------------------------------------------------------------------------
-__device__ __forceinline__ void load_q(const AttendParams &p, size_t row, bool ok, int kc, f16x8 *op, float &cs) {
-  float x[32];
-  const uint4 *src = (const uint4 *)((const uint16_t *)p.q + row * kD + 32 * kc);
-  float top = 0.f;
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const uint4 w = ok ? src[e] : make_uint4(0, 0, 0, 0);
-    const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      x[8 * e + 2 * i] = p.q_bf16 ? __uint_as_float(ww[i] << 16) : f16_bits_to_f32(ww[i] & 0xffffu);
-      x[8 * e + 2 * i + 1] = p.q_bf16 ? __uint_as_float(ww[i] & 0xffff0000u) : f16_bits_to_f32(ww[i] >> 16);
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x[8 * e + i]));
-  }
-  top = xor_max(top, 16);
-  top = xor_max(top, 32);
-  int ex = (int)((__float_as_uint(top) >> 23) & 0xffu);  // 0: all zero or tiny; 255: an infinity
-  ex = ex == 255 ? 127 : min(max(ex, 1), 253);
-  float f = __uint_as_float((uint32_t)(254 - ex) << 23);
-  cs = p.scale2 * __uint_as_float((uint32_t)ex << 23);
-  if (cs < 0.f) f = -f;  // a negative scale: into q, so that the largest product is the largest score
-  cs = fmaxf(fabsf(cs), 1e-37f);  // above 0: a hidden key's product of -inf stays -inf
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    u32x4 w;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = pk_f16_bits(x[8 * e + 2 * i] * f, x[8 * e + 2 * i + 1] * f);
-    op[e] = __builtin_bit_cast(f16x8, w);
-  }
-}
-
-// V words (8 tokens of a column) with infinities and NaN taken out; `bad` becomes non-zero where there were any.
-// A product with them would give 0 * inf to the rows that do not see them; add_not_finite puts them back.
-__device__ __forceinline__ u32x4 finite8(u32x4 w, uint32_t &bad) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint32_t x = ((w[i] & 0x7c007c00u) + 0x04000400u) & 0x80008000u;  // top bit of a half: all exponent bits set
-    bad |= x;
-    w[i] &= ~((x >> 15) * 0xffffu);
-  }
-  return w;
-}
-
-// infinities and NaN of V at tokens that the lane's row sees, into its columns 16 u + 4 g + (0..3): whatever the
-// weight (above zero), they make the result what they are
-template <int VT>
-__device__ __forceinline__ void add_not_finite(const uint8_t *v, int g, int nvis, f32x4 *o) {
-#pragma unroll 1
-  for (int t = 0; t < nvis && t < kPage; ++t)
-#pragma unroll
-    for (int u = 0; u < 8; ++u)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const uint32_t w = ((const uint16_t *)v)[vt_off(16 * u + 4 * g + e, t)];
-        const float x = VT == kVBF16 ? round_to(bf16_bits_to_f32(w), 0) : f16_bits_to_f32(w);
-        if (!(fabsf(x) < INFINITY)) o[u][e] += x;
-      }
-}
-
-// ---------------------------------------------------------------------------
-// The softmax step of one row tile over one page: scores to P operands, m and l of lane (g, n)'s row n
-// (l: the lane's own tokens only, summed over g at the end).  MASK: tokens at or past lim (relative to the page) do
-// not count.  Returns the factor that the row's O so far is to be multiplied by (1 where m stands).
-// ---------------------------------------------------------------------------
-template <bool MASK>
-__device__ __forceinline__ bool softmax_step(f32x4 *S, float cs, int nvis, int g, float &m, float &l, float &alpha,
-                                             f16x8 *P) {
-  float x[16];
-  float top = -INFINITY;
-#pragma unroll
-  for (int tau = 0; tau < 4; ++tau)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int k = 4 * i + tau;
-      x[k] = S[tau][i];
-      if (!MASK || 16 * g + k < nvis) top = fmaxf(top, x[k]);
-    }
-  top *= cs;
-  // the largest m may lag by kStale: most pages need no exchange between the row's four lanes and leave O as it is
-  const bool moved = __ballot(top > m + kStale) != 0;
-  alpha = 1.f;
-  if (moved) {
-    top = xor_max(top, 16);
-    top = xor_max(top, 32);
-    const float mn = fmaxf(m, top);
-    alpha = exp2_hw(m - mn);
-    m = mn;
-    l *= alpha;
-  }
-  float sum = 0.f;
-#pragma unroll
-  for (int k = 0; k < 16; ++k) {
-    x[k] = (!MASK || 16 * g + k < nvis) ? exp2_hw(__builtin_fmaf(x[k], cs, -m)) : 0.f;
-    sum += x[k];
-  }
-  l += sum;
-#pragma unroll
-  for (int kap = 0; kap < 2; ++kap) {
-    u32x4 w;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = pk_f16_bits(x[8 * kap + 2 * i], x[8 * kap + 2 * i + 1]);
-    P[kap] = __builtin_bit_cast(f16x8, w);
-  }
-  return moved;
-}
-
-__device__ __forceinline__ f32x4 mfma16(f16x8 a, f16x8 b, f32x4 c) {
-  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
-}
-
-// a partial (or, without slots, the output) of 8 columns of one row
-__device__ __forceinline__ void store_row8(const AttendParams &p, size_t row, int slot, int c0, const float *o, float m,
-                                           float l, bool sees) {
-  if (p.nslots == 0) {
-    const float inv = sees ? 1.f / l : 0.f;
-    float y[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) y[e] = sees ? o[e] * inv : 0.f;
-    uint4 w;
-    if (p.out_bf16) w = make_uint4(pk_bf16_bits(y[0], y[1]), pk_bf16_bits(y[2], y[3]), pk_bf16_bits(y[4], y[5]), pk_bf16_bits(y[6], y[7]));
-    else w = make_uint4(pk_f16_bits(y[0], y[1]), pk_f16_bits(y[2], y[3]), pk_f16_bits(y[4], y[5]), pk_f16_bits(y[6], y[7]));
-    *(uint4 *)((uint16_t *)p.out + row * kD + c0) = w;
-    return;
-  }
-  const size_t at = row * p.nslots + slot;
-  float4 *dst = (float4 *)(p.part_o + at * kD + c0);
-  dst[0] = make_float4(o[0], o[1], o[2], o[3]);
-  dst[1] = make_float4(o[4], o[5], o[6], o[7]);
-  if (c0 == 0) *(float2 *)(p.part_ml + 2 * at) = make_float2(m, l);
-}
-
-// ---------------------------------------------------------------------------
-// Few rows (up to 16 NT of a KV head and set per workgroup): each wave takes every fourth page of the range with all
-// rows, its operands straight from memory; the waves' results are joined in LDS.
-// ---------------------------------------------------------------------------
-template <int FMT, int RES, int VT, int NT>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NT <= 2 ? 2 : 1))) void paged_attend_kernel(const AttendParams p) {
-  typedef VTraits<VT> VTr;
-  const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int g = lane >> 4, n = lane & 15;
-  const int split = blockIdx.x, hkv = blockIdx.y % p.HKV, rb = blockIdx.y / p.HKV;
-  const AttendSet set = attend_set(p, blockIdx.z, split);
-  const int LG = p.L * p.G, R = set.n * LG, r0 = rb * 16 * NT;
-  if (r0 >= R) return;
-  const int pa = set.p0, pe = set.p1;
-  if (pa >= pe && p.nslots != 0) return;
-
-  __shared__ float s_m[4][16 * NT], s_l[4][16 * NT];
-  __shared__ __attribute__((aligned(16))) float s_o[4][16][kD + 4];
-  __shared__ float2 s_nf4[FMT == kFmtNf4 ? 256 : 1];
-  if constexpr (FMT == kFmtNf4) {
-    s_nf4[threadIdx.x] = make_float2(kAttendNF4[threadIdx.x & 15], kAttendNF4[threadIdx.x >> 4]);
-    __syncthreads();
-  }
-
-  f16x8 Q[NT][4];
-  float cs[NT], m[NT], l[NT];
-  int lim[NT];
-  int lo = 0x7fffffff, hi = 0;
-  f32x4 O[NT][8];
-#pragma unroll
-  for (int t = 0; t < NT; ++t) {
-    const int r = r0 + 16 * t + n;
-    const bool ok = r < R;
-    const int bi = ok ? r / LG : 0, j = ok ? r - bi * LG : 0, i = j / p.G;
-    const size_t row = ((size_t)(set.b0 + bi) * p.L + i) * p.HQ + hkv * p.G + (j - i * p.G);
-    load_q(p, row, ok, g, Q[t], cs[t]);
-    lim[t] = ok ? row_limit(p, set.b0 + bi, i) : 0x7fffffff;  // rows past the last are computed, and not stored
-    lo = min(lo, lim[t]);
-    hi = max(hi, ok ? lim[t] : 0);
-    m[t] = kNoMax;
-    l[t] = 0.f;
-#pragma unroll
-    for (int u = 0; u < 8; ++u) O[t][u] = f32x4{0.f, 0.f, 0.f, 0.f};
-  }
-#pragma unroll
-  for (int s = 1; s < 16; s <<= 1) {
-    lo = min(lo, __shfl_xor(lo, s));
-    hi = max(hi, __shfl_xor(hi, s));
-  }
-  lo = __builtin_amdgcn_readfirstlane(lo);
-  hi = __builtin_amdgcn_readfirstlane(hi);
-  const int32_t *bt = p.bt + (size_t)set.b0 * p.bt_stride;
-
-  for (int pg = pa + wv; pg < pe; pg += 4) {
-    const int t0 = pg * kPage;
-    if (t0 >= hi) break;  // no row sees this page or a later one
-    int id = bt[pg];
-    id = __builtin_amdgcn_readfirstlane((unsigned)id < (unsigned)p.num_pages ? id : 0);
-    const size_t blk = (size_t)id * p.HKV + hkv;
-    KRaw<FMT, RES> kr;
-    load_k<FMT, RES>(p, blk, lane, kr);
-    u32x4 V[16];
-    const u32x4 *vp = (const u32x4 *)(p.v + blk * (kD * kPage * 2));
-#pragma unroll
-    for (int i = 0; i < 16; ++i) V[i] = __builtin_nontemporal_load(vp + 64 * i + lane);
-
-    f32x4 S[NT][4];
-#pragma unroll
-    for (int tau = 0; tau < 4; ++tau) {
-      f16x8 K[4];
-      k_operands<FMT, RES>(kr, tau, s_nf4, K);
-#pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        f32x4 a = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) a = mfma16(K[e], Q[t][e], a);
-        S[t][tau] = a;
-      }
-    }
-    const bool full = lo >= t0 + kPage;  // every row sees the whole page
-    f16x8 P[NT][2];
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      float alpha;
-      const bool moved = full ? softmax_step<false>(S[t], cs[t], 64, g, m[t], l[t], alpha, P[t])
-                              : softmax_step<true>(S[t], cs[t], lim[t] - t0, g, m[t], l[t], alpha, P[t]);
-      if (moved)
-#pragma unroll
-        for (int u = 0; u < 8; ++u) O[t][u] *= alpha;
-    }
-    uint32_t bad = 0;
-    if (!full) {
-      u32x4 keep[2];
-      partial_page_masks(g, hi - t0, keep);  // slots that no row sees are not data
-#pragma unroll
-      for (int i = 0; i < 16; ++i)
-        V[i] = finite8(__builtin_bit_cast(u32x4, VTr::operand(V[i] & keep[i & 1])), bad);
-    }
-#pragma unroll
-    for (int u = 0; u < 8; ++u)
-#pragma unroll
-      for (int kap = 0; kap < 2; ++kap) {
-        const f16x8 a = full ? VTr::operand(V[2 * u + kap]) : __builtin_bit_cast(f16x8, V[2 * u + kap]);
-#pragma unroll
-        for (int t = 0; t < NT; ++t) O[t][u] = mfma16(a, P[t][kap], O[t][u]);
-      }
-    if (__ballot(bad != 0) != 0)
-#pragma unroll
-      for (int t = 0; t < NT; ++t) add_not_finite<VT>(p.v + blk * (kD * kPage * 2), g, lim[t] - t0, O[t]);
-  }
-
-  // join the four waves
-#pragma unroll
-  for (int t = 0; t < NT; ++t) {
-    l[t] = xor_sum(l[t], 16);
-    l[t] = xor_sum(l[t], 32);
-    if (g == 0) {
-      s_m[wv][16 * t + n] = m[t];
-      s_l[wv][16 * t + n] = l[t];
-    }
-  }
-  __syncthreads();
-#pragma unroll
-  for (int t = 0; t < NT; ++t) {
-    float M = kNoMax;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) M = fmaxf(M, s_m[w][16 * t + n]);
-    const float f = exp2_hw(m[t] - M);
-#pragma unroll
-    for (int u = 0; u < 8; ++u)
-      *(f32x4 *)&s_o[wv][n][16 * u + 4 * g] = O[t][u] * f;
-    __syncthreads();
-    const int rr = threadIdx.x >> 4, c0 = 8 * (threadIdx.x & 15);
-    const int r = r0 + 16 * t + rr;
-    if (r < R) {
-      float mm = kNoMax, ll = 0.f, o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int w = 0; w < 4; ++w) mm = fmaxf(mm, s_m[w][16 * t + rr]);
-#pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        ll += s_l[w][16 * t + rr] * exp2_hw(s_m[w][16 * t + rr] - mm);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) o[e] += s_o[w][rr][c0 + e];
-      }
-      const int bi = r / LG, j = r - bi * LG, i = j / p.G, b = set.b0 + bi;
-      const size_t row = ((size_t)b * p.L + i) * p.HQ + hkv * p.G + (j - i * p.G);
-      store_row8(p, row, set.slot, c0, o, mm, ll, row_limit(p, b, i) > 0);
-    }
-    __syncthreads();
-  }
-}
-
-// ---------------------------------------------------------------------------
-// Many rows: 16 NT rows to each of the W waves.  The workgroup dequantizes a page once, as operands in LDS (K: wave w
-// takes 8 / W of the eight (tile, half of the channels) units; V comes as it lies in the pool), and every wave reads
-// them for its rows.  Two pages are in flight: while a wave exponentiates page j and multiplies it with V, it computes
-// the scores of page j + 1, dequantizes its share of page j + 2 and has page j + 3's bytes under way, so that matrix
-// and vector instructions have independent work at any time, with one barrier a page.
-// ---------------------------------------------------------------------------
-template <int FMT>
-struct KUnit {  // one unit's bytes of lane (kc, m): token 4 m + tau, channels 32 kc + 16 h + (0..15)
-  uint32_t c0, c1;
-  uint16_t s, z;
-  uint4 res;
-};
-template <int FMT, int RES>
-__device__ __forceinline__ void load_unit(const AttendParams &p, size_t blk, int unit, int lane, KUnit<FMT> &r) {
-  const int kc = lane >> 4, m = lane & 15, tau = unit >> 1, h = unit & 1;
-  if constexpr (FMT == kFmtQ2) {
-    r.c0 = *(const uint32_t *)(p.k + blk * 2048 + (((tau >> 1) * 64 + lane) * 2 + (tau & 1)) * 8 + 4 * h);
-    const int at = (((tau >> 1) * 4 + kc) * 4 + (m >> 2)) * 8 + 4 * (tau & 1) + (m & 3);
-    r.s = ((const uint16_t *)(p.ks + blk * 512))[at];
-    r.z = ((const uint16_t *)(p.kz + blk * 512))[at];
-  } else {
-    const uint2 c = *(const uint2 *)(p.k + blk * 4096 + (tau * 64 + lane) * 16 + 8 * h);
-    r.c0 = c.x;
-    r.c1 = c.y;
-    if constexpr (FMT == kFmtNvfp4) r.s = (p.ks + blk * 512)[(4 * m + tau) * 8 + 2 * kc + h];
-    else r.s = ((const uint16_t *)(p.ks + blk * 256))[(4 * m + tau) * 2 + (kc >> 1)];
-  }
-  if constexpr (RES != kResNone) r.res = ((const uint4 *)(p.kr + blk * 8192))[64 * unit + lane];
-}
-template <int FMT, int RES>
-__device__ __forceinline__ void unit_to_lds(const KUnit<FMT> &r, int unit, int lane, const float2 *nf4, u32x4 *dst) {
-  const float s = FMT == kFmtNvfp4 ? fp8_pair<true, false>(r.s)[0] : f16_bits_to_f32(r.s);
-  const float z = FMT == kFmtQ2 ? f16_bits_to_f32(r.z) : 0.f;
-  f16x8 op[2];
-  k_half<FMT, RES>(r.c0, r.c1, s, z, r.res, nf4, op);
-  dst[(2 * unit) * 64 + lane] = __builtin_bit_cast(u32x4, op[0]);
-  dst[(2 * unit + 1) * 64 + lane] = __builtin_bit_cast(u32x4, op[1]);
-}
-
-template <int FMT, int RES, int VT, int NT, int W>
-__global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2))) void paged_attend_wide_kernel(
-    const AttendParams p) {
-  constexpr int kUnits = 8 / W, kVPieces = 16 / W;  // of a page, per wave
-  const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int g = lane >> 4, n = lane & 15;
-  const int nb = gridDim.x / p.HKV;  // the last rows, which see the most keys of a causal chunk, first
-  const int hkv = blockIdx.x % p.HKV, rb = nb - 1 - blockIdx.x / p.HKV, split = blockIdx.y;
-  const AttendSet set = attend_set(p, blockIdx.z, split);
-  const int LG = p.L * p.G, R = set.n * LG, r0 = (rb * W + wv) * 16 * NT;
-  if (rb * W * 16 * NT >= R) return;
-  const int pa = set.p0;
-  int pe = set.p1;
-  if (pa >= pe && p.nslots != 0) return;
-
-  __shared__ u32x4 s_k[2][16 * 64], s_v[2][16 * 64];
-  __shared__ float2 s_nf4[FMT == kFmtNf4 ? 256 : 1];
-  __shared__ int s_hi[W], s_lo[W], s_bad;
-
-  const int last = max(set.p1 - 1, pa);  // in the table also where the range is empty
-  const int32_t *bt = p.bt + (size_t)set.b0 * p.bt_stride;
-  auto block_of = [&](int pg) {  // pages past the range repeat its last one: loaded, never used
-    int id = bt[min(pg, last)];
-    id = __builtin_amdgcn_readfirstlane((unsigned)id < (unsigned)p.num_pages ? id : 0);
-    return (size_t)id * p.HKV + hkv;
-  };
-  KUnit<FMT> raw[kUnits];
-  auto load_raw = [&](size_t blk, KUnit<FMT> *r) {
-#pragma unroll
-    for (int i = 0; i < kUnits; ++i) load_unit<FMT, RES>(p, blk, wv * kUnits + i, lane, r[i]);
-  };
-  auto raw_to_lds = [&](int buf, const KUnit<FMT> *r) {
-#pragma unroll
-    for (int i = 0; i < kUnits; ++i) unit_to_lds<FMT, RES>(r[i], wv * kUnits + i, lane, s_nf4, s_k[buf]);
-  };
-  // V: straight into LDS; a bf16 pool's, which becomes the fp16 operand, through registers a page earlier
-  u32x4 vraw[VT == kVF16 ? 1 : kVPieces];
-  auto fetch_v = [&](size_t blk) {
-    if constexpr (VT != kVF16) {
-      const u32x4 *src = (const u32x4 *)(p.v + blk * (kD * kPage * 2));
-#pragma unroll
-      for (int i = 0; i < kVPieces; ++i) vraw[i] = src[(wv * kVPieces + i) * 64 + lane];
-    }
-  };
-  auto store_v = [&](size_t blk, int buf) {
-    const u32x4 *src = (const u32x4 *)(p.v + blk * (kD * kPage * 2));
-#pragma unroll
-    for (int i = 0; i < kVPieces; ++i) {
-      const int at = (wv * kVPieces + i) * 64;
-      if constexpr (VT == kVF16)
-        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)(src + at + lane),
-                                         (__attribute__((address_space(3))) void *)(&s_v[buf][at]), 16, 0, 0);
-      else
-        s_v[buf][at + lane] = __builtin_bit_cast(u32x4, VTraits<VT>::operand(vraw[i]));
-    }
-  };
-  // the first pages' bytes are under way while q and the rows' limits are read
-  size_t b0 = block_of(pa), b1 = block_of(pa + 1), b2 = block_of(pa + 2);
-  KUnit<FMT> raw0[kUnits];
-  load_raw(b0, raw0);
-  load_raw(b1, raw);
-  fetch_v(b0);
-  if constexpr (VT == kVF16) store_v(b0, 0);
-
-  f16x8 Q[NT][4];
-  float cs[NT], m[NT];
-  int lim[NT], lo = 0x7fffffff, hi = 0;
-  f32x4 O[NT][8], Ls[NT];
-#pragma unroll
-  for (int t = 0; t < NT; ++t) {
-    const int r = r0 + 16 * t + n;
-    const bool ok = r < R;
-    const int bi = ok ? r / LG : 0, j = ok ? r - bi * LG : 0, i = j / p.G;
-    const size_t row = ((size_t)(set.b0 + bi) * p.L + i) * p.HQ + hkv * p.G + (j - i * p.G);
-    load_q(p, row, ok, g, Q[t], cs[t]);
-    lim[t] = ok ? row_limit(p, set.b0 + bi, i) : 0x7fffffff;
-    lo = min(lo, lim[t]);
-    hi = max(hi, ok ? lim[t] : 0);
-    m[t] = kNoMax;
-    Ls[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int u = 0; u < 8; ++u) O[t][u] = f32x4{0.f, 0.f, 0.f, 0.f};
-  }
-#pragma unroll
-  for (int s = 1; s < 16; s <<= 1) {
-    lo = min(lo, __shfl_xor(lo, s));
-    hi = max(hi, __shfl_xor(hi, s));
-  }
-  if (lane == 0) {
-    s_lo[wv] = lo;
-    s_hi[wv] = hi;
-  }
-  if constexpr (FMT == kFmtNf4)
-    if (threadIdx.x < 256) s_nf4[threadIdx.x] = make_float2(kAttendNF4[threadIdx.x & 15], kAttendNF4[threadIdx.x >> 4]);
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < W; ++w) {
-    lo = min(lo, s_lo[w]);
-    hi = max(hi, s_hi[w]);
-  }
-  lo = __builtin_amdgcn_readfirstlane(lo);  // every row of the workgroup sees the keys below lo, none those from hi on
-  hi = __builtin_amdgcn_readfirstlane(hi);
-  pe = min(pe, (hi + kPage - 1) / kPage);
-
-  f32x4 S[NT][4];
-  auto scores = [&](int buf, f32x4 (*X)[4]) {
-#pragma unroll
-    for (int tau = 0; tau < 4; ++tau) {
-      f16x8 K[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) K[e] = __builtin_bit_cast(f16x8, s_k[buf][(4 * tau + e) * 64 + lane]);
-#pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        f32x4 a = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) a = mfma16(K[e], Q[t][e], a);
-        X[t][tau] = a;
-      }
-    }
-  };
-  const f16x8 one = {1, 1, 1, 1, 1, 1, 1, 1};
-  auto weights = [&](int t, f16x8 *P) {  // of S[t], against m[t]; their sum by a product with ones
-    float x[16];
-#pragma unroll
-    for (int tau = 0; tau < 4; ++tau)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) x[4 * i + tau] = exp2_hw(__builtin_fmaf(S[t][tau][i], cs[t], -m[t]));
-#pragma unroll
-    for (int kap = 0; kap < 2; ++kap) {
-      u32x4 w;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) w[i] = pk_f16_bits(x[8 * kap + 2 * i], x[8 * kap + 2 * i + 1]);
-      P[kap] = __builtin_bit_cast(f16x8, w);
-      Ls[t] = mfma16(one, P[kap], Ls[t]);
-    }
-  };
-
-  auto page_barrier = [&]() {  // loads into LDS are counted with the others, and no barrier waits for those
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-  };
-  if (pa < pe) {
-    if constexpr (VT != kVF16) store_v(b0, 0);
-    fetch_v(b1);
-    raw_to_lds(0, raw0);
-    raw_to_lds(1, raw);
-    load_raw(b2, raw);
-    page_barrier();
-    scores(0, S);
-    __syncthreads();
-    for (int pg = pa, cur = 0; pg < pe; ++pg, cur ^= 1) {
-      const size_t b3 = block_of(pg + 3);
-      store_v(b1, cur ^ 1);
-      fetch_v(b2);
-      raw_to_lds(cur, raw);
-      load_raw(b3, raw);
-      const int t0 = pg * kPage;
-      const bool full = lo >= t0 + kPage;
-      if (!full) {  // the last pages of a sequence or chunk
-        if (threadIdx.x == 0) s_bad = 0;
-        u32x4 keep[2];
-        uint32_t bad = 0;
-        partial_page_masks(g, hi - t0, keep);  // slots that no row sees are not data
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < kVPieces; ++i) {
-          const int at = (wv * kVPieces + i) * 64 + lane;
-          s_v[cur][at] = finite8(s_v[cur][at] & keep[(wv * kVPieces + i) & 1], bad);
-        }
-        if (bad) s_bad = 1;
-        __syncthreads();
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-          for (int tau = 0; tau < 4; ++tau)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              if (t0 + 16 * g + 4 * i + tau >= lim[t]) S[t][tau][i] = -INFINITY;
-      }
-      float top[NT];
-      bool lag = false;
-#pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        float x = S[t][0][0];
-#pragma unroll
-        for (int k = 1; k < 16; ++k) x = fmaxf(x, S[t][k >> 2][k & 3]);
-        top[t] = x * cs[t];
-        lag |= top[t] > m[t] + kStale;
-      }
-      if (__ballot(lag) != 0) {
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          const float mn = fmaxf(m[t], xor_max(xor_max(top[t], 16), 32));
-          const float alpha = exp2_hw(m[t] - mn);
-          m[t] = mn;
-          Ls[t] *= alpha;
-#pragma unroll
-          for (int u = 0; u < 8; ++u) O[t][u] *= alpha;
-        }
-      }
-      f16x8 P[NT][2];
-#pragma unroll
-      for (int t = 0; t < NT; ++t) weights(t, P[t]);
-      scores(cur ^ 1, S);
-#pragma unroll
-      for (int u = 0; u < 8; ++u)
-#pragma unroll
-        for (int kap = 0; kap < 2; ++kap) {
-          const f16x8 a = __builtin_bit_cast(f16x8, s_v[cur][(2 * u + kap) * 64 + lane]);
-#pragma unroll
-          for (int t = 0; t < NT; ++t) O[t][u] = mfma16(a, P[t][kap], O[t][u]);
-        }
-      if (!full && s_bad)
-#pragma unroll
-        for (int t = 0; t < NT; ++t) add_not_finite<VT>(p.v + b0 * (kD * kPage * 2), g, lim[t] - t0, O[t]);
-      b0 = b1;
-      b1 = b2;
-      b2 = b3;
-      page_barrier();
-    }
-  }
-
-#pragma unroll
-  for (int t = 0; t < NT; ++t) {
-    const int r = r0 + 16 * t + n;
-    if (r >= R) continue;
-    const int bi = r / LG, j = r - bi * LG, i = j / p.G;
-    const size_t row = ((size_t)(set.b0 + bi) * p.L + i) * p.HQ + hkv * p.G + (j - i * p.G);
-    const float l = Ls[t][0];
-    if (p.nslots == 0) {
-      const float inv = lim[t] > 0 ? 1.f / l : 0.f;
-#pragma unroll
-      for (int u = 0; u < 8; ++u) {
-        const f32x4 y = lim[t] > 0 ? O[t][u] * inv : f32x4{0.f, 0.f, 0.f, 0.f};
-        const uint2 w = p.out_bf16 ? make_uint2(pk_bf16_bits(y[0], y[1]), pk_bf16_bits(y[2], y[3]))
-                                   : make_uint2(pk_f16_bits(y[0], y[1]), pk_f16_bits(y[2], y[3]));
-        *(uint2 *)((uint16_t *)p.out + row * kD + 16 * u + 4 * g) = w;
-      }
-    } else {
-      const size_t at = row * p.nslots + set.slot;
-#pragma unroll
-      for (int u = 0; u < 8; ++u) *(f32x4 *)(p.part_o + at * kD + 16 * u + 4 * g) = O[t][u];
-      if (g == 0) *(float2 *)(p.part_ml + 2 * at) = make_float2(m[t], l);
-    }
-  }
-}
 
 // ---------------------------------------------------------------------------
 // Join of the partials: one workgroup per row; wave w adds the slots w, w + 4, ...
@@ -823,7 +17,7 @@ __global__ __launch_bounds__(256) void paged_attend_join_kernel(const AttendPara
   const bool sees = row_limit(p, b, i) > 0;
   const int sp = shared_pages_of(p, b), own = max((seq_len_of(p, b) + kPage - 1) / kPage - sp, 0);
   const int na = p.shared_slots ? min((sp + p.shared_ppw - 1) / p.shared_ppw, p.shared_slots) : 0;
-  const int nb = min((own + p.own_ppw - 1) / p.own_ppw, p.own_slots);
+  const int per = own_range(p, own), nb = p.own_slots ? min((own + per - 1) / per, p.own_slots) : 0;
   const float2 *ml = (const float2 *)p.part_ml + row * p.nslots;
   const float *po = p.part_o + row * p.nslots * kD;
   float m = kNoMax, l = 0.f;
@@ -880,94 +74,77 @@ __global__ __launch_bounds__(256) void paged_attend_join_kernel(const AttendPara
 
 // Launch plan of a call: page ranges of the shared and of the own pages
 struct AttendPlan {
-  int shared_slots, shared_ppw, own_slots, own_ppw, nslots;
+  int shared_slots, shared_ppw, own_slots, nslots;
   int shared_kind, shared_blocks, own_kind, own_blocks;
-  int own_pages;
+  bool both;  // one launch of 256-row workgroups over shared pages and of few-row ones over own pages
 };
 
 // the kernel for so many rows of a KV head and set, and the rows of its workgroup
-enum { kRows16 = 0, kRows32, kRows64, kRows128, kRows256 };
 static int kind_for(long rows) {
   return rows <= 16 ? kRows16 : (rows <= 32 ? kRows32 : (rows <= 64 ? kRows64 : (rows <= 128 ? kRows128 : kRows256)));
 }
 static long kind_rows(int kind) { return 16l << kind; }
 
+// Ranges of ppw pages so that `units` (pages over all sets, heads and row blocks) make about `want` workgroups
+static void page_ranges(long units, int pages, long want, int &ppw, int &slots) {
+  long w = (units + want - 1) / want;
+  w = (w + 3) / 4 * 4;  // a page for each of four waves
+  if (w > pages) w = (pages + 3) / 4 * 4;
+  ppw = (int)(w < 4 ? 4 : w);
+  slots = (pages + ppw - 1) / ppw;
+}
+
 static AttendPlan attend_plan(const ffa_paged_attend_args *a, int cus) {
   AttendPlan pl = {};
-  const int G = a->HQ / a->HKV;
   if (cus <= 0) cus = 256;
-  const long LG = (long)a->L * G;
-  auto ranges = [&](long units, int pages, int kind, int &ppw, int &slots) {
-    // units: pages over all sets, heads and row blocks; a workgroup of at least 4 pages, one per wave
-    const long want = (kind == kRows256 ? 1l : 2l) * cus;  // workgroups that fill the chip
-    long w = (units + want - 1) / want;
-    w = (w + 3) / 4 * 4;
-    ppw = (int)(w < 4 ? 4 : (w > pages ? (pages < 4 ? 4 : pages) : w));
-    slots = (pages + ppw - 1) / ppw;
-  };
-  int min_shared = 0;
-  if (a->ngroups > 0) {
-    long units = 0, rows = 0;
-    int pages = 0;
-    min_shared = a->group_pages_host[0];
-    for (int g = 0; g < a->ngroups; ++g) {
-      const long n = a->group_start_host[g + 1] - a->group_start_host[g];
-      const int gp = a->group_pages_host[g];
-      if (gp > 0 && n * LG > rows) rows = n * LG;
-      if (gp > pages) pages = gp;
-      if (gp < min_shared) min_shared = gp;
-    }
-    if (pages > 0) {
-      pl.shared_kind = kind_for(rows);
-      const long kr = kind_rows(pl.shared_kind);
-      pl.shared_blocks = (int)((rows + kr - 1) / kr);
-      for (int g = 0; g < a->ngroups; ++g) {
-        const long n = a->group_start_host[g + 1] - a->group_start_host[g];
-        units += (long)a->group_pages_host[g] * a->HKV * ((n * LG + kr - 1) / kr);
-      }
-      ranges(units, pages, pl.shared_kind, pl.shared_ppw, pl.shared_slots);
-    }
+  const long LG = (long)a->L * (a->HQ / a->HKV);
+  // workgroups that are resident at a time: one round of them (a second one that is not full costs as much)
+  auto resident = [&](int kind) { return (kind == kRows256 ? 1l : 2l) * cus; };
+  long units = 0, rows = 0;
+  int most = 0, least = a->ngroups > 0 ? a->group_pages_host[0] : 0;  // shared pages
+  for (int g = 0; g < a->ngroups; ++g) {
+    const long n = a->group_start_host[g + 1] - a->group_start_host[g];
+    const int gp = a->group_pages_host[g];
+    if (gp > 0 && n * LG > rows) rows = n * LG;
+    if (gp > most) most = gp;
+    if (gp < least) least = gp;
   }
-  pl.own_pages = (a->T + kPage - 1) / kPage - min_shared;
-  if (pl.own_pages < 0) pl.own_pages = 0;
+  const int own = (a->T + kPage - 1) / kPage - least;
   pl.own_kind = kind_for(LG);
   pl.own_blocks = (int)((LG + kind_rows(pl.own_kind) - 1) / kind_rows(pl.own_kind));
-  pl.own_ppw = 4;
-  if (pl.own_pages > 0) 
-    ranges((long)pl.own_pages * a->HKV * pl.own_blocks * a->B, pl.own_pages, pl.own_kind, pl.own_ppw, pl.own_slots);
+  if (own > 0) {
+    int ppw;  // of the longest sequence
+    page_ranges((long)own * a->HKV * pl.own_blocks * a->B, own, resident(pl.own_kind), ppw, pl.own_slots);
+  }
+  if (most > 0) {
+    pl.shared_kind = kind_for(rows);
+    const long kr = kind_rows(pl.shared_kind);
+    pl.shared_blocks = (int)((rows + kr - 1) / kr);
+    for (int g = 0; g < a->ngroups; ++g) {
+      const long n = a->group_start_host[g + 1] - a->group_start_host[g];
+      units += (long)a->group_pages_host[g] * a->HKV * ((n * LG + kr - 1) / kr);
+    }
+    long want = resident(pl.shared_kind);
+    // Both kinds in one launch: the shared pages get the share of the CUs that their work is of all, in us of a CU: a
+    // page of 256 rows 2.15, and 14 a workgroup; an own page of few rows 1.2.  64 sequences behind 32K tokens, own
+    // tokens up to 2000: 107 -> 86 us (two launches -> 56 %; 75 % 96), up to 8000 234 -> 197, 66 sequences of five groups
+    // 82 -> 74.  Own ranges too short for eight waves stay apart (256 sequences of 3 pages 91 -> 100).
+    const long pages = a->own_pages_host;
+    pl.both = pl.shared_kind == kRows256 && pl.own_kind <= kRows32 && own > 0 && pages >= 4l * a->B &&
+              (long)a->B * a->HKV * pl.own_slots < 1l << 30;
+    if (pl.both) {
+      const double many = 2.15 * units + 14. * cus, few = 1.2 * pages * a->HKV, share = many / (many + few);
+      want = (long)(want * (share < 0.4 ? 0.4 : share) + 0.5);
+    }
+    page_ranges(units, most, want, pl.shared_ppw, pl.shared_slots);
+    pl.both = pl.both && (long)a->HKV * pl.shared_blocks * pl.shared_slots * a->ngroups < 1l << 30;
+  }
   pl.nslots = pl.shared_slots + pl.own_slots;
   if (pl.shared_slots == 0 && pl.own_slots <= 1) {  // one range: no partials
     pl.own_slots = 1;
     pl.nslots = 0;
   }
   return pl;
-}
-
-template <int FMT, int RES, int VT>
-static void launch_attend(const AttendParams &p, int kind, int slots, int blocks, int sets, hipStream_t st) {
-  const dim3 few((unsigned)slots, (unsigned)(p.HKV * blocks), (unsigned)sets);
-  const dim3 wide((unsigned)(p.HKV * blocks), (unsigned)slots, (unsigned)sets);
-  switch (kind) {
-    case kRows16: hipLaunchKernelGGL((paged_attend_kernel<FMT, RES, VT, 1>), few, dim3(256), 0, st, p); break;
-    case kRows32: hipLaunchKernelGGL((paged_attend_kernel<FMT, RES, VT, 2>), few, dim3(256), 0, st, p); break;
-    case kRows64: hipLaunchKernelGGL((paged_attend_wide_kernel<FMT, RES, VT, 1, 4>), wide, dim3(256), 0, st, p); break;
-    case kRows128: hipLaunchKernelGGL((paged_attend_wide_kernel<FMT, RES, VT, 2, 4>), wide, dim3(256), 0, st, p); break;
-    default: hipLaunchKernelGGL((paged_attend_wide_kernel<FMT, RES, VT, 2, 8>), wide, dim3(512), 0, st, p);
-  }
-}
-
-template <int FMT>
-static void launch_attend_fmt(const AttendParams &p, int res, int vdt, int kind, int slots, int blocks, int sets,
-                              hipStream_t st) {
-#define FFA_CASE(RR, RC)                                                                \
-  if (res == RC) {                                                                      \
-    if (vdt == FFA_DT_BF16) launch_attend<FMT, RR, kVBF16>(p, kind, slots, blocks, sets, st);            \
-    else launch_attend<FMT, RR, kVF16>(p, kind, slots, blocks, sets, st);                                \
-  }
-  FFA_CASE(kResE4M3, FFA_DT_FP8_E4M3)
-  FFA_CASE(kResE5M2, FFA_DT_FP8_E5M2)
-  FFA_CASE(kResNone, FFA_DT_NONE)
-#undef FFA_CASE
 }
 
 static int attend_check(const ffa_paged_attend_args *a) {
@@ -1054,24 +231,27 @@ extern "C" int ffa_paged_attend(const ffa_paged_attend_args *a, void *stream) {
   p.shared_slots = pl.shared_slots;
   p.shared_ppw = pl.shared_ppw;
   p.own_slots = pl.own_slots;
-  p.own_ppw = pl.own_ppw;
   const hipStream_t st = (hipStream_t)stream;
-  auto launch = [&](int kind, int slots, int blocks, int sets) {
-    if (a->format == FFA_PAGES_Q2) launch_attend_fmt<kFmtQ2>(p, a->res_dtype, a->v_dtype, kind, slots, blocks, sets, st);
-    else if (a->format == FFA_PAGES_NVFP4) launch_attend_fmt<kFmtNvfp4>(p, a->res_dtype, a->v_dtype, kind, slots, blocks, sets, st);
-    else launch_attend_fmt<kFmtNf4>(p, a->res_dtype, a->v_dtype, kind, slots, blocks, sets, st);
+  auto launch = [&](int kind, int slots, int blocks, int sets, int own) {
+    const AttendLaunch l = {kind, slots, blocks, sets, own, a->res_dtype, a->v_dtype, st};
+    (a->format == FFA_PAGES_Q2 ? attend_q2 : (a->format == FFA_PAGES_NVFP4 ? attend_nvfp4 : attend_nf4))(p, l);
   };
-  if (pl.shared_slots > 0 && pl.own_slots > 0 && pl.shared_kind == pl.own_kind && a->ngroups + a->B <= 65535) {  // one launch
+  if (pl.both) {
     p.nshared = a->ngroups;
+    p.shared_blocks = pl.shared_blocks;
+    p.shared_wgs = a->HKV * pl.shared_blocks * pl.shared_slots * a->ngroups;
+    launch(pl.shared_kind, pl.shared_slots, pl.shared_blocks, a->ngroups, pl.own_kind);
+  } else if (pl.shared_slots > 0 && pl.own_slots > 0 && pl.shared_kind == pl.own_kind && a->ngroups + a->B <= 65535) {
+    p.nshared = a->ngroups;  // both in the grid of one kernel
     launch(pl.own_kind, pl.shared_slots > pl.own_slots ? pl.shared_slots : pl.own_slots,
-           pl.shared_blocks > pl.own_blocks ? pl.shared_blocks : pl.own_blocks, a->ngroups + a->B);
+           pl.shared_blocks > pl.own_blocks ? pl.shared_blocks : pl.own_blocks, a->ngroups + a->B, -1);
   } else {
     if (pl.shared_slots > 0) {
       p.nshared = a->ngroups;
-      launch(pl.shared_kind, pl.shared_slots, pl.shared_blocks, a->ngroups);
+      launch(pl.shared_kind, pl.shared_slots, pl.shared_blocks, a->ngroups, -1);
     }
     p.nshared = 0;
-    if (pl.own_slots > 0) launch(pl.own_kind, pl.own_slots, pl.own_blocks, a->B);
+    if (pl.own_slots > 0) launch(pl.own_kind, pl.own_slots, pl.own_blocks, a->B, -1);
   }
   if (pl.nslots > 0)
     hipLaunchKernelGGL(paged_attend_join_kernel, dim3((unsigned)rows), dim3(256), 0, st, p);

@@ -18,7 +18,8 @@ LIB_NAME = "libffa_mi355x.so"
 LIB_PATH = PKG_DIR / LIB_NAME
 
 SOURCES = ["q2fp8_decode.hip", "kfmt_decode.hip", "q2_quant.hip", "kfmt_quant.hip", "value_mean.hip",
-           "paged_attend.hip", "pages.hip"]
+           "paged_attend.hip", "paged_attend_q2.hip", "paged_attend_nvfp4.hip",
+           "paged_attend_nf4.hip", "pages.hip"]
 
 HIPCC_FLAGS = [
     "--offload-arch=gfx950",

@@ -484,7 +484,8 @@ typedef struct ffa_paged_attend_args {
   const int32_t *seq_group;   /* device, [B]: the group of each sequence */
   const int32_t *group_start_host;
   const int32_t *group_pages_host;
-  void *out; /* [B, L, HQ, 128] */
+  long own_pages_host; /* pages that all sequences hold past the shared ones, about: for the launch plan */
+  void *out;           /* [B, L, HQ, 128] */
   void *scratch;
   size_t scratch_bytes;
 } ffa_paged_attend_args;
