@@ -6,70 +6,75 @@ extern "C" int ffa_set_error_internal(int code, const char *msg);
 namespace ffa {
 
 // ---------------------------------------------------------------------------
-// Join of the partials: one workgroup per row; wave w adds the slots w, w + 4, ...
+// Join of the partials: WPR waves per row (4, or 1 where a row has few slots: a workgroup then takes four rows), each
+// with four slots' loads under way at a time
 // ---------------------------------------------------------------------------
-__global__ __launch_bounds__(256) void paged_attend_join_kernel(const AttendParams p) {
-  const int i = (blockIdx.x / p.HQ) % p.L, b = blockIdx.x / (p.HQ * p.L);
-  const size_t row = blockIdx.x;
+template <int WPR>
+__global__ __launch_bounds__(256) void paged_attend_join_kernel(const AttendParams p, int rows) {
   const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
-  __shared__ float s_m[4], s_l[4];
-  __shared__ float s_o[4][kD];
+  const int row = WPR == 4 ? blockIdx.x : 4 * blockIdx.x + wv;
+  if (row >= rows) return;  // (whole workgroups only where waves meet)
+  const int i = (row / p.HQ) % p.L, b = row / (p.HQ * p.L);
   const bool sees = row_limit(p, b, i) > 0;
   const int sp = shared_pages_of(p, b), own = max((seq_len_of(p, b) + kPage - 1) / kPage - sp, 0);
   const int na = p.shared_slots ? min((sp + p.shared_ppw - 1) / p.shared_ppw, p.shared_slots) : 0;
-  const int per = own_range(p, own), nb = p.own_slots ? min((own + per - 1) / per, p.own_slots) : 0;
-  const float2 *ml = (const float2 *)p.part_ml + row * p.nslots;
-  const float *po = p.part_o + row * p.nslots * kD;
+  int nb = 0;
+  if (p.own_slots) {
+    const int per = own_range(p, own);
+    nb = min((own + per - 1) / per, p.own_slots);
+  }
+  const float2 *ml = (const float2 *)p.part_ml + (size_t)row * p.nslots;
+  const float *po = p.part_o + (size_t)row * p.nslots * kD;
   float m = kNoMax, l = 0.f;
   float2 o = make_float2(0.f, 0.f);
   const int slots = sees ? na + nb : 0;
-  for (int s0 = wv; s0 < slots; s0 += 16) {  // four slots' loads at a time
+  for (int s0 = WPR == 4 ? wv : 0; s0 < slots; s0 += 4 * WPR) {
     float2 x[4], y[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int s = min(s0 + 4 * i, slots - 1), slot = s < na ? s : p.shared_slots + s - na;
-      x[i] = ml[slot];
-      y[i] = *(const float2 *)(po + (size_t)slot * kD + 2 * lane);
+    for (int k = 0; k < 4; ++k) {
+      const int s = min(s0 + WPR * k, slots - 1), slot = s < na ? s : p.shared_slots + s - na;
+      x[k] = ml[slot];
+      y[k] = *(const float2 *)(po + (size_t)slot * kD + 2 * lane);
     }
     float mn = m;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) mn = fmaxf(mn, x[i].x);
+    for (int k = 0; k < 4; ++k) mn = fmaxf(mn, x[k].x);
     const float fo = exp2_hw(m - mn);
     m = mn;
     l *= fo;
     o.x *= fo;
     o.y *= fo;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float f = s0 + 4 * i < slots ? exp2_hw(x[i].x - mn) : 0.f;
-      if (f != 0.f) {  // a slot read again, or far below the maximum, adds nothing
-        l += x[i].y * f;
-        o.x += y[i].x * f;
-        o.y += y[i].y * f;
+    for (int k = 0; k < 4; ++k)
+      if (s0 + WPR * k < slots) {
+        const float f = exp2_hw(x[k].x - mn);
+        l += x[k].y * f;
+        o.x += y[k].x * f;
+        o.y += y[k].y * f;
       }
+  }
+  if constexpr (WPR == 4) {
+    __shared__ float s_m[4], s_l[4];
+    __shared__ float s_o[4][kD];
+    if (lane == 0) {
+      s_m[wv] = m;
+      s_l[wv] = l;
     }
-  }
-  if (lane == 0) {
-    s_m[wv] = m;
-    s_l[wv] = l;
-  }
-  *(float2 *)&s_o[wv][2 * lane] = o;
-  __syncthreads();
-  if (wv == 0) {
-    const float M = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
-    float L = 0.f, x = 0.f, y = 0.f;
+    *(float2 *)&s_o[wv][2 * lane] = o;
+    __syncthreads();
+    if (wv != 0) return;
+    m = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
+    l = o.x = o.y = 0.f;
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
-      const float f = exp2_hw(s_m[w] - M);
-      L += s_l[w] * f;
-      x += s_o[w][2 * lane] * f;
-      y += s_o[w][2 * lane + 1] * f;
+      const float f = exp2_hw(s_m[w] - m);
+      l += s_l[w] * f;
+      o.x += s_o[w][2 * lane] * f;
+      o.y += s_o[w][2 * lane + 1] * f;
     }
-    const float inv = 1.f / L;
-    x = sees ? x * inv : 0.f;
-    y = sees ? y * inv : 0.f;
-    ((uint32_t *)p.out)[row * (kD / 2) + lane] = p.out_bf16 ? pk_bf16_bits(x, y) : pk_f16_bits(x, y);
   }
+  const float inv = 1.f / l, x = sees ? o.x * inv : 0.f, y = sees ? o.y * inv : 0.f;
+  ((uint32_t *)p.out)[(size_t)row * (kD / 2) + lane] = p.out_bf16 ? pk_bf16_bits(x, y) : pk_f16_bits(x, y);
 }
 
 // Launch plan of a call: page ranges of the shared and of the own pages
@@ -111,10 +116,16 @@ static AttendPlan attend_plan(const ffa_paged_attend_args *a, int cus) {
   }
   const int own = (a->T + kPage - 1) / kPage - least;
   pl.own_kind = kind_for(LG);
+  auto workgroups = [&](int kind) { return (LG + kind_rows(kind) - 1) / kind_rows(kind) * a->HKV * a->B; };
+  // Over few pages a workgroup's fixed 10-14 us count as much as its pages': smaller ones then, and ranges that are
+  // split (their partials are rows x 528 bytes, written and read) only where the chip is not half full
+  const bool brief = pl.own_kind > kRows64 && own < 48;
+  if (brief) pl.own_kind = workgroups(kRows128) > cus ? kRows128 : kRows64;
   pl.own_blocks = (int)((LG + kind_rows(pl.own_kind) - 1) / kind_rows(pl.own_kind));
   if (own > 0) {
     int ppw;  // of the longest sequence
     page_ranges((long)own * a->HKV * pl.own_blocks * a->B, own, resident(pl.own_kind), ppw, pl.own_slots);
+    if (brief && 2 * workgroups(pl.own_kind) >= cus) pl.own_slots = 1;
   }
   if (most > 0) {
     pl.shared_kind = kind_for(rows);
@@ -253,8 +264,10 @@ extern "C" int ffa_paged_attend(const ffa_paged_attend_args *a, void *stream) {
     p.nshared = 0;
     if (pl.own_slots > 0) launch(pl.own_kind, pl.own_slots, pl.own_blocks, a->B, -1);
   }
-  if (pl.nslots > 0)
-    hipLaunchKernelGGL(paged_attend_join_kernel, dim3((unsigned)rows), dim3(256), 0, st, p);
+  if (pl.nslots > 16 || (pl.nslots > 0 && rows < 8192))  // few rows: four waves each
+    hipLaunchKernelGGL(paged_attend_join_kernel<4>, dim3((unsigned)rows), dim3(256), 0, st, p, (int)rows);
+  else if (pl.nslots > 0)
+    hipLaunchKernelGGL(paged_attend_join_kernel<1>, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, p, (int)rows);
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? FFA_OK : ffa_set_error_internal(FFA_E_LAUNCH, hipGetErrorString(e));
 }

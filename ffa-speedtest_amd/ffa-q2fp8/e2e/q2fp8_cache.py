@@ -21,13 +21,18 @@ Here, for q2fp8, on the MI355X library:
   outside `pattern_layers` or with `use_ffa_decode=False` -- runs exact causal attention over the
   cache's own keys and values dequantized by `ffa_q2_paged_dequant` (the reference attends with
   FlashAttention to the keys its cache returns dequantized from every update, fp8fp8_cache.py:60-69,
-  84-89).  The exact attention itself is fp32 torch matmuls, as the reference's is a library call.
+  84-89).  The exact attention itself is fp32 torch matmuls, as the reference's is a library call; with
+  `paged_exact=True` those steps of fp16 / bf16 models run `PagedQ2Cache.attend` instead, which reads the
+  quantized pages themselves, and the pages that sequences share once.
+* Batch operations of transformers' caches (`batch_repeat_interleave`: samples of a prompt,
+  `batch_select_indices`, `reorder_cache`: beams, `crop`) fork and free pages (`ffa_mi355x.pages`) instead of
+  copying caches: whole pages are shared, partial last pages copied.
 
 The HF models apply RoPE (their half-split `rotate_half`) before `Cache.update`, so the cache receives
 rotated K and appends it with the quantize-append entry point; the fused K-projection + RoPE producer
 follows the reference producer's interleaved-pair RoPE instead and serves the benchmark path.
 
-Limits: all sequences of a batch have the same length (no padding), no beam search reordering.
+Limits: all sequences of a batch have the same length (no padding).
 """
 from __future__ import annotations
 
@@ -42,13 +47,16 @@ from transformers import AttentionInterface
 from transformers.cache_utils import Cache, CacheLayerMixin
 
 sys.path.insert(0, str(Path(__file__).resolve().parents[2]))  # ffa-speedtest_amd/
+from ffa_mi355x.attend import SharedPrefix  # noqa: E402
 from ffa_mi355x.decode import DecodeWorkspace  # noqa: E402
 from ffa_mi355x.paged import PAGE, PagedQ2Cache  # noqa: E402
+from ffa_mi355x.pages import PagePool  # noqa: E402
 
 __all__ = ["Q2FP8Cache", "Q2FP8PagedLayer", "ffa_q2fp8_attention", "enable_ffa_q2fp8"]
 
 ATTN_NAME = "ffa_q2fp8"
-DEFAULT_SETTINGS = dict(use_ffa_decode=True, BS=64, SBS=64, delta=5.0, use_fp8_residual=True, pattern_layers=None)
+DEFAULT_SETTINGS = dict(use_ffa_decode=True, BS=64, SBS=64, delta=5.0, use_fp8_residual=True, pattern_layers=None,
+                        paged_exact=False)
 # (layer index, layer) of the update() that ran last on this thread; the attention of that layer
 # takes it (and clears it), so a model run without a Q2FP8Cache cannot pick up a stale layer
 _current = threading.local()
@@ -70,6 +78,8 @@ class Q2FP8PagedLayer(CacheLayerMixin):
         self.seq_lens: Optional[torch.Tensor] = None
         self.seq_len = 0
         self._workspace: Optional[DecodeWorkspace] = None
+        self.pages: Optional[PagePool] = None  # from the first batch operation on: pages are shared and counted
+        self.shared: Optional[SharedPrefix] = None
 
     @property
     def capacity(self) -> int:
@@ -102,6 +112,8 @@ class Q2FP8PagedLayer(CacheLayerMixin):
         if self.seq_len + Tn > self.capacity:
             raise ValueError(f"cache holds {self.capacity} tokens, {self.seq_len + Tn} requested")
         pos = torch.full((B,), self.seq_len, dtype=torch.int32, device=self.device)
+        if self.pages is not None and -(-(self.seq_len + Tn) // PAGE) > -(-self.seq_len // PAGE):
+            self.pages.extend(self.block_table, self.seq_lens, Tn)
         self.pool.append(key_states.transpose(1, 2).contiguous(), value_states.transpose(1, 2).contiguous(), pos,
                          self.block_table)
         self.seq_len += Tn
@@ -127,11 +139,76 @@ class Q2FP8PagedLayer(CacheLayerMixin):
 
     def reset(self) -> None:
         self.seq_len = 0
+        self.shared = None
         if self.seq_lens is not None:
             self.seq_lens.zero_()
+        if self.pages is not None:
+            self.pages.refs.zero_()
+            self.block_table.fill_(-1)
+
+    # ------------------------------------------------------------------ batch operations
+    def _count_pages(self) -> PagePool:
+        """From fixed rows of pages to counted ones, in a pool that holds max_batch_size whole sequences and the copies
+        of their last pages that a fork makes before the parents go."""
+        if self.pages is None:
+            old, npg = self.pool, self.block_table.shape[1]
+            self.pool = PagedQ2Cache(self.max_batch_size * (npg + 1), old.HKV, self.device, res_dtype=old.res_dtype,
+                                     v_dtype=old.v_dtype)
+            for new, t in zip(self.pool.pools(), old.pools()):
+                new[: old.P].view(torch.uint8).copy_(t.view(torch.uint8))
+            self.block_table[:, -(-self.seq_len // PAGE):] = -1
+            self.pages = PagePool([self.pool])
+            self.pages.hold(self.block_table, self.seq_lens)
+        return self.pages
+
+    def _select(self, indices: torch.Tensor, check: bool) -> None:
+        if not self.is_initialized:
+            return
+        n = int(indices.numel())
+        if n > self.max_batch_size:
+            raise ValueError(f"batch {n} exceeds max_batch_size {self.max_batch_size}")
+        pages = self._count_pages()
+        child = pages.fork(self.block_table, self.seq_lens, indices.reshape(-1), check=check)
+        pages.free(self.block_table, self.seq_lens, check=check)
+        self.block_table = child
+        self.seq_lens = torch.full((n,), self.seq_len, dtype=torch.int32, device=self.device)
+        self.shared = None
+
+    def batch_repeat_interleave(self, repeats: int) -> None:
+        """Every sequence `repeats` times (samples of a prompt); the copies share its whole pages."""
+        if self.is_initialized:
+            self._select(torch.arange(self.block_table.shape[0]).repeat_interleave(repeats), True)
+            self.shared = SharedPrefix(self.block_table, self.seq_lens)
+
+    def batch_select_indices(self, indices: torch.Tensor) -> None:
+        """Sequences `indices` (a boolean mask or indices, from the end where negative) in this order."""
+        if self.is_initialized:
+            rows = torch.arange(self.block_table.shape[0])[indices.cpu()]
+            self._select(rows, True)
+            self.shared = SharedPrefix(self.block_table, self.seq_lens)
 
     def reorder_cache(self, beam_idx: torch.LongTensor) -> None:
-        raise NotImplementedError("beam search reordering is not supported by the paged q2fp8 cache")
+        """Beam search: beam i continues beam beam_idx[i] (within the batch).  Does not synchronise."""
+        self._select(beam_idx, False)
+
+    def crop(self, tokens_to_remove: int) -> None:
+        """Remove the newest -tokens_to_remove tokens (or, where positive, those past that length)."""
+        if not self.is_initialized or tokens_to_remove == 0:
+            return
+        length = min(tokens_to_remove, self.seq_len) if tokens_to_remove > 0 else max(self.seq_len + tokens_to_remove, 0)
+        first, end = -(-length // PAGE), -(-self.seq_len // PAGE)
+        if self.pages is not None and first < end:
+            tail = self.block_table[:, first:end].contiguous()
+            self.pages.free(tail, torch.full_like(self.seq_lens, tail.shape[1] * PAGE))
+            self.block_table[:, first:end] = -1
+        cut = length < self.seq_len
+        self.seq_len = length
+        self.seq_lens.fill_(length)
+        if self.pages is not None and cut and length % PAGE:
+            # the last page may be one that others share: tokens are appended to a copy
+            shared = self.shared
+            self._select(torch.arange(self.block_table.shape[0]), True)
+            self.shared = shared and SharedPrefix(self.block_table, self.seq_lens, group_sizes=shared.sizes)
 
     def offload(self):
         raise NotImplementedError("offloading is not supported by the paged q2fp8 cache")
@@ -178,7 +255,7 @@ def ffa_q2fp8_attention(module, query: torch.Tensor, key: torch.Tensor, value: t
 
     L == 1 with use_ffa_decode and the layer in pattern_layers: the pruned q2fp8 decode over the
     layer's paged cache (modeling_llama.py:293-321's branch); otherwise exact causal attention over
-    the cache's dequantized keys and values (:322-337)."""
+    the cache's keys and values (:322-337), dequantized, or with paged_exact as they lie in the pages."""
     settings = dict(DEFAULT_SETTINGS)
     settings.update(getattr(module.config, "attn_settings", None) or {})
     entry = getattr(_current, "entry", None)
@@ -204,7 +281,11 @@ def ffa_q2fp8_attention(module, query: torch.Tensor, key: torch.Tensor, value: t
         if hook is not None:
             hook(layer_idx, query[:, :, 0, :], out[:, 0], layer)
         return out, None
-    out = exact_attention(query, layer, scale)
+    if settings["paged_exact"] and query.dtype in (torch.float16, torch.bfloat16):
+        out = layer.pool.attend(query.transpose(1, 2).contiguous(), layer.block_table, layer.seq_lens, T=layer.seq_len,
+                                scale=scale, shared=layer.shared)
+    else:
+        out = exact_attention(query, layer, scale)
     hook = settings.get("on_exact")
     if hook is not None:
         hook(layer_idx, query, out, layer)
@@ -213,7 +294,7 @@ def ffa_q2fp8_attention(module, query: torch.Tensor, key: torch.Tensor, value: t
 
 def enable_ffa_q2fp8(model, **attn_settings: Any) -> None:
     """Route the model's attention through ffa_q2fp8_attention (registered once) with these settings
-    (BS, SBS, delta, use_fp8_residual, use_ffa_decode, pattern_layers; optional
+    (BS, SBS, delta, use_fp8_residual, use_ffa_decode, pattern_layers, paged_exact; optional
     on_decode(layer_idx, q, o, cache_layer) and on_exact(layer_idx, q, o, cache_layer) observers)."""
     AttentionInterface.register(ATTN_NAME, ffa_q2fp8_attention)
     cfg = model.config
