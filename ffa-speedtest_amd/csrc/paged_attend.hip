@@ -145,7 +145,7 @@ static AttendPlan attend_plan(const ffa_paged_attend_args *a, int cus) {
               (long)a->B * a->HKV * pl.own_slots < 1l << 30;
     if (pl.both) {
       const double many = 2.15 * units + 14. * cus, few = 1.2 * pages * a->HKV, share = many / (many + few);
-      want = (long)(want * (share < 0.4 ? 0.4 : share) + 0.5);
+      want = (long)(want * (share < 0.4 ? 0.4 : share)) + 1;
     }
     page_ranges(units, most, want, pl.shared_ppw, pl.shared_slots);
     pl.both = pl.both && (long)a->HKV * pl.shared_blocks * pl.shared_slots * a->ngroups < 1l << 30;
@@ -164,7 +164,7 @@ static int attend_check(const ffa_paged_attend_args *a) {
   if (!a) FFA_BAD("null args");
   if (a->B <= 0 || a->T <= 0 || a->L <= 0 || a->HQ <= 0 || a->HKV <= 0) FFA_BAD("bad dims");
   if (a->HQ % a->HKV) FFA_BAD("HQ must be a multiple of HKV");
-  if (a->B > 65535) FFA_NO("B is a grid dimension");
+  if (a->B > 65535 || a->HKV > 65535) FFA_NO("B and HKV are grid dimensions");
   if (a->T > 1 << 30) FFA_NO("T above 2^30 tokens");
   if (!(a->q_dtype == FFA_DT_F16 || a->q_dtype == FFA_DT_BF16)) FFA_BAD("q must be fp16 or bf16");
   if (!(a->v_dtype == FFA_DT_F16 || a->v_dtype == FFA_DT_BF16)) FFA_BAD("v dtype");
@@ -176,7 +176,7 @@ static int attend_check(const ffa_paged_attend_args *a) {
   if (!a->q || !a->k || !a->k_scale || !a->v || !a->block_table || !a->out) FFA_BAD("null pointer");
   if (a->format == FFA_PAGES_Q2 && !a->k_zero) FFA_BAD("2-bit pages need k_zero");
   if (a->res_dtype != FFA_DT_NONE && !a->k_residual) FFA_BAD("null residual");
-  if ((long)a->B * a->L * a->HQ > 0x7fffffffl) FFA_NO("more than 2^31 - 1 query rows");
+  if ((long)a->B * a->L * a->HQ > 1l << 30) FFA_NO("more than 2^30 query rows");
   if (a->ngroups < 0 || a->ngroups > a->B) FFA_BAD("ngroups must be within [0, B]");
   if (a->ngroups > 0) {
     if (!a->group_start || !a->group_pages || !a->seq_group || !a->group_start_host || !a->group_pages_host)
@@ -210,7 +210,6 @@ extern "C" int ffa_paged_attend(const ffa_paged_attend_args *a, void *stream) {
   if (a->scratch_bytes < rows * pl.nslots * (kD + 2) * sizeof(float) || (pl.nslots && !a->scratch))
     FFA_BAD("scratch below ffa_paged_attend_scratch()");
   if ((uintptr_t)a->scratch & 15) FFA_BAD("scratch must be a multiple of 16 bytes");
-  if ((long)pl.own_blocks * a->HKV > 65535 || (long)pl.shared_blocks * a->HKV > 65535) FFA_NO("more than 65535 row blocks");
   AttendParams p = {};
   p.q = a->q;
   p.k = a->k;

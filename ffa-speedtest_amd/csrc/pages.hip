@@ -413,6 +413,7 @@ extern "C" int ffa_pages_extend(const ffa_pages *pg, int32_t *block_table, int b
   bad = table_check(block_table, bt_stride, rows, seq_lens, errors);
   if (bad != FFA_OK) return bad;
   if (tokens < 0 || !scratch) FFA_BAD("extend needs a number of tokens and scratch");
+  if (ffa_pages_alloc_scratch(rows, tokens) > (size_t)1 << 30) FFA_NO("more than 2^30 pages in a call");
   const ffa::AllocArgs a = {pg->refs, block_table, nullptr, seq_lens, nullptr, scratch, errors,
                             pg->num_pages, rows, bt_stride, rows, tokens};
   hipLaunchKernelGGL(ffa::pages_alloc_kernel, dim3(1), dim3(1024), 0, (hipStream_t)stream, a);

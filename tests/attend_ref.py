@@ -66,8 +66,9 @@ def _logical_kv(cache, fmt, pages, residual):
     return k, v
 
 
-def reference(q, k, v, T, ql, scale):
+def reference(q, k, v, T, ql, scale, tokens=None):
     """q [L, HQ, 128] (torch), k, v [>= T, HKV, 128] f64 -> (o, bound) [L, HQ, 128] f64; rows past ql are zeros.
+    tokens: the query tokens to compute (default all; the others stay zeros).
 
     bound, by element, in units of the operands' arithmetic: each k is rounded once to fp16 (2^-11 relative, or
     2^-25 of the smallest normal), so a score is off by at most d = scale sum_c |q_c k_c| (2^-11 + 2^-17), the second
@@ -78,7 +79,7 @@ def reference(q, k, v, T, ql, scale):
     o = np.zeros((L, HQ, 128))
     bound = np.zeros((L, HQ, 128))
     qf = q.double().cpu().numpy()
-    for i in range(min(ql, L)):
+    for i in range(min(ql, L)) if tokens is None else tokens:
         n = T - ql + i + 1
         if n <= 0:
             continue

@@ -63,7 +63,7 @@ def test_c_entry_refuses(kw):
     assert rc == -1, N.lib().ffa_last_error()
 
 
-@pytest.mark.parametrize("kw", [dict(B=65536), dict(T=(1 << 30) + 64, bt_stride=1 << 25), dict(L=1 << 29, HQ=8)])
+@pytest.mark.parametrize("kw", [dict(B=65536), dict(HKV=65536, HQ=65536), dict(T=(1 << 30) + 64, bt_stride=1 << 25), dict(L=1 << 29, HQ=8)])
 def test_c_entry_unsupported(kw):
     a = _args(**kw)
     assert N.lib().ffa_paged_attend(ctypes.byref(a), None) == -2

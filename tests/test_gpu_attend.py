@@ -205,6 +205,59 @@ def test_shared_prefix(gpu, fmt, sizes, prefix, HQ, HKV, L):
     _check(cache, fmt, table, lens, q, out)
 
 
+@pytest.mark.parametrize("fmt,v", [("q2", torch.float16), ("nvfp4", torch.bfloat16), ("nf4", torch.float16)])
+@pytest.mark.parametrize("sizes,prefix,HQ,HKV,L", [
+    ([40], [700], 8, 1, 1),            # 320 rows over two workgroups, 8 own rows
+    ([17, 3, 30], [900, 64, 320], 16, 2, 3),  # uneven groups, drafts: 24 own rows; one group's rows fill a part
+])
+def test_shared_and_own_pages_in_one_launch(gpu, fmt, v, sizes, prefix, HQ, HKV, L):
+    """Own parts of several pages: both kinds of workgroup in one grid; some sequences end before the others' ranges."""
+    own = [L + (211 * b) % 700 for b in range(sum(sizes))]
+    cache, table, lens, sl, q = _forked(fmt, sizes, prefix, own, HQ, HKV, L, torch.bfloat16, 61, gpu, v=v)
+    plan = SharedPrefix(table, sl, group_sizes=sizes)
+    out = cache.attend(q, table, sl, shared=plan)
+    some = range(0, sum(sizes), 5)
+    _check(cache, fmt, table[list(some)], [lens[b] for b in some], q[list(some)], out[list(some)])
+    # without the plan, and with a capacity for T: other ranges of the same sums
+    for other in (cache.attend(q, table, sl), cache.attend(q, table, sl, T=64 * table.shape[1], shared=plan)):
+        assert torch.allclose(out.float(), other.float(), atol=2.0 ** -6, rtol=2.0 ** -7)
+
+
+@pytest.mark.parametrize("n,L,HQ,HKV", [
+    (3300, 150, 8, 2),    # 600 rows over 52 pages: 256-row workgroups, split ranges
+    (3200, 140, 64, 4),   # 8960 rows: the join by a wave per row
+    (1500, 300, 32, 4),   # few pages, many rows: smaller workgroups, ranges not split
+    (700, 100, 4, 4),     # 100 rows of each head: a workgroup's waves with two tiles, one and none
+])
+def test_chunks(gpu, n, L, HQ, HKV):
+    cache, table, sl, q = _batch("q2", [n], HQ, HKV, L, torch.float16, 67, gpu)
+    out = cache.attend(q, table, sl)
+    k, v = logical_kv(cache, "q2", table[0, :-(-n // 64)].tolist())
+    tokens = sorted({0, 1, 63, L // 2, L - 64, L - 2, L - 1} & set(range(L)))
+    o, bound = reference(q[0], k[:n], v[:n], n, L, SCALE, tokens)
+    assert_close(out[0, tokens], o[tokens], bound[tokens], q.dtype)
+    for i in range(0, L, 7):  # every part of the chunk against the same rows as short chunks of their own
+        part = cache.attend(q[:, i:i + 7].contiguous(), table, torch.tensor([n - L + min(i + 7, L)], device=gpu))
+        assert torch.allclose(part.float(), out[:, i:i + 7].float(), atol=2.0 ** -8, rtol=2.0 ** -8)
+
+
+def test_hidden_infinities_of_long_chunks(gpu):
+    """The same as test_hidden_infinities where 256 rows are a workgroup's and the ranges are split."""
+    n, L, HQ = 3200, 200, 4
+    cache, table, sl, q = _batch("nvfp4", [n], HQ, 1, L, torch.bfloat16, 71, gpu, v=torch.bfloat16)
+    v, k = torch.randn((3, 1, 128)), torch.randn((3, 1, 128))
+    v[0, 0, 5], v[1, 0, 7], v[2, 0, 9] = float("inf"), float("nan"), 3e38  # beyond the fp16 operand: an infinity
+    fill(cache, k, v, table[0], n - 100)
+    out = cache.attend(q, table, sl)[0].float()
+    first = L - 100  # the first query token that sees token n - 100
+    assert torch.isfinite(out[:first]).all()
+    assert torch.isinf(out[first:, :, 5]).all() and torch.isfinite(out[first, :, 7]).all()
+    assert torch.isnan(out[first + 1:, :, 7]).all() and torch.isfinite(out[first + 1, :, 9]).all()
+    assert torch.isinf(out[first + 2:, :, 9]).all()
+    rest = [c for c in range(128) if c not in (5, 7, 9)]
+    assert torch.isfinite(out[..., rest]).all()
+
+
 def test_shared_whole_pages_and_drafts(gpu):
     """Sequences of shared pages only: drafted tokens inside the shared pages, causal there."""
     cache, table, lens, sl, q = _forked("q2", [3], [128], [0, 0, 0], 8, 2, 4, torch.float16, 29, gpu)

@@ -52,6 +52,7 @@ def test_calls_refused():
     assert L.ffa_pages_fork(p, X, 4, 1, X, None, 1, 2 * X, X, X, None) == -1
     assert L.ffa_pages_fork(p, X, 4, 1, X, X, 1, X, X, X, None) == -1  # children into the parents' table
     assert L.ffa_pages_extend(p, X, 4, 1, X, -1, X, X, None) == -1
+    assert L.ffa_pages_extend(p, X, 1 << 24, 65535, X, 1 << 30, X, X, None) == -2  # more pages than the ranks count
     assert L.ffa_pages_count(p, X, 4, 1, X, 2, X, X, None) == -1
     assert L.ffa_pages_count(p, X, 4, 1, X, 1, None, X, None) == -1
     assert L.ffa_pages_compact(p, None, None, 1, X, None) == -1
