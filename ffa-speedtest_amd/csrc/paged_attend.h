@@ -590,15 +590,24 @@ struct ManyLds {
   int hi[W], lo[W], bad;
 };
 template <int FMT, int RES, int VT, int NT, int W>
-__device__ __forceinline__ void many_rows(const AttendParams &p, int split, int hkv, int rb, int z, ManyLds<FMT, W> &s) {
+__device__ __forceinline__ void many_rows(const AttendParams &p, int split, int hkv, int nth, int z, ManyLds<FMT, W> &s) {
   constexpr int kUnits = 8 / W, kVPieces = 16 / W;  // of a page, per wave
   const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, n = lane & 15;
   const AttendSet set = attend_set(p, z, split);
   // the set's row tiles over as few workgroups as hold them, evenly, and a workgroup's over its waves in turn
   const int LG = p.L * p.G, R = set.n * LG, tiles = (R + 15) / 16, blocks = (tiles + W * NT - 1) / (W * NT);
-  if (rb >= blocks) return;
-  const int per = (tiles + blocks - 1) / blocks, tile0 = rb * per + wv, tile_end = min((rb + 1) * per, tiles);
+  if (nth >= blocks) return;
+  const int per = (tiles + blocks - 1) / blocks;
+  // the set's nth workgroup: of one sequence's rows the last first, which see the most keys of a causal chunk; those
+  // past its q_lens, which see none, behind them
+  int rb = nth;
+  if (set.n == 1) {
+    const int ql = p.q_lens ? min(max(p.q_lens[set.b0], 0), p.L) : p.L;
+    const int live = ((ql * p.G + 15) / 16 + per - 1) / per;
+    if (nth < live) rb = live - 1 - nth;
+  }
+  const int tile0 = rb * per + wv, tile_end = min((rb + 1) * per, tiles);
   const int pa = set.p0;
   int pe = set.p1;
   if (pa >= pe && p.nslots != 0) return;
@@ -838,8 +847,10 @@ template <int FMT, int RES, int VT, int NT, int W>
 __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2))) void paged_attend_wide_kernel(
     const AttendParams p) {
   __shared__ ManyLds<FMT, W> s;
-  const int nb = gridDim.x / p.HKV;  // the last rows, which see the most keys of a causal chunk, first
-  many_rows<FMT, RES, VT, NT, W>(p, blockIdx.y, blockIdx.x % p.HKV, nb - 1 - blockIdx.x / p.HKV, blockIdx.z, s);
+  // KV head fastest (a head's workgroups, which read the same pages, on one XCD where heads are a multiple of 8), a set
+  // after the other (interleaved, batches of prompts took 0.85 to 1.3 of the time: 4 x 512 tokens 33 -> 28 us, 8 ragged
+  // ones of up to 2048 180 -> 226)
+  many_rows<FMT, RES, VT, NT, W>(p, blockIdx.y, blockIdx.x % p.HKV, blockIdx.x / p.HKV, blockIdx.z, s);
 }
 
 // Shared pages for many rows (256 a workgroup) and own pages for few (up to 16 NT), one launch: the first kind is
@@ -854,8 +865,8 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) void p
   } s;
   int x = blockIdx.x;
   if (x < p.shared_wgs) {
-    const int hkv = x % p.HKV, y = x / p.HKV, rb = y % p.shared_blocks, w = y / p.shared_blocks;
-    many_rows<FMT, RES, VT, 2, 8>(p, w % p.shared_slots, hkv, rb, w / p.shared_slots, s.many);
+    const int hkv = x % p.HKV, y = x / p.HKV, w = y / p.shared_blocks;
+    many_rows<FMT, RES, VT, 2, 8>(p, w % p.shared_slots, hkv, y % p.shared_blocks, w / p.shared_slots, s.many);
   } else {
     x -= p.shared_wgs;
     const int split = x % p.own_slots, y = x / p.own_slots;
