@@ -84,8 +84,9 @@ def append_rows(v: torch.Tensor, v_dtype: torch.dtype) -> torch.Tensor:
     return v.contiguous()
 
 
-def check_append_fits(pos: torch.Tensor, Tn: int, block_table: torch.Tensor, num_pages: int) -> None:
-    """Host-side bounds check of an append (positions and page ids must stay inside the table / pool)."""
+def check_append_fits(pos: torch.Tensor, Tn: int, block_table: torch.Tensor, num_pages: int, ragged: bool = False) -> None:
+    """Host-side bounds check of an append (positions and page ids must stay inside the table / pool): every row's
+    pages up to the batch's last position, or with ragged up to the row's own (PagePool's tables hold -1 past it)."""
     if block_table.shape[0] != pos.shape[0]:
         raise ValueError("block_table must have one row per sequence")
     if 0 < block_table.numel() <= _CHECK_ON_HOST and pos.device == block_table.device:
@@ -100,11 +101,12 @@ def check_append_fits(pos: torch.Tensor, Tn: int, block_table: torch.Tensor, num
         raise ValueError("append positions exceed the block table")
     used = table[:, : last // PAGE + 1]
     if int(used.min().item()) < 0 or int(used.max().item()) >= num_pages:
-        # rows of a ragged batch hold no pages past their own last position (PagePool leaves -1 there)
-        used, pos = torch.as_tensor(used).cpu(), pos.reshape(-1, 1).cpu()
-        used = used[torch.arange(used.shape[1]) <= (pos + (Tn - 1)) // PAGE]
-        if int(used.min()) < 0 or int(used.max()) >= num_pages:
-            raise ValueError("block table references pages outside the pool")
+        if ragged:
+            used, pos = torch.as_tensor(used).cpu(), pos.reshape(-1, 1).cpu()
+            used = used[torch.arange(used.shape[1]) <= (pos + (Tn - 1)) // PAGE]
+            if int(used.min()) >= 0 and int(used.max()) < num_pages:
+                return
+        raise ValueError("block table references pages outside the pool")
 
 
 class PagedQ2Cache:
@@ -127,8 +129,10 @@ class PagedQ2Cache:
         return [self.k_q, self.k_scale, self.k_zero, self.k_res, self.v]
 
     # ------------------------------------------------------------------ writes
-    def append(self, k: torch.Tensor, v: torch.Tensor | None, pos: torch.Tensor, block_table: torch.Tensor):
-        """g32-quantize k [B, Tn, HKV, 128] and write it (and v) at positions pos[b] + n."""
+    def append(self, k: torch.Tensor, v: torch.Tensor | None, pos: torch.Tensor, block_table: torch.Tensor,
+               ragged: bool = False):
+        """g32-quantize k [B, Tn, HKV, 128] and write it (and v) at positions pos[b] + n.  ragged: rows of the table hold
+        no pages past their own last position (as PagePool leaves them)."""
         B, Tn, HKV, D = k.shape
         if HKV != self.HKV or D != HEAD_DIM:
             raise ValueError("k shape does not match the cache")
@@ -141,7 +145,7 @@ class PagedQ2Cache:
             v_from, v_to = N.dtype_code(v.dtype), N.dtype_code(self.v_dtype)
         pos = pos.to(torch.int32).contiguous()
         block_table = block_table.to(torch.int32).contiguous()
-        check_append_fits(pos, Tn, block_table, self.P)
+        check_append_fits(pos, Tn, block_table, self.P, ragged)
         rc = N.lib().ffa_q2_quantize_g32_append_cast(
             k.data_ptr(), N.dtype_code(k.dtype), B, Tn, HKV, pos.data_ptr(), block_table.data_ptr(),
             block_table.shape[1], self.P, self.k_q.data_ptr(), self.k_scale.data_ptr(), self.k_zero.data_ptr(),

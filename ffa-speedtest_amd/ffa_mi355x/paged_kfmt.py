@@ -105,8 +105,10 @@ class PagedKfmtCache:
         """The pools, one page of each per page id."""
         return [self.k, self.k_scale, self.k_res, self.v]
 
-    def append(self, k: torch.Tensor, v: torch.Tensor | None, pos: torch.Tensor, block_table: torch.Tensor):
-        """Quantize k [B, Tn, HKV, 128] and write it (and v) at positions pos[b] + n."""
+    def append(self, k: torch.Tensor, v: torch.Tensor | None, pos: torch.Tensor, block_table: torch.Tensor,
+               ragged: bool = False):
+        """Quantize k [B, Tn, HKV, 128] and write it (and v) at positions pos[b] + n.  ragged: rows of the table hold no
+        pages past their own last position (as PagePool leaves them)."""
         B, Tn, HKV, D = k.shape
         if HKV != self.HKV or D != HEAD_DIM:
             raise ValueError("k shape does not match the cache")
@@ -119,7 +121,7 @@ class PagedKfmtCache:
             v_from, v_to = N.dtype_code(v.dtype), N.dtype_code(self.v_dtype)
         pos = pos.to(device=k.device, dtype=torch.int32).contiguous()
         block_table = block_table.to(device=k.device, dtype=torch.int32).contiguous()
-        check_append_fits(pos, Tn, block_table, self.P)
+        check_append_fits(pos, Tn, block_table, self.P, ragged)
         fn = N.lib().ffa_nvfp4_g16_append_cast if self.fmt == "nvfp4" else N.lib().ffa_nf4_g64_append_cast
         rc = fn(k.data_ptr(), N.dtype_code(k.dtype), B, Tn, HKV, pos.data_ptr(), block_table.data_ptr(),
                 block_table.shape[1], self.P, self.k.data_ptr(), self.k_scale.data_ptr(), self.k_res.data_ptr(),

@@ -6,7 +6,7 @@ page.  Forked sequences share whole pages and own a copy of the last partial one
 that another sequence holds:
 
     pool = PagePool([layer0_cache, layer1_cache, ...])
-    pool.extend(table, lens, 900)            # pages for a prompt; append its K and V to every layer
+    pool.extend(table, lens, 900)            # pages for prompts; append(..., ragged=True) fills every layer's
     children = pool.fork(table, lens, parents)   # samples, beams
     pool.free(table, lens)
     pool.extend(children, child_lens, 64)

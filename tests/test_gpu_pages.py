@@ -338,7 +338,7 @@ def test_samples_of_prompts(gpu, fmt):
         pool.extend(child, clens, n)
         for cache in layers:
             cache.append(torch.randn((6, n, HKV, 128), generator=g).to(gpu), torch.randn((6, n, HKV, 128), generator=g).to(gpu),
-                         clens, child)
+                         clens, child, ragged=True)
         clens = clens + n
         q = torch.randn((6, min(n, 5), HQ, 128), generator=g).to(torch.bfloat16).to(gpu)
         outs = [cache.attend(q, child, clens, shared=plan) for cache in layers]
