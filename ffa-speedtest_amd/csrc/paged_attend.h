@@ -311,8 +311,8 @@ __device__ __forceinline__ void add_not_finite(const uint8_t *v, int g, int nvis
 
 // ---------------------------------------------------------------------------
 // The softmax step of one row tile over one page: scores to P operands, m and l of lane (g, n)'s row n
-// (l: the lane's own tokens only, summed over g at the end).  MASK: tokens at or past lim (relative to the page) do
-// not count.  Returns the factor that the row's O so far is to be multiplied by (1 where m stands).
+// (l: the lane's own tokens only, summed over g at the end).  MASK: only the page's first nvis tokens count.  Returns
+// whether a maximum of the wave moved; alpha is then the factor of the row's O so far (1 where its m stands).
 // ---------------------------------------------------------------------------
 template <bool MASK>
 __device__ __forceinline__ bool softmax_step(f32x4 *S, float cs, int nvis, int g, float &m, float &l, float &alpha,
@@ -376,8 +376,8 @@ __device__ __forceinline__ void store_row4(const AttendParams &p, size_t row, in
 }
 
 // ---------------------------------------------------------------------------
-// Few rows (up to 16 NT of a KV head and set per workgroup): each wave takes every fourth page of the range with all
-// rows, its operands straight from memory; the waves' results are joined in LDS.
+// Few rows (up to 16 NT of a KV head and set per workgroup): each of the W waves takes every Wth page of the range
+// with all rows, its operands straight from memory; the waves' results are joined in LDS.
 // ---------------------------------------------------------------------------
 template <int FMT, int NT, int W>
 struct FewLds {

@@ -86,6 +86,15 @@ def _on(device: torch.device):
     return nullcontext() if device.index in (None, torch.cuda.current_device()) else torch.cuda.device(device)
 
 
+def _call(a: N.AttendArgs, dev: torch.device) -> int:
+    lib, ref = N.lib(), ctypes.byref(a)
+    need = lib.ffa_paged_attend_scratch(ref)
+    if need:
+        scratch = torch.empty(need, dtype=torch.uint8, device=dev)
+        a.scratch, a.scratch_bytes = scratch.data_ptr(), need
+    return lib.ffa_paged_attend(ref, N.stream_of(dev))
+
+
 def run_attend(fmt, q, k, k_scale, k_zero, k_res, v, block_table, seq_lens=None, *, T=None, q_lens=None, scale=None,
                use_fp8_residual=True, shared: SharedPrefix | None = None, out=None) -> torch.Tensor:
     """Exact attention of q [B, L, HQ, 128] (or [B, HQ, 128]) over the page pools of one format.
@@ -128,13 +137,15 @@ def run_attend(fmt, q, k, k_scale, k_zero, k_res, v, block_table, seq_lens=None,
         if q_lens.shape != (B,):
             raise ValueError("q_lens must be [B]")
         q_lens = _int32(q_lens, dev)
-    T, cols = max(int(T), 1), block_table.shape[1]  # T = 0: a batch of empty sequences
+    T, cols = int(T), block_table.shape[1]
     if cols * PAGE < T:
         raise ValueError("block_table must be [B, >= ceil(T/64)]")
     if out is None:
         out = torch.empty_like(q)
     elif out.shape != shape or out.dtype != q.dtype or out.device != dev or not out.is_contiguous():
         raise ValueError("out must be a contiguous tensor of q's shape, type and device")
+    if T <= 0:  # a batch of empty sequences
+        return out.zero_()
     res = k_res if use_fp8_residual else None
     groups = (0, None, None, None, None, None, 0)
     if shared is not None:
@@ -148,13 +159,10 @@ def run_attend(fmt, q, k, k_scale, k_zero, k_res, v, block_table, seq_lens=None,
         N.DT_NONE if res is None else N.dtype_code(res.dtype), v.data_ptr(), N.dtype_code(v.dtype), block_table.data_ptr(),
         cols, P, N.ptr(seq_lens), N.ptr(q_lens), B, T, L, HQ, HKV, _SCALE if scale is None else float(scale), *groups,
         out.data_ptr(), None, 0)
-    lib = N.lib()
-    with _on(dev):
-        ref = ctypes.byref(a)
-        need = lib.ffa_paged_attend_scratch(ref)
-        if need:
-            scratch = torch.empty(need, dtype=torch.uint8, device=dev)
-            a.scratch, a.scratch_bytes = scratch.data_ptr(), need
-        rc = lib.ffa_paged_attend(ref, N.stream_of(dev))
+    if dev.index == torch.cuda.current_device():
+        rc = _call(a, dev)
+    else:
+        with torch.cuda.device(dev):
+            rc = _call(a, dev)
     N.check(rc, "ffa_paged_attend")
     return out

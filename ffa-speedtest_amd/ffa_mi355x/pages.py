@@ -14,6 +14,7 @@ that another sequence holds:
 
 Everything runs on the current stream without synchronising, except for `check=True` (the default), which reads the
 call's error word and raises; `check=False` serves captured graphs and loops that look at `errors` now and then.
+Calls of one pool read and change its counts: they belong on one stream, or ordered.
 """
 from __future__ import annotations
 

@@ -499,7 +499,8 @@ int ffa_paged_attend(const ffa_paged_attend_args *args, void *stream);
  * counts the block-table rows that hold each page; a page is free while its count is 0.  New pages
  * are the lowest free ids, in (row, column) order: results depend on counts and tables alone.  Block
  * tables are [rows, bt_stride] int32, seq_lens [rows]; a row's pages are its first ceil(len / 64)
- * columns.  Page contents are copied whole, in every pool of the list.  Nothing synchronises: errors
+ * columns.  Page contents are copied whole, in every pool of the list.  Calls with the same counts must
+ * be ordered on one stream.  Nothing synchronises: errors
  * of the device data set bits in *errors (kept until the caller clears it) and in the call's own word
  * (scratch[0], call_errors): 1 not enough free pages, 2 a row that cannot be served (a parent outside
  * the batch, a length outside its row, a partial page that is free or outside the pool), 4 a page id

@@ -90,7 +90,7 @@ def reference(q, k, v, T, ql, scale, tokens=None):
                 w = np.exp(s - s.max())
                 w = w / w.sum()
                 o[i, h] = w @ vv
-                d = scale * (np.abs(kk) @ np.abs(qf[i, h])).max() * (2.0 ** -11 + 2.0 ** -17) + n * 2.0 ** -25
+                d = abs(scale) * (np.abs(kk) @ np.abs(qf[i, h])).max() * (2.0 ** -11 + 2.0 ** -17) + n * 2.0 ** -25
                 bound[i, h] = (np.expm1(2 * d) + 2.0 ** -11 + 2.0 ** -20) * (w @ np.abs(vv)) + n * 2.0 ** -25 * 2.0 ** -8
     return o, bound
 

@@ -94,6 +94,24 @@ def test_long_and_scale(gpu):
     _check(cache, "q2", table, lens, q, out, scale=0.03)
 
 
+@pytest.mark.parametrize("L,HQ", [(1, 4), (40, 8)])
+@pytest.mark.parametrize("scale", [-0.05, 0.0, 2.0])
+def test_other_scales(gpu, scale, L, HQ):
+    """Negative scales (the least product weighs most), 0 (a mean over the keys), scores far apart."""
+    cache, table, sl, q = _batch("nf4", [150], HQ, 1, L, torch.float16, 73, gpu)
+    _check(cache, "nf4", table, [150], q, cache.attend(q, table, sl, scale=scale), scale=scale)
+
+
+def test_empty_batch_of_sequences(gpu):
+    cache, table, _, q = _batch("q2", [64, 64], 4, 1, 2, torch.float16, 79, gpu)
+    for kw in (dict(seq_lens=torch.zeros(2, dtype=torch.int32, device=gpu)), dict(T=0),
+               dict(seq_lens=torch.full((2,), 64, device=gpu), T=0)):
+        out = torch.full_like(q, 7)
+        assert cache.attend(q, table, out=out, **kw) is out and (out == 0).all()
+    sl = torch.tensor([-3, 64], device=gpu)  # clamped
+    assert (cache.attend(q, table, sl)[0] == 0).all()
+
+
 def test_three_dimensions_out_and_strides(gpu):
     """[B, HQ, 128] queries, a strided view of them, int64 tables, a given output."""
     lens = [100, 77]
