@@ -326,6 +326,34 @@ def test_another_stream(gpu):
     assert torch.equal(want, got)
 
 
+def test_two_streams_and_two_graphs(gpu):
+    """Calls that overlap on two streams, and two captured calls replayed in turn, do not share partials."""
+    sets = [_batch("q2", [4000, 900], 8, 2, 1, torch.bfloat16, 83 + i, gpu) for i in range(2)]
+    want = [c.attend(q, t, sl, T=4000) for c, t, sl, q in sets]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    outs = [[], []]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for i, (c, t, sl, q) in enumerate(sets):
+            with torch.cuda.stream(streams[i]):
+                outs[i].append(c.attend(q, t, sl, T=4000))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want[i]) for i in range(2) for o in outs[i])
+    graphs, caught = [], []
+    for c, t, sl, q in sets:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            caught.append(c.attend(q, t, sl, T=4000))
+        graphs.append(g)
+    for order in ((0, 1), (1, 0), (0, 0, 1)):
+        for o in caught:
+            o.zero_()
+        for i in order:
+            graphs[i].replay()
+        torch.cuda.synchronize()
+        assert torch.equal(caught[0], want[0]) and torch.equal(caught[1], want[1])
+
+
 def test_repeatable(gpu):
     """The same bits every time (no order of atomics in them)."""
     cache, table, lens, sl, q = _forked("nf4", [5], [2000], [9] * 5, 8, 2, 1, torch.float16, 43, gpu)
