@@ -204,11 +204,13 @@ class Q2FP8PagedLayer(CacheLayerMixin):
         cut = length < self.seq_len
         self.seq_len = length
         self.seq_lens.fill_(length)
-        if self.pages is not None and cut and length % PAGE:
-            # the last page may be one that others share: tokens are appended to a copy
-            shared = self.shared
+        if self.pages is None or not cut:
+            return
+        shared = self.shared
+        if length % PAGE:  # the last page may be one that others share: tokens are appended to a copy
             self._select(torch.arange(self.block_table.shape[0]), True)
-            self.shared = shared and SharedPrefix(self.block_table, self.seq_lens, group_sizes=shared.sizes)
+        if shared is not None:  # pages that are gone are shared no more, also where the length is a page's end
+            self.shared = SharedPrefix(self.block_table, self.seq_lens, group_sizes=shared.sizes)
 
     def offload(self):
         raise NotImplementedError("offloading is not supported by the paged q2fp8 cache")

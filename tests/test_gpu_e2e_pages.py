@@ -191,3 +191,27 @@ def test_generate_with_beams(gpu):
                              eos_token_id=None)
     assert out.shape == (2, 76) and torch.equal(out[:, :70], ids)
     assert cache.layers[0].pages is not None and int(cache.layers[0].pages.errors.item()) == 0
+
+
+@pytest.mark.parametrize("keep", [0, 64, 128])
+def test_attention_after_a_crop_to_a_page(gpu, keep):
+    """Samples that share three pages, cut to a page's end (or to nothing) and continued apart: attention with the
+    layer's plan of shared pages is every sample's own."""
+    x = Both(_load(), 1, 3, gpu)
+    x.update(200)
+    x.layer.batch_repeat_interleave(3)
+    x.select([0, 0, 0])
+    x.update(10)
+    x.layer.crop(keep - 210)
+    x.cut(keep)
+    for n in (1, 90):
+        x.update(n)
+        x.check()
+        S = x.layer.seq_len
+        assert x.layer.shared.sizes == [3] and x.layer.shared.pages == [keep // 64]
+        q = torch.randn((3, n, 8, 128), generator=x.g).bfloat16().to(gpu)
+        out = x.layer.pool.attend(q, x.layer.block_table, x.layer.seq_lens, T=S, shared=x.layer.shared)
+        for b in range(3):
+            k, v = logical_kv(x.layer.pool, "q2", x.layer.block_table[b, : -(-S // 64)].tolist())
+            want, bound = reference(q[b], k[:S], v[:S], S, n, 1 / math.sqrt(128))
+            assert_close(out[b], want, bound, q.dtype, f"S={S} b={b}")
