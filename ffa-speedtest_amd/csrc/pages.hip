@@ -9,6 +9,7 @@
 // (page pair, 16 KB piece of a pool's page), wide loads of a piece before its stores.
 #include "ffa_common.h"
 #include "ffa_mi355x.h"
+#include "routes.h"
 
 extern "C" int ffa_set_error_internal(int code, const char *msg);
 
@@ -99,6 +100,7 @@ struct AllocArgs {
   int32_t *scratch;  // [0] error bits, [1] pages needed, [2 ..] ids
   int32_t *errors;
   int P, rows, cols, B, tokens;  // tokens < 0: fork
+  int checked;                   // fork: pages_fork_check_kernel left a word per row in scratch[2 ..]
 };
 
 // pages that row r gets: `cnt` from column `first` on.  Returns false for a row that cannot be served.
@@ -122,16 +124,44 @@ __device__ __forceinline__ bool row_need(const AllocArgs &a, int r, int &first, 
   return true;
 }
 
+// Fork: whether the parent of row r holds its whole pages t, t + n, ..: inside the pool, counts above 0 (a free one could
+// be given out as another's new page).  Rows that row_need refuses pass.
+__device__ __forceinline__ bool whole_pages_held(const AllocArgs &a, int r, int t, int n) {
+  const int par = a.parents[r];
+  if ((unsigned)par >= (unsigned)a.B) return true;
+  const int len = a.seq_lens[par];
+  if (len < 0 || len > a.cols * kPageTokens) return true;
+  const int32_t *from = a.parent_table + (size_t)par * a.cols;
+  const int full = len / kPageTokens;
+  int ok = 1;
+#pragma unroll 4
+  for (int j = t; j < full; j += n) {
+    const int id = from[j], in = (unsigned)id < (unsigned)a.P;
+    ok &= in & (a.refs[in ? id : 0] > 0);
+  }
+  return ok;
+}
+
+// the same by a workgroup per row (fork_check_apart)
+__global__ __launch_bounds__(256) void pages_fork_check_kernel(const AllocArgs a) {
+  const int bad = __syncthreads_or(!whole_pages_held(a, blockIdx.x, threadIdx.x, 256));
+  if (threadIdx.x == 0) a.scratch[2 + blockIdx.x] = bad;
+}
+
 __global__ __launch_bounds__(1024) void pages_alloc_kernel(const AllocArgs a) {
-  int need = 0, bad = 0;
+  int need = 0, bad = 0, page = 0;
+  if (a.tokens < 0 && !a.checked)
+    for (int r = threadIdx.x >> 6; r < a.rows; r += 16) page |= !whole_pages_held(a, r, threadIdx.x & 63, 64);
   for (int base = 0; base < a.rows; base += 1024) {
     const int r = base + threadIdx.x;
     int first = 0, cnt = 0, sum;
     if (r < a.rows && !row_need(a, r, first, cnt)) bad = 1;
+    if (r < a.rows && a.checked) page |= a.scratch[2 + r];
     block_rank(cnt, sum);
     need += sum;
   }
   bad = __syncthreads_or(bad);
+  page = __syncthreads_or(page);  // behind every read of the rows' words: the ids go over them
   // the lowest free pages, in order: 16 counts a thread and step
   int found = 0;
   for (int base = 0; base < a.P && found < need; base += 16 * 1024) {
@@ -153,7 +183,7 @@ __global__ __launch_bounds__(1024) void pages_alloc_kernel(const AllocArgs a) {
     found += sum;
   }
   __syncthreads();
-  const int err = (bad ? kErrRow : 0) | (found < need ? kErrFull : 0);
+  const int err = (bad ? kErrRow : 0) | (found < need ? kErrFull : 0) | (page ? kErrPage : 0);
   if (threadIdx.x == 0) {
     a.scratch[0] = err;
     a.scratch[1] = need;
@@ -176,10 +206,10 @@ __global__ __launch_bounds__(1024) void pages_alloc_kernel(const AllocArgs a) {
 }
 
 // Fork: workgroup (0, child) writes the child's row and counts the pages it shares; the others copy the pieces of its
-// partial page.  With an allocation that failed every child's row is empty (-1) and nothing else changes.
+// partial page.  Where the allocation found an error every child's row is empty (-1) and nothing else changes.
 __global__ __launch_bounds__(256) void pages_fork_kernel(const PoolSet s, const AllocArgs a, int tables) {
   const int r = blockIdx.y, par = a.parents[r];
-  const bool ok = (a.scratch[0] & 0xff) == 0;
+  const bool ok = a.scratch[0] == 0;
   const int len = ok ? a.seq_lens[par] : 0, full = len / kPageTokens, part = len % kPageTokens ? 1 : 0;
   int32_t *row = a.table + (size_t)r * a.cols;
   const int32_t *from = a.parent_table + (size_t)(ok ? par : 0) * a.cols;
@@ -190,11 +220,7 @@ __global__ __launch_bounds__(256) void pages_fork_kernel(const PoolSet s, const 
         int id = -1;
         if (j < full) {
           id = from[j];
-          if ((unsigned)id >= (unsigned)a.P) id = -1;
-          if (id < 0 || atomicAdd(&a.refs[id], 1) == 0) {
-            atomicOr(a.errors, kErrPage);
-            atomicOr(a.scratch, kErrPage << 8);  // beside the allocation's bits, which other workgroups read
-          }
+          if ((unsigned)id < (unsigned)a.P) atomicAdd(&a.refs[id], 1);
         }
         row[j] = id;
       }
@@ -393,8 +419,11 @@ extern "C" int ffa_pages_fork(const ffa_pages *pg, const int32_t *block_table, i
   if (bad != FFA_OK) return bad;
   if (B <= 0 || !parents || !child_table || !scratch) FFA_BAD("fork needs parents, a table for the children and scratch");
   if (child_table == block_table) FFA_BAD("the children's table cannot be the parents'");
+  const int checked = ffa::fork_check_apart(children, bt_stride);
   const ffa::AllocArgs a = {pg->refs, child_table, block_table, seq_lens, parents, scratch, errors,
-                            pg->num_pages, children, bt_stride, B, -1};
+                            pg->num_pages, children, bt_stride, B, -1, checked};
+  if (checked)
+    hipLaunchKernelGGL(ffa::pages_fork_check_kernel, dim3((unsigned)children), dim3(256), 0, (hipStream_t)stream, a);
   hipLaunchKernelGGL(ffa::pages_alloc_kernel, dim3(1), dim3(1024), 0, (hipStream_t)stream, a);
   for (int i = 0; i < pg->npools; i += ffa::kMaxPools) {
     const ffa::PoolSet s = pool_set(pg, i);
@@ -415,7 +444,7 @@ extern "C" int ffa_pages_extend(const ffa_pages *pg, int32_t *block_table, int b
   if (tokens < 0 || !scratch) FFA_BAD("extend needs a number of tokens and scratch");
   if (ffa_pages_alloc_scratch(rows, tokens) > (size_t)1 << 30) FFA_NO("more than 2^30 pages in a call");
   const ffa::AllocArgs a = {pg->refs, block_table, nullptr, seq_lens, nullptr, scratch, errors,
-                            pg->num_pages, rows, bt_stride, rows, tokens};
+                            pg->num_pages, rows, bt_stride, rows, tokens, 0};
   hipLaunchKernelGGL(ffa::pages_alloc_kernel, dim3(1), dim3(1024), 0, (hipStream_t)stream, a);
   return launched();
 }

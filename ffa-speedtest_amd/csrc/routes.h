@@ -85,4 +85,11 @@ inline int kproj_route(int M, int N, int cus) {
   return tiles(128, 64) >= cus ? kKproj128x64 : (tiles(64, 64) >= cus ? kKproj64x64 : kKproj32x64);
 }
 
+// Fork's check of the parents' whole pages: by a launch of its own, or by the one workgroup that ranks the free pages
+// (16 rows at a time).  us of a fork and free in a graph, in the workgroup / apart (without the check 11-26):
+//   4 children x 32 pages 11.6 / 13.4      64 x 64 13.9 / 14.8      64 x 256 16.1 / 14.8      16 x 1024 16.5 / 17.4
+//   64 of 64 parents x 256 20.3 / 16.9      64 x 1024 24 / 18      256 x 1024 53 / 22      256 x 2048 78 / 27
+// and without a graph, where the launches count, 20-21 / 22-24 up to 16384 entries, 24 / 22 at 65536.
+inline bool fork_check_apart(int children, int cols) { return (long)children * cols > 16384; }
+
 }  // namespace ffa

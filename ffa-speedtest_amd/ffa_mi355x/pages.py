@@ -127,8 +127,7 @@ class PagePool:
                                     self.errors.data_ptr(), self._stream())
         N.check(rc, "ffa_pages_fork")
         if check:
-            bits = int(scratch[0].item())
-            self._raise((bits & 0xff) | bits >> 8, "fork")
+            self._raise(int(scratch[0].item()), "fork")
         return child
 
     def extend(self, block_table: torch.Tensor, seq_lens: torch.Tensor, tokens: int, check: bool = True) -> None:

@@ -523,8 +523,8 @@ size_t ffa_pages_alloc_scratch(int rows, int tokens);
 
 /* Fork: child c continues sequence parents[c]: its row holds the parent's whole pages (counted once
  * more) and, where the length ends inside a page, a new page with that page's contents; columns past
- * them are -1.  child_table [children, bt_stride].  When the pages do not suffice or a row cannot be
- * served, every child's row is -1 and nothing else changes; scratch[1] is the number of new pages. */
+ * them are -1.  child_table [children, bt_stride].  On any error (1, 2, or 4: a whole page outside the pool
+ * or free) every child's row is -1 and nothing else changes; scratch[1] is the number of new pages. */
 int ffa_pages_fork(const ffa_pages *pages, const int32_t *block_table, int bt_stride, int B, const int32_t *seq_lens,
                    const int32_t *parents, int children, int32_t *child_table, int32_t *scratch, int32_t *errors,
                    void *stream);

@@ -356,3 +356,59 @@ def test_samples_of_prompts(gpu, fmt):
     for cache, out in zip(layers, first):  # the groups' sizes changed, so the page ranges may
         again = cache.attend(q[:4], child[:4], clens[:4], shared=plan)
         assert torch.allclose(again.float(), out[:4].float(), atol=2.0 ** -7, rtol=2.0 ** -7)
+
+
+@pytest.mark.parametrize("cols", [6, 9000])  # the check within the ranking, and by a launch of its own
+def test_fork_of_bad_whole_pages_changes_nothing(gpu, cols):
+    """A parent's whole page that is free (the next one to be given out, too) or outside the pool: no child, no count, no
+    copy, whichever child is the bad one's."""
+    pool, before = _pool(gpu, 40, fmts=("q2", "nf4"))
+    m = Model(40)
+    t, lens = [[-1] * cols for _ in range(2)], [0, 0]
+    td = _dev(t, gpu)
+    pool.extend(td, _dev(lens, gpu), 300)
+    m.extend(t, lens, 300)
+    lens = _dev([300, 300], gpu)
+    _same(pool, before, m)
+    for col in (0, 3):
+        for bad in (10, 39, 40, -1, 2 ** 31 - 1):  # 10: the lowest free page
+            wrong = td.clone()
+            wrong[1, col] = bad
+            for parents in ([1], [0, 1, 0]):
+                pool.errors.zero_()
+                with pytest.raises(ValueError):
+                    pool.fork(wrong, lens, _dev(parents, gpu))
+                assert (pool.fork(wrong, lens, _dev(parents, gpu), check=False) == -1).all()
+                assert int(pool.errors.item()) == 4
+                _same(pool, before, m)
+            child = pool.fork(wrong, lens, _dev([0], gpu))  # the other sequence is served
+            assert child.tolist() == m.fork(t, [300, 300], [0])
+            pool.free(child, lens[:1])
+            m.count(child.tolist(), [300], -1)
+            _same(pool, before, m)
+    wrong = td.clone()
+    wrong[0, 0], wrong[1, 4] = 39, 39  # a whole page and a partial one
+    pool.errors.zero_()
+    pool.fork(wrong, lens, _dev([0, 1], gpu), check=False)
+    assert int(pool.errors.item()) == 6
+    _same(pool, before, m)
+
+
+@pytest.mark.parametrize("children,cols", [(70, 30), (600, 90)])
+def test_fork_of_many_rows(gpu, children, cols):
+    """More children than one pass of the ranking workgroup's waves, by both ways of the check."""
+    pool, before = _pool(gpu, 2000, fmts=("nf4",), HKV=1)
+    m = Model(2000)
+    t, lens = [[-1] * cols for _ in range(3)], [0] * 3
+    td = _dev(t, gpu)
+    pool.extend(td, _dev(lens, gpu), 64 * cols - 7)
+    m.extend(t, lens, 64 * cols - 7)
+    lens = [64 * cols - 7, 64 * 11, 64 * 17 + 1]
+    parents = [(5 * c) % 3 for c in range(children)]
+    assert pool.fork(td, _dev(lens, gpu), _dev(parents, gpu)).tolist() == m.fork(t, lens, parents)
+    _same(pool, before, m)
+    wrong = td.clone()
+    wrong[2, 16] = 1999
+    with pytest.raises(ValueError):
+        pool.fork(wrong, _dev(lens, gpu), _dev(parents[:-2] + [2, 0], gpu))
+    _same(pool, before, m)

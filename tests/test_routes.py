@@ -82,3 +82,11 @@ def test_contiguous_decode_of_many_workgroups(routes):
     two = [(2, 512, 5.0), (1, 1280, 5.0), (1, 944, 5.0), (1, 8520, 8.0), (1, 8520, 1000.0)]
     got = routes(*(f"three_per_cu({nq}, {n}, 256, {d}f)" for nq, n, d in three + two))
     assert got == [1] * len(three) + [0] * len(two)
+
+
+def test_fork_checks(routes):
+    """The ranking workgroup checks up to 16384 entries of the parents' rows itself."""
+    inside = [(4, 32), (64, 64), (64, 256), (16, 1024), (1, 16384)]
+    apart = [(64, 1024), (256, 1024), (1, 16385), (65535, 1 << 24)]
+    got = routes(*(f"fork_check_apart({c}, {n})" for c, n in inside + apart))
+    assert got == [0] * len(inside) + [1] * len(apart)
