@@ -103,7 +103,8 @@ struct AllocArgs {
   int checked;                   // fork: pages_fork_check_kernel left a word per row in scratch[2 ..]
 };
 
-// pages that row r gets: `cnt` from column `first` on.  Returns false for a row that cannot be served.
+// pages that row r gets: `cnt` from column `first` on.  Returns false for a row that cannot be served (before any page is
+// given out; afterwards counts have grown, and only `first` and `cnt` are read).
 __device__ __forceinline__ bool row_need(const AllocArgs &a, int r, int &first, int &cnt) {
   first = cnt = 0;
   if (a.tokens < 0) {
@@ -121,7 +122,9 @@ __device__ __forceinline__ bool row_need(const AllocArgs &a, int r, int &first, 
   if (len < 0 || (long)len + a.tokens > (long)a.cols * kPageTokens) return false;
   first = (len + kPageTokens - 1) / kPageTokens;
   cnt = (len + a.tokens + kPageTokens - 1) / kPageTokens - first;
-  return true;
+  if (len % kPageTokens == 0) return true;
+  const int id = a.table[(size_t)r * a.cols + len / kPageTokens];  // the partial page, which the new tokens fill first
+  return (unsigned)id < (unsigned)a.P && a.refs[id] > 0;
 }
 
 // Fork: whether the parent of row r holds its whole pages t, t + n, ..: inside the pool, counts above 0 (a free one could

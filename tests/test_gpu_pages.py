@@ -412,3 +412,32 @@ def test_fork_of_many_rows(gpu, children, cols):
     with pytest.raises(ValueError):
         pool.fork(wrong, _dev(lens, gpu), _dev(parents[:-2] + [2, 0], gpu))
     _same(pool, before, m)
+
+
+@pytest.mark.parametrize("bad", [4, 29, 30, -1, -2 ** 31, 2 ** 31 - 1])  # 4: the lowest free page
+@pytest.mark.parametrize("tokens", [0, 1, 100])
+def test_extend_refuses_bad_partial_pages(gpu, bad, tokens):
+    """A last page, partly filled, that is free or outside the pool: no row gets pages (a free one could be given out as a
+    new page, its tokens beside others')."""
+    pool, before = _pool(gpu, 30, fmts=("q2",))
+    m = Model(30)
+    t, lens = [[-1] * 6 for _ in range(2)], [0, 0]
+    td = _dev(t, gpu)
+    pool.extend(td, _dev(lens, gpu), 100)
+    m.extend(t, lens, 100)
+    for row in (0, 1):
+        wrong = td.clone()
+        wrong[row, 1] = bad
+        given = wrong.clone()
+        pool.errors.zero_()
+        with pytest.raises(ValueError):
+            pool.extend(given, _dev([100, 100], gpu), tokens)
+        pool.extend(given, _dev([100, 100], gpu), tokens, check=False)
+        assert torch.equal(given, wrong) and int(pool.errors.item()) == 2
+        _same(pool, before, m)
+    at_end = td.clone()
+    at_end[:, 1] = bad  # past whole pages: written, not read
+    pool.extend(at_end, _dev([64, 64], gpu), tokens)
+    m.extend(t, [64, 64], tokens)
+    assert pool.refs.tolist() == m.refs
+    assert tokens == 0 or at_end.tolist() == t
