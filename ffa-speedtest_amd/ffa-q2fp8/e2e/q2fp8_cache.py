@@ -107,6 +107,8 @@ class Q2FP8PagedLayer(CacheLayerMixin):
         if not self.is_initialized:
             self.lazy_initialization(key_states, value_states)
         B, HKV, Tn, D = key_states.shape
+        if self.pages is not None and self.seq_len == 0 and 0 < B <= self.max_batch_size:
+            self._empty_rows(B)
         if B != self.block_table.shape[0] or HKV != self.pool.HKV:
             raise ValueError("key_states do not match the cache's batch / KV heads")
         if self.seq_len + Tn > self.capacity:
@@ -147,6 +149,14 @@ class Q2FP8PagedLayer(CacheLayerMixin):
             self.block_table.fill_(-1)
 
     # ------------------------------------------------------------------ batch operations
+    def _empty_rows(self, B: int) -> None:
+        """Rows for a batch of B, where no row holds a page: a new prompt may have another batch than the samples and
+        beams before it."""
+        if B != self.block_table.shape[0]:
+            self.block_table = torch.full((B, self.block_table.shape[1]), -1, dtype=torch.int32, device=self.device)
+            self.seq_lens = torch.zeros(B, dtype=torch.int32, device=self.device)
+            self.shared = None
+
     def _count_pages(self) -> PagePool:
         """From fixed rows of pages to counted ones, in a pool that holds max_batch_size whole sequences and the copies
         of their last pages that a fork makes before the parents go."""

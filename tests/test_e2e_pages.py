@@ -147,3 +147,28 @@ def test_crop_of_two_groups_twice(monkeypatch):
         x.check()
     x.crop(-192, 0)
     x.check()
+
+
+@pytest.mark.parametrize("empty", [lambda y: y.reset(), lambda y: y.crop(-10 ** 6)])
+def test_other_batches_after_an_empty_cache(monkeypatch, empty):
+    """One prompt, samples of it, emptied: the next prompt's batch is its own."""
+    x = Both(monkeypatch, 1, 5)
+    x.update(200)
+    x.repeat(3)
+    x.update(70)
+    for B in (1, 4, 5, 3):
+        empty(x.layer)
+        x.update(130, B)
+        x.check()
+        x.update(1)
+        x.check()
+        with pytest.raises(ValueError):  # with tokens cached the batch stands
+            x.layer.update(torch.zeros(B - 1 or 2, 1, 1, 128), torch.zeros(B - 1 or 2, 1, 1, 128))
+        x.check()
+    x.layer.batch_select_indices(torch.tensor([2, 0]))
+    x.rows = [x.rows[2], x.rows[0]]
+    x.check()
+    x.layer.reset()
+    for B in (0, 6):
+        with pytest.raises(ValueError):
+            x.layer.update(torch.zeros(B, 1, 1, 128), torch.zeros(B, 1, 1, 128))

@@ -215,3 +215,26 @@ def test_attention_after_a_crop_to_a_page(gpu, keep):
             k, v = logical_kv(x.layer.pool, "q2", x.layer.block_table[b, : -(-S // 64)].tolist())
             want, bound = reference(q[b], k[:S], v[:S], S, n, 1 / math.sqrt(128))
             assert_close(out[b], want, bound, q.dtype, f"S={S} b={b}")
+
+
+def test_a_new_prompt_after_samples(gpu):
+    """One prompt, samples, reset, prompts of other batches; decoded by the pruned kernel as a fresh layer's."""
+    C = _load()
+    x = Both(C, 1, 4, gpu)
+    x.update(200)
+    x.layer.batch_repeat_interleave(4)
+    x.select([0] * 4)
+    x.update(70)
+    for B in (1, 3):
+        x.layer.reset()
+        x.rows = [[torch.zeros(2, 0, 128), torch.zeros(2, 0, 128)] for _ in range(B)]
+        x.update(150)
+        x.check()
+        x.update(1)
+        x.check()
+        fresh = C.Q2FP8PagedLayer(B, x.cap)
+        fresh.update(*(torch.stack([r[j] for r in x.rows]).bfloat16().to(gpu) for j in range(2)))
+        q = torch.randn((B, 8, 128), generator=x.g).bfloat16().to(gpu)
+        outs = [y.pool.decode(q, y.block_table, y.seq_lens, T=y.capacity, workspace=y.workspace(8, 64, 64, q.dtype)).o
+                for y in (x.layer, fresh)]
+        assert torch.equal(*outs)
