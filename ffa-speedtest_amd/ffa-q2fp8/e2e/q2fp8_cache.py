@@ -175,8 +175,8 @@ class Q2FP8PagedLayer(CacheLayerMixin):
         if not self.is_initialized:
             return
         n = int(indices.numel())
-        if n > self.max_batch_size:
-            raise ValueError(f"batch {n} exceeds max_batch_size {self.max_batch_size}")
+        if not 0 < n <= self.max_batch_size:
+            raise ValueError(f"a batch of {n}: the cache holds 1 to {self.max_batch_size} sequences")
         pages = self._count_pages()
         child = pages.fork(self.block_table, self.seq_lens, indices.reshape(-1), check=check)
         pages.free(self.block_table, self.seq_lens, check=check)

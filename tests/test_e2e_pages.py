@@ -172,3 +172,20 @@ def test_other_batches_after_an_empty_cache(monkeypatch, empty):
     for B in (0, 6):
         with pytest.raises(ValueError):
             x.layer.update(torch.zeros(B, 1, 1, 128), torch.zeros(B, 1, 1, 128))
+
+
+def test_empty_selections_are_refused(monkeypatch):
+    """No sequence selected: refused before anything changes."""
+    x = Both(monkeypatch, 2, 4)
+    x.update(100)
+    for counted in (False, True):
+        for call in (lambda y: y.batch_repeat_interleave(0), lambda y: y.batch_select_indices(torch.zeros(len(x.rows), dtype=torch.bool)),
+                     lambda y: y.batch_select_indices(torch.tensor([], dtype=torch.long)),
+                     lambda y: y.reorder_cache(torch.tensor([], dtype=torch.long))):
+            with pytest.raises(ValueError):
+                call(x.layer)
+            x.check()
+        assert (x.layer.pages is not None) == counted
+        x.repeat(2 - counted)
+        x.update(30)
+        x.check()
