@@ -114,10 +114,15 @@ class Q2FP8PagedLayer(CacheLayerMixin):
         if self.seq_len + Tn > self.capacity:
             raise ValueError(f"cache holds {self.capacity} tokens, {self.seq_len + Tn} requested")
         pos = torch.full((B,), self.seq_len, dtype=torch.int32, device=self.device)
-        if self.pages is not None and -(-(self.seq_len + Tn) // PAGE) > -(-self.seq_len // PAGE):
+        first, end = -(-self.seq_len // PAGE), -(-(self.seq_len + Tn) // PAGE)
+        if self.pages is not None and end > first:
             self.pages.extend(self.block_table, self.seq_lens, Tn)
-        self.pool.append(key_states.transpose(1, 2).contiguous(), value_states.transpose(1, 2).contiguous(), pos,
-                         self.block_table)
+        try:
+            self.pool.append(key_states.transpose(1, 2).contiguous(), value_states.transpose(1, 2).contiguous(), pos,
+                             self.block_table)
+        except Exception:  # refused: the new pages hold nothing
+            self._drop_pages(first, end)
+            raise
         self.seq_len += Tn
         self.seq_lens.fill_(self.seq_len)
         self.last_query_len = Tn
@@ -171,6 +176,13 @@ class Q2FP8PagedLayer(CacheLayerMixin):
             self.pages.hold(self.block_table, self.seq_lens)
         return self.pages
 
+    def _drop_pages(self, first: int, end: int) -> None:
+        """Free the pages of columns [first, end) of every row."""
+        if self.pages is not None and first < end:
+            tail = self.block_table[:, first:end].contiguous()
+            self.pages.free(tail, torch.full_like(self.seq_lens, tail.shape[1] * PAGE))
+            self.block_table[:, first:end] = -1
+
     def _select(self, indices: torch.Tensor, check: bool) -> None:
         if not self.is_initialized:
             return
@@ -207,10 +219,7 @@ class Q2FP8PagedLayer(CacheLayerMixin):
             return
         length = min(tokens_to_remove, self.seq_len) if tokens_to_remove > 0 else max(self.seq_len + tokens_to_remove, 0)
         first, end = -(-length // PAGE), -(-self.seq_len // PAGE)
-        if self.pages is not None and first < end:
-            tail = self.block_table[:, first:end].contiguous()
-            self.pages.free(tail, torch.full_like(self.seq_lens, tail.shape[1] * PAGE))
-            self.block_table[:, first:end] = -1
+        self._drop_pages(first, end)
         cut = length < self.seq_len
         self.seq_len = length
         self.seq_lens.fill_(length)

@@ -189,3 +189,17 @@ def test_empty_selections_are_refused(monkeypatch):
         x.repeat(2 - counted)
         x.update(30)
         x.check()
+
+
+def test_refused_tokens_take_no_pages(monkeypatch):
+    """An append that is refused (here: a head dimension that the cache does not hold) after its pages were taken."""
+    x = Both(monkeypatch, 1, 3)
+    x.update(60)
+    x.repeat(3)
+    for n in (1, 300):  # inside the last page, and past it
+        for _ in range(3):
+            with pytest.raises(AssertionError):
+                x.layer.update(torch.zeros(3, 1, n, 64), torch.zeros(3, 1, n, 64))
+            x.check()
+    x.update(500)
+    x.check()
