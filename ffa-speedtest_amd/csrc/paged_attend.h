@@ -23,6 +23,7 @@ namespace ffa {
 
 enum { kFmtQ2 = 0, kFmtNvfp4 = 1, kFmtNf4 = 2 };
 constexpr float kNoMax = -1e30f;  // m of a row that has seen no key: below every score, and 2^(x - m) stays defined
+constexpr float kLeast = 0x1p-126f;  // least factor of a joined sum: an infinity times it stays one (times 0: NaN)
 constexpr float kStale = 8.f;     // log2 units a row's m may lag its maximum: p <= 2^8 fits the fp16 operand as well
 
 struct AttendParams {
@@ -282,7 +283,7 @@ __device__ __forceinline__ void load_q(const AttendParams &p, size_t row, bool o
 }
 
 // V words (8 tokens of a column) with infinities and NaN taken out; `bad` becomes non-zero where there were any.
-// A product with them would give 0 * inf to the rows that do not see them; add_not_finite puts them back.
+// A product with them would give 0 * inf, a NaN, to the rows that do not see them; add_not_finite puts them back.
 __device__ __forceinline__ u32x4 finite8(u32x4 w, uint32_t &bad) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -307,6 +308,40 @@ __device__ __forceinline__ void add_not_finite(const uint8_t *v, int g, int nvis
         const float x = VT == kVBF16 ? round_to(bf16_bits_to_f32(w), 0) : f16_bits_to_f32(w);
         if (!(fabsf(x) < INFINITY)) o[u][e] += x;
       }
+}
+
+// The sums o of a row tile after its pages pa, pa + step, .. below pe.  A page that all rows of a workgroup see is
+// multiplied as it is: an infinity of V comes out as one, or as NaN where the weight rounds to 0 or a later maximum
+// scales the sum by 0.  A column that is not finite becomes the sum of the infinities and NaN that the row sees in it,
+// if there are any: whatever its weights, the rows beside it and the order of the pages were.  `rows`: lanes of a row.
+template <int VT, class BlockOf>
+__device__ __forceinline__ void settle_not_finite(const AttendParams &p, BlockOf block_of, int pa, int pe, int step, int lane,
+                                                  bool rows, int lim, f32x4 *o) {
+  float any = 0.f;
+#pragma unroll
+  for (int u = 0; u < 8; ++u)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) any = __builtin_fmaf(o[u][e], 0.f, any);  // NaN, or 0
+  if (__ballot(rows && any != 0.f) == 0) return;
+  f32x4 sum[8];
+#pragma unroll
+  for (int u = 0; u < 8; ++u) sum[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+  for (int pg = pa; pg < pe; pg += step) {
+    const uint8_t *v = p.v + block_of(pg) * (kD * kPage * 2);
+    uint32_t bad = 0;
+#pragma unroll 1
+    for (int i = 0; i < 16; i += 4)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        finite8(__builtin_bit_cast(u32x4, VTraits<VT>::operand(((const u32x4 *)v)[64 * (i + j) + lane])), bad);
+    if (__ballot(bad != 0) != 0) add_not_finite<VT>(v, lane >> 4, lim - pg * kPage, sum);
+  }
+#pragma unroll
+  for (int u = 0; u < 8; ++u)
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (!(fabsf(o[u][e]) < INFINITY) && sum[u][e] != 0.f) o[u][e] = sum[u][e];
 }
 
 // ---------------------------------------------------------------------------
@@ -404,10 +439,13 @@ __device__ __forceinline__ void few_rows(const AttendParams &p, int split, int h
   KRaw<FMT, RES> kr;
   u32x4 V[16];
   size_t blk = 0;
-  auto load_page = [&](int pg) {
+  auto block_of = [&](int pg) {
     int id = bt[pg];
     id = __builtin_amdgcn_readfirstlane((unsigned)id < (unsigned)p.num_pages ? id : 0);
-    blk = (size_t)id * p.HKV + hkv;
+    return (size_t)id * p.HKV + hkv;
+  };
+  auto load_page = [&](int pg) {
+    blk = block_of(pg);
     load_k<FMT, RES>(p, blk, lane, kr);
     const uint4 *vp = (const uint4 *)(p.v + blk * (kD * kPage * 2));
 #pragma unroll
@@ -493,6 +531,10 @@ __device__ __forceinline__ void few_rows(const AttendParams &p, int split, int h
       for (int t = 0; t < NT; ++t) add_not_finite<VT>(p.v + blk * (kD * kPage * 2), g, lim[t] - t0, O[t]);
   }
 
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+    settle_not_finite<VT>(p, block_of, pa + wv, last, W, lane, r0 + 16 * t + n < R, lim[t], O[t]);
+
   // join the waves
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
@@ -509,7 +551,7 @@ __device__ __forceinline__ void few_rows(const AttendParams &p, int split, int h
     float M = kNoMax;
 #pragma unroll
     for (int w = 0; w < W; ++w) M = fmaxf(M, s.m[w][16 * t + n]);
-    const float f = exp2_hw(m[t] - M);
+    const float f = fmaxf(exp2_hw(m[t] - M), kLeast);
 #pragma unroll
     for (int u = 0; u < 8; ++u) *(f32x4 *)&s.o[wv][n][16 * u + 4 * g] = O[t][u] * f;
     __syncthreads();
@@ -832,6 +874,10 @@ __device__ __forceinline__ void many_rows(const AttendParams &p, int split, int 
   else if (any) pages(kOne);
   else pages(std::integral_constant<int, 0>());
 
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+    if (tile0 + W * t < tile_end)
+      settle_not_finite<VT>(p, block_of, pa, pe, 1, lane, 16 * (tile0 + W * t) + n < R, lim[t], O[t]);
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
     const int r = 16 * (tile0 + W * t) + n;

@@ -39,7 +39,7 @@ __global__ __launch_bounds__(256) void paged_attend_join_kernel(const AttendPara
     float mn = m;
 #pragma unroll
     for (int k = 0; k < 4; ++k) mn = fmaxf(mn, x[k].x);
-    const float fo = exp2_hw(m - mn);
+    const float fo = fmaxf(exp2_hw(m - mn), kLeast);
     m = mn;
     l *= fo;
     o.x *= fo;
@@ -47,7 +47,7 @@ __global__ __launch_bounds__(256) void paged_attend_join_kernel(const AttendPara
 #pragma unroll
     for (int k = 0; k < 4; ++k)
       if (s0 + WPR * k < slots) {
-        const float f = exp2_hw(x[k].x - mn);
+        const float f = fmaxf(exp2_hw(x[k].x - mn), kLeast);
         l += x[k].y * f;
         o.x += y[k].x * f;
         o.y += y[k].y * f;
@@ -67,7 +67,7 @@ __global__ __launch_bounds__(256) void paged_attend_join_kernel(const AttendPara
     l = o.x = o.y = 0.f;
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
-      const float f = exp2_hw(s_m[w] - m);
+      const float f = fmaxf(exp2_hw(s_m[w] - m), kLeast);
       l += s_l[w] * f;
       o.x += s_o[w][2 * lane] * f;
       o.y += s_o[w][2 * lane + 1] * f;

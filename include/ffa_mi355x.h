@@ -449,6 +449,7 @@ int ffa_kfmt_decode(const ffa_kfmt_decode_args *args, void *stream);
  * Rows that see no key (i >= qlen_b, an empty sequence, more query tokens than keys) are zeros.
  * q and out [B, L, HQ, 128] in fp16 or bf16; k is rounded to fp16 once, V of a bf16 pool likewise
  * (|v| <= 65504), products of fp16 operands are summed in fp32, and so are the softmax statistics.
+ * An infinity or NaN of V counts for every row that sees it, however small its weight, and for no other.
  *
  * Groups (ngroups > 0): sequences group_start[g] .. group_start[g + 1] - 1 share the pages of the
  * first group_pages[g] columns of their block-table rows (the first sequence's row is read), which

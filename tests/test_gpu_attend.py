@@ -396,3 +396,64 @@ def test_refusals_on_the_gpu(gpu):
     with pytest.raises(ValueError):
         cache.attend(q, table)
     assert np.isfinite(cache.attend(q, table, sl).float().cpu().numpy()).all()
+
+
+def _opposed(cache, table, b, n, HKV, at, depth, g):
+    """Keys of sequence b along one direction u, that at `at` against it: with queries along u and the returned scale its
+    score lies about `depth` log2 units below the others.  Its V holds an infinity, another key's a NaN."""
+    u = torch.sign(_rand(g, 128))
+    k, v = 0.5 * u + 0.05 * _rand(g, n, HKV, 128), _rand(g, n, HKV, 128)
+    k[at] = -u
+    v[at, :, 5], v[at, :, 6], v[at + 1, :, 7] = float("inf"), float("-inf"), float("nan")
+    fill(cache, k, v, table[b])
+    return u, depth * math.log(2) / 192
+
+
+@pytest.mark.parametrize("depth", [40, 200])  # below fp16's least weight, and below fp32's
+@pytest.mark.parametrize("fmt,v", [("q2", torch.float16), ("nf4", torch.bfloat16)])
+@pytest.mark.parametrize("n,L,HQ,HKV,at", [
+    (200, 1, 4, 1, 10), (200, 1, 4, 1, 190),      # a page that every row sees, and the last one
+    (200, 6, 8, 2, 10),                           # two tiles of rows
+    (200, 40, 2, 1, 70), (400, 100, 8, 2, 3),     # operands in LDS
+    (9000, 1, 8, 2, 700), (9000, 1, 8, 2, 8990),  # ranges of pages, joined
+    (3300, 150, 8, 2, 70), (3200, 140, 64, 4, 1), # ranges of a chunk
+])
+def test_infinities_of_small_weight(gpu, depth, fmt, v, n, L, HQ, HKV, at):
+    """A visible infinity counts whatever its weight, also one that rounds to 0 (0 * inf would be a NaN), in the page that
+    a row sees in part, in one that all rows see, and joined with ranges of far larger scores."""
+    g = torch.Generator().manual_seed(89)
+    cache, table, sl, _ = _batch(fmt, [n], HQ, HKV, 1, torch.float16, 89, gpu, v=v)
+    u, scale = _opposed(cache, table, 0, n, HKV, at, depth, g)
+    q = (u + 0.05 * _rand(g, 1, L, HQ, 128)).half().to(gpu)
+    out = cache.attend(q, table, sl, scale=scale)
+    sees = [i for i in range(L) if n - L + i >= at]
+    last = [i for i in range(L) if n - L + i >= at + 1]
+    assert (out[0, sees, :, 5] == float("inf")).all() and (out[0, sees, :, 6] == float("-inf")).all()
+    assert torch.isnan(out[0, last, :, 7]).all()
+    rest = [c for c in range(128) if c not in (5, 6, 7)]
+    assert torch.isfinite(out[..., rest]).all() and torch.isfinite(out[0, [i for i in range(L) if i not in sees]]).all()
+    some = sorted({0, L // 2, L - 1})
+    k, vv = logical_kv(cache, fmt, table[0, :-(-n // 64)].tolist())
+    o, bound = reference(q[0], k[:n], vv[:n], n, L, scale, some)
+    assert_close(out[0, some], o[some], bound[some], q.dtype)
+
+
+@pytest.mark.parametrize("own", [[30, 1, 60, 7], [300, 170, 500, 90]])
+@pytest.mark.parametrize("members,L,HQ", [(4, 1, 8), (4, 5, 64), (40, 1, 8)])
+def test_infinities_of_small_weight_in_shared_pages(gpu, members, L, HQ, own):
+    """The same in pages that sequences share: the call without the plan gives the same infinities."""
+    own = [own[b % 4] + L for b in range(members)]
+    cache, table, lens, sl, _ = _forked("q2", [members], [640], own, HQ, 1, L, torch.bfloat16, 97, gpu)
+    g = torch.Generator().manual_seed(97)
+    q = None
+    for b, n in enumerate(lens):  # the shared pages are written by every member, with the same values
+        u, scale = _opposed(cache, table, b, n, 1, 130, 40, torch.Generator().manual_seed(97))
+        q = q if q is not None else (u + 0.05 * _rand(g, members, L, HQ, 128)).bfloat16().to(gpu)
+    plan = SharedPrefix(table, sl)
+    assert plan.pages == [10]
+    a, b = cache.attend(q, table, sl, scale=scale, shared=plan), cache.attend(q, table, sl, scale=scale)
+    for out in (a, b):
+        assert (out[..., 5] == float("inf")).all() and (out[..., 6] == float("-inf")).all() and torch.isnan(out[..., 7]).all()
+    rest = [c for c in range(128) if c not in (5, 6, 7)]
+    assert torch.isfinite(a[..., rest]).all() and torch.isfinite(b[..., rest]).all()
+    assert torch.allclose(a[..., rest].float(), b[..., rest].float(), atol=2.0 ** -6, rtol=2.0 ** -7)
