@@ -2,7 +2,7 @@
 // sequences that share leading pages.
 //
 // Row (b, i, h) is query token i of sequence b at head h.  It sees the keys t < lim = len_b - qlen_b + i + 1 and
-//   out = sum_t p_t v_t / sum_t p_t,   p_t = 2^(s_t - m),   s_t = scale log2(e) q . k_t,   m >= max s_t - 8,
+//   out = sum_t p_t v_t / sum_t p_t,   p_t = 2^(s_t - m),   s_t = scale log2(e) q . k_t,   m + 8 <= max s_t <= m + 15,
 // one pass over the pages with a running m; k = code * scale + zero + residual (2-bit), level * scale + residual
 // (nvfp4, nf4) in fp32, rounded once to the fp16 matrix operand.  Partial results (m, sum p, sum p v) of page ranges
 // are fp32 and joined by q's row afterwards; a call whose rows each have one range writes the output directly.
@@ -24,7 +24,10 @@ namespace ffa {
 enum { kFmtQ2 = 0, kFmtNvfp4 = 1, kFmtNf4 = 2 };
 constexpr float kNoMax = -1e30f;  // m of a row that has seen no key: below every score, and 2^(x - m) stays defined
 constexpr float kLeast = 0x1p-126f;  // least factor of a joined sum: an infinity times it stays one (times 0: NaN)
-constexpr float kStale = 8.f;     // log2 units a row's m may lag its maximum: p <= 2^8 fits the fp16 operand as well
+// m lies kHead log2 units below the largest score when it is set, and may lag it by kStale more: p <= 2^15 fits the fp16
+// operand, whose steps of 2^-24 below 2^-14 are then at most 2^-32 of the largest weight.  (With kHead 0 they were up to
+// 2^-24 of it and smaller weights were lost: of 3300 tokens of 2^-25.7 each, 5.87e-5 together, 5.1e-5 came out.)
+constexpr float kHead = 8.f, kStale = 7.f;
 
 struct AttendParams {
   const void *q;
@@ -363,31 +366,30 @@ __device__ __forceinline__ bool softmax_step(f32x4 *S, float cs, int nvis, int g
       if (!MASK || 16 * g + k < nvis) top = fmaxf(top, x[k]);
     }
   top *= cs;
-  // the largest m may lag by kStale: most pages need no exchange between the row's four lanes and leave O as it is
-  const bool moved = __ballot(top > m + kStale) != 0;
+  // m may lag: most pages need no exchange between the row's four lanes and leave O as it is
+  const bool moved = __ballot(top > m + (kHead + kStale)) != 0;
   alpha = 1.f;
   if (moved) {
     top = xor_max(top, 16);
     top = xor_max(top, 32);
-    const float mn = fmaxf(m, top);
+    const float mn = fmaxf(m, top - kHead);
     alpha = exp2_hw(m - mn);
     m = mn;
     l *= alpha;
   }
-  float sum = 0.f;
 #pragma unroll
-  for (int k = 0; k < 16; ++k) {
-    x[k] = (!MASK || 16 * g + k < nvis) ? exp2_hw(__builtin_fmaf(x[k], cs, -m)) : 0.f;
-    sum += x[k];
-  }
-  l += sum;
+  for (int k = 0; k < 16; ++k) x[k] = (!MASK || 16 * g + k < nvis) ? exp2_hw(__builtin_fmaf(x[k], cs, -m)) : 0.f;
+  float sum = 0.f;  // of the weights as they are multiplied: their rounding then leaves a weighted mean of the same values
 #pragma unroll
   for (int kap = 0; kap < 2; ++kap) {
     u32x4 w;
 #pragma unroll
     for (int i = 0; i < 4; ++i) w[i] = pk_f16_bits(x[8 * kap + 2 * i], x[8 * kap + 2 * i + 1]);
     P[kap] = __builtin_bit_cast(f16x8, w);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sum += (float)P[kap][i];
   }
+  l += sum;
   return moved;
 }
 
@@ -791,12 +793,12 @@ __device__ __forceinline__ void many_rows(const AttendParams &p, int split, int 
 #pragma unroll
       for (int k = 1; k < 16; ++k) x = fmaxf(x, S[t][k >> 2][k & 3]);
       top[t] = x * cs[t];
-      lag |= top[t] > m[t] + kStale;
+      lag |= top[t] > m[t] + (kHead + kStale);
     }
     if (__ballot(lag) != 0) {
 #pragma unroll
       for (int t = 0; t < na(); ++t) {
-        const float mn = fmaxf(m[t], xor_max(xor_max(top[t], 16), 32));
+        const float mn = fmaxf(m[t], xor_max(xor_max(top[t], 16), 32) - kHead);
         const float alpha = exp2_hw(m[t] - mn);
         m[t] = mn;
         Ls[t] *= alpha;

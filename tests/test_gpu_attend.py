@@ -457,3 +457,45 @@ def test_infinities_of_small_weight_in_shared_pages(gpu, members, L, HQ, own):
     rest = [c for c in range(128) if c not in (5, 6, 7)]
     assert torch.isfinite(a[..., rest]).all() and torch.isfinite(b[..., rest]).all()
     assert torch.allclose(a[..., rest].float(), b[..., rest].float(), atol=2.0 ** -6, rtol=2.0 ** -7)
+
+
+@pytest.mark.parametrize("fmt", ["q2", "nvfp4", "nf4"])
+@pytest.mark.parametrize("n,L,HQ", [
+    (2000, 1, 4), (2000, 4, 8),     # one and two tiles of rows
+    (2000, 40, 1), (2000, 30, 4),   # operands in LDS
+    (9000, 1, 8), (3300, 150, 4),   # ranges of pages, joined
+])
+def test_constant_values(gpu, fmt, n, L, HQ):
+    """V of ones gives ones, whatever the weights round to: the sum below the fraction bar is that of the weights that are
+    multiplied.  (Both sums are chains of at most 52 pages x 32 fp32 additions, off by 52 x 32 x 2^-24 < 2^-13 each; half a
+    step of fp16 below 1 is 2^-12.)"""
+    g = torch.Generator().manual_seed(101)
+    cache, table, sl, _ = _batch(fmt, [n], HQ, 1, 1, torch.float16, 101, gpu)
+    u = torch.sign(_rand(g, 128))
+    k = (-u).repeat(n, 1, 1)
+    k[3::64] = u  # one key of every page above the others, which have one score
+    fill(cache, k, torch.ones(n, 1, 128), table[0])
+    q = u.expand(1, L, HQ, 128).half().contiguous().to(gpu)
+    for step in range(24):  # 2 to 4 log2 units below: weights that round by up to half a step either way
+        out = cache.attend(q, table, sl, scale=(2 + step / 12) * math.log(2) / 256)
+        assert (out == 1).all(), (step, out.float().min(), out.float().max())
+
+
+@pytest.mark.parametrize("fmt,v", [("q2", torch.float16), ("nvfp4", torch.bfloat16), ("nf4", torch.float16)])
+@pytest.mark.parametrize("depth", [20, 25, 27, 30])
+@pytest.mark.parametrize("n,L,HQ", [(2000, 1, 4), (2000, 4, 8), (2000, 30, 4), (9000, 1, 8), (3300, 150, 4)])
+def test_many_small_weights(gpu, fmt, v, depth, n, L, HQ):
+    """Keys far below the largest score, which together weigh something: their weights are not lost below fp16's steps."""
+    g = torch.Generator().manual_seed(103)
+    cache, table, sl, _ = _batch(fmt, [n], HQ, 1, 1, torch.float16, 103, gpu, v=v)
+    u = torch.sign(_rand(g, 128))
+    k, vv = (-u).repeat(n, 1, 1), torch.ones(n, 1, 128)
+    k[3], vv[3] = u, 0
+    fill(cache, k, vv, table[0])
+    q = u.expand(1, L, HQ, 128).half().contiguous().to(gpu)
+    scale = depth * math.log(2) / 256
+    out = cache.attend(q, table, sl, scale=scale)
+    k, vv = logical_kv(cache, fmt, table[0, :-(-n // 64)].tolist())
+    some = sorted({0, L // 2, L - 1})
+    o, bound = reference(q[0], k[:n], vv[:n], n, L, scale, some)
+    assert_close(out[0, some], o[some], bound[some], q.dtype)
