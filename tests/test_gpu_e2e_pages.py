@@ -238,3 +238,56 @@ def test_a_new_prompt_after_samples(gpu):
         outs = [y.pool.decode(q, y.block_table, y.seq_lens, T=y.capacity, workspace=y.workspace(8, 64, 64, q.dtype)).o
                 for y in (x.layer, fresh)]
         assert torch.equal(*outs)
+
+
+def _copying(C):
+    """The cache with every sequence's pages its own: batch operations copy them."""
+
+    class Layer(C.Q2FP8PagedLayer):
+        def _select(self, indices, check):
+            if not self.is_initialized:
+                return
+            old, table, idx = self.pool, self.block_table, indices.reshape(-1).cpu()
+            npg = table.shape[1]
+            self.pool = type(old)(len(idx) * npg, old.HKV, self.device, res_dtype=old.res_dtype, v_dtype=old.v_dtype)
+            source = table[idx.to(table.device)].reshape(-1).long()
+            for new, t in zip(self.pool.pools(), old.pools()):
+                new.view(torch.uint8).copy_(t.view(torch.uint8)[source])
+            self.block_table = torch.arange(len(idx) * npg, dtype=torch.int32, device=self.device).view(-1, npg)
+            self.seq_lens = torch.full((len(idx),), self.seq_len, dtype=torch.int32, device=self.device)
+
+    def cache(layers, batch, length):
+        made = C.Q2FP8Cache(num_layers=layers, max_batch_size=batch, max_cache_len=length)
+        made.layers = [Layer(batch, length, page_seed=i) for i in range(layers)]
+        return made
+
+    return cache
+
+
+@pytest.mark.parametrize("ffa_decode", [True, False])
+def test_beams_are_those_of_copied_caches(gpu, ffa_decode):
+    """transformers' beam search over shared pages: the same tokens and scores, bit for bit, as over caches that copy."""
+    from transformers import LlamaConfig, LlamaForCausalLM
+
+    C = _load()
+    cfg = LlamaConfig(vocab_size=96, hidden_size=512, intermediate_size=512, num_hidden_layers=2, num_attention_heads=4,
+                      num_key_value_heads=2, head_dim=128, max_position_embeddings=512)
+    torch.manual_seed(4)
+    model = LlamaForCausalLM(cfg).to(device=gpu, dtype=torch.bfloat16).eval()
+    C.enable_ffa_q2fp8(model, use_ffa_decode=ffa_decode, paged_exact=True)
+    ids = torch.randint(0, 96, (2, 120), generator=torch.Generator().manual_seed(5)).to(gpu)
+    runs = []
+    for make in (lambda *a: C.Q2FP8Cache(num_layers=a[0], max_batch_size=a[1], max_cache_len=a[2]), _copying(C)):
+        cache = make(2, 8, 256)
+        with torch.no_grad():
+            out = model.generate(ids, past_key_values=cache, max_new_tokens=30, num_beams=4, num_return_sequences=4,
+                                 do_sample=False, pad_token_id=0, eos_token_id=None, return_dict_in_generate=True,
+                                 output_scores=True)
+        runs.append((out.sequences, out.sequences_scores, out.beam_indices))
+        assert cache.get_seq_length() == 149
+    assert runs[0][0].shape == (8, 150) and torch.equal(runs[0][0][:, :120], ids.repeat_interleave(4, 0))
+    assert len({tuple(r) for r in runs[0][0].tolist()}) == 8
+    moved = runs[0][2][:, 1:30] - runs[0][2][:, :29]
+    assert (moved != 0).any()  # beams changed places
+    for a, b in zip(*runs):
+        assert torch.equal(a, b)
