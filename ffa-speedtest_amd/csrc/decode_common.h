@@ -306,6 +306,13 @@ enum { kChannel = 0, kG32 = 1, kChannelF32 = 2 };
 enum { kResNone = 0, kResE4M3 = 1, kResE5M2 = 2 };
 enum { kVF16 = 0, kVBF16 = 1 };
 
+// QLoRA NF4 levels (the published 16 normal-float values), as fp32
+static __constant__ float kNF4Levels[16] = {
+    -1.0f, -0.6961928009986877f, -0.5229921340942383f, -0.39491748809814453f, -0.28444138169288635f,
+    -0.18477343022823334f, -0.09105003625154495f, 0.0f, 0.07958029955625534f, 0.16093020141124725f,
+    0.24611230194568634f, 0.33791524171829224f, 0.44070982933044434f, 0.5626170039176941f,
+    0.7229568362236023f, 1.0f};
+
 // 8 fp8 residual bytes -> 8 fp16 (exact)
 template <int RES>
 __device__ __forceinline__ f16x8 fp8x8_to_f16x8(uint32_t lo, uint32_t hi) {

@@ -60,13 +60,6 @@ __device__ __forceinline__ uint32_t mul_pack_f16(float a, float sa, float b, flo
   return __builtin_bit_cast(uint32_t, h2{lo, hi});
 }
 
-// QLoRA NF4 levels (the published 16 normal-float values), as fp32
-__constant__ float kNF4Levels[16] = {
-    -1.0f, -0.6961928009986877f, -0.5229921340942383f, -0.39491748809814453f, -0.28444138169288635f,
-    -0.18477343022823334f, -0.09105003625154495f, 0.0f, 0.07958029955625534f, 0.16093020141124725f,
-    0.24611230194568634f, 0.33791524171829224f, 0.44070982933044434f, 0.5626170039176941f,
-    0.7229568362236023f, 1.0f};
-
 // two fp8 values (bytes 2*HI, 2*HI+1 of w) -> f32, exact
 template <bool E4M3, bool HI>
 __device__ __forceinline__ f32x2 fp8pair_f32(uint32_t w) {

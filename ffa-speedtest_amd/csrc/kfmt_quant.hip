@@ -260,22 +260,6 @@ __global__ __launch_bounds__(256) void nvfp4_quant8_kernel(const void *k, int T,
 // ---------------------------------------------------------------------------
 // nf4: per-channel absmax over T (splits, then a final pass), then codes
 // ---------------------------------------------------------------------------
-__constant__ float kNF4Book[16] = {-1.0f,
-                                   -0.6961928009986877f,
-                                   -0.5229921340942383f,
-                                   -0.39491748809814453f,
-                                   -0.28444138169288635f,
-                                   -0.18477343022823334f,
-                                   -0.09105003625154495f,
-                                   0.0f,
-                                   0.07958029955625534f,
-                                   0.16093020141124725f,
-                                   0.24611230194568634f,
-                                   0.33791524171829224f,
-                                   0.44070982933044434f,
-                                   0.5626170039176941f,
-                                   0.7229568362236023f,
-                                   1.0f};
 constexpr int kNF4Tok = 256;  // tokens per absmax split
 
 __global__ __launch_bounds__(256) void nf4_absmax_kernel(const void *k, int kdt, int T, int C, int nsplit,
@@ -326,8 +310,8 @@ __global__ __launch_bounds__(256) void nf4_quant_kernel(const void *k, int kdt, 
     // bucketize(x, midpoints) (right=False): count of midpoints < x
     int idx = 0;
 #pragma unroll
-    for (int j = 0; j < 15; ++j) idx += ((kNF4Book[j] + kNF4Book[j + 1]) * 0.5f < x) ? 1 : 0;
-    res[row * D + d] = (uint8_t)f32_to_fp8(kv - kNF4Book[idx] * sc, e4m3);
+    for (int j = 0; j < 15; ++j) idx += ((kNF4Levels[j] + kNF4Levels[j + 1]) * 0.5f < x) ? 1 : 0;
+    res[row * D + d] = (uint8_t)f32_to_fp8(kv - kNF4Levels[idx] * sc, e4m3);
     pk |= (uint32_t)idx << (4 * e);
   }
   packed[row * DP + byte] = (uint8_t)pk;
@@ -379,8 +363,8 @@ __global__ __launch_bounds__(256) void kfmt_group_append_kernel(const void *k, i
       const float x = fminf(fmaxf(__fdiv_rn(kv[e], sc), -1.0f), 1.0f);
       int idx = 0;
 #pragma unroll
-      for (int j = 0; j < 15; ++j) idx += ((kNF4Book[j] + kNF4Book[j + 1]) * 0.5f < x) ? 1 : 0;
-      rw[e >> 2] |= f32_to_fp8(kv[e] - kNF4Book[idx] * sc, res_e4m3) << (8 * (e & 3));
+      for (int j = 0; j < 15; ++j) idx += ((kNF4Levels[j] + kNF4Levels[j + 1]) * 0.5f < x) ? 1 : 0;
+      rw[e >> 2] |= f32_to_fp8(kv[e] - kNF4Levels[idx] * sc, res_e4m3) << (8 * (e & 3));
       cw[e >> 3] |= (uint32_t)idx << (4 * (e & 7));
     }
     if (wr && (c16 & 3) == 0) ((uint16_t *)s_pages)[prow * 2 + (c16 >> 2)] = (uint16_t)f32_to_f16_bits(sc);
@@ -425,7 +409,7 @@ __device__ __forceinline__ float nf4_turn(float sc, float mid) {
   if ((u & 1u) ? (double)f < v : (double)f <= v) f = __uint_as_float(__float_as_uint(f) + (f < 0.f ? 0xffffffffu : 1u));
   return f;
 }
-__device__ __forceinline__ float nf4_mid(int j) { return (kNF4Book[j] + kNF4Book[j + 1]) * 0.5f; }
+__device__ __forceinline__ float nf4_mid(int j) { return (kNF4Levels[j] + kNF4Levels[j + 1]) * 0.5f; }
 __device__ __forceinline__ uint32_t nf4_index_div(float kv, float sc) {
   const float x = fminf(fmaxf(__fdiv_rn(kv, sc), -1.0f), 1.0f);
   uint32_t idx = 0;
@@ -462,7 +446,7 @@ __global__ __launch_bounds__(256) void kfmt_page_append_kernel(const void *k, in
   const int hkv = blockIdx.x, b = blockIdx.z;
   const PageTile pt = page_tile(pos, bt, bt_stride, num_pages, b, blockIdx.y, Tn);
   if (pt.page < 0) return;  // the whole workgroup
-  if (NF4 && threadIdx.x < 16) s_book[threadIdx.x] = kNF4Book[threadIdx.x];  // read after page_tile_k's barriers
+  if (NF4 && threadIdx.x < 16) s_book[threadIdx.x] = kNF4Levels[threadIdx.x];  // read after page_tile_k's barriers
   const size_t row0 = (size_t)b * Tn * HKV + hkv, blk = (size_t)pt.page * HKV + hkv;
   float x[32];
   page_tile_k<KDT>(k, row0, HKV, pt, s_t, x);

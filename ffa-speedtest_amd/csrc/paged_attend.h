@@ -52,13 +52,6 @@ struct AttendParams {
   int shared_blocks, shared_wgs;  // of the launch of both kinds
 };
 
-// QLoRA NF4 levels (the published 16 normal-float values)
-__constant__ float kAttendNF4[16] = {
-    -1.0f, -0.6961928009986877f, -0.5229921340942383f, -0.39491748809814453f, -0.28444138169288635f,
-    -0.18477343022823334f, -0.09105003625154495f, 0.0f, 0.07958029955625534f, 0.16093020141124725f,
-    0.24611230194568634f, 0.33791524171829224f, 0.44070982933044434f, 0.5626170039176941f,
-    0.7229568362236023f, 1.0f};
-
 __device__ __forceinline__ int seq_len_of(const AttendParams &p, int b) {
   return p.seq_lens ? min(max(p.seq_lens[b], 0), p.T) : p.T;
 }
@@ -433,7 +426,7 @@ __device__ __forceinline__ void few_rows(const AttendParams &p, int split, int h
   const int pa = set.p0, pe = set.p1;
   if (pa >= pe && p.nslots != 0) return;
   if constexpr (FMT == kFmtNf4) {
-    if (threadIdx.x < 256) s.nf4[threadIdx.x] = make_float2(kAttendNF4[threadIdx.x & 15], kAttendNF4[threadIdx.x >> 4]);
+    if (threadIdx.x < 256) s.nf4[threadIdx.x] = make_float2(kNF4Levels[threadIdx.x & 15], kNF4Levels[threadIdx.x >> 4]);
     __syncthreads();
   }
 
@@ -730,7 +723,7 @@ __device__ __forceinline__ void many_rows(const AttendParams &p, int split, int 
     s.hi[wv] = hi;
   }
   if constexpr (FMT == kFmtNf4)
-    if (threadIdx.x < 256) s.nf4[threadIdx.x] = make_float2(kAttendNF4[threadIdx.x & 15], kAttendNF4[threadIdx.x >> 4]);
+    if (threadIdx.x < 256) s.nf4[threadIdx.x] = make_float2(kNF4Levels[threadIdx.x & 15], kNF4Levels[threadIdx.x >> 4]);
   __syncthreads();
 #pragma unroll
   for (int w = 0; w < W; ++w) {
