@@ -16,6 +16,7 @@
 
 #include "decode_common.h"
 #include "ffa_mi355x.h"
+#include "routes.h"
 
 #include <type_traits>
 
@@ -914,9 +915,6 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) void p
     few_rows<FMT, RES, VT, NT, 8>(p, split, y % p.HKV, 0, p.nshared + y / p.HKV, s.few);
   }
 }
-
-// the kernel for so many rows of a KV head and set, and the rows of its workgroup
-enum { kRows16 = 0, kRows32, kRows64, kRows128, kRows256 };
 
 // One launch over `sets` sets (own < 0), or one of both kinds: shared pages by 256 rows a workgroup, own pages by the
 // kernel for few rows of kind `own`.

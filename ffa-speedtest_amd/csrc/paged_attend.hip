@@ -84,27 +84,10 @@ struct AttendPlan {
   bool both;  // one launch of 256-row workgroups over shared pages and of few-row ones over own pages
 };
 
-// the kernel for so many rows of a KV head and set, and the rows of its workgroup
-static int kind_for(long rows) {
-  return rows <= 16 ? kRows16 : (rows <= 32 ? kRows32 : (rows <= 64 ? kRows64 : (rows <= 128 ? kRows128 : kRows256)));
-}
-static long kind_rows(int kind) { return 16l << kind; }
-
-// Ranges of ppw pages so that `units` (pages over all sets, heads and row blocks) make about `want` workgroups
-static void page_ranges(long units, int pages, long want, int &ppw, int &slots) {
-  long w = (units + want - 1) / want;
-  w = (w + 3) / 4 * 4;  // a page for each of four waves
-  if (w > pages) w = (pages + 3) / 4 * 4;
-  ppw = (int)(w < 4 ? 4 : w);
-  slots = (pages + ppw - 1) / ppw;
-}
-
 static AttendPlan attend_plan(const ffa_paged_attend_args *a, int cus) {
   AttendPlan pl = {};
   if (cus <= 0) cus = 256;
   const long LG = (long)a->L * (a->HQ / a->HKV);
-  // workgroups that are resident at a time: one round of them (a second one that is not full costs as much)
-  auto resident = [&](int kind) { return (kind == kRows256 ? 1l : 2l) * cus; };
   long units = 0, rows = 0;
   int most = 0, least = a->ngroups > 0 ? a->group_pages_host[0] : 0;  // shared pages
   for (int g = 0; g < a->ngroups; ++g) {
@@ -115,38 +98,25 @@ static AttendPlan attend_plan(const ffa_paged_attend_args *a, int cus) {
     if (gp < least) least = gp;
   }
   const int own = (a->T + kPage - 1) / kPage - least;
-  pl.own_kind = kind_for(LG);
-  auto workgroups = [&](int kind) { return (LG + kind_rows(kind) - 1) / kind_rows(kind) * a->HKV * a->B; };
-  // Over few pages a workgroup's fixed 10-14 us count as much as its pages': smaller ones then, and ranges that are
-  // split (their partials are rows x 528 bytes, written and read) only where the chip is not half full
-  const bool brief = pl.own_kind > kRows64 && own < 48;
-  if (brief) pl.own_kind = workgroups(kRows128) > cus ? kRows128 : kRows64;
-  pl.own_blocks = (int)((LG + kind_rows(pl.own_kind) - 1) / kind_rows(pl.own_kind));
+  const long heads = (long)a->B * a->HKV;
+  pl.own_kind = attend_own_kind(LG, heads, own, cus);
+  pl.own_blocks = (int)attend_blocks(LG, pl.own_kind);
   if (own > 0) {
     int ppw;  // of the longest sequence
-    page_ranges((long)own * a->HKV * pl.own_blocks * a->B, own, resident(pl.own_kind), ppw, pl.own_slots);
-    if (brief && 2 * workgroups(pl.own_kind) >= cus) pl.own_slots = 1;
+    page_ranges((long)own * heads * pl.own_blocks, own, attend_resident(pl.own_kind, cus), ppw, pl.own_slots);
+    if (attend_one_range(LG, heads, own, cus)) pl.own_slots = 1;
   }
   if (most > 0) {
-    pl.shared_kind = kind_for(rows);
-    const long kr = kind_rows(pl.shared_kind);
-    pl.shared_blocks = (int)((rows + kr - 1) / kr);
+    pl.shared_kind = attend_kind(rows);
+    pl.shared_blocks = (int)attend_blocks(rows, pl.shared_kind);
     for (int g = 0; g < a->ngroups; ++g) {
       const long n = a->group_start_host[g + 1] - a->group_start_host[g];
-      units += (long)a->group_pages_host[g] * a->HKV * ((n * LG + kr - 1) / kr);
+      units += (long)a->group_pages_host[g] * a->HKV * attend_blocks(n * LG, pl.shared_kind);
     }
-    long want = resident(pl.shared_kind);
-    // Both kinds in one launch: the shared pages get the share of the CUs that their work is of all, in us of a CU: a
-    // page of 256 rows 2.15, and 14 a workgroup; an own page of few rows 1.2.  64 sequences behind 32K tokens, own
-    // tokens up to 2000: 107 -> 86 us (two launches -> 56 %; 75 % 96), up to 8000 234 -> 197, 66 sequences of five groups
-    // 82 -> 74.  Own ranges too short for eight waves stay apart (256 sequences of 3 pages 91 -> 100).
-    const long pages = a->own_pages_host;
-    pl.both = pl.shared_kind == kRows256 && pl.own_kind <= kRows32 && own > 0 && pages >= 4l * a->B &&
-              (long)a->B * a->HKV * pl.own_slots < 1l << 30;
-    if (pl.both) {
-      const double many = 2.15 * units + 14. * cus, few = 1.2 * pages * a->HKV, share = many / (many + few);
-      want = (long)(want * (share < 0.4 ? 0.4 : share)) + 1;
-    }
+    long want = attend_resident(pl.shared_kind, cus);
+    pl.both = attend_both(pl.shared_kind, pl.own_kind, a->own_pages_host, a->B) && own > 0 &&
+              heads * pl.own_slots < 1l << 30;
+    if (pl.both) want = attend_shared_wgs(units, a->own_pages_host * a->HKV, cus);
     page_ranges(units, most, want, pl.shared_ppw, pl.shared_slots);
     pl.both = pl.both && (long)a->HKV * pl.shared_blocks * pl.shared_slots * a->ngroups < 1l << 30;
   }
@@ -263,7 +233,7 @@ extern "C" int ffa_paged_attend(const ffa_paged_attend_args *a, void *stream) {
     p.nshared = 0;
     if (pl.own_slots > 0) launch(pl.own_kind, pl.own_slots, pl.own_blocks, a->B, -1);
   }
-  if (pl.nslots > 0 && rows <= 2048)  // (4224 rows of 18 slots 69.5 -> 66 us by a wave each, 2048 the same or 1 % slower)
+  if (pl.nslots > 0 && !join_by_wave((long)rows))
     hipLaunchKernelGGL(paged_attend_join_kernel<4>, dim3((unsigned)rows), dim3(256), 0, st, p, (int)rows);
   else if (pl.nslots > 0)
     hipLaunchKernelGGL(paged_attend_join_kernel<1>, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, p, (int)rows);

@@ -92,4 +92,55 @@ inline int kproj_route(int M, int N, int cus) {
 // and without a graph, where the launches count, 20-21 / 22-24 up to 16384 entries, 24 / 22 at 65536.
 inline bool fork_check_apart(int children, int cols) { return (long)children * cols > 16384; }
 
+// Exact attention over the pages: the kernel for so many rows of a KV head and set (a sequence, or a group that shares
+// pages), and the rows of its workgroup.  Up to 32 rows operands come straight from memory (17-32 rows through LDS: five
+// drafted tokens of 8 sequences, nf4, 215 -> 335 us); from 33 on through LDS (16 rows x 4 behind 32K tokens 53 -> 41).
+enum { kRows16 = 0, kRows32, kRows64, kRows128, kRows256 };
+inline long attend_kind_rows(int kind) { return 16l << kind; }
+inline long attend_blocks(long rows, int kind) { return (rows + attend_kind_rows(kind) - 1) / attend_kind_rows(kind); }
+inline int attend_kind(long rows) {
+  return rows <= 16 ? kRows16 : (rows <= 32 ? kRows32 : (rows <= 64 ? kRows64 : (rows <= 128 ? kRows128 : kRows256)));
+}
+// workgroups that are resident at a time: one round of them (a second one that is not full costs as much)
+inline long attend_resident(int kind, int cus) { return (kind == kRows256 ? 1l : 2l) * cus; }
+
+// Chunks of many rows over fewer than 48 pages, where a workgroup's fixed 10-14 us count as much as its pages': smaller
+// workgroups then, and ranges that are split (their partials are rows x 528 bytes, written and read) only where the chip
+// is not half full.  A prompt of 700 tokens 56 -> 22 us, 4 of 1024 81 -> 73.  heads: sequences x KV heads.
+inline bool attend_brief(long rows, int pages) { return attend_kind(rows) > kRows64 && pages < 48; }
+inline int attend_own_kind(long rows, long heads, int pages, int cus) {
+  if (!attend_brief(rows, pages)) return attend_kind(rows);
+  return attend_blocks(rows, kRows128) * heads > cus ? kRows128 : kRows64;
+}
+inline bool attend_one_range(long rows, long heads, int pages, int cus) {
+  return attend_brief(rows, pages) && 2 * attend_blocks(rows, attend_own_kind(rows, heads, pages, cus)) * heads >= cus;
+}
+
+// Ranges of ppw pages so that `units` (pages over all sets, heads and row blocks) make about `want` workgroups
+inline void page_ranges(long units, int pages, long want, int &ppw, int &slots) {
+  long w = (units + want - 1) / want;
+  w = (w + 3) / 4 * 4;  // a page for each of four waves
+  if (w > pages) w = (pages + 3) / 4 * 4;
+  ppw = (int)(w < 4 ? 4 : w);
+  slots = (pages + ppw - 1) / ppw;
+}
+
+// Shared pages of 256-row workgroups and own pages of few rows in one launch: 64 sequences behind 32K tokens, own tokens
+// up to 2000, 107 -> 86 us, up to 8000 234 -> 197; 66 sequences of five groups 82 -> 74.  Own ranges too short for eight
+// waves stay apart (256 sequences of 3 pages 91 -> 100).
+inline bool attend_both(int shared_kind, int own_kind, long own_pages, int B) {
+  return shared_kind == kRows256 && own_kind <= kRows32 && own_pages >= 4l * B;
+}
+// The shared pages' workgroups there: the share of the CUs that their work is of all, in us of a CU: a page of 256 rows
+// 2.15, and 14 a workgroup; an own page of a KV head 1.2.  (Fixed shares of 50 / 63 / 75 / 88 / 100 %: the first case above 86 /
+// 97 / 96 / 103 / 109 us, the groups 84 / 84 / 74 / 74 / 79, 16 x 5 drafts behind 64K tokens 278 / 230 / 199 / 176 / 169.)
+inline long attend_shared_wgs(long units, long own_head_pages, int cus) {
+  const double many = 2.15 * units + 14. * cus, few = 1.2 * own_head_pages, share = many / (many + few);
+  return (long)(cus * (share < 0.4 ? 0.4 : share)) + 1;
+}
+
+// The join of a row's partials by one wave, four rows a workgroup, rather than by four waves: 4224 rows of 18 slots 69.5
+// -> 66 us, 2048 the same or 1 % slower
+inline bool join_by_wave(long rows) { return rows > 2048; }
+
 }  // namespace ffa

@@ -90,3 +90,32 @@ def test_fork_checks(routes):
     apart = [(64, 1024), (256, 1024), (1, 16385), (65535, 1 << 24)]
     got = routes(*(f"fork_check_apart({c}, {n})" for c, n in inside + apart))
     assert got == [0] * len(inside) + [1] * len(apart)
+
+
+def test_attention_kernels(routes):
+    """The kernel by the rows of a KV head; smaller workgroups and whole ranges for chunks over few pages (256 CUs)."""
+    want = {"kRows16": (1, 16), "kRows32": (17, 32), "kRows64": (33, 64), "kRows128": (65, 128), "kRows256": (129, 1 << 30)}
+    for kind, sizes in want.items():
+        assert routes(*(f"attend_kind({n}) == {kind}" for n in sizes)) == [1, 1], kind
+        assert routes(*(f"attend_own_kind({n}, 8, 48, 256) == {kind}" for n in sizes)) == [1, 1], kind  # not few pages
+    # (rows, sequences x KV heads, pages): prompts of 700 tokens (4 rows a token, 8 heads), 4 of 1024, three of 701 with
+    # 64 query heads; decode steps and drafts stay with the kernel of their rows
+    cases = {(2800, 8, 11): ("kRows64", 1), (4096, 32, 16): ("kRows128", 1), (5608, 24, 11): ("kRows128", 1),
+             (400, 1, 47): ("kRows64", 0), (8192, 8, 256): ("kRows256", 0), (4, 128, 10): ("kRows16", 0),
+             (20, 64, 10): ("kRows32", 0)}
+    for (rows, heads, pages), (kind, one) in cases.items():
+        assert routes(f"attend_own_kind({rows}, {heads}, {pages}, 256) == {kind}",
+                      f"attend_one_range({rows}, {heads}, {pages}, 256)") == [1, one], (rows, heads, pages)
+
+
+def test_attention_launches(routes):
+    """Shared and own pages in one launch, and the shared pages' workgroups; the join."""
+    both = [("kRows256", "kRows16", 1000, 64), ("kRows256", "kRows32", 264, 66)]
+    apart = [("kRows256", "kRows16", 768, 256), ("kRows128", "kRows16", 1000, 64), ("kRows256", "kRows64", 1000, 64)]
+    assert routes(*(f"attend_both({s}, {o}, {n}, {B})" for s, o, n, B in both + apart)) == [1] * 2 + [0] * 3
+    # 64 sequences behind 32K tokens with some 1000 own pages: about 56 %; drafts behind 64K tokens with few own pages:
+    # nearly all; hardly any shared pages: 40 % at the least
+    some, most, least = routes("attend_shared_wgs(512 * 8, 1050 * 8, 256)", "attend_shared_wgs(1024 * 8 * 2, 70 * 8, 256)",
+                               "attend_shared_wgs(8, 1 << 24, 256)")
+    assert 0.5 * 256 <= some <= 0.62 * 256 and most >= 0.95 * 256 and least == 103
+    assert routes("join_by_wave(2048)", "join_by_wave(2049)", "join_by_wave(4224)") == [0, 1, 1]
