@@ -23,10 +23,11 @@ Here, for q2fp8, on the MI355X library:
   FlashAttention to the keys its cache returns dequantized from every update, fp8fp8_cache.py:60-69,
   84-89).  The exact attention itself is fp32 torch matmuls, as the reference's is a library call; with
   `paged_exact=True` those steps of fp16 / bf16 models run `PagedQ2Cache.attend` instead, which reads the
-  quantized pages themselves, and the pages that sequences share once.
+  quantized pages themselves, and the pages that samples of a prompt share once (after `reorder_cache`, which
+  reads nothing back, every beam's pages for it alone).
 * Batch operations of transformers' caches (`batch_repeat_interleave`: samples of a prompt,
   `batch_select_indices`, `reorder_cache`: beams, `crop`) fork and free pages (`ffa_mi355x.pages`) instead of
-  copying caches: whole pages are shared, partial last pages copied.
+  copying caches: whole pages are shared, partial last pages copied.  Every layer counts its own pages.
 
 The HF models apply RoPE (their half-split `rotate_half`) before `Cache.update`, so the cache receives
 rotated K and appends it with the quantize-append entry point; the fused K-projection + RoPE producer
@@ -210,7 +211,8 @@ class Q2FP8PagedLayer(CacheLayerMixin):
             self.shared = SharedPrefix(self.block_table, self.seq_lens)
 
     def reorder_cache(self, beam_idx: torch.LongTensor) -> None:
-        """Beam search: beam i continues beam beam_idx[i] (within the batch).  Does not synchronise."""
+        """Beam search: beam i continues beam beam_idx[i] (within the batch).  Does not synchronise, and makes no plan
+        of the shared pages (a read of the table): exact steps then read every beam's pages for it alone."""
         self._select(beam_idx, False)
 
     def crop(self, tokens_to_remove: int) -> None:

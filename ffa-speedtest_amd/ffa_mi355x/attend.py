@@ -27,7 +27,8 @@ class SharedPrefix:
 
     group_sizes: sequences per group, in batch order (their sum is the batch); by default a sequence belongs to
     the group before it if its first page is that group's.  A group's shared pages are the longest run of equal
-    leading page ids that lie wholly inside every member (seq_lens).  Reads block_table and seq_lens on the host
+    leading page ids that lie wholly inside every member (seq_lens): one level, so requests behind one short system
+    prompt and each with samples of its own are better given as groups of samples (group_sizes).  Reads block_table and seq_lens on the host
     (once: make it when sequences are forked, not per step).  It stays valid while the members keep those pages;
     their own pages and lengths may change, so it serves every step until a fork, free or compaction."""
 
