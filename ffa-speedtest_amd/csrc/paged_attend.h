@@ -16,13 +16,15 @@
 
 #include "decode_common.h"
 #include "ffa_mi355x.h"
+#include "mxfp4.h"
 #include "routes.h"
 
 #include <type_traits>
 
 namespace ffa {
 
-enum { kFmtQ2 = 0, kFmtNvfp4 = 1, kFmtNf4 = 2 };
+enum { kFmtQ2 = 0, kFmtNvfp4 = 1, kFmtNf4 = 2, kFmtMxfp4 = 3 };
+enum { kVMxfp4 = 2 };  // V of mxfp4 pages, beside kVF16 and kVBF16
 constexpr float kNoMax = -1e30f;  // m of a row that has seen no key: below every score, and 2^(x - m) stays defined
 constexpr float kLeast = 0x1p-126f;  // least factor of a joined sum: an infinity times it stays one (times 0: NaN)
 // m lies kHead log2 units below the largest score when it is set, and may lag it by kStale more: p <= 2^15 fits the fp16
@@ -51,6 +53,7 @@ struct AttendParams {
   int nshared;
   int shared_slots, shared_ppw, own_slots;
   int shared_blocks, shared_wgs;  // of the launch of both kinds
+  const uint8_t *vs;              // mxfp4 pages: V's scales
 };
 
 __device__ __forceinline__ int seq_len_of(const AttendParams &p, int b) {
@@ -307,6 +310,15 @@ __device__ __forceinline__ void add_not_finite(const uint8_t *v, int g, int nvis
       }
 }
 
+// the same of an mxfp4 page: NaN into the columns of the blocks that are NaN at a token that the lane's row sees
+__device__ __forceinline__ void add_nan_blocks(const uint8_t *vs, int nvis, f32x4 *o) {
+#pragma unroll 1
+  for (int t = 0; t < nvis && t < kPage; ++t)
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
+      if (vs[(u >> 1) * kPage + t] == kMxNan) o[u] = f32x4{NAN, NAN, NAN, NAN};
+}
+
 // The sums o of a row tile after its pages pa, pa + step, .. below pe.  A page that all rows of a workgroup see is
 // multiplied as it is: an infinity of V comes out as one, or as NaN where the weight rounds to 0 or a later maximum
 // scales the sum by 0.  A column that is not finite becomes the sum of the infinities and NaN that the row sees in it,
@@ -416,6 +428,55 @@ struct FewLds {
   float o[W][16][kD + 4];
   float2 nf4[FMT == kFmtNf4 ? 256 : 1];
 };
+// The waves' results of the rows r0 .. joined in LDS and stored.  m, l, O: as softmax_step leaves them.
+template <int NT, int W, class Lds>
+__device__ __forceinline__ void join_waves(const AttendParams &p, const AttendSet &set, int hkv, int r0, float *m, float *l,
+                                           f32x4 (*O)[8], Lds &s) {
+  const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int g = lane >> 4, n = lane & 15, LG = p.L * p.G, R = set.n * LG;
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    l[t] = xor_sum(l[t], 16);
+    l[t] = xor_sum(l[t], 32);
+    if (g == 0) {
+      s.m[wv][16 * t + n] = m[t];
+      s.l[wv][16 * t + n] = l[t];
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    float M = kNoMax;
+#pragma unroll
+    for (int w = 0; w < W; ++w) M = fmaxf(M, s.m[w][16 * t + n]);
+    const float f = fmaxf(exp2_hw(m[t] - M), kLeast);
+#pragma unroll
+    for (int u = 0; u < 8; ++u) *(f32x4 *)&s.o[wv][n][16 * u + 4 * g] = O[t][u] * f;
+    __syncthreads();
+    constexpr int C = 32 / W;  // columns per thread
+    const int rr = threadIdx.x / (kD / C), c0 = C * (threadIdx.x % (kD / C));
+    const int r = r0 + 16 * t + rr;
+    if (r < R) {
+      float mm = kNoMax, ll = 0.f, o[C] = {};
+#pragma unroll
+      for (int w = 0; w < W; ++w) mm = fmaxf(mm, s.m[w][16 * t + rr]);
+#pragma unroll
+      for (int w = 0; w < W; ++w) {
+        ll += s.l[w][16 * t + rr] * exp2_hw(s.m[w][16 * t + rr] - mm);
+#pragma unroll
+        for (int e = 0; e < C; ++e) o[e] += s.o[w][rr][c0 + e];
+      }
+      const int bi = r / LG, j = r - bi * LG, i = j / p.G, b = set.b0 + bi;
+      const size_t row = ((size_t)b * p.L + i) * p.HQ + hkv * p.G + (j - i * p.G);
+      const bool sees = row_limit(p, b, i) > 0;
+#pragma unroll
+      for (int e = 0; e < C; e += 4)
+        store_row4(p, row, set.slot, c0 + e, f32x4{o[e], o[e + 1], o[e + 2], o[e + 3]}, mm, ll, sees);
+    }
+    __syncthreads();
+  }
+}
+
 template <int FMT, int RES, int VT, int NT, int W>
 __device__ __forceinline__ void few_rows(const AttendParams &p, int split, int hkv, int rb, int z, FewLds<FMT, NT, W> &s) {
   typedef VTraits<VT> VTr;
@@ -531,48 +592,7 @@ __device__ __forceinline__ void few_rows(const AttendParams &p, int split, int h
   for (int t = 0; t < NT; ++t)
     settle_not_finite<VT>(p, block_of, pa + wv, last, W, lane, r0 + 16 * t + n < R, lim[t], O[t]);
 
-  // join the waves
-#pragma unroll
-  for (int t = 0; t < NT; ++t) {
-    l[t] = xor_sum(l[t], 16);
-    l[t] = xor_sum(l[t], 32);
-    if (g == 0) {
-      s.m[wv][16 * t + n] = m[t];
-      s.l[wv][16 * t + n] = l[t];
-    }
-  }
-  __syncthreads();
-#pragma unroll
-  for (int t = 0; t < NT; ++t) {
-    float M = kNoMax;
-#pragma unroll
-    for (int w = 0; w < W; ++w) M = fmaxf(M, s.m[w][16 * t + n]);
-    const float f = fmaxf(exp2_hw(m[t] - M), kLeast);
-#pragma unroll
-    for (int u = 0; u < 8; ++u) *(f32x4 *)&s.o[wv][n][16 * u + 4 * g] = O[t][u] * f;
-    __syncthreads();
-    constexpr int C = 32 / W;  // columns per thread
-    const int rr = threadIdx.x / (kD / C), c0 = C * (threadIdx.x % (kD / C));
-    const int r = r0 + 16 * t + rr;
-    if (r < R) {
-      float mm = kNoMax, ll = 0.f, o[C] = {};
-#pragma unroll
-      for (int w = 0; w < W; ++w) mm = fmaxf(mm, s.m[w][16 * t + rr]);
-#pragma unroll
-      for (int w = 0; w < W; ++w) {
-        ll += s.l[w][16 * t + rr] * exp2_hw(s.m[w][16 * t + rr] - mm);
-#pragma unroll
-        for (int e = 0; e < C; ++e) o[e] += s.o[w][rr][c0 + e];
-      }
-      const int bi = r / LG, j = r - bi * LG, i = j / p.G, b = set.b0 + bi;
-      const size_t row = ((size_t)b * p.L + i) * p.HQ + hkv * p.G + (j - i * p.G);
-      const bool sees = row_limit(p, b, i) > 0;
-#pragma unroll
-      for (int e = 0; e < C; e += 4)
-        store_row4(p, row, set.slot, c0 + e, f32x4{o[e], o[e + 1], o[e + 2], o[e + 3]}, mm, ll, sees);
-    }
-    __syncthreads();
-  }
+  join_waves<NT, W>(p, set, hkv, r0, m, l, O, s);
 }
 
 template <int FMT, int RES, int VT, int NT>
@@ -606,13 +626,19 @@ __device__ __forceinline__ void load_unit(const AttendParams &p, size_t blk, int
     const uint2 c = *(const uint2 *)(p.k + blk * 4096 + (tau * 64 + lane) * 16 + 8 * h);
     r.c0 = c.x;
     r.c1 = c.y;
-    if constexpr (FMT == kFmtNvfp4) r.s = (p.ks + blk * 512)[(4 * m + tau) * 8 + 2 * kc + h];
+    if constexpr (FMT == kFmtMxfp4) r.s = (p.ks + blk * kMxScales)[kc * kPage + 4 * m + tau];
+    else if constexpr (FMT == kFmtNvfp4) r.s = (p.ks + blk * 512)[(4 * m + tau) * 8 + 2 * kc + h];
     else r.s = ((const uint16_t *)(p.ks + blk * 256))[(4 * m + tau) * 2 + (kc >> 1)];
   }
   if constexpr (RES != kResNone) r.res = ((const uint4 *)(p.kr + blk * 8192))[64 * unit + lane];
 }
 template <int FMT, int RES>
 __device__ __forceinline__ void unit_to_lds(const KUnit<FMT> &r, int unit, int lane, const float2 *nf4, u32x4 *dst) {
+  if constexpr (FMT == kFmtMxfp4) {
+    dst[(2 * unit) * 64 + lane] = __builtin_bit_cast(u32x4, mx_operand(r.c0, mx_factor(r.s)));
+    dst[(2 * unit + 1) * 64 + lane] = __builtin_bit_cast(u32x4, mx_operand(r.c1, mx_factor(r.s)));
+    return;
+  }
   const float s = FMT == kFmtNvfp4 ? fp8_pair<true, false>(r.s)[0] : f16_bits_to_f32(r.s);
   const float z = FMT == kFmtQ2 ? f16_bits_to_f32(r.z) : 0.f;
   f16x8 op[2];
@@ -666,10 +692,19 @@ __device__ __forceinline__ void many_rows(const AttendParams &p, int split, int 
 #pragma unroll
     for (int i = 0; i < kUnits; ++i) unit_to_lds<FMT, RES>(r[i], wv * kUnits + i, lane, s.nf4, s.k[buf]);
   };
-  // V: straight into LDS; a bf16 pool's, which becomes the fp16 operand, through registers a page earlier
-  u32x4 vraw[VT == kVF16 ? 1 : kVPieces];
+  // V: straight into LDS; a bf16 or mxfp4 pool's, which becomes the fp16 operand, through registers a page earlier
+  u32x4 vraw[VT == kVF16 || VT == kVMxfp4 ? 1 : kVPieces];
+  uint32_t vcode[VT == kVMxfp4 ? kVPieces : 1];
+  uint2 vscale[VT == kVMxfp4 ? kVPieces : 1];
   auto fetch_v = [&](size_t blk) {
-    if constexpr (VT != kVF16) {
+    if constexpr (VT == kVMxfp4) {
+#pragma unroll
+      for (int i = 0; i < kVPieces; ++i) {  // piece (u, kap): channel 16 u + n, tokens 16 g + 8 kap + (0..7)
+        const int u = (wv * kVPieces + i) >> 1, kap = (wv * kVPieces + i) & 1;
+        vcode[i] = *(const uint32_t *)(p.v + blk * kMxCodes + ((u >> 1) * 64 + lane) * 16 + (u & 1) * 8 + 4 * kap);
+        vscale[i] = *(const uint2 *)(p.vs + blk * kMxScales + (u >> 1) * kPage + 16 * g + 8 * kap);
+      }
+    } else if constexpr (VT != kVF16) {
       const u32x4 *src = (const u32x4 *)(p.v + blk * (kD * kPage * 2));
 #pragma unroll
       for (int i = 0; i < kVPieces; ++i) vraw[i] = src[(wv * kVPieces + i) * 64 + lane];
@@ -680,7 +715,9 @@ __device__ __forceinline__ void many_rows(const AttendParams &p, int split, int 
 #pragma unroll
     for (int i = 0; i < kVPieces; ++i) {
       const int at = (wv * kVPieces + i) * 64;
-      if constexpr (VT == kVF16)
+      if constexpr (VT == kVMxfp4)
+        s.v[buf][at + lane] = __builtin_bit_cast(u32x4, mx_operand(vcode[i], vscale[i]));
+      else if constexpr (VT == kVF16)
         __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)(src + at + lane),
                                          (__attribute__((address_space(3))) void *)(&s.v[buf][at]), 16, 0, 0);
       else
@@ -814,7 +851,10 @@ __device__ __forceinline__ void many_rows(const AttendParams &p, int split, int 
       }
     if (!full && s.bad)
 #pragma unroll
-      for (int t = 0; t < na(); ++t) add_not_finite<VT>(p.v + blk * (kD * kPage * 2), g, lim[t] - t0, O[t]);
+      for (int t = 0; t < na(); ++t) {
+        if constexpr (VT == kVMxfp4) add_nan_blocks(p.vs + blk * kMxScales, lim[t] - t0, O[t]);
+        else add_not_finite<VT>(p.v + blk * (kD * kPage * 2), g, lim[t] - t0, O[t]);
+      }
   };
   constexpr std::integral_constant<int, NT> kAll = {};
   constexpr std::integral_constant<int, 1> kOne = {};
@@ -870,10 +910,11 @@ __device__ __forceinline__ void many_rows(const AttendParams &p, int split, int 
   else if (any) pages(kOne);
   else pages(std::integral_constant<int, 0>());
 
+  if constexpr (VT != kVMxfp4)  // which has no infinities
 #pragma unroll
-  for (int t = 0; t < NT; ++t)
-    if (tile0 + W * t < tile_end)
-      settle_not_finite<VT>(p, block_of, pa, pe, 1, lane, 16 * (tile0 + W * t) + n < R, lim[t], O[t]);
+    for (int t = 0; t < NT; ++t)
+      if (tile0 + W * t < tile_end)
+        settle_not_finite<VT>(p, block_of, pa, pe, 1, lane, 16 * (tile0 + W * t) + n < R, lim[t], O[t]);
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
     const int r = 16 * (tile0 + W * t) + n;
@@ -953,5 +994,6 @@ static void launch_format(const AttendParams &p, const AttendLaunch &a) {
 void attend_q2(const AttendParams &p, const AttendLaunch &a);
 void attend_nvfp4(const AttendParams &p, const AttendLaunch &a);
 void attend_nf4(const AttendParams &p, const AttendLaunch &a);
+void attend_mxfp4(const AttendParams &p, const AttendLaunch &a);
 
 }  // namespace ffa

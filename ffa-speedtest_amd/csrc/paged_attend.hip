@@ -128,7 +128,8 @@ static AttendPlan attend_plan(const ffa_paged_attend_args *a, int cus) {
   return pl;
 }
 
-static int attend_check(const ffa_paged_attend_args *a) {
+// v_scale: of mxfp4 pages, whose entry points alone take them
+static int attend_check(const ffa_paged_attend_args *a, const uint8_t *v_scale) {
 #define FFA_BAD(msg) return ffa_set_error_internal(FFA_E_INVALID, msg)
 #define FFA_NO(msg) return ffa_set_error_internal(FFA_E_UNSUPPORTED, msg)
   if (!a) FFA_BAD("null args");
@@ -137,10 +138,11 @@ static int attend_check(const ffa_paged_attend_args *a) {
   if (a->B > 65535 || a->HKV > 65535) FFA_NO("B and HKV are grid dimensions");
   if (a->T > 1 << 30) FFA_NO("T above 2^30 tokens");
   if (!(a->q_dtype == FFA_DT_F16 || a->q_dtype == FFA_DT_BF16)) FFA_BAD("q must be fp16 or bf16");
-  if (!(a->v_dtype == FFA_DT_F16 || a->v_dtype == FFA_DT_BF16)) FFA_BAD("v dtype");
-  if (a->format < FFA_PAGES_Q2 || a->format > FFA_PAGES_NF4) FFA_BAD("page format");
+  if (v_scale ? a->v_dtype != FFA_DT_NONE : !(a->v_dtype == FFA_DT_F16 || a->v_dtype == FFA_DT_BF16)) FFA_BAD("v dtype");
+  if (v_scale ? a->format != FFA_PAGES_MXFP4 : a->format < FFA_PAGES_Q2 || a->format > FFA_PAGES_NF4) FFA_BAD("page format");
   if (!(a->res_dtype == FFA_DT_FP8_E4M3 || a->res_dtype == FFA_DT_FP8_E5M2 || a->res_dtype == FFA_DT_NONE))
     FFA_BAD("residual dtype must be fp8 or none");
+  if (v_scale && (a->res_dtype != FFA_DT_NONE || a->k_residual || a->k_zero)) FFA_BAD("mxfp4 pages hold codes and scales alone");
   if (a->bt_stride <= 0 || a->num_pages <= 0) FFA_BAD("empty block table or pool");
   if ((long)a->bt_stride * kPage < a->T) FFA_BAD("block table has fewer than ceil(T/64) columns");
   if (!a->q || !a->k || !a->k_scale || !a->v || !a->block_table || !a->out) FFA_BAD("null pointer");
@@ -158,22 +160,18 @@ static int attend_check(const ffa_paged_attend_args *a) {
     }
   }
   const uintptr_t al = (uintptr_t)a->q | (uintptr_t)a->k | (uintptr_t)a->v | (uintptr_t)a->out |
-                       (uintptr_t)a->k_residual | (uintptr_t)a->k_scale | (uintptr_t)a->k_zero;
+                       (uintptr_t)a->k_residual | (uintptr_t)a->k_scale | (uintptr_t)a->k_zero | (uintptr_t)v_scale;
   if (al & 15) FFA_BAD("q, out and the pools must be multiples of 16 bytes");
   return FFA_OK;
 }
 
-}  // namespace ffa
-
-extern "C" size_t ffa_paged_attend_scratch(const ffa_paged_attend_args *a) {
-  using namespace ffa;
-  if (attend_check(a) != FFA_OK) return 0;
+static size_t attend_scratch(const ffa_paged_attend_args *a, const uint8_t *v_scale) {
+  if (attend_check(a, v_scale) != FFA_OK) return 0;
   return (size_t)a->B * a->L * a->HQ * attend_plan(a, device_cus()).nslots * (kD + 2) * sizeof(float);
 }
 
-extern "C" int ffa_paged_attend(const ffa_paged_attend_args *a, void *stream) {
-  using namespace ffa;
-  const int bad = attend_check(a);
+static int attend_run(const ffa_paged_attend_args *a, const uint8_t *v_scale, void *stream) {
+  const int bad = attend_check(a, v_scale);
   if (bad != FFA_OK) return bad;
   const AttendPlan pl = attend_plan(a, device_cus());
   const size_t rows = (size_t)a->B * a->L * a->HQ;
@@ -187,6 +185,7 @@ extern "C" int ffa_paged_attend(const ffa_paged_attend_args *a, void *stream) {
   p.kz = (const uint8_t *)a->k_zero;
   p.kr = a->k_residual;
   p.v = (const uint8_t *)a->v;
+  p.vs = v_scale;
   p.bt = a->block_table;
   p.seq_lens = a->seq_lens;
   p.q_lens = a->q_lens;
@@ -214,7 +213,8 @@ extern "C" int ffa_paged_attend(const ffa_paged_attend_args *a, void *stream) {
   const hipStream_t st = (hipStream_t)stream;
   auto launch = [&](int kind, int slots, int blocks, int sets, int own) {
     const AttendLaunch l = {kind, slots, blocks, sets, own, a->res_dtype, a->v_dtype, st};
-    (a->format == FFA_PAGES_Q2 ? attend_q2 : (a->format == FFA_PAGES_NVFP4 ? attend_nvfp4 : attend_nf4))(p, l);
+    (v_scale ? attend_mxfp4
+             : (a->format == FFA_PAGES_Q2 ? attend_q2 : (a->format == FFA_PAGES_NVFP4 ? attend_nvfp4 : attend_nf4)))(p, l);
   };
   if (pl.both) {
     p.nshared = a->ngroups;
@@ -239,6 +239,21 @@ extern "C" int ffa_paged_attend(const ffa_paged_attend_args *a, void *stream) {
     hipLaunchKernelGGL(paged_attend_join_kernel<1>, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, p, (int)rows);
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? FFA_OK : ffa_set_error_internal(FFA_E_LAUNCH, hipGetErrorString(e));
+}
+
+}  // namespace ffa
+
+extern "C" size_t ffa_paged_attend_scratch(const ffa_paged_attend_args *a) { return ffa::attend_scratch(a, nullptr); }
+
+extern "C" int ffa_paged_attend(const ffa_paged_attend_args *a, void *stream) { return ffa::attend_run(a, nullptr, stream); }
+
+extern "C" size_t ffa_mxfp4_attend_scratch(const ffa_paged_attend_args *a, const uint8_t *v_scale) {
+  return v_scale ? ffa::attend_scratch(a, v_scale) : 0;
+}
+
+extern "C" int ffa_mxfp4_attend(const ffa_paged_attend_args *a, const uint8_t *v_scale, void *stream) {
+  if (!v_scale) FFA_BAD("null pointer");
+  return ffa::attend_run(a, v_scale, stream);
 }
 #undef FFA_BAD
 #undef FFA_NO

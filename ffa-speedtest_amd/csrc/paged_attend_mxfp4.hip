@@ -1,0 +1,298 @@
+// Exact attention over mxfp4 pages (keys and values in 4 bits): the kernel for few rows, and the builds of paged_attend.h
+// for many.
+//
+// Few rows are bound by the pages' bytes (136 a token and head) only while the vector unit keeps up: the bytes of a
+// 16-bit cache's token bring four tokens to convert.  K's codes become the fp16 operand by one conversion a pair, which
+// applies the block's power of two.  V's powers of two belong to tokens, of which a V^T operand holds eight, so they
+// multiply the weights: for each block of 32 columns the weights' operand is w_t 2^(e_t - R), R the largest e so far, and
+// V's codes are converted as they are.  In a page that every row sees whole, and whose e lie within 14 of R, that is a
+// packed product of fp16 pairs, exact; other pages take the same in fp32, with what a row does not see left out.  A NaN
+// block thereby reaches the rows that see it and no other.  The weights' sum is a product with ones, of the weights as
+// they are rounded.
+// (The block-scaled matrix instruction on the codes themselves needs neither conversion, but it sums the products of a
+// group of channels on a common 14-bit grid: 256 + 2^-6 = 256 there, where sums in 32 bits keep 2^-15.)
+#include "paged_attend.h"
+
+namespace ffa {
+
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+
+// One (page, KV head) as lane (g, n) takes it: K, and V with its scales.  Each half is loaded for the next page as soon
+// as this page's is used.
+struct MxKeys {
+  u32x4 code[4];
+  uint32_t scale;  // tokens 4 n + (0..3), block g
+};
+struct MxValues {
+  u32x4 code[4], scale[4];  // block cb, tokens 16 g + (0..15)
+  uint32_t every;           // block g, tokens 4 n + (0..3): each scale of the page in one lane
+};
+__device__ __forceinline__ void load_keys(const AttendParams &p, size_t blk, int lane, MxKeys &r) {
+  r.scale = ((const uint32_t *)(p.ks + blk * kMxScales))[lane];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r.code[i] = __builtin_nontemporal_load((const u32x4 *)(p.k + blk * kMxCodes) + 64 * i + lane);
+}
+__device__ __forceinline__ void load_values(const AttendParams &p, size_t blk, int lane, MxValues &r) {
+  const uint8_t *vs = p.vs + blk * kMxScales;
+  r.every = ((const uint32_t *)vs)[lane];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r.scale[i] = ((const u32x4 *)vs)[4 * i + (lane >> 4)];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r.code[i] = __builtin_nontemporal_load((const u32x4 *)(p.v + blk * kMxCodes) + 64 * i + lane);
+}
+
+// The largest scale byte of a page's first `tokens` tokens (NaN blocks apart), wave-uniform
+__device__ __forceinline__ int page_scale(uint32_t every, int lane, int tokens) {
+  int best = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int byte = (every >> (8 * j)) & 0xffu;
+    if (byte != kMxNan && 4 * (lane & 15) + j < tokens) best = max(best, byte);
+  }
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) best = max(best, __shfl_xor(best, d));
+  return __builtin_amdgcn_readfirstlane(best);
+}
+
+template <int NT, int W>
+__device__ __forceinline__ void few_rows_mx(const AttendParams &p, int split, int hkv, int rb, int z, FewLds<kFmtMxfp4, NT, W> &s) {
+  const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int g = lane >> 4, n = lane & 15;
+  const AttendSet set = attend_set(p, z, split);
+  const int LG = p.L * p.G, R = set.n * LG, r0 = rb * 16 * NT;
+  if (r0 >= R) return;
+  const int pa = set.p0, pe = set.p1;
+  if (pa >= pe && p.nslots != 0) return;
+
+  const int32_t *bt = p.bt + (size_t)set.b0 * p.bt_stride;
+  auto page_id = [&](int pg) { return bt[max(min(pg, pe - 1), pa)]; };  // past the range its last page: loaded, never used
+  auto block = [&](int id) {
+    id = __builtin_amdgcn_readfirstlane((unsigned)id < (unsigned)p.num_pages ? id : 0);
+    return (size_t)id * p.HKV + hkv;
+  };
+  MxKeys K;
+  MxValues V;
+  size_t blk = 0;
+  int id = 0;
+  if (pa < pe) {
+    blk = block(page_id(pa + wv));
+    id = page_id(pa + wv + W);
+    load_keys(p, blk, lane, K);
+    load_values(p, blk, lane, V);
+  }
+
+  f16x8 Q[NT][4];
+  float cs[NT], m[NT];
+  int lim[NT];
+  int lo = 0x7fffffff, hi = 0;
+  f32x4 O[NT][8], Ls[NT];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    const int r = r0 + 16 * t + n;
+    const bool ok = r < R;
+    const int bi = ok ? r / LG : 0, j = ok ? r - bi * LG : 0, i = j / p.G;
+    const size_t row = ((size_t)(set.b0 + bi) * p.L + i) * p.HQ + hkv * p.G + (j - i * p.G);
+    load_q(p, row, ok, g, Q[t], cs[t]);
+    lim[t] = ok ? row_limit(p, set.b0 + bi, i) : 0x7fffffff;  // rows past the last are computed, and not stored
+    lo = min(lo, lim[t]);
+    hi = max(hi, ok ? lim[t] : 0);
+    m[t] = kNoMax;
+    Ls[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int u = 0; u < 8; ++u) O[t][u] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+#pragma unroll
+  for (int d = 1; d < 16; d <<= 1) {
+    lo = min(lo, __shfl_xor(lo, d));
+    hi = max(hi, __shfl_xor(hi, d));
+  }
+  lo = __builtin_amdgcn_readfirstlane(lo);
+  hi = __builtin_amdgcn_readfirstlane(hi);
+
+  const f16x8 one = {1, 1, 1, 1, 1, 1, 1, 1};
+  int vtop = kMxLow;  // R + 127
+  const int last = min(pe, (hi + kPage - 1) / kPage);  // no row sees a later page
+  for (int pg = pa + wv; pg < last; pg += W) {
+    const int t0 = pg * kPage;
+    f32x4 S[NT][4];
+#pragma unroll
+    for (int tau = 0; tau < 4; ++tau) {
+      const float ks = mx_factor((K.scale >> (8 * tau)) & 0xffu);
+      f16x8 op[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) op[e] = mx_operand(K.code[tau][e], ks);
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        f32x4 a = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) a = mfma16(op[e], Q[t][e], a);
+        S[t][tau] = a;
+      }
+    }
+    blk = block(id);
+    id = page_id(pg + 2 * W);
+    load_keys(p, blk, lane, K);
+
+    const bool full = lo >= t0 + kPage;  // every row sees the whole page
+    if (!full)
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int tau = 0; tau < 4; ++tau)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (t0 + 16 * g + 4 * i + tau >= lim[t]) S[t][tau][i] = -INFINITY;
+    u32x4 w16[NT][2];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      float top = S[t][0][0];
+#pragma unroll
+      for (int k = 1; k < 16; ++k) top = fmaxf(top, S[t][k >> 2][k & 3]);
+      top *= cs[t];
+      if (__ballot(top > m[t] + (kHead + kStale)) != 0) {
+        const float mn = fmaxf(m[t], xor_max(xor_max(top, 16), 32) - kHead), alpha = exp2_hw(m[t] - mn);
+        m[t] = mn;
+        Ls[t] *= alpha;
+#pragma unroll
+        for (int u = 0; u < 8; ++u) O[t][u] *= alpha;
+      }
+#pragma unroll
+      for (int k = 0; k < 16; k += 2) {  // tokens 16 g + k, + 1
+        const float a = exp2_hw(__builtin_fmaf(S[t][k & 3][k >> 2], cs[t], -m[t]));
+        const float b = exp2_hw(__builtin_fmaf(S[t][(k + 1) & 3][k >> 2], cs[t], -m[t]));
+        w16[t][k >> 3][(k >> 1) & 3] = pk_f16_bits(a, b);
+      }
+#pragma unroll
+      for (int kap = 0; kap < 2; ++kap) Ls[t] = mfma16(one, __builtin_bit_cast(f16x8, w16[t][kap]), Ls[t]);
+    }
+    // scales of the page: above R, or more than 14 below it?
+    bool packed = full;
+    {
+      const u16x2 a = __builtin_bit_cast(u16x2, V.every & 0x00ff00ffu), b = __builtin_bit_cast(u16x2, (V.every >> 8) & 0x00ff00ffu);
+      const u16x2 most = __builtin_elementwise_max(a, b), least = __builtin_elementwise_min(a, b);
+      if (__ballot(max(most[0], most[1]) > vtop) != 0) {
+        const int now = max(vtop, page_scale(V.every, lane, hi - t0));
+        const float f = now - vtop > 126 ? 0.f : mx_factor(127 + vtop - now);
+        vtop = now;
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int u = 0; u < 8; ++u) O[t][u] *= f;
+        packed = packed && __ballot(max(most[0], most[1]) > vtop) == 0;  // no NaN block
+      }
+      packed = packed && __ballot((int)min(least[0], least[1]) < vtop - 14) == 0;
+    }
+    if (packed) {
+      const uint32_t base = (uint32_t)(vtop - 15) * 0x01010101u;
+#pragma unroll
+      for (int cb = 0; cb < 4; ++cb) {
+        f16x8 P[NT][2];
+#pragma unroll
+        for (int kap = 0; kap < 2; ++kap)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            // four bytes 127 + e to the upper bytes of the fp16 numbers 2^(e - R)
+            const uint32_t x = (V.scale[cb][2 * kap + i] - base) << 2;
+            const f16x2 f[2] = {bits_f16x2(__builtin_amdgcn_perm(0, x, 0x010c000cu)), bits_f16x2(__builtin_amdgcn_perm(0, x, 0x030c020cu))};
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+#pragma unroll
+              for (int t = 0; t < NT; ++t) {
+                const f16x2 y = bits_f16x2(w16[t][kap][2 * i + e]) * f[e];
+                P[t][kap][4 * i + 2 * e] = y[0];
+                P[t][kap][4 * i + 2 * e + 1] = y[1];
+              }
+          }
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int kap = 0; kap < 2; ++kap) {
+            const f16x8 a = mx_operand(V.code[cb][2 * h + kap], 1.0f);
+#pragma unroll
+            for (int t = 0; t < NT; ++t) O[t][2 * cb + h] = mfma16(a, P[t][kap], O[t][2 * cb + h]);
+          }
+      }
+    } else {
+#pragma unroll
+      for (int cb = 0; cb < 4; ++cb) {
+        f16x8 P[NT][2];
+        asm("" : "+v"(V.code[cb]));  // else the compiler converts V for both branches before them, in 64 more registers
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          const int nvis = lim[t] - t0 - 16 * g;  // of the lane's tokens
+          asm("" : "+v"(w16[t][0]), "+v"(w16[t][1]));  // nor the weights in fp32 for all four blocks
+#pragma unroll
+          for (int k = 0; k < 16; ++k) {
+            const int byte = (V.scale[cb][k >> 2] >> (8 * (k & 3))) & 0xffu;
+            // byte - vtop <= 0 for what a row sees, but for NaN blocks
+            const float f = byte == kMxNan ? NAN : mx_factor(max(127 + min(byte - vtop, 0), 0));
+            const float w = (float)__builtin_bit_cast(f16x8, w16[t][k >> 3])[k & 7];
+            P[t][k >> 3][k & 7] = (_Float16)(k < nvis ? w * f : 0.f);
+          }
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int kap = 0; kap < 2; ++kap) {
+            const f16x8 a = mx_operand(V.code[cb][2 * h + kap], 1.0f);
+#pragma unroll
+            for (int t = 0; t < NT; ++t) O[t][2 * cb + h] = mfma16(a, P[t][kap], O[t][2 * cb + h]);
+          }
+      }
+    }
+    load_values(p, blk, lane, V);
+  }
+  float l[NT];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    l[t] = g == 0 ? Ls[t][0] : 0.f;  // join_waves sums over g
+#pragma unroll
+    for (int u = 0; u < 8; ++u) O[t][u] *= mx_factor(vtop);
+  }
+  join_waves<NT, W>(p, set, hkv, r0, m, l, O, s);
+}
+
+template <int NT>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void mxfp4_attend_kernel(const AttendParams p) {
+  __shared__ FewLds<kFmtMxfp4, NT, 4> s;
+  few_rows_mx<NT, 4>(p, blockIdx.x, blockIdx.y % p.HKV, blockIdx.y / p.HKV, blockIdx.z, s);
+}
+
+// Shared pages for many rows and own pages for few in one launch, as paged_attend_both_kernel
+template <int NT>
+__global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) void mxfp4_attend_both_kernel(const AttendParams p) {
+  __shared__ union Lds {
+    FewLds<kFmtMxfp4, NT, 8> few;
+    ManyLds<kFmtMxfp4, 8> many;
+    __device__ Lds() {}
+  } s;
+  int x = blockIdx.x;
+  if (x < p.shared_wgs) {
+    const int hkv = x % p.HKV, y = x / p.HKV, w = y / p.shared_blocks;
+    many_rows<kFmtMxfp4, kResNone, kVMxfp4, 2, 8>(p, w % p.shared_slots, hkv, y % p.shared_blocks, w / p.shared_slots, s.many);
+  } else {
+    x -= p.shared_wgs;
+    const int split = x % p.own_slots, y = x / p.own_slots;
+    few_rows_mx<NT, 8>(p, split, y % p.HKV, 0, p.nshared + y / p.HKV, s.few);
+  }
+}
+
+void attend_mxfp4(const AttendParams &p, const AttendLaunch &a) {
+  if (a.own >= 0) {
+    const dim3 grid((unsigned)(p.shared_wgs + (long)p.B * p.HKV * p.own_slots));
+    if (a.own == kRows16) hipLaunchKernelGGL(mxfp4_attend_both_kernel<1>, grid, dim3(512), 0, a.st, p);
+    else hipLaunchKernelGGL(mxfp4_attend_both_kernel<2>, grid, dim3(512), 0, a.st, p);
+    return;
+  }
+  const dim3 few((unsigned)a.slots, (unsigned)(p.HKV * a.blocks), (unsigned)a.sets);
+  const dim3 wide((unsigned)(p.HKV * a.blocks), (unsigned)a.slots, (unsigned)a.sets);
+  switch (a.kind) {
+    case kRows16: hipLaunchKernelGGL(mxfp4_attend_kernel<1>, few, dim3(256), 0, a.st, p); break;
+    case kRows32: hipLaunchKernelGGL(mxfp4_attend_kernel<2>, few, dim3(256), 0, a.st, p); break;
+    case kRows64: hipLaunchKernelGGL((paged_attend_wide_kernel<kFmtMxfp4, kResNone, kVMxfp4, 1, 4>), wide, dim3(256), 0, a.st, p); break;
+    case kRows128: hipLaunchKernelGGL((paged_attend_wide_kernel<kFmtMxfp4, kResNone, kVMxfp4, 2, 4>), wide, dim3(256), 0, a.st, p); break;
+    default: hipLaunchKernelGGL((paged_attend_wide_kernel<kFmtMxfp4, kResNone, kVMxfp4, 2, 8>), wide, dim3(512), 0, a.st, p);
+  }
+}
+
+}  // namespace ffa

@@ -139,6 +139,26 @@ inline long attend_shared_wgs(long units, long own_head_pages, int cus) {
   return (long)(cus * (share < 0.4 ? 0.4 : share)) + 1;
 }
 
+// mxfp4 appends by tiles of 64 tokens rather than by pairs of positions; units: heads of q, K and V.
+inline bool mx_by_tiles(int B, int Tn, int units) { return Tn >= 16; }
+// workgroups that share a tile's units (each computes the tile's angles): n waves' worth of four units
+inline long mx_tile_splits(long tiles, long n) {
+  const long want = (2048 + tiles - 1) / tiles;
+  return want < n ? want : n;
+}
+
+// Rotary positions on given rows: tokens of a workgroup, which computes their angles, and workgroups that share a tile's
+// rows (each computing the angles again).
+inline int rope_tokens(long tokens, int most) {
+  int n = 1;
+  while (n < most && tokens > 1024l * n) n *= 2;
+  return n;
+}
+inline long rope_splits(long tiles, long rows) {
+  const long want = (1024 + tiles - 1) / tiles, can = (rows + 31) / 32;
+  return want < can ? want : can;
+}
+
 // The join of a row's partials by one wave, four rows a workgroup, rather than by four waves: 4224 rows of 18 slots 69.5
 // -> 66 us, 2048 the same or 1 % slower
 inline bool join_by_wave(long rows) { return rows > 2048; }

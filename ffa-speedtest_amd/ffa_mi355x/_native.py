@@ -18,7 +18,7 @@ DT_F16, DT_BF16, DT_F32, DT_FP8_E4M3, DT_FP8_E5M2, DT_NONE = range(6)
 LAYOUT_CONTIG, LAYOUT_PAGED = 0, 1
 SCALE_CHANNEL, SCALE_G32 = 0, 1
 KFMT_FP8_E4M3, KFMT_FP8_E5M2, KFMT_NVFP4, KFMT_NF4 = range(4)
-PAGES_Q2, PAGES_NVFP4, PAGES_NF4 = range(3)
+PAGES_Q2, PAGES_NVFP4, PAGES_NF4, PAGES_MXFP4 = range(4)
 KSCALE_NONE, KSCALE_TOKEN, KSCALE_BLOCK, KSCALE_CHANNEL, KSCALE_G16, KSCALE_G64 = range(6)
 
 EXPORTS = (
@@ -51,6 +51,11 @@ EXPORTS = (
     "ffa_nf4_g64_append_cast",
     "ffa_paged_attend_scratch",
     "ffa_paged_attend",
+    "ffa_rope_axes",
+    "ffa_mxfp4_append",
+    "ffa_mxfp4_dequant",
+    "ffa_mxfp4_attend_scratch",
+    "ffa_mxfp4_attend",
     "ffa_pages_copy",
     "ffa_pages_alloc_scratch",
     "ffa_pages_fork",
@@ -201,6 +206,80 @@ class AttendArgs(ctypes.Structure):
     ]
 
 
+class RopeAxesArgs(ctypes.Structure):
+    _fields_ = [
+        ("q", ctypes.c_void_p),
+        ("q_out", ctypes.c_void_p),
+        ("k", ctypes.c_void_p),
+        ("k_out", ctypes.c_void_p),
+        ("dtype", ctypes.c_int),
+        ("B", ctypes.c_int),
+        ("T", ctypes.c_int),
+        ("HQ", ctypes.c_int),
+        ("HKV", ctypes.c_int),
+        ("q_batch", ctypes.c_long),
+        ("q_token", ctypes.c_long),
+        ("q_head", ctypes.c_long),
+        ("q_out_batch", ctypes.c_long),
+        ("q_out_token", ctypes.c_long),
+        ("q_out_head", ctypes.c_long),
+        ("k_batch", ctypes.c_long),
+        ("k_token", ctypes.c_long),
+        ("k_head", ctypes.c_long),
+        ("k_out_batch", ctypes.c_long),
+        ("k_out_token", ctypes.c_long),
+        ("k_out_head", ctypes.c_long),
+        ("pairs", ctypes.c_void_p),
+        ("positions", ctypes.c_void_p),
+        ("positions64", ctypes.c_int),
+        ("axes", ctypes.c_int),
+        ("pos_axis", ctypes.c_long),
+        ("pos_batch", ctypes.c_long),
+        ("adjacent", ctypes.c_int),
+        ("inverse", ctypes.c_int),
+    ]
+
+
+class MXFP4AppendArgs(ctypes.Structure):
+    _fields_ = [
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("q", ctypes.c_void_p),
+        ("dtype", ctypes.c_int),
+        ("B", ctypes.c_int),
+        ("T", ctypes.c_int),
+        ("HKV", ctypes.c_int),
+        ("HQ", ctypes.c_int),
+        ("k_batch", ctypes.c_long),
+        ("k_token", ctypes.c_long),
+        ("k_head", ctypes.c_long),
+        ("v_batch", ctypes.c_long),
+        ("v_token", ctypes.c_long),
+        ("v_head", ctypes.c_long),
+        ("q_batch", ctypes.c_long),
+        ("q_token", ctypes.c_long),
+        ("q_head", ctypes.c_long),
+        ("pairs", ctypes.c_void_p),
+        ("positions", ctypes.c_void_p),
+        ("positions64", ctypes.c_int),
+        ("axes", ctypes.c_int),
+        ("pos_axis", ctypes.c_long),
+        ("pos_batch", ctypes.c_long),
+        ("adjacent", ctypes.c_int),
+        ("pos", ctypes.c_void_p),
+        ("block_table", ctypes.c_void_p),
+        ("bt_stride", ctypes.c_int),
+        ("num_pages", ctypes.c_int),
+        ("k_pages", ctypes.c_void_p),
+        ("k_scale", ctypes.c_void_p),
+        ("v_pages", ctypes.c_void_p),
+        ("v_scale", ctypes.c_void_p),
+        ("q_out", ctypes.c_void_p),
+        ("k_values", ctypes.c_void_p),
+        ("v_values", ctypes.c_void_p),
+    ]
+
+
 class Pages(ctypes.Structure):
     _fields_ = [
         ("pools", ctypes.c_void_p),
@@ -287,6 +366,16 @@ def lib() -> ctypes.CDLL:
         L.ffa_paged_attend_scratch.restype = ctypes.c_size_t
         L.ffa_paged_attend.argtypes = [ctypes.POINTER(AttendArgs), vp]
         L.ffa_paged_attend.restype = ci
+        L.ffa_rope_axes.argtypes = [ctypes.POINTER(RopeAxesArgs), vp]
+        L.ffa_rope_axes.restype = ci
+        L.ffa_mxfp4_append.argtypes = [ctypes.POINTER(MXFP4AppendArgs), vp]
+        L.ffa_mxfp4_append.restype = ci
+        L.ffa_mxfp4_dequant.argtypes = [vp, vp, vp, vp, vp, ci, ci, vp, ci, ci, ci, vp, vp, ci, vp]
+        L.ffa_mxfp4_dequant.restype = ci
+        L.ffa_mxfp4_attend_scratch.argtypes = [ctypes.POINTER(AttendArgs), vp]
+        L.ffa_mxfp4_attend_scratch.restype = ctypes.c_size_t
+        L.ffa_mxfp4_attend.argtypes = [ctypes.POINTER(AttendArgs), vp, vp]
+        L.ffa_mxfp4_attend.restype = ci
         pg, cz = ctypes.POINTER(Pages), ctypes.c_size_t
         L.ffa_pages_copy.argtypes = [pg, vp, vp, ci, vp]
         L.ffa_pages_alloc_scratch.argtypes = [ci, ci]

@@ -3,7 +3,7 @@
 The reference attends to its cache's dequantized keys with a library call whenever it does not prune
 (ffa-fp8fp8/e2e/modeling_llama.py:322-337).  Here the kernel reads the quantized pages themselves: L query
 tokens per sequence (a decode step, drafted tokens, a prompt's chunk), causal at the sequence's end.
-`PagedQ2Cache.attend` and `PagedKfmtCache.attend` call `run_attend`.
+`PagedQ2Cache.attend`, `PagedKfmtCache.attend` and `PagedMXFP4Cache.attend` call `run_attend`.
 """
 from __future__ import annotations
 
@@ -18,7 +18,7 @@ from .decode import HEAD_DIM
 
 PAGE = 64
 _SCALE = 1.0 / math.sqrt(HEAD_DIM)
-_FORMATS = {"q2": N.PAGES_Q2, "nvfp4": N.PAGES_NVFP4, "nf4": N.PAGES_NF4}
+_FORMATS = {"q2": N.PAGES_Q2, "nvfp4": N.PAGES_NVFP4, "nf4": N.PAGES_NF4, "mxfp4": N.PAGES_MXFP4}
 
 
 class SharedPrefix:
@@ -87,23 +87,27 @@ def _on(device: torch.device):
     return nullcontext() if device.index in (None, torch.cuda.current_device()) else torch.cuda.device(device)
 
 
-def _call(a: N.AttendArgs, dev: torch.device) -> int:
+def _call(a: N.AttendArgs, v_scale: torch.Tensor | None, dev: torch.device) -> int:
     lib, ref = N.lib(), ctypes.byref(a)
-    need = lib.ffa_paged_attend_scratch(ref)
+    if v_scale is None:
+        more, size, run = (), lib.ffa_paged_attend_scratch, lib.ffa_paged_attend
+    else:
+        more, size, run = (v_scale.data_ptr(),), lib.ffa_mxfp4_attend_scratch, lib.ffa_mxfp4_attend
+    need = size(ref, *more)
     if need:
         scratch = torch.empty(need, dtype=torch.uint8, device=dev)
         a.scratch, a.scratch_bytes = scratch.data_ptr(), need
-    return lib.ffa_paged_attend(ref, N.stream_of(dev))
+    return run(ref, *more, N.stream_of(dev))
 
 
 def run_attend(fmt, q, k, k_scale, k_zero, k_res, v, block_table, seq_lens=None, *, T=None, q_lens=None, scale=None,
-               use_fp8_residual=True, shared: SharedPrefix | None = None, out=None) -> torch.Tensor:
+               use_fp8_residual=True, shared: SharedPrefix | None = None, out=None, v_scale=None) -> torch.Tensor:
     """Exact attention of q [B, L, HQ, 128] (or [B, HQ, 128]) over the page pools of one format.
 
     Query token i of sequence b sits at position seq_lens[b] - q_lens[b] + i and sees the keys up to its own;
     query tokens i >= q_lens[b] (padding of a batch of uneven chunks) and rows that see no key give zeros.
     seq_lens counts the query tokens, which are in the cache already.  T: the largest length (read from the
-    device when not given); a capacity serves, and lets a captured graph's sequences grow.
+    device when not given); a capacity serves, and lets a captured graph's sequences grow.  v_scale: of mxfp4 pools.
     Returns out (allocated unless given) in q's shape and type."""
     if q.ndim not in (3, 4):
         raise ValueError(f"q must be [B, L, HQ, 128] or [B, HQ, 128], got {tuple(q.shape)}")
@@ -157,13 +161,13 @@ def run_attend(fmt, q, k, k_scale, k_zero, k_res, v, block_table, seq_lens=None,
         groups = shared._args
     a = N.AttendArgs(  # in the order of the fields: one call instead of thirty assignments
         q.data_ptr(), N.dtype_code(q.dtype), _FORMATS[fmt], k.data_ptr(), k_scale.data_ptr(), N.ptr(k_zero), N.ptr(res),
-        N.DT_NONE if res is None else N.dtype_code(res.dtype), v.data_ptr(), N.dtype_code(v.dtype), block_table.data_ptr(),
-        cols, P, N.ptr(seq_lens), N.ptr(q_lens), B, T, L, HQ, HKV, _SCALE if scale is None else float(scale), *groups,
+        N.DT_NONE if res is None else N.dtype_code(res.dtype), v.data_ptr(), N.DT_NONE if v_scale is not None else N.dtype_code(v.dtype),
+        block_table.data_ptr(), cols, P, N.ptr(seq_lens), N.ptr(q_lens), B, T, L, HQ, HKV, _SCALE if scale is None else float(scale), *groups,
         out.data_ptr(), None, 0)
     if dev.index == torch.cuda.current_device():
-        rc = _call(a, dev)
+        rc = _call(a, v_scale, dev)
     else:
         with torch.cuda.device(dev):
-            rc = _call(a, dev)
-    N.check(rc, "ffa_paged_attend")
+            rc = _call(a, v_scale, dev)
+    N.check(rc, "ffa_paged_attend" if v_scale is None else "ffa_mxfp4_attend")
     return out

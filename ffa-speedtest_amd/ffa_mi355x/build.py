@@ -19,7 +19,7 @@ LIB_PATH = PKG_DIR / LIB_NAME
 
 SOURCES = ["q2fp8_decode.hip", "kfmt_decode.hip", "q2_quant.hip", "kfmt_quant.hip", "value_mean.hip",
            "paged_attend.hip", "paged_attend_q2.hip", "paged_attend_nvfp4.hip",
-           "paged_attend_nf4.hip", "pages.hip"]
+           "paged_attend_nf4.hip", "paged_attend_mxfp4.hip", "pages.hip", "mxfp4_cache.hip", "rope_axes.hip"]
 
 HIPCC_FLAGS = [
     "--offload-arch=gfx950",

@@ -1,0 +1,178 @@
+"""Rotary positions with several axes (time, height and width of video; height and width of images; plain text).
+
+The reference rotates keys by cos / sin tables of one axis (ffa-q2fp8/fused_kproj_rope_q2fp8.py:10-37, here
+`rope.py`).  `AxisRope` keeps the frequency and the axis of each of the 64 pairs of channels; `rotate` turns given
+queries and keys (both in one launch), and `PagedMXFP4Cache.append_rotary` turns while it stores.
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+
+import torch
+
+from . import _native as N
+from .attend import _on
+from .decode import HEAD_DIM
+
+PAIRS = HEAD_DIM // 2
+_DTYPES = (torch.float16, torch.bfloat16, torch.float32)
+
+
+def strided_rows(x: torch.Tensor) -> tuple[torch.Tensor, tuple[int, int, int]]:
+    """x [B, T, H, 128] and its strides (elements; 0 where a dimension has one entry) as the kernels take rows: 128
+    contiguous channels, every address a multiple of 16 bytes.  Others are copied."""
+    def strides(t):
+        return tuple(s if n > 1 else 0 for s, n in zip(t.stride()[:3], t.shape[:3]))
+
+    step = 16 // x.element_size()
+    if x.stride(3) != 1 or any(s % step for s in strides(x)):
+        x = x.contiguous()
+    if x.data_ptr() % 16:
+        x = x.clone(memory_format=torch.contiguous_format)
+    return x, strides(x)
+
+
+class AxisRope:
+    """Rotary positions of 128 channels: pair j of a token turns by positions[axis of j] * frequency j.
+
+    sections: pairs of each axis, 64 in all.  order: "blocks" gives axis 0 the first sections[0] pairs, axis 1 the
+    next ones, ...; "cycled" gives the pairs to the axes in turn while they have pairs left.
+    pairs: "half" turns channels (j, j + 64), as transformers' rotate_half; "adjacent" (2 j, 2 j + 1).
+    base: frequency j is base^(-j / 64); inv_freq [64] gives other ones (scaled or stretched).
+    """
+
+    def __init__(self, sections, base: float = 10000.0, device="cuda", *, pairs: str = "half", order: str = "blocks",
+                 inv_freq=None):
+        sections = [int(n) for n in sections]
+        if not sections or min(sections) < 0 or sum(sections) != PAIRS:
+            raise ValueError(f"sections must sum to {PAIRS} pairs, got {sections}")
+        if pairs not in ("half", "adjacent"):
+            raise ValueError('pairs must be "half" or "adjacent"')
+        if order not in ("blocks", "cycled"):
+            raise ValueError('order must be "blocks" or "cycled"')
+        if inv_freq is None:
+            if not base > 0:
+                raise ValueError("base must be positive")
+            freq = [float(base) ** (-j / PAIRS) for j in range(PAIRS)]
+        else:
+            freq = torch.as_tensor(inv_freq).detach().double().reshape(-1).tolist()
+            if len(freq) != PAIRS:
+                raise ValueError(f"inv_freq must hold {PAIRS} frequencies, got {len(freq)}")
+        if order == "blocks":
+            axis = [a for a, n in enumerate(sections) for _ in range(n)]
+        else:
+            axis, left = [], list(sections)
+            while len(axis) < PAIRS:
+                for a in range(len(sections)):
+                    if left[a]:
+                        axis.append(a)
+                        left[a] -= 1
+        self.sections, self.axes, self.axis = sections, len(sections), axis
+        self.inv_freq = freq
+        self.adjacent = pairs == "adjacent"
+        self.device = torch.device(device)
+        turns = torch.tensor([f / (2 * math.pi) for f in freq], dtype=torch.float64)
+        # ffa_rope_pair: {double turns; int64 axis}
+        self.table = torch.stack([turns.view(torch.int64), torch.tensor(axis)], 1).contiguous().to(self.device)
+
+    def _positions(self, positions: torch.Tensor, B: int, T: int, dev) -> tuple[torch.Tensor, int, int]:
+        """positions [axes, B, T], [axes, T] for every sequence, or [B, T] of one axis -> (them, strides)."""
+        if positions.dtype not in (torch.int32, torch.int64):
+            raise ValueError(f"positions must be int32 or int64, got {positions.dtype}")
+        if positions.device != dev:
+            raise ValueError(f"positions are on {positions.device}, the rows on {dev}")
+        shape = tuple(positions.shape)
+        if shape == (self.axes, B, T):
+            p = positions
+        elif shape == (self.axes, T):
+            p = positions[:, None].expand(self.axes, B, T)
+        elif self.axes == 1 and shape == (B, T):
+            p = positions[None]
+        else:
+            raise ValueError(f"positions must be [{self.axes}, {B}, {T}] or [{self.axes}, {T}], got {shape}")
+        if T > 1 and p.stride(2) != 1:
+            p = p.contiguous()
+        return p, p.stride(0), p.stride(1)
+
+    def _check(self, x: torch.Tensor, what: str, like: torch.Tensor | None = None) -> None:
+        if x.ndim != 4 or x.shape[3] != HEAD_DIM:
+            raise ValueError(f"{what} must be [B, T, H, {HEAD_DIM}], got {tuple(x.shape)}")
+        if x.dtype not in _DTYPES:
+            raise NotImplementedError(f"{what} must be fp16, bf16 or fp32, got {x.dtype}")
+        if x.device.type != "cuda" or self.table.device != x.device:
+            raise ValueError(f"{what} is on {x.device}, the rotation on {self.table.device}: both must be on one GPU")
+        if like is not None and (x.shape[:2] != like.shape[:2] or x.dtype != like.dtype):
+            raise ValueError("q and k must have the same sequences, tokens and type")
+
+    def _run(self, positions, q, k, inverse, inplace):
+        B, T, HQ, _ = q.shape
+        HKV = 0 if k is None else k.shape[2]
+        if q.numel() == 0:
+            HQ = 0
+        if HKV and k.numel() == 0:
+            HKV = 0
+        pos, pos_axis, pos_batch = self._positions(positions, B, T, q.device)
+        outs, args = [], []
+        for x in (q, k):
+            if x is None:
+                args.append((None, None, (0, 0, 0), (0, 0, 0)))
+                continue
+            src, st = strided_rows(x)
+            if inplace:
+                if src is not x:
+                    raise ValueError("rows turned in place must have contiguous channels and 16-byte aligned strides")
+                if any(n > 1 and s == 0 for n, s in zip(x.shape, x.stride())):
+                    raise ValueError("rows turned in place must not be expanded")
+                out, ot = x, st
+            else:
+                out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+                ot = tuple(out.stride()[:3])
+            outs.append(out)
+            args.append((src, out, st, ot))
+        if HQ == 0 and HKV == 0:
+            return outs
+        (q_in, q_out, qs, qo), (k_in, k_out, ks, ko) = args
+        if HQ == 0:  # k alone, in q's place
+            (q_in, q_out, qs, qo), HQ, HKV = (k_in, k_out, ks, ko), HKV, 0
+        a = N.RopeAxesArgs(
+            q_in.data_ptr(), q_out.data_ptr(), N.ptr(k_in), N.ptr(k_out), N.dtype_code(q.dtype), B, T, HQ, HKV, *qs, *qo, *ks,
+            *ko, self.table.data_ptr(), pos.data_ptr(), int(pos.dtype is torch.int64), self.axes, pos_axis, pos_batch,
+            int(self.adjacent), int(inverse))
+        with _on(q.device):
+            rc = N.lib().ffa_rope_axes(ctypes.byref(a), N.stream_of(q.device))
+        N.check(rc, "ffa_rope_axes")
+        return outs
+
+    def rotate(self, positions: torch.Tensor, q: torch.Tensor, k: torch.Tensor | None = None, *, inverse: bool = False,
+               inplace: bool = False):
+        """q [B, T, H, 128] (and k, with heads of its own) turned by positions [axes, B, T] (or [axes, T] for every
+        sequence; int32 or int64), angles in 64 bits, one rounding to the rows' type.  inverse: turned back, which is
+        also the gradient; `rotate` records it where q or k needs one.  inplace: into q and k themselves.
+        Returns q, or (q, k) where k is given."""
+        self._check(q, "q")
+        if k is not None:
+            self._check(k, "k", q)
+        if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+            if inplace:
+                raise ValueError("rows that need gradients are not turned in place")
+            got = _Rotate.apply(self, positions, inverse, q, k)
+        else:
+            got = self._run(positions, q, k, inverse, inplace)
+        return got[0] if k is None else (got[0], got[1])
+
+
+class _Rotate(torch.autograd.Function):
+    """rotate with its gradient: the rotation back (linear, so the gradient's own is the rotation again)."""
+
+    @staticmethod
+    def forward(ctx, rope, positions, inverse, q, k):
+        ctx.rope, ctx.inverse, ctx.two = rope, inverse, k is not None
+        ctx.save_for_backward(positions)
+        return tuple(rope._run(positions, q, k, inverse, False))
+
+    @staticmethod
+    def backward(ctx, gq, gk=None):
+        (positions,) = ctx.saved_tensors
+        got = _Rotate.apply(ctx.rope, positions, not ctx.inverse, gq, gk)
+        return None, None, None, got[0], got[1] if ctx.two else None

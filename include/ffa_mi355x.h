@@ -46,6 +46,10 @@
  *   ffa_pages_*               no reference counterpart: copying, forking, extending, freeing and
  *                             compacting the pages of the paged caches (the reference grows one
  *                             contiguous cache by torch.cat, ffa-fp8fp8/e2e/fp8fp8_cache.py:84-89)
+ *   ffa_mxfp4_*               no reference counterpart: a paged cache of keys and values in 4 bits, its append
+ *                             (with or without rotary positions), read-back and exact attention
+ *   ffa_rope_axes             apply_rope of given q and k with positions of one to four axes (the reference
+ *                             rotates k by tables of one axis, ffa-q2fp8/fused_kproj_rope_q2fp8.py:10-37)
  *   ffa_kproj_rope            F.linear + apply_rope of every reference producer, e.g.
  *                             ffa-fp8fp8/fused_kproj_rope_fp8fp8.py:80-88,
  *                             ffa-nvfp4fp8/fused_kproj_rope_nvfp4fp8.py:131-139,
@@ -460,7 +464,7 @@ int ffa_kfmt_decode(const ffa_kfmt_decode_args *args, void *stream);
  * partials of the page ranges.  Calls that share scratch must be ordered on one stream.  Block-table
  * entries outside [0, num_pages) read page 0.
  */
-enum { FFA_PAGES_Q2 = 0, FFA_PAGES_NVFP4 = 1, FFA_PAGES_NF4 = 2 };
+enum { FFA_PAGES_Q2 = 0, FFA_PAGES_NVFP4 = 1, FFA_PAGES_NF4 = 2, FFA_PAGES_MXFP4 = 3 /* ffa_mxfp4_attend */ };
 typedef struct ffa_paged_attend_args {
   const void *q; /* [B, L, HQ, 128] */
   int q_dtype;   /* F16 or BF16, also out's */
@@ -494,6 +498,112 @@ typedef struct ffa_paged_attend_args {
 /* Bytes of scratch that a call with these arguments needs (scratch and scratch_bytes are not read). */
 size_t ffa_paged_attend_scratch(const ffa_paged_attend_args *args);
 int ffa_paged_attend(const ffa_paged_attend_args *args, void *stream);
+
+/*
+ * The cache that holds keys and values in 4 bits (no reference counterpart): MXFP4 pages.  Per token and
+ * KV head, blocks of 32 channels of e2m1 codes with one power of two:
+ *   value = level[code] * 2^(byte - 127),  level = 0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives,
+ *   byte: the smallest power of two of which the block's largest magnitude is at most seven, within
+ *         105 .. 140 (values of 2^-23 .. 49152, each exact in fp16 and bf16); 255 where the block holds an
+ *         infinity or NaN: its codes are 0 and its values NaN,
+ *   code: the nearest level (ties to the even code; beyond 6 the largest).
+ * 64-token pages of four pools:
+ *   k [P, HKV, 64, 64] u8        K codes; token t, channels 2 j, 2 j + 1 (low half first) in byte
+ *                                ((t % 4 * 4 + j / 16) * 16 + t / 4) * 16 + j % 16 of the block
+ *   k_scale [P, HKV, 4, 64] u8   bytes of 32 channels, token by token
+ *   v [P, HKV, 128, 32] u8       V codes; channel c, tokens t = 2 i, 2 i + 1 (low half first) in byte
+ *                                ((c / 32 * 4 + t / 16) * 16 + c % 16) * 16 + c / 16 % 2 * 8 + t % 16 / 2
+ *   v_scale [P, HKV, 4, 64] u8
+ * Two tokens share a byte of V: an append of the second leaves the first, and calls that write tokens of
+ * one page are ordered on one stream.
+ */
+
+/*
+ * Rotary positions with several axes.  Pair j (0..63) of a token turns by
+ *   angle = positions[axis_j][token] * 2 pi turns_j   (64 bits; sine and cosine of the remainder in 32),
+ *   (a, b) -> (a cos - b sin, b cos + a sin),   inverse: -angle (the gradient of the rotation),
+ * with (a, b) the channels (j, j + 64), or (2 j, 2 j + 1) with `adjacent`.  One rounding, to the rows' type.
+ * pairs: device, [64].  positions: device, element (axis, b, t) at axis * pos_axis + b * pos_batch + t, int32 or
+ * int64; axes outside [0, axes) read axis 0.
+ */
+typedef struct ffa_rope_pair {
+  double turns;
+  int64_t axis;
+} ffa_rope_pair;
+/*
+ * q [B, T, HQ, 128] and k [B, T, HKV, 128] (k may be NULL with HKV = 0) of one type (F16/BF16/F32), rows of 128
+ * contiguous channels at the given strides (elements; addresses and strides multiples of 16 bytes); q_out and
+ * k_out likewise, each its input itself (in place) or memory that shares nothing with the inputs.
+ */
+typedef struct ffa_rope_axes_args {
+  const void *q;
+  void *q_out;
+  const void *k;
+  void *k_out;
+  int dtype;
+  int B, T, HQ, HKV;
+  long q_batch, q_token, q_head;
+  long q_out_batch, q_out_token, q_out_head;
+  long k_batch, k_token, k_head;
+  long k_out_batch, k_out_token, k_out_head;
+  const ffa_rope_pair *pairs;
+  const void *positions;
+  int positions64; /* positions are int64 */
+  int axes;
+  long pos_axis, pos_batch;
+  int adjacent;
+  int inverse;
+} ffa_rope_axes_args;
+int ffa_rope_axes(const ffa_rope_axes_args *args, void *stream);
+
+/*
+ * Append to mxfp4 pages: token n of sequence b goes to position pos[b] + n.  k and v [B, T, HKV, 128] of one
+ * type (F16/BF16/F32), strided as in ffa_rope_axes_args; v may be NULL (K alone is written).  With pairs, k
+ * turns before it is quantized (in 32 bits, unrounded), and q [B, T, HQ, 128] (or NULL with HQ = 0) of the same type
+ * into q_out [B, T, HQ, 128], contiguous; positions NULL: pos[b] + n on every axis.  k_values, v_values
+ * [B, T, HKV, 128] of the same type (or NULL): the values as the pages hold them.  Nothing is written for a
+ * token whose position lies outside its block-table row or whose page id is outside [0, num_pages); its
+ * q_out and values are.
+ */
+typedef struct ffa_mxfp4_append_args {
+  const void *k, *v, *q;
+  int dtype;
+  int B, T, HKV, HQ;
+  long k_batch, k_token, k_head;
+  long v_batch, v_token, v_head;
+  long q_batch, q_token, q_head;
+  const ffa_rope_pair *pairs; /* or NULL */
+  const void *positions;      /* or NULL */
+  int positions64;
+  int axes;
+  long pos_axis, pos_batch;
+  int adjacent;
+  const int32_t *pos;
+  const int32_t *block_table;
+  int bt_stride;
+  int num_pages;
+  uint8_t *k_pages, *k_scale, *v_pages, *v_scale;
+  void *q_out;
+  void *k_values, *v_values;
+} ffa_mxfp4_append_args;
+int ffa_mxfp4_append(const ffa_mxfp4_append_args *args, void *stream);
+
+/*
+ * mxfp4 pages -> contiguous K and V [B, T, HKV, 128] in out_dtype (F16/BF16/F32), exact.  T is a multiple of
+ * 64; tokens at or past seq_lens[b] (NULL: every sequence holds T tokens) are zeros.  Block-table entries
+ * outside [0, num_pages) read page 0.
+ */
+int ffa_mxfp4_dequant(const uint8_t *k_pages, const uint8_t *k_scale, const uint8_t *v_pages, const uint8_t *v_scale,
+                      const int32_t *block_table, int bt_stride, int num_pages, const int32_t *seq_lens, int B, int T,
+                      int HKV, void *k_out, void *v_out, int out_dtype, void *stream);
+
+/*
+ * ffa_paged_attend over mxfp4 pages: args as there with format FFA_PAGES_MXFP4, v the V codes, v_dtype and
+ * res_dtype FFA_DT_NONE, k_zero and k_residual NULL; v_scale beside them.  Keys and values enter the products
+ * exactly; the weights, times V's powers of two where rows are few, are rounded to fp16.
+ */
+size_t ffa_mxfp4_attend_scratch(const ffa_paged_attend_args *args, const uint8_t *v_scale);
+int ffa_mxfp4_attend(const ffa_paged_attend_args *args, const uint8_t *v_scale, void *stream);
 
 /*
  * Management of the pages of one or several caches (layers) that share page ids.  refs [num_pages]
