@@ -54,6 +54,7 @@ struct AttendParams {
   int shared_slots, shared_ppw, own_slots;
   int shared_blocks, shared_wgs;  // of the launch of both kinds
   const uint8_t *vs;              // mxfp4 pages: V's scales
+  int even;                       // even ranges over the batch's pages, about this many; 0: ranges by sequence
 };
 
 __device__ __forceinline__ int seq_len_of(const AttendParams &p, int b) {
@@ -70,6 +71,55 @@ __device__ __forceinline__ int shared_pages_of(const AttendParams &p, int b) {
 __device__ __forceinline__ int own_range(const AttendParams &p, int pages) {
   return max((pages + 4 * p.own_slots - 1) / (4 * p.own_slots), 1) * 4;
 }
+__device__ __forceinline__ int pages_of(const AttendParams &p, int b) {
+  return b < p.B ? (seq_len_of(p, b) + kPage - 1) / kPage : 0;
+}
+
+// Even ranges: the pages of all sequences, which the host need not know, in ranges of equal length (but for each
+// sequence's last), so that the workgroups of a ragged batch have the same work.  Every wave adds the lengths up for itself.
+// Inclusive sum over the lanes up to each.
+__device__ __forceinline__ int lanes_sum(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, true);  // row_shr 1, 2, 4, 8
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xF, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, false);  // row_bcast 15 into rows 1 and 3
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, false);  // row_bcast 31 into rows 2 and 3
+  return x;
+}
+// pages per range: a page for each of four waves at least
+__device__ __forceinline__ int even_range(const AttendParams &p) {
+  const int lane = threadIdx.x & 63;
+  long all = 0;
+  for (int b = 0; b < p.B; b += 64) all += __builtin_amdgcn_readlane(lanes_sum(pages_of(p, b + lane)), 63);
+  return (int)((all + 4l * p.even - 1) / (4l * p.even) > 0 ? (all + 4l * p.even - 1) / (4l * p.even) * 4 : 4);
+}
+// The sequence of range x and the range within it (b = B: none), or the first range of sequence `of` and its ranges
+struct EvenRange {
+  int b, split, ppw;
+};
+__device__ __forceinline__ EvenRange even_find(const AttendParams &p, int x, int of) {
+  const int lane = threadIdx.x & 63, ppw = even_range(p);
+  int before = 0;
+  for (int b = 0; b < p.B; b += 64) {
+    const int n = (pages_of(p, b + lane) + ppw - 1) / ppw, to = before + lanes_sum(n);
+    if (of >= 0) {
+      if (of < b + 64) {
+        const int k = __builtin_amdgcn_readlane(n, of - b);
+        return EvenRange{k, __builtin_amdgcn_readlane(to, of - b) - k, ppw};
+      }
+    } else {
+      const uint64_t past = __ballot(to > x);
+      if (past) {
+        const int k = __builtin_ctzll(past);
+        return EvenRange{b + k, x - __builtin_amdgcn_readlane(to - n, k), ppw};
+      }
+    }
+    before = __builtin_amdgcn_readlane(to, 63);
+  }
+  return EvenRange{p.B, 0, ppw};
+}
+
 // keys that query token i of sequence b sees: positions below this
 __device__ __forceinline__ int row_limit(const AttendParams &p, int b, int i) {
   const int len = seq_len_of(p, b);
@@ -413,7 +463,7 @@ __device__ __forceinline__ void store_row4(const AttendParams &p, size_t row, in
                    : make_uint2(pk_f16_bits(y[0], y[1]), pk_f16_bits(y[2], y[3]));
     return;
   }
-  const size_t at = row * p.nslots + slot;
+  const size_t at = p.even ? row : row * p.nslots + slot;
   *(f32x4 *)(p.part_o + at * kD + c0) = o;
   if (c0 == 0) *(float2 *)(p.part_ml + 2 * at) = make_float2(m, l);
 }
@@ -467,7 +517,8 @@ __device__ __forceinline__ void join_waves(const AttendParams &p, const AttendSe
         for (int e = 0; e < C; ++e) o[e] += s.o[w][rr][c0 + e];
       }
       const int bi = r / LG, j = r - bi * LG, i = j / p.G, b = set.b0 + bi;
-      const size_t row = ((size_t)b * p.L + i) * p.HQ + hkv * p.G + (j - i * p.G);
+      const size_t row = p.even ? ((size_t)set.slot * p.HKV + hkv) * LG + r
+                                : ((size_t)b * p.L + i) * p.HQ + hkv * p.G + (j - i * p.G);
       const bool sees = row_limit(p, b, i) > 0;
 #pragma unroll
       for (int e = 0; e < C; e += 4)

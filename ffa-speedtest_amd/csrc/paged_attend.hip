@@ -16,6 +16,7 @@ __global__ __launch_bounds__(256) void paged_attend_join_kernel(const AttendPara
   if (row >= rows) return;  // (whole workgroups only where waves meet)
   const int i = (row / p.HQ) % p.L, b = row / (p.HQ * p.L);
   const bool sees = row_limit(p, b, i) > 0;
+  size_t first = (size_t)row * p.nslots, step = 1;  // the row's partials
   const int sp = shared_pages_of(p, b), own = max((seq_len_of(p, b) + kPage - 1) / kPage - sp, 0);
   const int na = p.shared_slots ? min((sp + p.shared_ppw - 1) / p.shared_ppw, p.shared_slots) : 0;
   int nb = 0;
@@ -23,8 +24,15 @@ __global__ __launch_bounds__(256) void paged_attend_join_kernel(const AttendPara
     const int per = own_range(p, own);
     nb = min((own + per - 1) / per, p.own_slots);
   }
-  const float2 *ml = (const float2 *)p.part_ml + (size_t)row * p.nslots;
-  const float *po = p.part_o + (size_t)row * p.nslots * kD;
+  if (p.even) {
+    const EvenRange e = even_find(p, 0, __builtin_amdgcn_readfirstlane(b));
+    const int h = row % p.HQ, hkv = h / p.G, LG = p.L * p.G;
+    nb = e.b;
+    step = (size_t)p.HKV * LG;
+    first = e.split * step + (size_t)hkv * LG + i * p.G + (h - hkv * p.G);
+  }
+  const float2 *ml = (const float2 *)p.part_ml + first;
+  const float *po = p.part_o + first * kD;
   float m = kNoMax, l = 0.f;
   float2 o = make_float2(0.f, 0.f);
   const int slots = sees ? na + nb : 0;
@@ -32,9 +40,10 @@ __global__ __launch_bounds__(256) void paged_attend_join_kernel(const AttendPara
     float2 x[4], y[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      const int s = min(s0 + WPR * k, slots - 1), slot = s < na ? s : p.shared_slots + s - na;
+      const int s = min(s0 + WPR * k, slots - 1);
+      const size_t slot = step * (s < na ? s : p.shared_slots + s - na);
       x[k] = ml[slot];
-      y[k] = *(const float2 *)(po + (size_t)slot * kD + 2 * lane);
+      y[k] = *(const float2 *)(po + slot * kD + 2 * lane);
     }
     float mn = m;
 #pragma unroll
@@ -82,9 +91,13 @@ struct AttendPlan {
   int shared_slots, shared_ppw, own_slots, nslots;
   int shared_kind, shared_blocks, own_kind, own_blocks;
   bool both;  // one launch of 256-row workgroups over shared pages and of few-row ones over own pages
+  int even;   // even ranges over the batch's pages, about this many (mxfp4's few-row kernels)
+  size_t parts(const ffa_paged_attend_args *a) const {  // partials of the call
+    return (size_t)(even ? even + a->B : (long)a->B * nslots) * a->L * a->HQ;
+  }
 };
 
-static AttendPlan attend_plan(const ffa_paged_attend_args *a, int cus) {
+static AttendPlan attend_plan(const ffa_paged_attend_args *a, int cus, bool mxfp4) {
   AttendPlan pl = {};
   if (cus <= 0) cus = 256;
   const long LG = (long)a->L * (a->HQ / a->HKV);
@@ -121,6 +134,8 @@ static AttendPlan attend_plan(const ffa_paged_attend_args *a, int cus) {
     pl.both = pl.both && (long)a->HKV * pl.shared_blocks * pl.shared_slots * a->ngroups < 1l << 30;
   }
   pl.nslots = pl.shared_slots + pl.own_slots;
+  if (mxfp4 && a->ngroups == 0 && a->seq_lens && pl.own_kind <= kRows32 && pl.own_slots > 1)
+    pl.even = mx_even_ranges(a->B, a->HKV, pl.own_kind, cus);
   if (pl.shared_slots == 0 && pl.own_slots <= 1) {  // one range: no partials
     pl.own_slots = 1;
     pl.nslots = 0;
@@ -167,15 +182,15 @@ static int attend_check(const ffa_paged_attend_args *a, const uint8_t *v_scale) 
 
 static size_t attend_scratch(const ffa_paged_attend_args *a, const uint8_t *v_scale) {
   if (attend_check(a, v_scale) != FFA_OK) return 0;
-  return (size_t)a->B * a->L * a->HQ * attend_plan(a, device_cus()).nslots * (kD + 2) * sizeof(float);
+  return attend_plan(a, device_cus(), v_scale != nullptr).parts(a) * (kD + 2) * sizeof(float);
 }
 
 static int attend_run(const ffa_paged_attend_args *a, const uint8_t *v_scale, void *stream) {
   const int bad = attend_check(a, v_scale);
   if (bad != FFA_OK) return bad;
-  const AttendPlan pl = attend_plan(a, device_cus());
-  const size_t rows = (size_t)a->B * a->L * a->HQ;
-  if (a->scratch_bytes < rows * pl.nslots * (kD + 2) * sizeof(float) || (pl.nslots && !a->scratch))
+  const AttendPlan pl = attend_plan(a, device_cus(), v_scale != nullptr);
+  const size_t rows = (size_t)a->B * a->L * a->HQ, parts = pl.parts(a);
+  if (a->scratch_bytes < parts * (kD + 2) * sizeof(float) || (parts && !a->scratch))
     FFA_BAD("scratch below ffa_paged_attend_scratch()");
   if ((uintptr_t)a->scratch & 15) FFA_BAD("scratch must be a multiple of 16 bytes");
   AttendParams p = {};
@@ -194,7 +209,8 @@ static int attend_run(const ffa_paged_attend_args *a, const uint8_t *v_scale, vo
   p.seq_group = a->seq_group;
   p.out = a->out;
   p.part_o = (float *)a->scratch;
-  p.part_ml = p.part_o + rows * pl.nslots * kD;
+  p.part_ml = p.part_o + parts * kD;
+  p.even = pl.even;
   p.bt_stride = a->bt_stride;
   p.num_pages = a->num_pages;
   p.ngroups = a->ngroups;
@@ -231,7 +247,8 @@ static int attend_run(const ffa_paged_attend_args *a, const uint8_t *v_scale, vo
       launch(pl.shared_kind, pl.shared_slots, pl.shared_blocks, a->ngroups, -1);
     }
     p.nshared = 0;
-    if (pl.own_slots > 0) launch(pl.own_kind, pl.own_slots, pl.own_blocks, a->B, -1);
+    if (pl.even) launch(pl.own_kind, pl.even + a->B, pl.own_blocks, 1, -1);
+    else if (pl.own_slots > 0) launch(pl.own_kind, pl.own_slots, pl.own_blocks, a->B, -1);
   }
   if (pl.nslots > 0 && !join_by_wave((long)rows))
     hipLaunchKernelGGL(paged_attend_join_kernel<4>, dim3((unsigned)rows), dim3(256), 0, st, p, (int)rows);

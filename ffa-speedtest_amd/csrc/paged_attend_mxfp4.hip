@@ -6,8 +6,8 @@
 // applies the block's power of two.  V's powers of two belong to tokens, of which a V^T operand holds eight, so they
 // multiply the weights: for each block of 32 columns the weights' operand is w_t 2^(e_t - R), R the largest e so far, and
 // V's codes are converted as they are.  In a page that every row sees whole, and whose e lie within 14 of R, that is a
-// packed product of fp16 pairs, exact; other pages take the same in fp32, with what a row does not see left out.  A NaN
-// block thereby reaches the rows that see it and no other.  The weights' sum is a product with ones, of the weights as
+// packed product of fp16 pairs, exact; other pages, put off to the end of a run of 64, take it in fp32, with what a row does
+// not see left out.  A NaN block thereby reaches the rows that see it and no other.  The weights' sum is a product with ones, of the weights as
 // they are rounded.
 // (The block-scaled matrix instruction on the codes themselves needs neither conversion, but it sums the products of a
 // group of channels on a common 14-bit grid: 256 + 2^-6 = 256 there, where sums in 32 bits keep 2^-15.)
@@ -18,7 +18,8 @@ namespace ffa {
 typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
 
 // One (page, KV head) as lane (g, n) takes it: K, and V with its scales.  Each half is loaded for the next page as soon
-// as this page's is used.
+// as this page's is used.  (The pages that need care are a loop of their own: as a branch of this one they cost it 30
+// registers, whose spills, waited for in order behind the next page's loads, took 1.4 times as long with two row tiles.)
 struct MxKeys {
   u32x4 code[4];
   uint32_t scale;  // tokens 4 n + (0..3), block g
@@ -58,7 +59,14 @@ template <int NT, int W>
 __device__ __forceinline__ void few_rows_mx(const AttendParams &p, int split, int hkv, int rb, int z, FewLds<kFmtMxfp4, NT, W> &s) {
   const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, n = lane & 15;
-  const AttendSet set = attend_set(p, z, split);
+  AttendSet set;
+  if (p.even) {
+    const EvenRange e = even_find(p, split, -1);
+    if (e.b >= p.B) return;
+    set = AttendSet{e.b, 1, e.split * e.ppw, min((e.split + 1) * e.ppw, pages_of(p, e.b)), split};
+  } else {
+    set = attend_set(p, z, split);
+  }
   const int LG = p.L * p.G, R = set.n * LG, r0 = rb * 16 * NT;
   if (r0 >= R) return;
   const int pa = set.p0, pe = set.p1;
@@ -72,10 +80,9 @@ __device__ __forceinline__ void few_rows_mx(const AttendParams &p, int split, in
   };
   MxKeys K;
   MxValues V;
-  size_t blk = 0;
   int id = 0;
   if (pa < pe) {
-    blk = block(page_id(pa + wv));
+    const size_t blk = block(page_id(pa + wv));
     id = page_id(pa + wv + W);
     load_keys(p, blk, lane, K);
     load_values(p, blk, lane, V);
@@ -111,10 +118,8 @@ __device__ __forceinline__ void few_rows_mx(const AttendParams &p, int split, in
 
   const f16x8 one = {1, 1, 1, 1, 1, 1, 1, 1};
   int vtop = kMxLow;  // R + 127
-  const int last = min(pe, (hi + kPage - 1) / kPage);  // no row sees a later page
-  for (int pg = pa + wv; pg < last; pg += W) {
-    const int t0 = pg * kPage;
-    f32x4 S[NT][4];
+  f32x4 S[NT][4];
+  auto scores = [&]() {
 #pragma unroll
     for (int tau = 0; tau < 4; ++tau) {
       const float ks = mx_factor((K.scale >> (8 * tau)) & 0xffu);
@@ -129,27 +134,16 @@ __device__ __forceinline__ void few_rows_mx(const AttendParams &p, int split, in
         S[t][tau] = a;
       }
     }
-    blk = block(id);
-    id = page_id(pg + 2 * W);
-    load_keys(p, blk, lane, K);
-
-    const bool full = lo >= t0 + kPage;  // every row sees the whole page
-    if (!full)
-#pragma unroll
-      for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int tau = 0; tau < 4; ++tau)
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (t0 + 16 * g + 4 * i + tau >= lim[t]) S[t][tau][i] = -INFINITY;
-    u32x4 w16[NT][2];
+  };
+  u32x4 w16[NT][2];  // the weights, tokens 16 g + 8 kap + (0..7)
+  auto weights = [&]() {
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       float top = S[t][0][0];
 #pragma unroll
       for (int k = 1; k < 16; ++k) top = fmaxf(top, S[t][k >> 2][k & 3]);
       top *= cs[t];
-      if (__ballot(top > m[t] + (kHead + kStale)) != 0) {
+      if (__ballot(top > m[t] + (kHead + kStale)) != 0) [[unlikely]] {
         const float mn = fmaxf(m[t], xor_max(xor_max(top, 16), 32) - kHead), alpha = exp2_hw(m[t] - mn);
         m[t] = mn;
         Ls[t] *= alpha;
@@ -165,24 +159,52 @@ __device__ __forceinline__ void few_rows_mx(const AttendParams &p, int split, in
 #pragma unroll
       for (int kap = 0; kap < 2; ++kap) Ls[t] = mfma16(one, __builtin_bit_cast(f16x8, w16[t][kap]), Ls[t]);
     }
-    // scales of the page: above R, or more than 14 below it?
-    bool packed = full;
-    {
-      const u16x2 a = __builtin_bit_cast(u16x2, V.every & 0x00ff00ffu), b = __builtin_bit_cast(u16x2, (V.every >> 8) & 0x00ff00ffu);
-      const u16x2 most = __builtin_elementwise_max(a, b), least = __builtin_elementwise_min(a, b);
-      if (__ballot(max(most[0], most[1]) > vtop) != 0) {
-        const int now = max(vtop, page_scale(V.every, lane, hi - t0));
-        const float f = now - vtop > 126 ? 0.f : mx_factor(127 + vtop - now);
-        vtop = now;
+  };
+  // R up to the page's largest scale; whether all of its scales then lie within 14 below R
+  auto scales = [&](int t0) {
+    const u16x2 a = __builtin_bit_cast(u16x2, V.every & 0x00ff00ffu), b = __builtin_bit_cast(u16x2, (V.every >> 8) & 0x00ff00ffu);
+    const u16x2 most = __builtin_elementwise_max(a, b), least = __builtin_elementwise_min(a, b);
+    const int up = max((int)most[0], (int)most[1]), low = min((int)least[0], (int)least[1]);
+    if (__ballot(up > vtop) != 0) [[unlikely]] {
+      const int now = max(vtop, page_scale(V.every, lane, hi - t0));
+      const float f = now - vtop > 126 ? 0.f : mx_factor(127 + vtop - now);
+      vtop = now;
 #pragma unroll
-        for (int t = 0; t < NT; ++t)
+      for (int t = 0; t < NT; ++t)
 #pragma unroll
-          for (int u = 0; u < 8; ++u) O[t][u] *= f;
-        packed = packed && __ballot(max(most[0], most[1]) > vtop) == 0;  // no NaN block
-      }
-      packed = packed && __ballot((int)min(least[0], least[1]) < vtop - 14) == 0;
+        for (int u = 0; u < 8; ++u) O[t][u] *= f;
     }
-    if (packed) {
+    return __ballot(up > vtop || low < vtop - 14) == 0;
+  };
+  auto values = [&](int cb, const f16x8 (*P)[2]) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int kap = 0; kap < 2; ++kap) {
+        const f16x8 a = mx_operand(V.code[cb][2 * h + kap], 1.0f);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) O[t][2 * cb + h] = mfma16(a, P[t][kap], O[t][2 * cb + h]);
+      }
+  };
+
+  const int last = min(pe, (hi + kPage - 1) / kPage);  // no row sees a later page
+  // 64 pages of the wave at a time: those that every row sees whole and whose scales lie together, then the others
+#pragma unroll 1
+  for (int p0 = pa + wv; p0 < last; p0 += 64 * W) {
+    uint64_t others = 0;
+#pragma unroll 1
+    for (int i = 0, pg = p0; i < 64 && pg < last; ++i, pg += W) {
+      const size_t next = block(id);
+      id = page_id(pg + 2 * W);
+      if (lo < (pg + 1) * kPage || !scales(pg * kPage)) [[unlikely]] {
+        others |= 1ull << i;
+        load_keys(p, next, lane, K);
+        load_values(p, next, lane, V);
+        continue;
+      }
+      scores();
+      load_keys(p, next, lane, K);
+      weights();
       const uint32_t base = (uint32_t)(vtop - 15) * 0x01010101u;
 #pragma unroll
       for (int cb = 0; cb < 4; ++cb) {
@@ -190,57 +212,60 @@ __device__ __forceinline__ void few_rows_mx(const AttendParams &p, int split, in
 #pragma unroll
         for (int kap = 0; kap < 2; ++kap)
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
+          for (int j = 0; j < 2; ++j) {
             // four bytes 127 + e to the upper bytes of the fp16 numbers 2^(e - R)
-            const uint32_t x = (V.scale[cb][2 * kap + i] - base) << 2;
+            const uint32_t x = (V.scale[cb][2 * kap + j] - base) << 2;
             const f16x2 f[2] = {bits_f16x2(__builtin_amdgcn_perm(0, x, 0x010c000cu)), bits_f16x2(__builtin_amdgcn_perm(0, x, 0x030c020cu))};
 #pragma unroll
             for (int e = 0; e < 2; ++e)
 #pragma unroll
               for (int t = 0; t < NT; ++t) {
-                const f16x2 y = bits_f16x2(w16[t][kap][2 * i + e]) * f[e];
-                P[t][kap][4 * i + 2 * e] = y[0];
-                P[t][kap][4 * i + 2 * e + 1] = y[1];
+                const f16x2 y = bits_f16x2(w16[t][kap][2 * j + e]) * f[e];
+                P[t][kap][4 * j + 2 * e] = y[0];
+                P[t][kap][4 * j + 2 * e + 1] = y[1];
               }
           }
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int kap = 0; kap < 2; ++kap) {
-            const f16x8 a = mx_operand(V.code[cb][2 * h + kap], 1.0f);
-#pragma unroll
-            for (int t = 0; t < NT; ++t) O[t][2 * cb + h] = mfma16(a, P[t][kap], O[t][2 * cb + h]);
-          }
+        values(cb, P);
       }
-    } else {
+      load_values(p, next, lane, V);
+    }
+    if (others == 0) [[likely]] continue;
+#pragma unroll 1
+    for (; others != 0; others &= others - 1) {
+      const int pg = p0 + W * __builtin_ctzll(others), t0 = pg * kPage;
+      const size_t blk = block(page_id(pg));
+      load_keys(p, blk, lane, K);
+      load_values(p, blk, lane, V);
+      scales(t0);
+      scores();
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int tau = 0; tau < 4; ++tau)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (t0 + 16 * g + 4 * i + tau >= lim[t]) S[t][tau][i] = -INFINITY;
+      weights();
 #pragma unroll
       for (int cb = 0; cb < 4; ++cb) {
         f16x8 P[NT][2];
-        asm("" : "+v"(V.code[cb]));  // else the compiler converts V for both branches before them, in 64 more registers
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          const int nvis = lim[t] - t0 - 16 * g;  // of the lane's tokens
-          asm("" : "+v"(w16[t][0]), "+v"(w16[t][1]));  // nor the weights in fp32 for all four blocks
+        for (int t = 0; t < NT; ++t)
 #pragma unroll
           for (int k = 0; k < 16; ++k) {
             const int byte = (V.scale[cb][k >> 2] >> (8 * (k & 3))) & 0xffu;
             // byte - vtop <= 0 for what a row sees, but for NaN blocks
             const float f = byte == kMxNan ? NAN : mx_factor(max(127 + min(byte - vtop, 0), 0));
             const float w = (float)__builtin_bit_cast(f16x8, w16[t][k >> 3])[k & 7];
-            P[t][k >> 3][k & 7] = (_Float16)(k < nvis ? w * f : 0.f);
+            P[t][k >> 3][k & 7] = (_Float16)(t0 + 16 * g + k < lim[t] ? w * f : 0.f);
           }
-        }
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int kap = 0; kap < 2; ++kap) {
-            const f16x8 a = mx_operand(V.code[cb][2 * h + kap], 1.0f);
-#pragma unroll
-            for (int t = 0; t < NT; ++t) O[t][2 * cb + h] = mfma16(a, P[t][kap], O[t][2 * cb + h]);
-          }
+        values(cb, P);
       }
     }
-    load_values(p, blk, lane, V);
+    if (p0 + 64 * W < last) {
+      load_keys(p, block(page_id(p0 + 64 * W)), lane, K);
+      load_values(p, block(page_id(p0 + 64 * W)), lane, V);
+    }
   }
   float l[NT];
 #pragma unroll

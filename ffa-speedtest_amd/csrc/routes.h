@@ -104,6 +104,14 @@ inline int attend_kind(long rows) {
 // workgroups that are resident at a time: one round of them (a second one that is not full costs as much)
 inline long attend_resident(int kind, int cus) { return (kind == kRows256 ? 1l : 2l) * cus; }
 
+// Even page ranges of a batch of mxfp4 pages for few rows: about one round of workgroups in all (kernels of either kind run
+// two a CU), each sequence's last range being a part of one.
+inline int mx_even_ranges(int B, int HKV, int kind, int cus) {
+  const long all = attend_resident(kind, cus) / HKV > 0 ? attend_resident(kind, cus) / HKV : 1;
+  const long n = all - B > all / 2 ? all - B : all / 2;
+  return (int)(n > 0 ? n : 1);
+}
+
 // Chunks of many rows over fewer than 48 pages, where a workgroup's fixed 10-14 us count as much as its pages': smaller
 // workgroups then, and ranges that are split (their partials are rows x 528 bytes, written and read) only where the chip
 // is not half full.  A prompt of 700 tokens 56 -> 22 us, 4 of 1024 81 -> 73.  heads: sequences x KV heads.
