@@ -21,7 +21,7 @@ from . import _native as N
 from .attend import _int32, _on
 from .decode import HEAD_DIM
 from .paged import PAGE, check_append_fits
-from .rope_axes import AxisRope, strided_rows
+from .rope_axes import _NO_STRIDES, AxisRope, _launch, rows_like, strided_rows
 
 _DTYPES = (torch.float16, torch.bfloat16, torch.float32)
 
@@ -71,13 +71,13 @@ class PagedMXFP4Cache:
         if v is not None and v.shape != k.shape:
             raise ValueError("v must have the shape of k")
         dev = self.k.device
-        for x, what in ((q, "q"), (k, "k"), (v, "v")):
+        for x in (k, v, q):
             if x is None:
                 continue
             if x.dtype not in _DTYPES:
-                raise NotImplementedError(f"{what} must be fp16, bf16 or fp32, got {x.dtype}")
-            if x.device.type != "cuda" or x.device != dev:
-                raise ValueError(f"{what} is on {x.device}, the cache on {dev}: both must be on one GPU")
+                raise NotImplementedError(f"rows must be fp16, bf16 or fp32, got {x.dtype}")
+            if x.device != dev or dev.type != "cuda":
+                raise ValueError(f"rows are on {x.device}, the cache on {dev}: both must be on one GPU")
         HQ = 0
         if rope is not None and rope.table.device != dev:
             raise ValueError(f"the rotation is on {rope.table.device}, the cache on {dev}")
@@ -85,22 +85,22 @@ class PagedMXFP4Cache:
             if q.ndim != 4 or q.shape[:2] != k.shape[:2] or q.shape[3] != HEAD_DIM or q.dtype != k.dtype:
                 raise ValueError("q must be [B, Tn, HQ, 128] of k's type")
             HQ = q.shape[2]
-        if tuple(pos.shape) != (B,) or block_table.ndim != 2 or block_table.shape[0] != B:
+        if pos.shape != (B,) or block_table.ndim != 2 or block_table.shape[0] != B:
             raise ValueError("pos must be [B] and block_table [B, n]")
         out_type = k.dtype
         if v is not None and v.dtype != k.dtype:  # fp32 holds both
             k, v = k.float(), v.float()
             q = None if q is None else q.float()
-        q_out = None if q is None else torch.empty(q.shape, dtype=q.dtype, device=dev)
-        k_values = torch.empty(k.shape, dtype=k.dtype, device=dev) if values else None
-        v_values = torch.empty(k.shape, dtype=k.dtype, device=dev) if values and v is not None else None
+        q_out = None if q is None else rows_like(q)
+        k_values = rows_like(k) if values else None
+        v_values = rows_like(v) if values and v is not None else None
         if k.numel():
             pos, block_table = _int32(pos, dev), _int32(block_table, dev)
             if check:
                 check_append_fits(pos, Tn, block_table, self.P, ragged)
-            (k, ks), none = strided_rows(k), (None, (0, 0, 0))
-            v, vs = none if v is None else strided_rows(v)
-            q, qs = none if not HQ else strided_rows(q)
+            k, ks = strided_rows(k)
+            v, vs = (None, _NO_STRIDES) if v is None else strided_rows(v)
+            q, qs = strided_rows(q) if HQ else (None, _NO_STRIDES)
             p, p_axis, p_batch, axes = None, 0, 0, 0
             if rope is not None:
                 axes = rope.axes
@@ -108,14 +108,14 @@ class PagedMXFP4Cache:
                     p, p_axis, p_batch = rope._positions(positions, B, Tn, dev)
             a = N.MXFP4AppendArgs(
                 k.data_ptr(), N.ptr(v), N.ptr(q), N.dtype_code(k.dtype), B, Tn, HKV, HQ, *ks, *vs, *qs,
-                None if rope is None else rope.table.data_ptr(), N.ptr(p), int(p is not None and p.dtype is torch.int64), axes,
-                p_axis, p_batch, int(rope is not None and rope.adjacent), pos.data_ptr(), block_table.data_ptr(),
+                None if rope is None else rope.table.data_ptr(), N.ptr(p), p is not None and p.dtype is torch.int64, axes,
+                p_axis, p_batch, rope is not None and rope.adjacent, pos.data_ptr(), block_table.data_ptr(),
                 block_table.shape[1], self.P, self.k.data_ptr(), self.k_scale.data_ptr(), self.v.data_ptr(),
                 self.v_scale.data_ptr(), N.ptr(q_out), N.ptr(k_values), N.ptr(v_values))
-            with _on(dev):
-                rc = N.lib().ffa_mxfp4_append(ctypes.byref(a), N.stream_of(dev))
-            N.check(rc, "ffa_mxfp4_append")
-        return [x if x is None or x.dtype is out_type else x.to(out_type) for x in (q_out, k_values, v_values)]
+            N.check(_launch(N.lib().ffa_mxfp4_append, a, dev), "ffa_mxfp4_append")
+        if k.dtype is not out_type:
+            return [x if x is None else x.to(out_type) for x in (q_out, k_values, v_values)]
+        return [q_out, k_values, v_values]
 
     # ------------------------------------------------------------------ reads
     def dequantize(self, block_table: torch.Tensor, T: int, seq_lens: torch.Tensor | None = None,

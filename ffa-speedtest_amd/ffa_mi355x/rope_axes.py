@@ -17,20 +17,34 @@ from .decode import HEAD_DIM
 
 PAIRS = HEAD_DIM // 2
 _DTYPES = (torch.float16, torch.bfloat16, torch.float32)
+_NO_STRIDES = (0, 0, 0)
+
+
+def _launch(fn, args: ctypes.Structure, device: torch.device) -> int:
+    if device.index == torch.cuda.current_device():
+        return fn(ctypes.byref(args), N.stream_of(device))
+    with _on(device):
+        return fn(ctypes.byref(args), N.stream_of(device))
 
 
 def strided_rows(x: torch.Tensor) -> tuple[torch.Tensor, tuple[int, int, int]]:
     """x [B, T, H, 128] and its strides (elements; 0 where a dimension has one entry) as the kernels take rows: 128
     contiguous channels, every address a multiple of 16 bytes.  Others are copied."""
-    def strides(t):
-        return tuple(s if n > 1 else 0 for s, n in zip(t.stride()[:3], t.shape[:3]))
-
-    step = 16 // x.element_size()
-    if x.stride(3) != 1 or any(s % step for s in strides(x)):
+    if not x.is_contiguous():
+        step = 16 // x.element_size()
+        strides = tuple([s if n > 1 else 0 for s, n in zip(x.stride()[:3], x.shape[:3])])
+        if x.stride(3) == 1 and not (strides[0] % step or strides[1] % step or strides[2] % step or x.data_ptr() % 16):
+            return x, strides
         x = x.contiguous()
     if x.data_ptr() % 16:
         x = x.clone(memory_format=torch.contiguous_format)
-    return x, strides(x)
+    b, t, h, _ = x.stride()
+    return x, (b, t, h)
+
+
+def rows_like(x: torch.Tensor) -> torch.Tensor:
+    """Contiguous rows of x's shape and type (empty_like: a third of empty's time on the host)."""
+    return torch.empty_like(x) if x.is_contiguous() else torch.empty(x.shape, dtype=x.dtype, device=x.device)
 
 
 class AxisRope:
@@ -84,6 +98,8 @@ class AxisRope:
             raise ValueError(f"positions are on {positions.device}, the rows on {dev}")
         shape = tuple(positions.shape)
         if shape == (self.axes, B, T):
+            if positions.is_contiguous():
+                return positions, B * T, T
             p = positions
         elif shape == (self.axes, T):
             p = positions[:, None].expand(self.axes, B, T)
@@ -95,53 +111,46 @@ class AxisRope:
             p = p.contiguous()
         return p, p.stride(0), p.stride(1)
 
-    def _check(self, x: torch.Tensor, what: str, like: torch.Tensor | None = None) -> None:
+    def _check(self, x: torch.Tensor, what: str) -> None:
         if x.ndim != 4 or x.shape[3] != HEAD_DIM:
             raise ValueError(f"{what} must be [B, T, H, {HEAD_DIM}], got {tuple(x.shape)}")
         if x.dtype not in _DTYPES:
             raise NotImplementedError(f"{what} must be fp16, bf16 or fp32, got {x.dtype}")
-        if x.device.type != "cuda" or self.table.device != x.device:
+        if self.table.device != x.device or x.device.type != "cuda":
             raise ValueError(f"{what} is on {x.device}, the rotation on {self.table.device}: both must be on one GPU")
-        if like is not None and (x.shape[:2] != like.shape[:2] or x.dtype != like.dtype):
-            raise ValueError("q and k must have the same sequences, tokens and type")
+
+    @staticmethod
+    def _rows(x: torch.Tensor, inplace: bool):
+        """What the kernel reads and writes for x: input, strides, output, strides."""
+        src, st = strided_rows(x)
+        if not inplace:
+            hs = x.shape[2] * HEAD_DIM
+            return src, st, rows_like(x), (x.shape[1] * hs, hs, HEAD_DIM)
+        if src is not x:
+            raise ValueError("rows turned in place must have contiguous channels and 16-byte aligned strides")
+        if any(n > 1 and s == 0 for n, s in zip(x.shape, x.stride())):
+            raise ValueError("rows turned in place must not be expanded")
+        return x, st, x, st
 
     def _run(self, positions, q, k, inverse, inplace):
+        dev, dtype = q.device, q.dtype
         B, T, HQ, _ = q.shape
-        HKV = 0 if k is None else k.shape[2]
-        if q.numel() == 0:
-            HQ = 0
-        if HKV and k.numel() == 0:
-            HKV = 0
-        pos, pos_axis, pos_batch = self._positions(positions, B, T, q.device)
-        outs, args = [], []
-        for x in (q, k):
-            if x is None:
-                args.append((None, None, (0, 0, 0), (0, 0, 0)))
-                continue
-            src, st = strided_rows(x)
-            if inplace:
-                if src is not x:
-                    raise ValueError("rows turned in place must have contiguous channels and 16-byte aligned strides")
-                if any(n > 1 and s == 0 for n, s in zip(x.shape, x.stride())):
-                    raise ValueError("rows turned in place must not be expanded")
-                out, ot = x, st
-            else:
-                out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-                ot = tuple(out.stride()[:3])
-            outs.append(out)
-            args.append((src, out, st, ot))
-        if HQ == 0 and HKV == 0:
+        pos, pos_axis, pos_batch = self._positions(positions, B, T, dev)
+        q_in, qs, q_out, qo = self._rows(q, inplace)
+        HKV, k_in, ks, k_out, ko = 0, None, _NO_STRIDES, None, _NO_STRIDES
+        if k is not None:
+            HKV = k.shape[2]
+            k_in, ks, k_out, ko = self._rows(k, inplace)
+        outs = (q_out,) if k is None else (q_out, k_out)
+        if B == 0 or T == 0 or HQ + HKV == 0:
             return outs
-        (q_in, q_out, qs, qo), (k_in, k_out, ks, ko) = args
         if HQ == 0:  # k alone, in q's place
-            (q_in, q_out, qs, qo), HQ, HKV = (k_in, k_out, ks, ko), HKV, 0
+            q_in, qs, q_out, qo, HQ, HKV = k_in, ks, k_out, ko, HKV, 0
         a = N.RopeAxesArgs(
-            q_in.data_ptr(), q_out.data_ptr(), N.ptr(k_in), N.ptr(k_out), N.dtype_code(q.dtype), B, T, HQ, HKV, *qs, *qo, *ks,
-            *ko, self.table.data_ptr(), pos.data_ptr(), int(pos.dtype is torch.int64), self.axes, pos_axis, pos_batch,
-            int(self.adjacent), int(inverse))
-        with _on(q.device):
-            rc = N.lib().ffa_rope_axes(ctypes.byref(a), N.stream_of(q.device))
-        N.check(rc, "ffa_rope_axes")
+            q_in.data_ptr(), q_out.data_ptr(), N.ptr(k_in), N.ptr(k_out), N.dtype_code(dtype), B, T, HQ, HKV, *qs, *qo, *ks, *ko,
+            self.table.data_ptr(), pos.data_ptr(), pos.dtype is torch.int64, self.axes, pos_axis, pos_batch, self.adjacent,
+            inverse)
+        N.check(_launch(N.lib().ffa_rope_axes, a, dev), "ffa_rope_axes")
         return outs
 
     def rotate(self, positions: torch.Tensor, q: torch.Tensor, k: torch.Tensor | None = None, *, inverse: bool = False,
@@ -152,14 +161,16 @@ class AxisRope:
         Returns q, or (q, k) where k is given."""
         self._check(q, "q")
         if k is not None:
-            self._check(k, "k", q)
+            self._check(k, "k")
+            if k.shape[:2] != q.shape[:2] or k.dtype != q.dtype:
+                raise ValueError("q and k must have the same sequences, tokens and type")
         if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
             if inplace:
                 raise ValueError("rows that need gradients are not turned in place")
             got = _Rotate.apply(self, positions, inverse, q, k)
         else:
             got = self._run(positions, q, k, inverse, inplace)
-        return got[0] if k is None else (got[0], got[1])
+        return got[0] if k is None else got
 
 
 class _Rotate(torch.autograd.Function):
@@ -169,7 +180,7 @@ class _Rotate(torch.autograd.Function):
     def forward(ctx, rope, positions, inverse, q, k):
         ctx.rope, ctx.inverse, ctx.two = rope, inverse, k is not None
         ctx.save_for_backward(positions)
-        return tuple(rope._run(positions, q, k, inverse, False))
+        return rope._run(positions, q, k, inverse, False)
 
     @staticmethod
     def backward(ctx, gq, gk=None):
