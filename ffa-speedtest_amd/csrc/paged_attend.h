@@ -87,22 +87,19 @@ __device__ __forceinline__ int lanes_sum(int x) {
   x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, false);  // row_bcast 31 into rows 2 and 3
   return x;
 }
-// pages per range: a page for each of four waves at least
-__device__ __forceinline__ int even_range(const AttendParams &p) {
-  const int lane = threadIdx.x & 63;
-  long all = 0;
-  for (int b = 0; b < p.B; b += 64) all += __builtin_amdgcn_readlane(lanes_sum(pages_of(p, b + lane)), 63);
-  return (int)((all + 4l * p.even - 1) / (4l * p.even) > 0 ? (all + 4l * p.even - 1) / (4l * p.even) * 4 : 4);
-}
 // The sequence of range x and the range within it (b = B: none), or the first range of sequence `of` and its ranges
 struct EvenRange {
   int b, split, ppw;
 };
 __device__ __forceinline__ EvenRange even_find(const AttendParams &p, int x, int of) {
-  const int lane = threadIdx.x & 63, ppw = even_range(p);
+  const int lane = threadIdx.x & 63, mine = pages_of(p, lane);
+  long all = __builtin_amdgcn_readlane(lanes_sum(mine), 63);
+  for (int b = 64; b < p.B; b += 64) all += __builtin_amdgcn_readlane(lanes_sum(pages_of(p, b + lane)), 63);
+  // pages per range: a page for each of four waves at least
+  const int ppw = all <= 4l * p.even ? 4 : (int)((all + 4l * p.even - 1) / (4l * p.even)) * 4;
   int before = 0;
   for (int b = 0; b < p.B; b += 64) {
-    const int n = (pages_of(p, b + lane) + ppw - 1) / ppw, to = before + lanes_sum(n);
+    const int n = ((b == 0 ? mine : pages_of(p, b + lane)) + ppw - 1) / ppw, to = before + lanes_sum(n);
     if (of >= 0) {
       if (of < b + 64) {
         const int k = __builtin_amdgcn_readlane(n, of - b);
@@ -302,19 +299,19 @@ __device__ __forceinline__ void k_operands(const KRaw<FMT, RES> &r, int tau, con
 __device__ __forceinline__ void load_q(const AttendParams &p, size_t row, bool ok, int kc, f16x8 *op, float &cs) {
   float x[32];
   const uint4 *src = (const uint4 *)((const uint16_t *)p.q + row * kD + 32 * kc);
+  uint4 w[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) w[e] = ok ? src[e] : make_uint4(0, 0, 0, 0);
+  if (p.q_bf16) {  // one branch: a choice for each element became one each
+#pragma unroll
+    for (int e = 0; e < 4; ++e) raw8_to_f32<1>(Raw8<1>{{w[e]}}, x + 8 * e);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) raw8_to_f32<0>(Raw8<0>{{w[e]}}, x + 8 * e);
+  }
   float top = 0.f;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const uint4 w = ok ? src[e] : make_uint4(0, 0, 0, 0);
-    const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      x[8 * e + 2 * i] = p.q_bf16 ? __uint_as_float(ww[i] << 16) : f16_bits_to_f32(ww[i] & 0xffffu);
-      x[8 * e + 2 * i + 1] = p.q_bf16 ? __uint_as_float(ww[i] & 0xffff0000u) : f16_bits_to_f32(ww[i] >> 16);
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x[8 * e + i]));
-  }
+  for (int i = 0; i < 32; ++i) top = fmaxf(top, fabsf(x[i]));
   top = xor_max(top, 16);
   top = xor_max(top, 32);
   int ex = (int)((__float_as_uint(top) >> 23) & 0xffu);  // 0: all zero or tiny; 255: an infinity

@@ -42,6 +42,15 @@ __device__ __forceinline__ void load_values(const AttendParams &p, size_t blk, i
   for (int i = 0; i < 4; ++i) r.code[i] = __builtin_nontemporal_load((const u32x4 *)(p.v + blk * kMxCodes) + 64 * i + lane);
 }
 
+// The largest of the first 16 lanes' x (lane n: row n's), wave-uniform
+__device__ __forceinline__ int row16_max(int x) {
+  x = max(x, __builtin_amdgcn_update_dpp(0, x, kRowRor8, 0xF, 0xF, false));
+  x = max(x, __builtin_amdgcn_update_dpp(0, x, kRowRor4, 0xF, 0xF, false));
+  x = max(x, __builtin_amdgcn_update_dpp(0, x, kRowRor2, 0xF, 0xF, false));
+  x = max(x, __builtin_amdgcn_update_dpp(0, x, kRowRor1, 0xF, 0xF, false));
+  return __builtin_amdgcn_readfirstlane(x);
+}
+
 // The largest scale byte of a page's first `tokens` tokens (NaN blocks apart), wave-uniform
 __device__ __forceinline__ int page_scale(uint32_t every, int lane, int tokens) {
   int best = 0;
@@ -50,9 +59,7 @@ __device__ __forceinline__ int page_scale(uint32_t every, int lane, int tokens) 
     const int byte = (every >> (8 * j)) & 0xffu;
     if (byte != kMxNan && 4 * (lane & 15) + j < tokens) best = max(best, byte);
   }
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) best = max(best, __shfl_xor(best, d));
-  return __builtin_amdgcn_readfirstlane(best);
+  return __builtin_amdgcn_readfirstlane((int)wave_max((float)best));
 }
 
 template <int NT, int W>
@@ -108,13 +115,8 @@ __device__ __forceinline__ void few_rows_mx(const AttendParams &p, int split, in
 #pragma unroll
     for (int u = 0; u < 8; ++u) O[t][u] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
-#pragma unroll
-  for (int d = 1; d < 16; d <<= 1) {
-    lo = min(lo, __shfl_xor(lo, d));
-    hi = max(hi, __shfl_xor(hi, d));
-  }
-  lo = __builtin_amdgcn_readfirstlane(lo);
-  hi = __builtin_amdgcn_readfirstlane(hi);
+  lo = -row16_max(-lo);
+  hi = row16_max(hi);
 
   const f16x8 one = {1, 1, 1, 1, 1, 1, 1, 1};
   int vtop = kMxLow;  // R + 127
