@@ -42,6 +42,51 @@ __device__ __forceinline__ void load_values(const AttendParams &p, size_t blk, i
   for (int i = 0; i < 4; ++i) r.code[i] = __builtin_nontemporal_load((const u32x4 *)(p.v + blk * kMxCodes) + 64 * i + lane);
 }
 
+// With two row tiles a page's registers are short: the wave's pages then come through LDS, two ahead of use and in no
+// registers (five drafted tokens of 8 sequences 88 -> 79 us, of 2 35 -> 29; with one tile, which memory bounds, 121 -> 125).
+// What is read from there goes by the instruction itself: the compiler makes every read of LDS it knows of wait for all
+// copies under way.
+struct MxSlot {
+  u32x4 k[4][64], v[4][64];
+  uint32_t ks[64], vs[64];
+};
+constexpr int kSlotLoads = 10;
+__device__ __forceinline__ void copy_page(const AttendParams &p, size_t blk, int lane, MxSlot &s) {
+  typedef const __attribute__((address_space(1))) void *From;
+  typedef __attribute__((address_space(3))) void *To;
+  __builtin_amdgcn_global_load_lds((From)(p.ks + blk * kMxScales + 4 * lane), (To)s.ks, 4, 0, 0);
+  __builtin_amdgcn_global_load_lds((From)(p.vs + blk * kMxScales + 4 * lane), (To)s.vs, 4, 0, 0);
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    __builtin_amdgcn_global_load_lds((From)(p.k + blk * kMxCodes + 1024 * i + 16 * lane), (To)s.k[i], 16, 0, kNonTemporal);
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    __builtin_amdgcn_global_load_lds((From)(p.v + blk * kMxCodes + 1024 * i + 16 * lane), (To)s.v[i], 16, 0, kNonTemporal);
+}
+__device__ __forceinline__ uint32_t lds_address(const void *p) {
+  return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void *)p;
+}
+__device__ __forceinline__ void read_keys(const MxSlot &s, int lane, MxKeys &K, uint32_t &every) {
+  const uint32_t a = lds_address(&s) + 16 * lane, b = lds_address(&s) + 8192 + 4 * lane;
+  asm volatile(
+      "ds_read_b32 %4, %7\n ds_read_b32 %5, %7 offset:256\n ds_read_b128 %0, %6\n ds_read_b128 %1, %6 offset:1024\n"
+      " ds_read_b128 %2, %6 offset:2048\n ds_read_b128 %3, %6 offset:3072\n s_waitcnt lgkmcnt(0)"
+      : "=&v"(K.code[0]), "=&v"(K.code[1]), "=&v"(K.code[2]), "=&v"(K.code[3]), "=&v"(K.scale), "=&v"(every)
+      : "v"(a), "v"(b)
+      : "memory");
+}
+__device__ __forceinline__ void read_values(const MxSlot &s, int lane, MxValues &V) {
+  const uint32_t a = lds_address(&s) + 4096 + 16 * lane, b = lds_address(&s) + 8448 + 16 * (lane >> 4);
+  asm volatile(
+      "ds_read_b128 %4, %9\n ds_read_b128 %5, %9 offset:64\n ds_read_b128 %6, %9 offset:128\n ds_read_b128 %7, %9 offset:192\n"
+      " ds_read_b128 %0, %8\n ds_read_b128 %1, %8 offset:1024\n ds_read_b128 %2, %8 offset:2048\n ds_read_b128 %3, %8 offset:3072\n"
+      " s_waitcnt lgkmcnt(0)"
+      : "=&v"(V.code[0]), "=&v"(V.code[1]), "=&v"(V.code[2]), "=&v"(V.code[3]), "=&v"(V.scale[0]), "=&v"(V.scale[1]),
+        "=&v"(V.scale[2]), "=&v"(V.scale[3])
+      : "v"(a), "v"(b)
+      : "memory");
+}
+
 // The largest of the first 16 lanes' x (lane n: row n's), wave-uniform
 __device__ __forceinline__ int row16_max(int x) {
   x = max(x, __builtin_amdgcn_update_dpp(0, x, kRowRor8, 0xF, 0xF, false));
@@ -63,7 +108,15 @@ __device__ __forceinline__ int page_scale(uint32_t every, int lane, int tokens) 
 }
 
 template <int NT, int W>
-__device__ __forceinline__ void few_rows_mx(const AttendParams &p, int split, int hkv, int rb, int z, FewLds<kFmtMxfp4, NT, W> &s) {
+union MxLds {
+  FewLds<kFmtMxfp4, NT, W> join;
+  MxSlot slot[NT == 2 ? W : 1][NT == 2 ? 2 : 1];
+  __device__ MxLds() {}
+};
+
+template <int NT, int W>
+__device__ __forceinline__ void few_rows_mx(const AttendParams &p, int split, int hkv, int rb, int z, MxLds<NT, W> &s) {
+  constexpr bool kRing = NT == 2;
   const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, n = lane & 15;
   AttendSet set;
@@ -91,8 +144,14 @@ __device__ __forceinline__ void few_rows_mx(const AttendParams &p, int split, in
   if (pa < pe) {
     const size_t blk = block(page_id(pa + wv));
     id = page_id(pa + wv + W);
-    load_keys(p, blk, lane, K);
-    load_values(p, blk, lane, V);
+    if constexpr (kRing) {
+      copy_page(p, blk, lane, s.slot[wv][0]);
+      copy_page(p, block(id), lane, s.slot[wv][1]);
+      id = page_id(pa + wv + 2 * W);
+    } else {
+      load_keys(p, blk, lane, K);
+      load_values(p, blk, lane, V);
+    }
   }
 
   f16x8 Q[NT][4];
@@ -197,16 +256,29 @@ __device__ __forceinline__ void few_rows_mx(const AttendParams &p, int split, in
 #pragma unroll 1
     for (int i = 0, pg = p0; i < 64 && pg < last; ++i, pg += W) {
       const size_t next = block(id);
-      id = page_id(pg + 2 * W);
+      id = page_id(pg + (kRing ? 3 : 2) * W);
+      MxSlot &slot = s.slot[kRing ? wv : 0][kRing ? i & 1 : 0];
+      if constexpr (kRing) {
+        __builtin_amdgcn_s_waitcnt(0x0f70 | kSlotLoads);  // vmcnt: the next page's copies may be under way
+        read_keys(slot, lane, K, V.every);
+      }
       if (lo < (pg + 1) * kPage || !scales(pg * kPage)) [[unlikely]] {
         others |= 1ull << i;
-        load_keys(p, next, lane, K);
-        load_values(p, next, lane, V);
+        if constexpr (kRing) {
+          copy_page(p, next, lane, slot);
+        } else {
+          load_keys(p, next, lane, K);
+          load_values(p, next, lane, V);
+        }
         continue;
       }
       scores();
-      load_keys(p, next, lane, K);
+      if constexpr (!kRing) load_keys(p, next, lane, K);
       weights();
+      if constexpr (kRing) {
+        read_values(slot, lane, V);
+        copy_page(p, next, lane, slot);  // its last page is read
+      }
       const uint32_t base = (uint32_t)(vtop - 15) * 0x01010101u;
 #pragma unroll
       for (int cb = 0; cb < 4; ++cb) {
@@ -229,7 +301,7 @@ __device__ __forceinline__ void few_rows_mx(const AttendParams &p, int split, in
           }
         values(cb, P);
       }
-      load_values(p, next, lane, V);
+      if constexpr (!kRing) load_values(p, next, lane, V);
     }
     if (others == 0) [[likely]] continue;
 #pragma unroll 1
@@ -264,7 +336,7 @@ __device__ __forceinline__ void few_rows_mx(const AttendParams &p, int split, in
         values(cb, P);
       }
     }
-    if (p0 + 64 * W < last) {
+    if (!kRing && p0 + 64 * W < last) {
       load_keys(p, block(page_id(p0 + 64 * W)), lane, K);
       load_values(p, block(page_id(p0 + 64 * W)), lane, V);
     }
@@ -276,12 +348,16 @@ __device__ __forceinline__ void few_rows_mx(const AttendParams &p, int split, in
 #pragma unroll
     for (int u = 0; u < 8; ++u) O[t][u] *= mx_factor(vtop);
   }
-  join_waves<NT, W>(p, set, hkv, r0, m, l, O, s);
+  if constexpr (kRing) {  // the waves' copies, used or not, have arrived: their place is the join's
+    __builtin_amdgcn_s_waitcnt(0x0f70);
+    __syncthreads();
+  }
+  join_waves<NT, W>(p, set, hkv, r0, m, l, O, s.join);
 }
 
 template <int NT>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void mxfp4_attend_kernel(const AttendParams p) {
-  __shared__ FewLds<kFmtMxfp4, NT, 4> s;
+  __shared__ MxLds<NT, 4> s;
   few_rows_mx<NT, 4>(p, blockIdx.x, blockIdx.y % p.HKV, blockIdx.y / p.HKV, blockIdx.z, s);
 }
 
@@ -289,7 +365,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void m
 template <int NT>
 __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) void mxfp4_attend_both_kernel(const AttendParams p) {
   __shared__ union Lds {
-    FewLds<kFmtMxfp4, NT, 8> few;
+    MxLds<NT, 8> few;
     ManyLds<kFmtMxfp4, 8> many;
     __device__ Lds() {}
   } s;
