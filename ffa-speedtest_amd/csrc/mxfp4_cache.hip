@@ -70,12 +70,13 @@ __device__ __forceinline__ void held_row(const MxRow &r, float *x) {
 // ---------------------------------------------------------------------------
 // by tiles of 64 tokens
 // ---------------------------------------------------------------------------
+constexpr int kAnglePitch = 66;  // a token's angles in LDS, 16 bytes apart from a power of two: eight tokens' meet in few banks
 struct MxTile {
   int b, page, n0, lo, hi;  // slots [lo, hi) of the page are new tokens n0 + slot; page -1: nothing is written
 };
 
 template <int DT, int TURN>
-__device__ __forceinline__ void tile_k(const MxAppendParams &p, const MxTile &tl, int h, int half, const float2 (*cs)[64]) {
+__device__ __forceinline__ void tile_k(const MxAppendParams &p, const MxTile &tl, int h, int half, const float2 (*cs)[kAnglePitch]) {
   const int lane = threadIdx.x & 63, l = lane & 7, m = 8 * half + (lane >> 3);
   Row16<DT> w[4];
 #pragma unroll
@@ -120,7 +121,7 @@ __device__ __forceinline__ void tile_k(const MxAppendParams &p, const MxTile &tl
 }
 
 template <int DT, int TURN>
-__device__ __forceinline__ void tile_q(const MxAppendParams &p, const MxTile &tl, int h, int half, const float2 (*cs)[64]) {
+__device__ __forceinline__ void tile_q(const MxAppendParams &p, const MxTile &tl, int h, int half, const float2 (*cs)[kAnglePitch]) {
   const int lane = threadIdx.x & 63, l = lane & 7;
   Row16<DT> w[4];
 #pragma unroll
@@ -187,13 +188,8 @@ __device__ __forceinline__ void tile_v(const MxAppendParams &p, const MxTile &tl
     for (int i = 0; i < 8; ++i) {
       if (t0 + i < tl.lo || t0 + i >= tl.hi) continue;
       const float f = value_factor(byte[i]);
-      const size_t at = ((((size_t)tl.b * p.T + tl.n0 + t0 + i) * p.HKV + h) * kD + 4 * c);
-      if constexpr (DT == 2)
-        *(float4 *)((float *)p.v_values + at) = make_float4(y[0][i] * f, y[1][i] * f, y[2][i] * f, y[3][i] * f);
-      else if constexpr (DT == 1)
-        *(uint2 *)((uint16_t *)p.v_values + at) = make_uint2(pk_bf16_bits(y[0][i] * f, y[1][i] * f), pk_bf16_bits(y[2][i] * f, y[3][i] * f));
-      else
-        *(uint2 *)((uint16_t *)p.v_values + at) = make_uint2(pk_f16_bits(y[0][i] * f, y[1][i] * f), pk_f16_bits(y[2][i] * f, y[3][i] * f));
+      const float held[4] = {y[0][i] * f, y[1][i] * f, y[2][i] * f, y[3][i] * f};
+      store_values<DT, 4, false>(p.v_values, (((size_t)tl.b * p.T + tl.n0 + t0 + i) * p.HKV + h) * kD + 4 * c, held);
     }
   }
   if (tl.page < 0) return;
@@ -242,7 +238,7 @@ __device__ __forceinline__ void tile_v(const MxAppendParams &p, const MxTile &tl
 
 template <int DT, int TURN>
 __global__ __launch_bounds__(256) void mxfp4_append_tiles_kernel(const MxAppendParams p) {
-  __shared__ float2 cs[TURN == kTurnNone ? 1 : 64][64];
+  __shared__ float2 cs[TURN == kTurnNone ? 1 : 64][kAnglePitch];
   __shared__ u32x4 words[4][64];
   const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   MxTile tl;
@@ -260,15 +256,16 @@ __global__ __launch_bounds__(256) void mxfp4_append_tiles_kernel(const MxAppendP
     }
     __syncthreads();
   }
-  // units: two a head of q, two of K, four of V; the waves of the tile's workgroups in turn
-  const int nq = TURN == kTurnNone ? 0 : 2 * p.HQ, nk = 2 * p.HKV, units = nq + nk + (p.v ? 4 * p.HKV : 0);
+  // units: two a head of K, four of V, two of q, the waves of the tile's workgroups in turn; q, which only turns, last (a 16K
+  // prompt's append 93 -> 89 us)
+  const int nk = 2 * p.HKV, kv = nk + (p.v ? 4 * p.HKV : 0), units = kv + (TURN == kTurnNone ? 0 : 2 * p.HQ);
   for (int u = blockIdx.y * 4 + wv; u < units; u += 4 * gridDim.y) {
-    if (u < nq) {
-      if constexpr (TURN != kTurnNone) tile_q<DT, TURN>(p, tl, u >> 1, u & 1, cs);
-    } else if (u < nq + nk) {
-      tile_k<DT, TURN>(p, tl, (u - nq) >> 1, (u - nq) & 1, cs);
+    if (u < nk) {
+      tile_k<DT, TURN>(p, tl, u >> 1, u & 1, cs);
+    } else if (u < kv) {
+      tile_v<DT>(p, tl, (u - nk) >> 2, (u - nk) & 3, (uint32_t *)words[wv]);
     } else {
-      tile_v<DT>(p, tl, (u - nq - nk) >> 2, (u - nq - nk) & 3, (uint32_t *)words[wv]);
+      if constexpr (TURN != kTurnNone) tile_q<DT, TURN>(p, tl, (u - kv) >> 1, (u - kv) & 1, cs);
     }
   }
 }
@@ -375,7 +372,8 @@ static void launch_append(MxAppendParams &p, hipStream_t st) {
   if (mx_by_tiles(p.B, p.T, units)) {
     p.tiles = page_tiles(p.T);
     const long x = (long)p.B * p.tiles, n = (2l * (units - (p.v ? p.HKV : 0)) + (p.v ? 4l * p.HKV : 0) + 3) / 4;
-    hipLaunchKernelGGL((mxfp4_append_tiles_kernel<DT, TURN>), dim3((unsigned)x, (unsigned)mx_tile_splits(x, n)), dim3(256), 0, st, p);
+    hipLaunchKernelGGL((mxfp4_append_tiles_kernel<DT, TURN>), dim3((unsigned)x, (unsigned)mx_tile_splits(x, n, device_cus())), dim3(256), 0, st,
+                       p);
   } else {
     p.tiles = p.T / 2 + 1;
     hipLaunchKernelGGL((mxfp4_append_tokens_kernel<DT, TURN>), dim3((unsigned)((long)p.B * p.tiles), (unsigned)((units + 31) / 32)),
@@ -450,10 +448,7 @@ __global__ __launch_bounds__(256) void mxfp4_dequant_kernel(const MxReadParams p
     float x[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) x[e] = t0 + i < n ? y[e][i] * f : 0.f;
-    const size_t at = ((size_t)(row0 + t0 + i) * p.HKV + h) * kD + 4 * cq;
-    if constexpr (DT == 2) *(float4 *)((float *)p.v + at) = make_float4(x[0], x[1], x[2], x[3]);
-    else if constexpr (DT == 1) *(uint2 *)((uint16_t *)p.v + at) = make_uint2(pk_bf16_bits(x[0], x[1]), pk_bf16_bits(x[2], x[3]));
-    else *(uint2 *)((uint16_t *)p.v + at) = make_uint2(pk_f16_bits(x[0], x[1]), pk_f16_bits(x[2], x[3]));
+    store_values<DT, 4>(p.v, ((size_t)(row0 + t0 + i) * p.HKV + h) * kD + 4 * cq, x);
   }
 }
 

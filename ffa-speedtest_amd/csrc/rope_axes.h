@@ -60,17 +60,23 @@ __device__ __forceinline__ void rope_turn(const float2 *cs, int l, float *x) {
   }
 }
 
-// eight elements at `at`, as loaded, to the type DT at `at` of p
-template <int DT>
-__device__ __forceinline__ void store8(void *p, size_t at, const float *x) {
-  uint4 *d = (uint4 *)((uint8_t *)p + at * (DT == 2 ? 4 : 2));
-  if constexpr (DT == 2) {
-    d[0] = make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
-    d[1] = make_uint4(__float_as_uint(x[4]), __float_as_uint(x[5]), __float_as_uint(x[6]), __float_as_uint(x[7]));
-  } else if constexpr (DT == 1) {
-    d[0] = make_uint4(pk_bf16_bits(x[0], x[1]), pk_bf16_bits(x[2], x[3]), pk_bf16_bits(x[4], x[5]), pk_bf16_bits(x[6], x[7]));
-  } else {
-    d[0] = make_uint4(pk_f16_bits(x[0], x[1]), pk_f16_bits(x[2], x[3]), pk_f16_bits(x[4], x[5]), pk_f16_bits(x[6], x[7]));
+// N (4 or 8) values to elements `at` .. of p, of type DT.  NT: not kept in the caches, as nothing reads them soon (a 16K
+// prompt's append 95 -> 93 us, read-backs 132 -> 124; but its V's values, 8 bytes a lane, so 89 -> 94)
+template <int DT, int N, bool NT = true>
+__device__ __forceinline__ void store_values(void *p, size_t at, const float *x) {
+  typedef uint32_t Words __attribute__((ext_vector_type(DT != 2 && N == 4 ? 2 : 4)));
+  constexpr int kPer = DT == 2 ? 1 : 2, kWords = DT != 2 && N == 4 ? 2 : 4;  // values a word, words a store
+  Words *d = (Words *)((uint8_t *)p + at * (DT == 2 ? 4 : 2));
+#pragma unroll
+  for (int i = 0; i < N / (kPer * kWords); ++i) {
+    Words w;
+#pragma unroll
+    for (int e = 0; e < kWords; ++e) {
+      const float *y = x + (i * kWords + e) * kPer;
+      w[e] = DT == 2 ? __float_as_uint(y[0]) : (DT == 1 ? pk_bf16_bits(y[0], y[kPer - 1]) : pk_f16_bits(y[0], y[kPer - 1]));
+    }
+    if constexpr (NT) __builtin_nontemporal_store(w, d + i);
+    else d[i] = w;
   }
 }
 
@@ -90,8 +96,8 @@ __device__ __forceinline__ void row_values(const Row16<DT> &r, float *x) {
 }
 template <int DT>
 __device__ __forceinline__ void store_row(void *p, long at, int l, const float *x) {
-  store8<DT>(p, (size_t)(at + 8 * l), x);
-  store8<DT>(p, (size_t)(at + 64 + 8 * l), x + 8);
+  store_values<DT, 8>(p, (size_t)(at + 8 * l), x);
+  store_values<DT, 8>(p, (size_t)(at + 64 + 8 * l), x + 8);
 }
 
 }  // namespace ffa

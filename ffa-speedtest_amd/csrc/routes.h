@@ -149,9 +149,11 @@ inline long attend_shared_wgs(long units, long own_head_pages, int cus) {
 
 // mxfp4 appends by tiles of 64 tokens rather than by pairs of positions; units: heads of q, K and V.
 inline bool mx_by_tiles(int B, int Tn, int units) { return Tn >= 16; }
-// workgroups that share a tile's units (each computes the tile's angles): n waves' worth of four units
-inline long mx_tile_splits(long tiles, long n) {
-  const long want = (2048 + tiles - 1) / tiles;
+// workgroups that share a tile's units (each computes the tile's angles), of n fours of them: one round, four a CU.  us of a
+// 16K prompt, 32 + 8 heads, at 1, 2, 3, 4, 8 and 16 workgroups a tile  - / 99 / 95 / 94 / 107 / 109; 4 x 1500 tokens at 6, 8,
+// 11 and 22  38.0 / 37.4 / 39.0 / 41.1
+inline long mx_tile_splits(long tiles, long n, int cus) {
+  const long want = (4l * cus + tiles - 1) / tiles;
   return want < n ? want : n;
 }
 
