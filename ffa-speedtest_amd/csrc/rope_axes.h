@@ -20,8 +20,31 @@ struct RopeParams {
   int positions64, axes, inverse;
 };
 
-// cos and sin of pair j of token t of sequence b (own: its position there).  The product in turns, in 64 bits: at
-// position 2^20 it is off by 2^-33 turns, where 32 bits would be by 2^-4; then the remainder in 32.
+// cos and sin of 2 pi r, |r| <= 1/2, each within 2^-40 before its rounding to fp32: the remainder from the next quarter turn
+// (|x| <= pi / 4) by the Taylor sums, whose first terms left out are x^15 / 15! < 2^-45 and x^16 / 16! < 2^-49.
+__device__ __forceinline__ float2 cos_sin_turns(double r) {
+  const double k = rint(4.0 * r), x = (r - 0.25 * k) * 6.283185307179586476925287, y = x * x;
+  double s = 1.0 / 6227020800.0, c = -1.0 / 87178291200.0;
+  s = fma(s, y, -1.0 / 39916800.0);
+  s = fma(s, y, 1.0 / 362880.0);
+  s = fma(s, y, -1.0 / 5040.0);
+  s = fma(s, y, 1.0 / 120.0);
+  s = fma(s, y, -1.0 / 6.0);
+  s = fma(s * y, x, x);
+  c = fma(c, y, 1.0 / 479001600.0);
+  c = fma(c, y, -1.0 / 3628800.0);
+  c = fma(c, y, 1.0 / 40320.0);
+  c = fma(c, y, -1.0 / 720.0);
+  c = fma(c, y, 1.0 / 24.0);
+  c = fma(c, y, -0.5);
+  c = fma(c, y, 1.0);
+  const int q = (int)k & 3;
+  const float fc = (float)c, fs = (float)s, a = q & 1 ? fs : fc, b = q & 1 ? fc : fs;  // (c, s) (-s, c) (-c, -s) (s, -c)
+  return make_float2(q == 1 || q == 2 ? -a : a, q & 2 ? -b : b);
+}
+
+// cos and sin of pair j of token t of sequence b (own: its position there).  All of it in 64 bits up to the one rounding: at
+// position 2^20 the product in turns is off by 2^-33, where 32 bits would be by 2^-4.
 __device__ __forceinline__ float2 rope_angle(const RopeParams &p, int j, int b, int t, long own) {
   const ffa_rope_pair pr = p.pairs[j];
   long pos = own;
@@ -31,32 +54,28 @@ __device__ __forceinline__ float2 rope_angle(const RopeParams &p, int j, int b, 
     pos = p.positions64 ? ((const int64_t *)p.positions)[at] : ((const int32_t *)p.positions)[at];
   }
   const double a = (double)pos * pr.turns;
-  float s, c;
-  sincospif(2.f * (float)(a - rint(a)), &s, &c);
-  return make_float2(c, p.inverse ? -s : s);
+  const float2 f = cos_sin_turns(a - rint(a));
+  return make_float2(f.x, p.inverse ? -f.y : f.y);
 }
 
-// x of lane l turned by the token's cos and sin cs[64]
+// x of lane l turned by the token's cos and sin cs[64]: two products and their sum, each rounded (not fused, as which
+// product were the exact one would be a matter of taste, and what is then quantized should not depend on it)
+__device__ __forceinline__ void turn_pair(float2 f, float &a, float &b) {
+#pragma clang fp contract(off)
+  const float ac = a * f.x, bs = b * f.y, bc = b * f.x, as = a * f.y;
+  a = ac - bs;
+  b = bc + as;
+}
 template <int TURN>
 __device__ __forceinline__ void rope_turn(const float2 *cs, int l, float *x) {
   if constexpr (TURN == kTurnHalf) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float2 f = cs[8 * l + i];
-      const float a = x[i], b = x[8 + i];
-      x[i] = __builtin_fmaf(a, f.x, -b * f.y);
-      x[8 + i] = __builtin_fmaf(b, f.x, a * f.y);
-    }
+    for (int i = 0; i < 8; ++i) turn_pair(cs[8 * l + i], x[i], x[8 + i]);
   } else if constexpr (TURN == kTurnAdjacent) {
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float2 f = cs[32 * h + 4 * l + i];
-        const float a = x[8 * h + 2 * i], b = x[8 * h + 2 * i + 1];
-        x[8 * h + 2 * i] = __builtin_fmaf(a, f.x, -b * f.y);
-        x[8 * h + 2 * i + 1] = __builtin_fmaf(b, f.x, a * f.y);
-      }
+      for (int i = 0; i < 4; ++i) turn_pair(cs[32 * h + 4 * l + i], x[8 * h + 2 * i], x[8 * h + 2 * i + 1]);
   }
 }
 
