@@ -369,7 +369,7 @@ __global__ __launch_bounds__(256) void mxfp4_append_tokens_kernel(const MxAppend
 template <int DT, int TURN>
 static void launch_append(MxAppendParams &p, hipStream_t st) {
   const int units = (TURN == kTurnNone ? 0 : p.HQ) + p.HKV + (p.v ? p.HKV : 0);
-  if (mx_by_tiles(p.B, p.T, units)) {
+  if (mx_by_tiles(p.B, p.T, units, TURN != kTurnNone)) {
     p.tiles = page_tiles(p.T);
     const long x = (long)p.B * p.tiles, n = (2l * (units - (p.v ? p.HKV : 0)) + (p.v ? 4l * p.HKV : 0) + 3) / 4;
     hipLaunchKernelGGL((mxfp4_append_tiles_kernel<DT, TURN>), dim3((unsigned)x, (unsigned)mx_tile_splits(x, n, device_cus())), dim3(256), 0, st,

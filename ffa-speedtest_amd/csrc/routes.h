@@ -147,8 +147,16 @@ inline long attend_shared_wgs(long units, long own_head_pages, int cus) {
   return (long)(cus * (share < 0.4 ? 0.4 : share)) + 1;
 }
 
-// mxfp4 appends by tiles of 64 tokens rather than by pairs of positions; units: heads of q, K and V.
-inline bool mx_by_tiles(int B, int Tn, int units) { return Tn >= 16; }
+// mxfp4 appends by tiles of 64 tokens rather than by pairs of positions; units: heads of q, K and V.  Tiles store whole
+// pieces; pairs have no idle lanes where a page takes few tokens, and with rotary positions fewer angles a workgroup.
+// us by tiles / by pairs, with positions, 32 + 8 heads: 1 sequence of 1024 tokens 9.5 / 6.4, of 2048 15.5 / 12.6, of 4096
+// 21.2 / 22.1, of 16K 59 / 75; 64 of 64 24.8 / 21.9, of 128 39 / 39, of 256 63 / 74; 256 of 32 57 / 40, of 64 71 / 74; 8 + 1
+// heads, 1 of 8192 14.2 / 12.5, of 16K 18.6 / 21.2.  Without, 8 heads: 1 of 1 token 3.4 / 4.0, 8 of 1 3.6 / 4.3, 64 of 1 5.0 /
+// 4.4, of 16 7.3 / 6.6, of 32 7.4 / 8.9; 256 of 16 25 / 16, of 32 25 / 24, of 64 25 / 41; 1 head, 256 of 1 4.1 / 4.6.
+inline bool mx_by_tiles(int B, int Tn, int units, bool rotary) {
+  if (rotary) return Tn >= 64 && (long)B * Tn * units >= 160000;
+  return Tn >= 32 || (long)B * units <= 512;
+}
 // workgroups that share a tile's units (each computes the tile's angles), of n fours of them: one round, four a CU.  us of a
 // 16K prompt, 32 + 8 heads, at 1, 2, 3, 4, 8 and 16 workgroups a tile  - / 99 / 95 / 94 / 107 / 109; 4 x 1500 tokens at 6, 8,
 // 11 and 22  38.0 / 37.4 / 39.0 / 41.1
@@ -158,7 +166,9 @@ inline long mx_tile_splits(long tiles, long n, int cus) {
 }
 
 // Rotary positions on given rows: tokens of a workgroup, which computes their angles, and workgroups that share a tile's
-// rows (each computing the angles again).
+// rows (each computing the angles again), for 1024 workgroups.  us for 256 / 512 / 1024 / 2048 of them, 32 + 8 heads, 1024
+// tokens 5.2 / 4.9 / 4.6 / 5.8, 2048 10.1 / 6.4 / 6.1 / 6.9, 4096 18.7 / 15.7 / 15.3 / 15.2; 8 + 1 heads, 2048 tokens 4.8 /
+// 4.1 / 4.2 / 5.6, 8192 7.7 / 7.6 / 7.0 / 7.5.
 inline int rope_tokens(long tokens, int most) {
   int n = 1;
   while (n < most && tokens > 1024l * n) n *= 2;

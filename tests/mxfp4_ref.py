@@ -101,12 +101,12 @@ def rotate(x, positions, axis, freq, adjacent, inverse=False):
 
 
 def turn_bound(x, adjacent):
-    """How far fp32 may leave a turned element from the 64-bit one: the sine and cosine are off by at most 2^-22 (the
-    remainder in turns is rounded to fp32, at most 1/2 in size: 2^-26 turns = 2 pi 2^-26 < 2^-23 in the angle; the
-    functions add two steps of 2^-24), the product and the fused sum by 2^-24 of |a| + |b| each."""
+    """How far the turn may leave an element from the 64-bit one: sine and cosine are rounded to fp32 once (2^-25; before
+    that they are within 2^-40, and the angle, at positions up to 2^20, within 2^-30), the two products and their sum once
+    each (2^-24 of |a| + |b| for the products together, and as much for the sum)."""
     a = np.abs(np.asarray(x, dtype=np.float64))
     if adjacent:
         s = np.repeat(a[..., ::2] + a[..., 1::2], 2, axis=-1)
     else:
         s = np.concatenate([a[..., :64] + a[..., 64:]] * 2, -1)
-    return s * (2.0 ** -22 + 2.0 ** -23)
+    return s * (2.0 ** -25 + 2.0 ** -23 + 2.0 ** -29)

@@ -69,6 +69,15 @@ def test_rotate_far_positions(gpu):
     assert (np.abs(_f64(got) - want) <= limit).all()
 
 
+def test_rotate_many_tokens(gpu):
+    """Sixteen tokens a workgroup, the last one's fewer; two sequences in one workgroup."""
+    g = torch.Generator().manual_seed(9)
+    rope, q, k = AxisRope((64,), device=gpu), _rand(g, 2, 8205, 1, 128).bfloat16().to(gpu), _rand(g, 2, 8205, 1, 128).bfloat16().to(gpu)
+    pos = torch.randint(0, 2 ** 20, (1, 2, 8205), generator=g).to(gpu)
+    for x, y in zip((q, k), rope.rotate(pos, q, k)):
+        _check_turned(y, x, pos, rope)
+
+
 def test_rotate_strides_and_in_place(gpu):
     """Views of a joined projection, heads before tokens, one position row for all sequences, and in place."""
     g = torch.Generator().manual_seed(7)
@@ -329,6 +338,59 @@ def test_append_rotary(gpu, dtype, pairs, B, T, HQ, HKV, pos):
     assert cache.append_rotary(None, k, v, p, table.to(gpu), rope, own, True) is None
 
 
+@pytest.mark.parametrize("dtype,pairs,B,T,HQ,HKV,pos", [
+    ("bf16", "half", 2, 90, 900, 2, [33, 64]),     # a long prompt's kernel, at the size of its tiles' edges
+    ("fp32", "adjacent", 1, 64, 2600, 1, [63]),    # a token in the first tile, 63 in the second
+    ("fp16", "half", 1, 131, 1300, 3, [0]),
+])
+def test_append_rotary_of_many_heads(gpu, dtype, pairs, B, T, HQ, HKV, pos):
+    test_append_rotary(gpu, dtype, pairs, B, T, HQ, HKV, pos)
+
+
+def test_append_at_once_and_in_parts(gpu):
+    """A prompt in one call, in pieces of several sizes, and the same without the turn: the same bytes and values."""
+    g = torch.Generator().manual_seed(53)
+    rope, T, pos = AxisRope((64,), device=gpu), 2300, [17, 128]
+    cache, table, k, v = _append_case(g, 2, T, 8, torch.bfloat16, gpu, pos)
+    q, table = _rand(g, 2, T, 24, 128).bfloat16().to(gpu), table.to(gpu)
+    start = [t.clone() for t in cache.pools()]
+    p = torch.tensor(pos, dtype=torch.int32, device=gpu)
+    whole = cache.append_rotary(q, k, v, p, table, rope, None, True, values=True)
+    want = R.to_numpy(cache)
+    for cuts in ([1, 2, 66, 67, 130, 1000, 2300], [63, 64, 2299, 2300]):
+        for t, s in zip(cache.pools(), start):
+            t.copy_(s)
+        got, at = [], 0
+        for cut in cuts:
+            got.append(cache.append_rotary(q[:, at:cut], k[:, at:cut], v[:, at:cut], p + at, table, rope, None, True, values=True))
+            at = cut
+        _same_pools(cache, want)
+        for i in range(3):
+            assert torch.equal(torch.cat([x[i] for x in got], 1).nan_to_num(7.0), whole[i].nan_to_num(7.0))
+    for t, s in zip(cache.pools(), start):
+        t.copy_(s)
+    cache.append(k, v, p, table, True)
+    want, at = R.to_numpy(cache), 0
+    for t, s in zip(cache.pools(), start):
+        t.copy_(s)
+    for cut in (1, 2, 5, 70, 2300):
+        cache.append(k[:, at:cut], v[:, at:cut], p + at, table, True)
+        at = cut
+    _same_pools(cache, want)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("B,T,HKV", [(70, 1, 4), (140, 3, 2), (300, 2, 1), (33, 31, 8)])
+def test_append_of_many_sequences(gpu, dtype, B, T, HKV):
+    g = torch.Generator().manual_seed(59)
+    pos = [(37 * b) % 130 for b in range(B)]
+    cache, table, k, v = _append_case(g, B, T, HKV, TYPES[dtype], gpu, pos)
+    want = _expect(R.to_numpy(cache), table, pos, _f64(k), _f64(v))
+    kh, vh = cache.append(k, v, torch.tensor(pos, dtype=torch.int32, device=gpu), table.to(gpu), ragged=True, values=True)
+    _same_pools(cache, want)
+    assert np.array_equal(_f64(kh), R.held(_f64(k)), equal_nan=True) and np.array_equal(_f64(vh), R.held(_f64(v)), equal_nan=True)
+
+
 def test_append_rotary_refusals(gpu):
     cache, rope = R.make_cache(2, 1, gpu), AxisRope((64,), device=gpu)
     k, pos, table = torch.zeros(1, 2, 1, 128, device=gpu), torch.zeros(1, dtype=torch.int32, device=gpu), torch.zeros(1, 1, dtype=torch.int32, device=gpu)
@@ -433,6 +495,23 @@ def _check(cache, table, lens, q, out, q_lens=None, scale=SCALE, tokens=None, sl
 def test_attend_lengths(gpu, lens, HQ, HKV, L, dtype):
     cache, table, sl, q = _batch(lens, HQ, HKV, L, TYPES[dtype], 3, gpu)
     _check(cache, table, lens, q, cache.attend(q, table, sl))
+
+
+@pytest.mark.parametrize("B,HQ,HKV,L", [(65, 8, 2, 1), (70, 4, 1, 5), (130, 16, 4, 1), (700, 2, 1, 1)])
+def test_attend_many_sequences(gpu, B, HQ, HKV, L):
+    """More sequences than a wave has lanes, than half a round of workgroups and than a whole one; lengths from none to
+    several page ranges, in no order."""
+    g = torch.Generator().manual_seed(B)
+    lens = torch.randint(0, 300, (B,), generator=g).tolist()
+    lens[0], lens[B // 2], lens[63], lens[64] = 0, 3000, 64, 0
+    lens[B - 1] = 1 if B % 2 else 2100
+    cache, table, sl, q = _batch(lens, HQ, HKV, L, torch.bfloat16, 83, gpu)
+    out = cache.attend(q, table, sl)
+    some = sorted({0, B // 2, 62, 63, 64, B - 1} | set(range(1, B, 1 + B // 12)))
+    _check(cache, table[some], [lens[b] for b in some], q[some], out[some])
+    alone = torch.cat([cache.attend(q[b:b + 1], table[b:b + 1], sl[b:b + 1]) for b in range(B)])
+    assert torch.allclose(alone.float(), out.float(), atol=2.0 ** -7, rtol=2.0 ** -7)
+    assert torch.equal(cache.attend(q, table, torch.zeros_like(sl), T=100), torch.zeros_like(out))
 
 
 def test_attend_long_and_scale(gpu):

@@ -119,3 +119,30 @@ def test_attention_launches(routes):
                                "attend_shared_wgs(8, 1 << 24, 256)")
     assert 0.5 * 256 <= some <= 0.62 * 256 and most >= 0.95 * 256 and least == 103
     assert routes("join_by_wave(2048)", "join_by_wave(2049)", "join_by_wave(4224)") == [0, 1, 1]
+
+
+def test_mxfp4_appends(routes):
+    """Whole tiles for long appends, and without rotary positions for few heads and sequences; pairs of positions for the rest."""
+    tiles = [(1, 4096, 48, "true"), (1, 16384, 48, "true"), (1, 16384, 10, "true"), (256, 64, 48, "true"), (64, 256, 48, "true"),
+             (1, 2 ** 31 - 1, 48, "true"), (1, 1, 16, "false"), (8, 1, 16, "false"), (256, 1, 2, "false"), (64, 32, 16, "false"),
+             (256, 64, 16, "false"), (1, 2 ** 31 - 1, 16, "false"), (65535, 2 ** 20, 2048, "false")]
+    pairs = [(1, 1, 48, "true"), (64, 1, 48, "true"), (1, 2048, 48, "true"), (256, 32, 48, "true"), (1, 8192, 10, "true"),
+             (16, 128, 48, "true"), (64, 1, 16, "false"), (64, 16, 16, "false"), (256, 16, 16, "false")]
+    got = routes(*(f"mx_by_tiles({B}, {Tn}, {units}, {rotary})" for B, Tn, units, rotary in tiles + pairs))
+    assert got == [1] * len(tiles) + [0] * len(pairs)
+    # one round of four workgroups a CU, but no workgroup without a unit
+    assert routes("mx_tile_splits(256, 24, 256)", "mx_tile_splits(1, 24, 256)", "mx_tile_splits(94, 24, 256)",
+                  "mx_tile_splits(5000, 24, 256)") == [4, 24, 11, 1]
+
+
+def test_mxfp4_page_ranges(routes):
+    """Ranges for about one round of workgroups, each sequence's last being a part of one; never none."""
+    assert routes("mx_even_ranges(16, 8, kRows16, 256)", "mx_even_ranges(1, 8, kRows32, 256)", "mx_even_ranges(60, 8, kRows16, 256)",
+                  "mx_even_ranges(4096, 8, kRows16, 256)", "mx_even_ranges(1, 4096, kRows16, 256)") == [48, 63, 32, 32, 1]
+
+
+def test_rotary_workgroups(routes):
+    """About 1024 workgroups: more tokens each from 1024 on, several for a token's rows below."""
+    assert routes(*(f"rope_tokens({n}, 16)" for n in (1, 1024, 1025, 4096, 16384, 10 ** 9))) == [1, 1, 2, 4, 16, 16]
+    assert routes("rope_splits(1, 40)", "rope_splits(64, 40)", "rope_splits(1024, 160)", "rope_splits(1, 1)", "rope_splits(600, 640)") \
+        == [2, 2, 1, 1, 2]
