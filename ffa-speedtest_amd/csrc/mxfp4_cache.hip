@@ -8,6 +8,7 @@
 //           words for whole 16-byte pieces in LDS, so that every store of a wave is 1 KB.
 //   tokens  eight lanes take two tokens of a head that share bytes, whichever of them are new, and write the bytes one by
 //           one: a decode step's rows in one round.
+// mx_by_tiles says which takes a call.
 #include "rope_axes.h"
 #include "routes.h"
 

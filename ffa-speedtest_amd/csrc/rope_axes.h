@@ -58,8 +58,8 @@ __device__ __forceinline__ float2 rope_angle(const RopeParams &p, int j, int b, 
   return make_float2(f.x, p.inverse ? -f.y : f.y);
 }
 
-// x of lane l turned by the token's cos and sin cs[64]: two products and their sum, each rounded (not fused, as which
-// product were the exact one would be a matter of taste, and what is then quantized should not depend on it)
+// x of lane l turned by the token's cos and sin cs[64].  Two products and their sum, each rounded: a fused sum would keep
+// one of the products exact, and the codes of what is quantized next would depend on which.  It takes no longer.
 __device__ __forceinline__ void turn_pair(float2 f, float &a, float &b) {
 #pragma clang fp contract(off)
   const float ac = a * f.x, bs = b * f.y, bc = b * f.x, as = a * f.y;

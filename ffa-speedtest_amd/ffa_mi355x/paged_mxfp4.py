@@ -65,10 +65,11 @@ class PagedMXFP4Cache:
         return tuple(got) if values else got[0]
 
     def _append(self, q, k, v, pos, block_table, rope, positions, ragged, values, check):
-        if k.ndim != 4 or k.shape[2] != self.HKV or k.shape[3] != HEAD_DIM:
+        shape = k.shape
+        if len(shape) != 4 or shape[2] != self.HKV or shape[3] != HEAD_DIM:
             raise ValueError("k shape does not match the cache")
-        B, Tn, HKV, _ = k.shape
-        if v is not None and v.shape != k.shape:
+        B, Tn, HKV, _ = shape
+        if v is not None and v.shape != shape:
             raise ValueError("v must have the shape of k")
         dev = self.k.device
         for x in (k, v, q):
@@ -76,15 +77,16 @@ class PagedMXFP4Cache:
                 continue
             if x.dtype not in _DTYPES:
                 raise NotImplementedError(f"rows must be fp16, bf16 or fp32, got {x.dtype}")
-            if x.device != dev or dev.type != "cuda":
+            if x.device != dev or not x.is_cuda:
                 raise ValueError(f"rows are on {x.device}, the cache on {dev}: both must be on one GPU")
         HQ = 0
         if rope is not None and rope.table.device != dev:
             raise ValueError(f"the rotation is on {rope.table.device}, the cache on {dev}")
         if q is not None:
-            if q.ndim != 4 or q.shape[:2] != k.shape[:2] or q.shape[3] != HEAD_DIM or q.dtype != k.dtype:
+            shape = q.shape
+            if len(shape) != 4 or shape[0] != B or shape[1] != Tn or shape[3] != HEAD_DIM or q.dtype != k.dtype:
                 raise ValueError("q must be [B, Tn, HQ, 128] of k's type")
-            HQ = q.shape[2]
+            HQ = shape[2]
         if pos.shape != (B,) or block_table.ndim != 2 or block_table.shape[0] != B:
             raise ValueError("pos must be [B] and block_table [B, n]")
         out_type = k.dtype
@@ -135,7 +137,7 @@ class PagedMXFP4Cache:
         if Tp < 0 or Tp > block_table.shape[1] * PAGE:
             raise ValueError("T exceeds the block table")
         if seq_lens is not None:
-            if tuple(seq_lens.shape) != (B,):
+            if seq_lens.shape != (B,):
                 raise ValueError("seq_lens must be [B]")
             seq_lens = _int32(seq_lens, dev)
         k = torch.empty((B, Tp, self.HKV, HEAD_DIM), dtype=out_dtype, device=dev)

@@ -111,25 +111,30 @@ class AxisRope:
             p = p.contiguous()
         return p, p.stride(0), p.stride(1)
 
-    def _check(self, x: torch.Tensor, what: str) -> None:
-        if x.ndim != 4 or x.shape[3] != HEAD_DIM:
-            raise ValueError(f"{what} must be [B, T, H, {HEAD_DIM}], got {tuple(x.shape)}")
+    def _check(self, x: torch.Tensor, what: str) -> torch.Size:
+        shape = x.shape
+        if len(shape) != 4 or shape[3] != HEAD_DIM:
+            raise ValueError(f"{what} must be [B, T, H, {HEAD_DIM}], got {tuple(shape)}")
         if x.dtype not in _DTYPES:
             raise NotImplementedError(f"{what} must be fp16, bf16 or fp32, got {x.dtype}")
-        if self.table.device != x.device or x.device.type != "cuda":
+        if self.table.device != x.device or not x.is_cuda:
             raise ValueError(f"{what} is on {x.device}, the rotation on {self.table.device}: both must be on one GPU")
+        return shape
 
     @staticmethod
     def _rows(x: torch.Tensor, inplace: bool):
         """What the kernel reads and writes for x: input, strides, output, strides."""
         src, st = strided_rows(x)
         if not inplace:
-            hs = x.shape[2] * HEAD_DIM
-            return src, st, rows_like(x), (x.shape[1] * hs, hs, HEAD_DIM)
+            out = rows_like(x)
+            b, t, h, _ = out.stride()
+            return src, st, out, (b, t, h)
         if src is not x:
             raise ValueError("rows turned in place must have contiguous channels and 16-byte aligned strides")
         if any(n > 1 and s == 0 for n, s in zip(x.shape, x.stride())):
             raise ValueError("rows turned in place must not be expanded")
+        if not x.is_inference():
+            torch.autograd.graph.increment_version(x)  # a graph that saved x must not use it turned
         return x, st, x, st
 
     def _run(self, positions, q, k, inverse, inplace):
@@ -157,13 +162,15 @@ class AxisRope:
                inplace: bool = False):
         """q [B, T, H, 128] (and k, with heads of its own) turned by positions [axes, B, T] (or [axes, T] for every
         sequence; int32 or int64), angles in 64 bits, one rounding to the rows' type.  inverse: turned back, which is
-        also the gradient; `rotate` records it where q or k needs one.  inplace: into q and k themselves.
+        also the gradient; `rotate` records it where q or k needs one.  inplace: into q and k themselves, which must not overlap.
         Returns q, or (q, k) where k is given."""
-        self._check(q, "q")
+        B, T, _, _ = self._check(q, "q")
         if k is not None:
-            self._check(k, "k")
-            if k.shape[:2] != q.shape[:2] or k.dtype != q.dtype:
+            Bk, Tk, _, _ = self._check(k, "k")
+            if Bk != B or Tk != T or k.dtype != q.dtype:
                 raise ValueError("q and k must have the same sequences, tokens and type")
+            if inplace and k.numel() and k.data_ptr() == q.data_ptr():
+                raise ValueError("q and k turned in place must not overlap")
         if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
             if inplace:
                 raise ValueError("rows that need gradients are not turned in place")

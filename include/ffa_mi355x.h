@@ -48,7 +48,7 @@
  *                             contiguous cache by torch.cat, ffa-fp8fp8/e2e/fp8fp8_cache.py:84-89)
  *   ffa_mxfp4_*               no reference counterpart: a paged cache of keys and values in 4 bits, its append
  *                             (with or without rotary positions), read-back and exact attention
- *   ffa_rope_axes             apply_rope of given q and k with positions of one to four axes (the reference
+ *   ffa_rope_axes             apply_rope of given q and k with positions of several axes (the reference
  *                             rotates k by tables of one axis, ffa-q2fp8/fused_kproj_rope_q2fp8.py:10-37)
  *   ffa_kproj_rope            F.linear + apply_rope of every reference producer, e.g.
  *                             ffa-fp8fp8/fused_kproj_rope_fp8fp8.py:80-88,
@@ -520,9 +520,10 @@ int ffa_paged_attend(const ffa_paged_attend_args *args, void *stream);
 
 /*
  * Rotary positions with several axes.  Pair j (0..63) of a token turns by
- *   angle = positions[axis_j][token] * 2 pi turns_j   (64 bits; sine and cosine of the remainder in 32),
+ *   angle = positions[axis_j][token] * 2 pi turns_j   (64 bits; sine and cosine rounded once to fp32),
  *   (a, b) -> (a cos - b sin, b cos + a sin),   inverse: -angle (the gradient of the rotation),
- * with (a, b) the channels (j, j + 64), or (2 j, 2 j + 1) with `adjacent`.  One rounding, to the rows' type.
+ * with (a, b) the channels (j, j + 64), or (2 j, 2 j + 1) with `adjacent`.  Products and sums are fp32, rounded each,
+ * the result once more to the rows' type.
  * pairs: device, [64].  positions: device, element (axis, b, t) at axis * pos_axis + b * pos_batch + t, int32 or
  * int64; axes outside [0, axes) read axis 0.
  */
@@ -559,7 +560,7 @@ int ffa_rope_axes(const ffa_rope_axes_args *args, void *stream);
 /*
  * Append to mxfp4 pages: token n of sequence b goes to position pos[b] + n.  k and v [B, T, HKV, 128] of one
  * type (F16/BF16/F32), strided as in ffa_rope_axes_args; v may be NULL (K alone is written).  With pairs, k
- * turns before it is quantized (in 32 bits, unrounded), and q [B, T, HQ, 128] (or NULL with HQ = 0) of the same type
+ * turns before it is quantized (in fp32: not rounded to its type between), and q [B, T, HQ, 128] (or NULL with HQ = 0) of the same type
  * into q_out [B, T, HQ, 128], contiguous; positions NULL: pos[b] + n on every axis.  k_values, v_values
  * [B, T, HKV, 128] of the same type (or NULL): the values as the pages hold them.  Nothing is written for a
  * token whose position lies outside its block-table row or whose page id is outside [0, num_pages); its

@@ -107,6 +107,24 @@ def test_rotate_strides_and_in_place(gpu):
         rope.rotate(pos, q[:, :1].expand(B, T, HQ, 128), inplace=True)
 
 
+def test_rotate_in_place_beside_a_graph(gpu):
+    """What autograd saved before it was turned in place is refused in the backward pass; q and k at one address are."""
+    rope, pos = AxisRope((64,), device=gpu), torch.arange(5, device=gpu)[None]
+    w = torch.randn(1, 5, 2, 128, device=gpu, requires_grad=True)
+    x = torch.randn(1, 5, 2, 128, device=gpu)
+    loss = (w * x).sum()
+    rope.rotate(pos, x, inplace=True)
+    with pytest.raises(RuntimeError):
+        loss.backward()
+    with torch.inference_mode():
+        y = x.clone()
+        assert torch.equal(rope.rotate(pos, y, inplace=True), rope.rotate(pos, x))
+    with pytest.raises(ValueError):
+        rope.rotate(pos, x, x[:, :, :1], inplace=True)
+    with pytest.raises(ValueError):
+        rope.rotate(pos, w, inplace=True)
+
+
 def test_rotate_empty_and_refusals(gpu):
     rope = AxisRope((64,), device=gpu)
     q = torch.zeros(2, 0, 4, 128, device=gpu)
