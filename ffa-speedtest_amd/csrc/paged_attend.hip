@@ -112,12 +112,13 @@ static AttendPlan attend_plan(const ffa_paged_attend_args *a, int cus, bool mxfp
   }
   const int own = (a->T + kPage - 1) / kPage - least;
   const long heads = (long)a->B * a->HKV;
-  pl.own_kind = attend_own_kind(LG, heads, own, cus);
+  const bool mx_own = mxfp4 && a->ngroups == 0;
+  pl.own_kind = mx_own && mx_by_sixteens(LG, heads, own, cus) ? kRows16 : attend_own_kind(LG, heads, own, cus);
   pl.own_blocks = (int)attend_blocks(LG, pl.own_kind);
   if (own > 0) {
     int ppw;  // of the longest sequence
     page_ranges((long)own * heads * pl.own_blocks, own, attend_resident(pl.own_kind, cus), ppw, pl.own_slots);
-    if (attend_one_range(LG, heads, own, cus)) pl.own_slots = 1;
+    if (mx_own && pl.own_kind <= kRows32 ? mx_one_range(pl.own_kind, own) : attend_one_range(LG, heads, own, cus)) pl.own_slots = 1;
   }
   if (most > 0) {
     pl.shared_kind = attend_kind(rows);
@@ -134,8 +135,8 @@ static AttendPlan attend_plan(const ffa_paged_attend_args *a, int cus, bool mxfp
     pl.both = pl.both && (long)a->HKV * pl.shared_blocks * pl.shared_slots * a->ngroups < 1l << 30;
   }
   pl.nslots = pl.shared_slots + pl.own_slots;
-  if (mxfp4 && a->ngroups == 0 && a->seq_lens && pl.own_kind <= kRows32 && pl.own_slots > 1)
-    pl.even = mx_even_ranges(a->B, a->HKV, pl.own_kind, cus);
+  if (mx_own && a->seq_lens && pl.own_kind <= kRows32 && pl.own_slots > 1)
+    pl.even = mx_even_ranges(a->B, a->HKV * pl.own_blocks, pl.own_kind, cus);
   if (pl.shared_slots == 0 && pl.own_slots <= 1) {  // one range: no partials
     pl.own_slots = 1;
     pl.nslots = 0;

@@ -105,9 +105,9 @@ inline int attend_kind(long rows) {
 inline long attend_resident(int kind, int cus) { return (kind == kRows256 ? 1l : 2l) * cus; }
 
 // Even page ranges of a batch of mxfp4 pages for few rows: about one round of workgroups in all (kernels of either kind run
-// two a CU), each sequence's last range being a part of one.
-inline int mx_even_ranges(int B, int HKV, int kind, int cus) {
-  const long all = attend_resident(kind, cus) / HKV > 0 ? attend_resident(kind, cus) / HKV : 1;
+// two a CU), each sequence's last range being a part of one.  units: KV heads x row blocks.
+inline int mx_even_ranges(int B, int units, int kind, int cus) {
+  const long all = attend_resident(kind, cus) / units > 0 ? attend_resident(kind, cus) / units : 1;
   const long n = all - B > all / 2 ? all - B : all / 2;
   return (int)(n > 0 ? n : 1);
 }
@@ -123,6 +123,20 @@ inline int attend_own_kind(long rows, long heads, int pages, int cus) {
 inline bool attend_one_range(long rows, long heads, int pages, int cus) {
   return attend_brief(rows, pages) && 2 * attend_blocks(rows, attend_own_kind(rows, heads, pages, cus)) * heads >= cus;
 }
+
+// mxfp4 pages, own ranges.  Where the chip is not full, rows by sixteens, each reading the pages again, rather than by the
+// kernels for more of them, whose start and join cost more than the pages: workgroups of 16 rows up to one round over few pages,
+// to a quarter of one over more.  us by the rows' kind / by sixteens, 32 + 8 heads: 5 tokens of 1 sequence of 512 11.5 / 7.9
+// (with one range each), of 4000 16.2 / 12.7, of 32000 25 / 22, of 8 of 4000 26 / 24, of 9000 34.7 / 35.5, of 16 of 1500 23 /
+// 14, of 2000 24 / 26, of 64 of 512 18 / 21; 16 of 1 of 700 13.9 / 8.8, of 9000 22 / 17, of 4 of 2000 20.6 / 19.7, of 16 of 700
+// 21 / 12; 32 of 4 of 2000 21 / 26; a prompt of 200 10.6 / 9.3, of 500 16.7 / 18.6.
+inline bool mx_by_sixteens(long rows, long heads, int pages, int cus) {
+  const long n = attend_blocks(rows, kRows16) * heads;
+  return rows > 16 && (pages <= 24 ? n <= 2l * cus : 2 * n <= cus && n * pages <= 32l * cus);
+}
+// ... and ranges that are not split, which saves the join: 300 tokens of 1 sequence 10.8 -> 7.5 us, 1000 11.9 -> 9.2, 1500 12.1 ->
+// 11.0, 2048 11.3 -> 11.8; 16 of 1000 15.2 -> 11.2; 5 tokens by the kernel for 32 rows, 1000 16.5 -> 14.4, 1500 16.7 -> 17.1.
+inline bool mx_one_range(int kind, int pages) { return kind == kRows16 ? pages <= 24 : (kind == kRows32 && pages <= 16); }
 
 // Ranges of ppw pages so that `units` (pages over all sets, heads and row blocks) make about `want` workgroups
 inline void page_ranges(long units, int pages, long want, int &ppw, int &slots) {

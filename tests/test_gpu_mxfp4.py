@@ -660,6 +660,43 @@ def test_attend_many_small_weights(gpu, depth, n, L, HQ):
     _check(cache, table, [n], q, out, scale=scale, tokens=sorted({0, L // 2, L - 1}))
 
 
+# Where sequences and KV heads leave CUs idle their rows go by sixteens to as many workgroups.  The same cases beside so many
+# copies of their sequences that the kernels for 17 to 256 rows take them.
+@pytest.mark.parametrize("copies,case", [
+    (300, (test_attend_lengths, [130, 40], 14, 2, 3, "fp16")),       # 21 rows, ranges not split
+    (200, (test_attend_lengths, [2600, 1700, 0], 20, 4, 5, "bf16")),  # 25 rows, even ranges of a ragged batch
+    (300, (test_attend_lengths, [200, 5], 16, 1, 5, "bf16")),        # 80 rows
+    (300, (test_attend_lengths, [300], 48, 1, 1, "fp16")),           # 48 rows
+    (300, (test_attend_padded_batch,)), (300, (test_attend_large_queries,)),
+    (300, (test_attend_other_scales, -0.05, 6, 4)), (300, (test_attend_other_scales, 0.0, 40, 8)),
+    (300, (test_attend_other_scales, -0.05, 40, 8)), (300, (test_attend_other_scales, 2.0, 40, 8)),
+    (100, (test_attend_chunks, 3300, 150, 8, 2)), (20, (test_attend_chunks, 1500, 300, 32, 4)),
+    (300, (test_attend_chunks, 700, 100, 4, 4)), (150, (test_attend_chunks, 3300, 71, 2, 2)),
+    *[(n, (test_attend_nan_blocks, *x, where)) for where in ("first", "last")
+      for n, x in ((200, (200, 70, 4)), (300, (200, 9, 16)), (300, (200, 5, 4)), (150, (9000, 5, 4)), (300, (200, 10, 4)),
+                   (150, (4000, 15, 4)), (100, (3300, 150, 4)))],
+    *[(300, (test_attend_sizes_of_values, n, L, 4, power)) for power in (13, 0, -20) for n, L in ((300, 5), (300, 40), (4000, 6))],
+    *[(300, (test_attend_constant_values, *x)) for x in ((2000, 4, 8), (2000, 40, 1), (2000, 30, 4))],
+    (100, (test_attend_constant_values, 3300, 150, 4)),
+    *[(n, (test_attend_many_small_weights, depth, *x)) for depth in (20, 30)
+      for n, x in ((300, (2000, 4, 8)), (300, (2000, 30, 4)), (100, (3300, 150, 4)))],
+])
+def test_attend_among_copies(gpu, monkeypatch, copies, case):
+    attend = PagedMXFP4Cache.attend
+
+    def crowded(self, q, table, lens=None, *, q_lens=None, **kw):
+        got = attend(self, *(t.repeat(copies, *[1] * (t.ndim - 1)) for t in (q, table, lens)),
+                     q_lens=None if q_lens is None else q_lens.repeat(copies), **kw)
+        got = got.view(copies, *q.shape)
+        # copies differ by where their ranges end: by each's bound, far below a step and a half of the type
+        assert torch.allclose(got[0].float(), got[-1].float(), rtol=2.0 ** -6, atol=2.0 ** -6 * float(got[0].float().nan_to_num(0).abs().max()),
+                              equal_nan=True)
+        return got[copies // 2]
+
+    monkeypatch.setattr(PagedMXFP4Cache, "attend", crowded)
+    case[0](gpu, *case[1:])
+
+
 def _forked(sizes, prefix, own, HQ, HKV, L, dtype, seed, dev):
     g = torch.Generator().manual_seed(seed)
     lens, b = [], 0
