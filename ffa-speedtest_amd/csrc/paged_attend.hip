@@ -118,7 +118,8 @@ static AttendPlan attend_plan(const ffa_paged_attend_args *a, int cus, bool mxfp
   if (own > 0) {
     int ppw;  // of the longest sequence
     page_ranges((long)own * heads * pl.own_blocks, own, attend_resident(pl.own_kind, cus), ppw, pl.own_slots);
-    if (mx_own && pl.own_kind <= kRows32 ? mx_one_range(pl.own_kind, own) : attend_one_range(LG, heads, own, cus)) pl.own_slots = 1;
+    if (mx_own && mx_one_range(pl.own_kind, own)) pl.own_slots = 1;
+    if (!(mx_own && pl.own_kind <= kRows32) && attend_one_range(LG, heads, own, cus)) pl.own_slots = 1;
   }
   if (most > 0) {
     pl.shared_kind = attend_kind(rows);

@@ -135,8 +135,9 @@ inline bool mx_by_sixteens(long rows, long heads, int pages, int cus) {
   return rows > 16 && (pages <= 24 ? n <= 2l * cus : 2 * n <= cus && n * pages <= 32l * cus);
 }
 // ... and ranges that are not split, which saves the join: 300 tokens of 1 sequence 10.8 -> 7.5 us, 1000 11.9 -> 9.2, 1500 12.1 ->
-// 11.0, 2048 11.3 -> 11.8; 16 of 1000 15.2 -> 11.2; 5 tokens by the kernel for 32 rows, 1000 16.5 -> 14.4, 1500 16.7 -> 17.1.
-inline bool mx_one_range(int kind, int pages) { return kind == kRows16 ? pages <= 24 : (kind == kRows32 && pages <= 16); }
+// 11.0, 2048 11.3 -> 11.8; 16 of 1000 15.2 -> 11.2; 5 tokens by the kernel for 32 rows, 1000 16.5 -> 14.4, 1500 16.7 -> 17.1; 12
+// of 32 sequences by the one for 64, 500 23 -> 16, 1000 30 -> 26, 2000 42 -> 46.
+inline bool mx_one_range(int kind, int pages) { return pages <= (kind == kRows16 ? 24 : 16) && kind <= kRows64; }
 
 // Ranges of ppw pages so that `units` (pages over all sets, heads and row blocks) make about `want` workgroups
 inline void page_ranges(long units, int pages, long want, int &ppw, int &slots) {
