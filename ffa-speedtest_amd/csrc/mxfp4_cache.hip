@@ -476,8 +476,8 @@ extern "C" int ffa_mxfp4_append(const ffa_mxfp4_append_args *a, void *stream) {
                        (uintptr_t)a->k_values | (uintptr_t)a->v_values | (uintptr_t)a->k_pages | (uintptr_t)a->k_scale |
                        (uintptr_t)a->v_pages | (uintptr_t)a->v_scale;
   if ((off | al) & 15) FFA_BAD("rows and pools must start at multiples of 16 bytes");
-  if (a->T > 1 << 30 || a->HKV > 1 << 16 || a->HQ > 1 << 20 || (long)a->B * (a->T / 2 + 1) > 0x7fffffffl)
-    FFA_NO("more workgroups than a grid holds");
+  const long wgs = (long)a->B * (mx_by_tiles(a->B, a->T, a->HQ + (a->v ? 2 : 1) * a->HKV, a->pairs) ? page_tiles(a->T) : a->T / 2 + 1);
+  if (a->T > 1 << 30 || a->HKV > 1 << 16 || a->HQ > 1 << 20 || wgs > kMostWorkgroups) FFA_NO("more workgroups than a grid holds");
   MxAppendParams p = {};
   p.rope = RopeParams{a->pairs, a->positions, a->pos_axis, a->pos_batch, a->positions64, a->axes, 0};
   p.k = a->k;
@@ -527,7 +527,7 @@ extern "C" int ffa_mxfp4_dequant(const uint8_t *k_pages, const uint8_t *k_scale,
   const uintptr_t al = (uintptr_t)k_pages | (uintptr_t)k_scale | (uintptr_t)v_pages | (uintptr_t)v_scale | (uintptr_t)k_out |
                        (uintptr_t)v_out;
   if (al & 15) FFA_BAD("outputs and pools must be multiples of 16 bytes");
-  if (HKV > 32768 || (long)B * (T / kPage) > 0x7fffffffl) FFA_NO("more workgroups than a grid holds");
+  if (HKV > 32768 || (long)B * (T / kPage) > kMostWorkgroups) FFA_NO("more workgroups than a grid holds");
   MxReadParams p = {k_pages, k_scale, v_pages, v_scale, block_table, seq_lens, bt_stride, num_pages, T, HKV, T / kPage, k_out, v_out};
   const dim3 grid((unsigned)((long)B * p.tiles), (unsigned)((6 * HKV + 3) / 4));
   const hipStream_t st = (hipStream_t)stream;

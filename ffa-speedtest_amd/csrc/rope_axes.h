@@ -11,6 +11,7 @@
 
 namespace ffa {
 
+constexpr long kMostWorkgroups = (1l << 24) - 1;  // workgroups of 256 threads in a dimension: fewer than 2^32 threads
 enum { kTurnNone = 0, kTurnHalf = 1, kTurnAdjacent = 2 };
 
 struct RopeParams {

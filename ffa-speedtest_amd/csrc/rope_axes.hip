@@ -104,7 +104,7 @@ extern "C" int ffa_rope_axes(const ffa_rope_axes_args *a, void *stream) {
   p.HKV = a->HKV;
   p.tokens = rope_tokens(all, kRopeTokens);
   const long tiles = (all + p.tokens - 1) / p.tokens;
-  if (tiles > 0x7fffffff) FFA_NO("more than 2^35 tokens");
+  if (tiles > kMostWorkgroups) FFA_NO("more than 2^28 tokens");
   const dim3 grid((unsigned)tiles, (unsigned)rope_splits(tiles, (long)p.tokens * H));
   const hipStream_t st = (hipStream_t)stream;
   if (a->dtype == FFA_DT_F32) launch_rope<2>(p, a->adjacent, grid, st);

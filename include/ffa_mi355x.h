@@ -514,8 +514,9 @@ int ffa_paged_attend(const ffa_paged_attend_args *args, void *stream);
  *   v [P, HKV, 128, 32] u8       V codes; channel c, tokens t = 2 i, 2 i + 1 (low half first) in byte
  *                                ((c / 32 * 4 + t / 16) * 16 + c % 16) * 16 + c / 16 % 2 * 8 + t % 16 / 2
  *   v_scale [P, HKV, 4, 64] u8
- * Two tokens share a byte of V: an append of the second leaves the first, and calls that write tokens of
- * one page are ordered on one stream.
+ * Two tokens share a byte of V: an append of the second leaves the first.  Calls that write tokens of one
+ * page are ordered on one stream, and of one call's sequences a single one writes to a page (ffa_pages_fork
+ * gives each its own).
  */
 
 /*

@@ -147,6 +147,14 @@ def test_rope_entry_unsupported():
     assert N.lib().ffa_rope_axes(None, None) == -1
 
 
+def test_calls_beyond_a_grid():
+    """More workgroups than a grid of 2^32 threads holds."""
+    assert N.lib().ffa_rope_axes(ctypes.byref(_rope_args(B=1 << 14, T=1 << 15)), None) == -2
+    assert N.lib().ffa_mxfp4_append(ctypes.byref(_append_args(B=1 << 25, T=1)), None) == -2
+    assert N.lib().ffa_mxfp4_append(ctypes.byref(_append_args(B=1 << 18, T=1 << 13, pairs=None, HQ=0, q=None)), None) == -2
+    assert N.lib().ffa_mxfp4_dequant(4096, 4096, 4096, 4096, 4096, 2, 4, None, 1 << 24, 64, 2, 4096, 4096, N.DT_F16, None) == -2
+
+
 def _append_args(**kw):
     a = N.MXFP4AppendArgs()
     a.k = a.v = a.q = a.pairs = a.pos = a.block_table = a.k_pages = a.k_scale = a.v_pages = a.v_scale = a.q_out = 4096
