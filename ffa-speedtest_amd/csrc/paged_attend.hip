@@ -92,8 +92,12 @@ struct AttendPlan {
   int shared_kind, shared_blocks, own_kind, own_blocks;
   bool both;  // one launch of 256-row workgroups over shared pages and of few-row ones over own pages
   int even;   // even ranges over the batch's pages, about this many (mxfp4's few-row kernels)
+  long even_slots(const ffa_paged_attend_args *a) const {  // at most: a range of T's pages takes four
+    const long n = ((a->T + kPage - 1) / kPage + 3) / 4 * (long)a->B;
+    return n < even + a->B ? n : even + a->B;
+  }
   size_t parts(const ffa_paged_attend_args *a) const {  // partials of the call
-    return (size_t)(even ? even + a->B : (long)a->B * nslots) * a->L * a->HQ;
+    return (size_t)(even ? even_slots(a) : (long)a->B * nslots) * a->L * a->HQ;
   }
 };
 
@@ -249,7 +253,7 @@ static int attend_run(const ffa_paged_attend_args *a, const uint8_t *v_scale, vo
       launch(pl.shared_kind, pl.shared_slots, pl.shared_blocks, a->ngroups, -1);
     }
     p.nshared = 0;
-    if (pl.even) launch(pl.own_kind, pl.even + a->B, pl.own_blocks, 1, -1);
+    if (pl.even) launch(pl.own_kind, (int)pl.even_slots(a), pl.own_blocks, 1, -1);
     else if (pl.own_slots > 0) launch(pl.own_kind, pl.own_slots, pl.own_blocks, a->B, -1);
   }
   if (pl.nslots > 0 && !join_by_wave((long)rows))

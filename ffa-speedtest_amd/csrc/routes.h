@@ -128,16 +128,17 @@ inline bool attend_one_range(long rows, long heads, int pages, int cus) {
 // kernels for more of them, whose start and join cost more than the pages: workgroups of 16 rows up to one round over few pages,
 // to a quarter of one over more.  us by the rows' kind / by sixteens, 32 + 8 heads: 5 tokens of 1 sequence of 512 11.5 / 7.9
 // (with one range each), of 4000 16.2 / 12.7, of 32000 25 / 22, of 8 of 4000 26 / 24, of 9000 34.7 / 35.5, of 16 of 1500 23 /
-// 14, of 2000 24 / 26, of 64 of 512 18 / 21; 16 of 1 of 700 13.9 / 8.8, of 9000 22 / 17, of 4 of 2000 20.6 / 19.7, of 16 of 700
-// 21 / 12; 32 of 4 of 2000 21 / 26; a prompt of 200 10.6 / 9.3, of 500 16.7 / 18.6.
+// 14, of 2000 24 / 16, of 64 of 512 18 / 21; 16 of 1 of 700 13.9 / 8.8, of 9000 22 / 17, of 4 of 2000 20.6 / 19.7, of 16 of 700
+// 21 / 12; 32 of 4 of 2000 20 / 14; a prompt of 200 10.6 / 9.3, of 500 16.7 / 18.6.
 inline bool mx_by_sixteens(long rows, long heads, int pages, int cus) {
   const long n = attend_blocks(rows, kRows16) * heads;
-  return rows > 16 && (pages <= 24 ? n <= 2l * cus : 2 * n <= cus && n * pages <= 32l * cus);
+  return rows > 16 && (pages <= 32 ? n <= 2l * cus : 2 * n <= cus && n * pages <= 32l * cus);
 }
-// ... and ranges that are not split, which saves the join: 300 tokens of 1 sequence 10.8 -> 7.5 us, 1000 11.9 -> 9.2, 1500 12.1 ->
-// 11.0, 2048 11.3 -> 11.8; 16 of 1000 15.2 -> 11.2; 5 tokens by the kernel for 32 rows, 1000 16.5 -> 14.4, 1500 16.7 -> 17.1; 12
+// ... and ranges that are not split, which saves the join (3.8 us, and 2 of the host's): 300 tokens of 1 sequence 10.8 -> 7.5 us,
+// 1000 11.9 -> 9.2, 2000 10.5 -> 12.7 (called one by one 14.7 -> 12.7), 2500 10.5 -> 14.6; 16 of 2000 16.5 -> 16.0, 32 of 2000 22 -> 17; 5
+// of 8 of 2000 18 -> 15, of 32 of 2000 31 -> 23; 5 tokens by the kernel for 32 rows, 1000 16.5 -> 14.4, 1500 16.7 -> 17.1; 12
 // of 32 sequences by the one for 64, 500 23 -> 16, 1000 30 -> 26, 2000 42 -> 46.
-inline bool mx_one_range(int kind, int pages) { return pages <= (kind == kRows16 ? 24 : 16) && kind <= kRows64; }
+inline bool mx_one_range(int kind, int pages) { return pages <= (kind == kRows16 ? 32 : 16) && kind <= kRows64; }
 
 // Ranges of ppw pages so that `units` (pages over all sets, heads and row blocks) make about `want` workgroups
 inline void page_ranges(long units, int pages, long want, int &ppw, int &slots) {

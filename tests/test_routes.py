@@ -151,10 +151,10 @@ def test_rotary_workgroups(routes):
 def test_mxfp4_rows_by_sixteens(routes):
     """Rows by sixteens where that was measured to be the faster one (32 + 8 heads, 256 CUs), in ranges that are not split."""
     yes = [(20, 8, 8), (20, 8, 24), (20, 8, 63), (20, 8, 500), (20, 64, 63), (20, 128, 24), (20, 256, 8), (64, 8, 11), (64, 8, 141),
-           (64, 32, 63), (64, 128, 11), (128, 8, 63), (256, 8, 32), (800, 8, 4)]
-    no = [(16, 8, 8), (20, 64, 141), (20, 128, 32), (20, 512, 8), (128, 32, 32), (128, 128, 11), (2000, 8, 8), (8192, 8, 256), (4, 1, 1)]
+           (64, 32, 63), (64, 128, 11), (128, 8, 63), (256, 8, 32), (128, 32, 32), (800, 8, 4)]
+    no = [(16, 8, 8), (20, 64, 141), (20, 128, 33), (20, 512, 8), (128, 32, 33), (128, 128, 11), (2000, 8, 8), (8192, 8, 256), (4, 1, 1)]
     got = routes(*(f"mx_by_sixteens({rows}, {heads}, {pages}, 256)" for rows, heads, pages in yes + no))
     assert got == [1] * len(yes) + [0] * len(no)
-    one = [("kRows16", 1), ("kRows16", 24), ("kRows32", 16), ("kRows64", 16)]
-    several = [("kRows16", 25), ("kRows32", 17), ("kRows64", 17), ("kRows128", 1), ("kRows256", 1)]
+    one = [("kRows16", 1), ("kRows16", 32), ("kRows32", 16), ("kRows64", 16)]
+    several = [("kRows16", 33), ("kRows32", 17), ("kRows64", 17), ("kRows128", 1), ("kRows256", 1)]
     assert routes(*(f"mx_one_range({kind}, {pages})" for kind, pages in one + several)) == [1] * len(one) + [0] * len(several)
