@@ -1,7 +1,7 @@
 // Exact attention over mxfp4 pages (keys and values in 4 bits): the kernel for few rows, the one for the most, and the
 // builds of paged_attend.h between them.
 //
-// Few rows (16 sequences of 8K-64K, 32 + 8 heads: 120 us, 5.9 TB/s; five drafted tokens of 8: 76 us, 4.1) are bound by
+// Few rows (16 sequences of 8K-64K, 32 + 8 heads: 120 us, 5.9 TB/s; five drafted tokens of 8: 74 us, 4.2) are bound by
 // the pages' bytes (136 a token and head) only while the vector unit keeps up: the bytes of a 16-bit cache's token bring
 // four tokens to convert.  K's codes become the fp16 operand by one conversion a pair, which applies the block's power of
 // two.  V's powers of two belong to tokens, of which a V^T operand holds eight, so they multiply the weights: for each
@@ -44,48 +44,51 @@ __device__ __forceinline__ void load_values(const AttendParams &p, size_t blk, i
 }
 
 // With two row tiles a page's registers are short: the wave's pages then come through LDS, two ahead of use and in no
-// registers (five drafted tokens of 8 sequences 88 -> 79 us, of 2 35 -> 29; with one tile, which memory bounds, 121 -> 125).
-// What is read from there goes by the instruction itself: the compiler makes every read of LDS it knows of wait for all
-// copies under way.
+// registers (five drafted tokens of 8 sequences 88 -> 74 us, of 2 35 -> 29; with one tile, 120.9 -> 121.6, one token after 2000
+// 12.6 -> 14.5).  The copies are buffer loads, for whose data the compiler waits nowhere: the waits below are all there are.
+// (Global loads into LDS make each wait of the kernel one for every load under way, those of the next page too: 77 us.)
 struct MxSlot {
   u32x4 k[4][64], v[4][64];
   uint32_t ks[64], vs[64];
 };
 constexpr int kSlotLoads = 10;
-__device__ __forceinline__ void copy_page(const AttendParams &p, size_t blk, int lane, MxSlot &s) {
-  typedef const __attribute__((address_space(1))) void *From;
-  typedef __attribute__((address_space(3))) void *To;
-  __builtin_amdgcn_global_load_lds((From)(p.ks + blk * kMxScales + 4 * lane), (To)s.ks, 4, 0, 0);
-  __builtin_amdgcn_global_load_lds((From)(p.vs + blk * kMxScales + 4 * lane), (To)s.vs, 4, 0, 0);
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    __builtin_amdgcn_global_load_lds((From)(p.k + blk * kMxCodes + 1024 * i + 16 * lane), (To)s.k[i], 16, 0, kNonTemporal);
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    __builtin_amdgcn_global_load_lds((From)(p.v + blk * kMxCodes + 1024 * i + 16 * lane), (To)s.v[i], 16, 0, kNonTemporal);
+typedef __attribute__((address_space(3))) void *LdsTo;
+__device__ __forceinline__ void copy_256(const uint8_t *from, int lane, void *to) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(make_rsrc(from, 256), (LdsTo)to, 4, 4 * lane, 0, 0, 0);
 }
-__device__ __forceinline__ uint32_t lds_address(const void *p) {
-  return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void *)p;
+__device__ __forceinline__ void copy_1k(const uint8_t *from, int lane, void *to) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(make_rsrc(from, 1024), (LdsTo)to, 16, 16 * lane, 0, 0, kNonTemporal);
+}
+__device__ __forceinline__ void copy_page(const AttendParams &p, size_t blk, int lane, MxSlot &s) {
+  // what was read from the slot has arrived before anything is copied there
+  __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
+  asm volatile("" ::: "memory");
+  copy_256(p.ks + blk * kMxScales, lane, s.ks);
+  copy_256(p.vs + blk * kMxScales, lane, s.vs);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) copy_1k(p.k + blk * kMxCodes + 1024 * i, lane, s.k[i]);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) copy_1k(p.v + blk * kMxCodes + 1024 * i, lane, s.v[i]);
+  asm volatile("" ::: "memory");
+}
+// the oldest page's copies have arrived: those of at most one other may be under way
+__device__ __forceinline__ void await_page() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0x0f70 | kSlotLoads);  // vmcnt
+  asm volatile("" ::: "memory");
 }
 __device__ __forceinline__ void read_keys(const MxSlot &s, int lane, MxKeys &K, uint32_t &every) {
-  const uint32_t a = lds_address(&s) + 16 * lane, b = lds_address(&s) + 8192 + 4 * lane;
-  asm volatile(
-      "ds_read_b32 %4, %7\n ds_read_b32 %5, %7 offset:256\n ds_read_b128 %0, %6\n ds_read_b128 %1, %6 offset:1024\n"
-      " ds_read_b128 %2, %6 offset:2048\n ds_read_b128 %3, %6 offset:3072\n s_waitcnt lgkmcnt(0)"
-      : "=&v"(K.code[0]), "=&v"(K.code[1]), "=&v"(K.code[2]), "=&v"(K.code[3]), "=&v"(K.scale), "=&v"(every)
-      : "v"(a), "v"(b)
-      : "memory");
+  K.scale = s.ks[lane];
+  every = s.vs[lane];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) K.code[i] = s.k[i][lane];
 }
 __device__ __forceinline__ void read_values(const MxSlot &s, int lane, MxValues &V) {
-  const uint32_t a = lds_address(&s) + 4096 + 16 * lane, b = lds_address(&s) + 8448 + 16 * (lane >> 4);
-  asm volatile(
-      "ds_read_b128 %4, %9\n ds_read_b128 %5, %9 offset:64\n ds_read_b128 %6, %9 offset:128\n ds_read_b128 %7, %9 offset:192\n"
-      " ds_read_b128 %0, %8\n ds_read_b128 %1, %8 offset:1024\n ds_read_b128 %2, %8 offset:2048\n ds_read_b128 %3, %8 offset:3072\n"
-      " s_waitcnt lgkmcnt(0)"
-      : "=&v"(V.code[0]), "=&v"(V.code[1]), "=&v"(V.code[2]), "=&v"(V.code[3]), "=&v"(V.scale[0]), "=&v"(V.scale[1]),
-        "=&v"(V.scale[2]), "=&v"(V.scale[3])
-      : "v"(a), "v"(b)
-      : "memory");
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    V.scale[i] = ((const u32x4 *)s.vs)[4 * i + (lane >> 4)];
+    V.code[i] = s.v[i][lane];
+  }
 }
 
 // The largest of the first 16 lanes' x (lane n: row n's), wave-uniform
@@ -143,13 +146,14 @@ __device__ __forceinline__ void few_rows_mx(const AttendParams &p, int split, in
   MxValues V;
   int id = 0;
   if (pa < pe) {
-    const size_t blk = block(page_id(pa + wv));
-    id = page_id(pa + wv + W);
+    const int id0 = page_id(pa + wv), id1 = page_id(pa + wv + W);
     if constexpr (kRing) {
-      copy_page(p, blk, lane, s.slot[wv][0]);
-      copy_page(p, block(id), lane, s.slot[wv][1]);
       id = page_id(pa + wv + 2 * W);
+      copy_page(p, block(id0), lane, s.slot[wv][0]);
+      copy_page(p, block(id1), lane, s.slot[wv][1]);
     } else {
+      id = id1;
+      const size_t blk = block(id0);
       load_keys(p, blk, lane, K);
       load_values(p, blk, lane, V);
     }
@@ -256,16 +260,21 @@ __device__ __forceinline__ void few_rows_mx(const AttendParams &p, int split, in
     uint64_t others = 0;
 #pragma unroll 1
     for (int i = 0, pg = p0; i < 64 && pg < last; ++i, pg += W) {
-      const size_t next = block(id);
-      id = page_id(pg + (kRing ? 3 : 2) * W);
+      size_t next = 0;
+      auto find_next = [&]() {
+        next = block(id);
+        id = page_id(pg + (kRing ? 3 : 2) * W);
+      };
+      if constexpr (!kRing) find_next();
       MxSlot &slot = s.slot[kRing ? wv : 0][kRing ? i & 1 : 0];
       if constexpr (kRing) {
-        __builtin_amdgcn_s_waitcnt(0x0f70 | kSlotLoads);  // vmcnt: the next page's copies may be under way
+        await_page();
         read_keys(slot, lane, K, V.every);
       }
       if (lo < (pg + 1) * kPage || !scales(pg * kPage)) [[unlikely]] {
         others |= 1ull << i;
         if constexpr (kRing) {
+          find_next();
           copy_page(p, next, lane, slot);
         } else {
           load_keys(p, next, lane, K);
@@ -278,7 +287,8 @@ __device__ __forceinline__ void few_rows_mx(const AttendParams &p, int split, in
       weights();
       if constexpr (kRing) {
         read_values(slot, lane, V);
-        copy_page(p, next, lane, slot);  // its last page is read
+        find_next();  // (before the copies: await_page counts those alone)
+        copy_page(p, next, lane, slot);
       }
       const uint32_t base = (uint32_t)(vtop - 15) * 0x01010101u;
 #pragma unroll
