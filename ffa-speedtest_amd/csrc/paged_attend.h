@@ -54,7 +54,9 @@ struct AttendParams {
   int shared_slots, shared_ppw, own_slots;
   int shared_blocks, shared_wgs;  // of the launch of both kinds
   const uint8_t *vs;              // mxfp4 pages: V's scales
-  int even;                       // even ranges over the batch's pages, about this many; 0: ranges by sequence
+  int even;                       // even ranges over the batch's pages, this many of one round; 0: ranges by sequence
+  int even_grow;                  // up to which multiple of the first their pages are looked for
+  float even_share;               // fours of pages a range, as a share of all
 };
 
 __device__ __forceinline__ int seq_len_of(const AttendParams &p, int b) {
@@ -91,15 +93,30 @@ __device__ __forceinline__ int lanes_sum(int x) {
 struct EvenRange {
   int b, split, ppw;
 };
+// x / d rounded up, inv about 1 / d (x below 2^24, as pages are: a quotient from fp32 is off by one at most)
+__device__ __forceinline__ int ceil_div(int x, int d, float inv) {
+  x += d - 1;
+  const int q = (int)((float)x * inv), r = x - q * d;
+  return q + (r >= d ? 1 : 0) - (r < 0 ? 1 : 0);
+}
 __device__ __forceinline__ EvenRange even_find(const AttendParams &p, int x, int of) {
   const int lane = threadIdx.x & 63, mine = pages_of(p, lane);
-  long all = __builtin_amdgcn_readlane(lanes_sum(mine), 63);
-  for (int b = 64; b < p.B; b += 64) all += __builtin_amdgcn_readlane(lanes_sum(pages_of(p, b + lane)), 63);
-  // pages per range: a page for each of four waves at least
-  const int ppw = all <= 4l * p.even ? 4 : (int)((all + 4l * p.even - 1) / (4l * p.even)) * 4;
+  float all = (float)__builtin_amdgcn_readlane(lanes_sum(mine), 63);
+  for (int b = 64; b < p.B; b += 64) all += (float)__builtin_amdgcn_readlane(lanes_sum(pages_of(p, b + lane)), 63);
+  // Pages per range: a page for each of four waves at least, and a share of the pages that leaves each sequence a part of a
+  // range (p.even_grow 1), or the least that makes no more than p.even ranges, but for twice the average (2: at most
+  // p.even / 2 + B ranges then).
+  int ppw = 4 * max((int)ceilf(all * p.even_share), 1);
+  const int step = (ppw + 31) / 32 * 4, most = p.even_grow * ppw;
+  float inv = __builtin_amdgcn_rcpf((float)ppw);
+  for (; ppw < most; ppw += step, inv = __builtin_amdgcn_rcpf((float)ppw)) {
+    int n = __builtin_amdgcn_readlane(lanes_sum(ceil_div(mine, ppw, inv)), 63);
+    for (int b = 64; b < p.B; b += 64) n += __builtin_amdgcn_readlane(lanes_sum(ceil_div(pages_of(p, b + lane), ppw, inv)), 63);
+    if (n <= p.even) break;
+  }
   int before = 0;
   for (int b = 0; b < p.B; b += 64) {
-    const int n = ((b == 0 ? mine : pages_of(p, b + lane)) + ppw - 1) / ppw, to = before + lanes_sum(n);
+    const int n = ceil_div(b == 0 ? mine : pages_of(p, b + lane), ppw, inv), to = before + lanes_sum(n);
     if (of >= 0) {
       if (of < b + 64) {
         const int k = __builtin_amdgcn_readlane(n, of - b);
@@ -151,6 +168,16 @@ __device__ __forceinline__ AttendSet attend_set(const AttendParams &p, int z, in
   s.p0 += split * ppw;
   s.p1 = min(s.p0 + ppw, s.p1);
   return s;
+}
+// ... or even range `split`; sets of no sequence past the last
+__device__ __forceinline__ AttendSet even_set(const AttendParams &p, int split) {
+  const EvenRange e = even_find(p, split, -1);
+  if (e.b >= p.B) return AttendSet{0, 0, 0, 0, split};
+  return AttendSet{e.b, 1, e.split * e.ppw, min((e.split + 1) * e.ppw, pages_of(p, e.b)), split};
+}
+// where row r (of R = L G) of a set of even ranges keeps its partial
+__device__ __forceinline__ size_t even_row(const AttendParams &p, int split, int hkv, int r) {
+  return ((size_t)split * p.HKV + hkv) * p.L * p.G + r;
 }
 
 // ---------------------------------------------------------------------------
@@ -514,8 +541,7 @@ __device__ __forceinline__ void join_waves(const AttendParams &p, const AttendSe
         for (int e = 0; e < C; ++e) o[e] += s.o[w][rr][c0 + e];
       }
       const int bi = r / LG, j = r - bi * LG, i = j / p.G, b = set.b0 + bi;
-      const size_t row = p.even ? ((size_t)set.slot * p.HKV + hkv) * LG + r
-                                : ((size_t)b * p.L + i) * p.HQ + hkv * p.G + (j - i * p.G);
+      const size_t row = p.even ? even_row(p, set.slot, hkv, r) : ((size_t)b * p.L + i) * p.HQ + hkv * p.G + (j - i * p.G);
       const bool sees = row_limit(p, b, i) > 0;
 #pragma unroll
       for (int e = 0; e < C; e += 4)
@@ -706,7 +732,7 @@ __device__ __forceinline__ void many_rows(const AttendParams &p, int split, int 
   constexpr int kUnits = 8 / W, kVPieces = 16 / W;  // of a page, per wave
   const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, n = lane & 15;
-  const AttendSet set = attend_set(p, z, split);
+  const AttendSet set = FMT == kFmtMxfp4 && p.even ? even_set(p, split) : attend_set(p, z, split);
   // the set's row tiles over as few workgroups as hold them, evenly, and a workgroup's over its waves in turn
   const int LG = p.L * p.G, R = set.n * LG, tiles = (R + 15) / 16, blocks = (tiles + W * NT - 1) / (W * NT);
   if (nth >= blocks) return;
@@ -968,7 +994,8 @@ __device__ __forceinline__ void many_rows(const AttendParams &p, int split, int 
     const int r = 16 * (tile0 + W * t) + n;
     if (tile0 + W * t >= tile_end || r >= R) continue;
     const int bi = r / LG, j = r - bi * LG, i = j / p.G;
-    const size_t row = ((size_t)(set.b0 + bi) * p.L + i) * p.HQ + hkv * p.G + (j - i * p.G);
+    const size_t row = FMT == kFmtMxfp4 && p.even ? even_row(p, set.slot, hkv, r)
+                                                  : ((size_t)(set.b0 + bi) * p.L + i) * p.HQ + hkv * p.G + (j - i * p.G);
 #pragma unroll
     for (int u = 0; u < 8; ++u) store_row4(p, row, set.slot, 16 * u + 4 * g, O[t][u], m[t], Ls[t][0], lim[t] > 0);
   }

@@ -91,10 +91,11 @@ struct AttendPlan {
   int shared_slots, shared_ppw, own_slots, nslots;
   int shared_kind, shared_blocks, own_kind, own_blocks;
   bool both;  // one launch of 256-row workgroups over shared pages and of few-row ones over own pages
-  int even;   // even ranges over the batch's pages, about this many (mxfp4's few-row kernels)
+  int even;   // even ranges over the batch's pages, this many of one round (mxfp4)
   long even_slots(const ffa_paged_attend_args *a) const {  // at most: a range of T's pages takes four
     const long n = ((a->T + kPage - 1) / kPage + 3) / 4 * (long)a->B;
-    return n < even + a->B ? n : even + a->B;
+    const long most = mx_even_slots(even, a->B);
+    return n < most ? n : most;
   }
   size_t parts(const ffa_paged_attend_args *a) const {  // partials of the call
     return (size_t)(even ? even_slots(a) : (long)a->B * nslots) * a->L * a->HQ;
@@ -140,8 +141,8 @@ static AttendPlan attend_plan(const ffa_paged_attend_args *a, int cus, bool mxfp
     pl.both = pl.both && (long)a->HKV * pl.shared_blocks * pl.shared_slots * a->ngroups < 1l << 30;
   }
   pl.nslots = pl.shared_slots + pl.own_slots;
-  if (mx_own && a->seq_lens && pl.own_kind <= kRows32 && pl.own_slots > 1)
-    pl.even = mx_even_ranges(a->B, a->HKV * pl.own_blocks, pl.own_kind, cus);
+  if (mx_own && a->seq_lens && (pl.own_kind <= kRows32 || pl.own_blocks == 1) && pl.own_slots > 1)
+    pl.even = mx_even_ranges((long)a->HKV * pl.own_blocks, pl.own_kind, cus);
   if (pl.shared_slots == 0 && pl.own_slots <= 1) {  // one range: no partials
     pl.own_slots = 1;
     pl.nslots = 0;
@@ -217,6 +218,8 @@ static int attend_run(const ffa_paged_attend_args *a, const uint8_t *v_scale, vo
   p.part_o = (float *)a->scratch;
   p.part_ml = p.part_o + parts * kD;
   p.even = pl.even;
+  p.even_grow = mx_even_search(pl.even, a->B, pl.own_kind) ? 2 : 1;
+  p.even_share = pl.even ? 0.25f / (float)(p.even_grow == 2 ? pl.even : pl.even - a->B) : 0.f;
   p.bt_stride = a->bt_stride;
   p.num_pages = a->num_pages;
   p.ngroups = a->ngroups;

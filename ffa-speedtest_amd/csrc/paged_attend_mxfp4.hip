@@ -123,14 +123,7 @@ __device__ __forceinline__ void few_rows_mx(const AttendParams &p, int split, in
   constexpr bool kRing = NT == 2;
   const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, n = lane & 15;
-  AttendSet set;
-  if (p.even) {
-    const EvenRange e = even_find(p, split, -1);
-    if (e.b >= p.B) return;
-    set = AttendSet{e.b, 1, e.split * e.ppw, min((e.split + 1) * e.ppw, pages_of(p, e.b)), split};
-  } else {
-    set = attend_set(p, z, split);
-  }
+  const AttendSet set = p.even ? even_set(p, split) : attend_set(p, z, split);
   const int LG = p.L * p.G, R = set.n * LG, r0 = rb * 16 * NT;
   if (r0 >= R) return;
   const int pa = set.p0, pe = set.p1;
@@ -412,7 +405,7 @@ __device__ __forceinline__ void many_rows_mx(const AttendParams &p, int split, i
   constexpr int NT = 2, W = 8;
   const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, n = lane & 15;
-  const AttendSet set = attend_set(p, z, split);
+  const AttendSet set = p.even ? even_set(p, split) : attend_set(p, z, split);
   const int LG = p.L * p.G, R = set.n * LG, tiles = (R + 15) / 16, blocks = (tiles + W * NT - 1) / (W * NT);
   if (nth >= blocks) return;
   const int per = (tiles + blocks - 1) / blocks;
@@ -704,7 +697,7 @@ __device__ __forceinline__ void many_rows_mx(const AttendParams &p, int split, i
     const int r = 16 * (tile0 + W * t) + n;
     if (tile0 + W * t >= tile_end || r >= R) continue;
     const int bi = r / LG, j = r - bi * LG, i = j / p.G;
-    const size_t row = ((size_t)(set.b0 + bi) * p.L + i) * p.HQ + hkv * p.G + (j - i * p.G);
+    const size_t row = p.even ? even_row(p, set.slot, hkv, r) : ((size_t)(set.b0 + bi) * p.L + i) * p.HQ + hkv * p.G + (j - i * p.G);
 #pragma unroll
     for (int u = 0; u < 8; ++u) store_row4(p, row, set.slot, 16 * u + 4 * g, O[t][u], m[t], Ls[t][0], lim[t] > 0);
   }
@@ -720,7 +713,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void m
   __shared__ MxLds<NT, 4> s;
   // Ranges are the grid's fast order, but where about as many of them may be none as not: a CU then got two while another got
   // none (one token of 32 sequences of 3000, 34 -> 28 us; of 3 of 9000, where few are none, 15.4 -> 16.3).
-  const bool last = p.even && p.even <= p.B;
+  const bool last = p.even && p.even <= 2 * p.B;
   const int split = last ? blockIdx.y : blockIdx.x, u = last ? blockIdx.x : blockIdx.y;
   few_rows_mx<NT, 4>(p, split, u % p.HKV, u / p.HKV, blockIdx.z, s);
 }
@@ -752,7 +745,7 @@ void attend_mxfp4(const AttendParams &p, const AttendLaunch &a) {
     return;
   }
   const unsigned slots = (unsigned)a.slots, units = (unsigned)(p.HKV * a.blocks);
-  const dim3 few = p.even && p.even <= p.B ? dim3(units, slots, (unsigned)a.sets) : dim3(slots, units, (unsigned)a.sets);
+  const dim3 few = p.even && p.even <= 2 * p.B ? dim3(units, slots, (unsigned)a.sets) : dim3(slots, units, (unsigned)a.sets);
   const dim3 wide((unsigned)(p.HKV * a.blocks), (unsigned)a.slots, (unsigned)a.sets);
   switch (a.kind) {
     case kRows16: hipLaunchKernelGGL(mxfp4_attend_kernel<1>, few, dim3(256), 0, a.st, p); break;

@@ -104,13 +104,17 @@ inline int attend_kind(long rows) {
 // workgroups that are resident at a time: one round of them (a second one that is not full costs as much)
 inline long attend_resident(int kind, int cus) { return (kind == kRows256 ? 1l : 2l) * cus; }
 
-// Even page ranges of a batch of mxfp4 pages for few rows: about one round of workgroups in all (kernels of either kind run
-// two a CU), each sequence's last range being a part of one.  units: KV heads x row blocks.
-inline int mx_even_ranges(int B, int units, int kind, int cus) {
-  const long all = attend_resident(kind, cus) / units > 0 ? attend_resident(kind, cus) / units : 1;
-  const long n = all - B > all / 2 ? all - B : all / 2;
+// Even page ranges of a batch of mxfp4 pages: one round of workgroups in all, each sequence's last range being a part of
+// one.  units: KV heads x row blocks.
+inline int mx_even_ranges(long units, int kind, int cus) {
+  const long n = attend_resident(kind, cus) / units;
   return (int)(n > 0 ? n : 1);
 }
+// ... whose length is looked for rather than taken from the average, which costs the start of each workgroup and of the join
+// about half a us: one token of 40 ragged sequences of up to 9000 64 -> 57 us, 5 of 30 64 -> 51, 12 of 8 of 4000 31.5 -> 27; one of 8 of
+// up to 9000 18.5 -> 19.4, 5 of 8 of up to 64K 68 -> 70.
+inline bool mx_even_search(int even, int B, int kind) { return kind > kRows32 || 4l * B >= even; }
+inline long mx_even_slots(int even, int B) { return even / 2 + B > even ? even / 2 + B : even; }  // at most
 
 // Chunks of many rows over fewer than 48 pages, where a workgroup's fixed 10-14 us count as much as its pages': smaller
 // workgroups then, and ranges that are split (their partials are rows x 528 bytes, written and read) only where the chip

@@ -136,9 +136,12 @@ def test_mxfp4_appends(routes):
 
 
 def test_mxfp4_page_ranges(routes):
-    """Ranges for about one round of workgroups, each sequence's last being a part of one; never none."""
-    assert routes("mx_even_ranges(16, 8, kRows16, 256)", "mx_even_ranges(1, 8, kRows32, 256)", "mx_even_ranges(60, 8, kRows16, 256)",
-                  "mx_even_ranges(4096, 8, kRows16, 256)", "mx_even_ranges(1, 4096, kRows16, 256)") == [48, 63, 32, 32, 1]
+    """Ranges for one round of workgroups (never none), and looked for where sequences' last ones are many among them."""
+    assert routes("mx_even_ranges(8, kRows16, 256)", "mx_even_ranges(16, kRows32, 256)", "mx_even_ranges(8, kRows256, 256)",
+                  "mx_even_ranges(4096, kRows16, 256)") == [64, 32, 32, 1]
+    assert routes("mx_even_slots(64, 8)", "mx_even_slots(64, 40)", "mx_even_slots(1, 1)") == [64, 72, 1]
+    assert routes("mx_even_search(64, 40, kRows16)", "mx_even_search(64, 30, kRows32)", "mx_even_search(64, 8, kRows64)",
+                  "mx_even_search(64, 8, kRows16)", "mx_even_search(64, 8, kRows32)") == [1, 1, 1, 0, 0]
 
 
 def test_rotary_workgroups(routes):
