@@ -667,6 +667,10 @@ def test_attend_many_small_weights(gpu, depth, n, L, HQ):
     (200, (test_attend_lengths, [2600, 1700, 0], 20, 4, 5, "bf16")),  # 25 rows, even ranges of a ragged batch
     (300, (test_attend_lengths, [200, 5], 16, 1, 5, "bf16")),        # 80 rows
     (300, (test_attend_lengths, [300], 48, 1, 1, "fp16")),           # 48 rows
+    (40, (test_attend_lengths, [2600, 1700, 0, 3100], 16, 2, 6, "bf16")),   # 48 rows, even ranges
+    (30, (test_attend_lengths, [3100, 0, 1700, 2600], 16, 2, 14, "fp16")),  # 112 rows
+    (12, (test_attend_lengths, [64, 1700, 3100, 2600], 16, 2, 30, "bf16")),  # 240 rows
+    (25, (test_attend_nan_blocks, 9000, 10, 4, "first")), (25, (test_attend_nan_blocks, 9000, 10, 4, "last")),
     (300, (test_attend_padded_batch,)), (300, (test_attend_large_queries,)),
     (300, (test_attend_other_scales, -0.05, 6, 4)), (300, (test_attend_other_scales, 0.0, 40, 8)),
     (300, (test_attend_other_scales, -0.05, 40, 8)), (300, (test_attend_other_scales, 2.0, 40, 8)),
@@ -695,6 +699,29 @@ def test_attend_among_copies(gpu, monkeypatch, copies, case):
 
     monkeypatch.setattr(PagedMXFP4Cache, "attend", crowded)
     case[0](gpu, *case[1:])
+
+
+@pytest.mark.parametrize("L,HQ", [(1, 4), (3, 16), (6, 16), (14, 16), (31, 16)])
+def test_attend_padded_ragged_batches(gpu, L, HQ):
+    """Sequences of none to 52 pages with none to all of L query tokens, in kernels for 2 to 248 rows."""
+    g = torch.Generator().manual_seed(L)
+    B = 60 if L < 14 else 24
+    lens = torch.randint(0, 3300, (B,), generator=g).tolist()
+    lens[3], lens[-1], lens[7] = 3300, 0, 2
+    ql = [min(int(x), n) for x, n in zip(torch.randint(0, L + 1, (B,), generator=g), lens)]
+    cache, table, sl, q = _batch(lens, HQ, 2, L, torch.bfloat16, 97, gpu)
+    for b, n in enumerate(ql):
+        q[b, n:] = float("nan")
+    out = cache.attend(q, table, sl, q_lens=torch.tensor(ql, device=gpu))
+    for b in range(B):
+        assert (out[b, ql[b]:] == 0).all()
+        assert torch.isfinite(out[b]).all()
+    some = [b for b in range(0, B, 5) if ql[b]]
+    for b in some:
+        rows = sorted({0, ql[b] // 2, ql[b] - 1})
+        k, v = R.logical_kv(cache, table[b, :-(-lens[b] // 64)].tolist())
+        o, bound = reference(q[b], k[:lens[b]], v[:lens[b]], lens[b], ql[b], SCALE, rows)
+        assert_close(out[b][rows], o[rows], bound[rows], q.dtype, f"sequence {b}")
 
 
 def _forked(sizes, prefix, own, HQ, HKV, L, dtype, seed, dev):
