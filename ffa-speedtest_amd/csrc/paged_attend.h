@@ -93,7 +93,7 @@ __device__ __forceinline__ int lanes_sum(int x) {
 struct EvenRange {
   int b, split, ppw;
 };
-// x / d rounded up, inv about 1 / d (x below 2^24, as pages are: a quotient from fp32 is off by one at most)
+// x / d rounded up, inv about 1 / d (quotients of pages by a range's are below 2^11: from fp32 they are off by one at most)
 __device__ __forceinline__ int ceil_div(int x, int d, float inv) {
   x += d - 1;
   const int q = (int)((float)x * inv), r = x - q * d;
@@ -103,9 +103,9 @@ __device__ __forceinline__ EvenRange even_find(const AttendParams &p, int x, int
   const int lane = threadIdx.x & 63, mine = pages_of(p, lane);
   float all = (float)__builtin_amdgcn_readlane(lanes_sum(mine), 63);
   for (int b = 64; b < p.B; b += 64) all += (float)__builtin_amdgcn_readlane(lanes_sum(pages_of(p, b + lane)), 63);
-  // Pages per range: a page for each of four waves at least, and a share of the pages that leaves each sequence a part of a
-  // range (p.even_grow 1), or the least that makes no more than p.even ranges, but for twice the average (2: at most
-  // p.even / 2 + B ranges then).
+  // Pages per range: a page for each of four waves at least, and a share of all that leaves each sequence a part of a range
+  // besides (p.even_grow 1), or the least that makes no more than p.even ranges, up to twice the average (2).  At most
+  // the larger of p.even and p.even / 2 + B ranges either way.
   int ppw = 4 * max((int)ceilf(all * p.even_share), 1);
   const int step = (ppw + 31) / 32 * 4, most = p.even_grow * ppw;
   float inv = __builtin_amdgcn_rcpf((float)ppw);

@@ -219,7 +219,8 @@ static int attend_run(const ffa_paged_attend_args *a, const uint8_t *v_scale, vo
   p.part_ml = p.part_o + parts * kD;
   p.even = pl.even;
   p.even_grow = mx_even_search(pl.even, a->B, pl.own_kind) ? 2 : 1;
-  p.even_share = pl.even ? 0.25f / (float)(p.even_grow == 2 ? pl.even : pl.even - a->B) : 0.f;
+  const int aim = p.even_grow == 2 ? pl.even : (pl.even - a->B > pl.even / 2 ? pl.even - a->B : pl.even / 2);
+  p.even_share = 0.25f / (float)(aim > 0 ? aim : 1);
   p.bt_stride = a->bt_stride;
   p.num_pages = a->num_pages;
   p.ngroups = a->ngroups;

@@ -112,8 +112,8 @@ inline int mx_even_ranges(long units, int kind, int cus) {
 }
 // ... whose length is looked for rather than taken from the average, which costs the start of each workgroup and of the join
 // about half a us: one token of 40 ragged sequences of up to 9000 64 -> 57 us, 5 of 30 64 -> 51, 12 of 8 of 4000 31.5 -> 27; one of 8 of
-// up to 9000 18.5 -> 19.4, 5 of 8 of up to 64K 68 -> 70.
-inline bool mx_even_search(int even, int B, int kind) { return kind > kRows32 || 4l * B >= even; }
+// up to 9000 18.5 -> 19.4, 5 of 8 of up to 64K 68 -> 70, one of 400 of up to 4000 (seven rounds of loads each time) 46.5 -> 52.
+inline bool mx_even_search(int even, int B, int kind) { return B <= 256 && (kind > kRows32 || 4l * B >= even); }
 inline long mx_even_slots(int even, int B) { return even / 2 + B > even ? even / 2 + B : even; }  // at most
 
 // Chunks of many rows over fewer than 48 pages, where a workgroup's fixed 10-14 us count as much as its pages': smaller

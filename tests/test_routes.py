@@ -141,7 +141,7 @@ def test_mxfp4_page_ranges(routes):
                   "mx_even_ranges(4096, kRows16, 256)") == [64, 32, 32, 1]
     assert routes("mx_even_slots(64, 8)", "mx_even_slots(64, 40)", "mx_even_slots(1, 1)") == [64, 72, 1]
     assert routes("mx_even_search(64, 40, kRows16)", "mx_even_search(64, 30, kRows32)", "mx_even_search(64, 8, kRows64)",
-                  "mx_even_search(64, 8, kRows16)", "mx_even_search(64, 8, kRows32)") == [1, 1, 1, 0, 0]
+                  "mx_even_search(64, 8, kRows16)", "mx_even_search(64, 8, kRows32)", "mx_even_search(512, 400, kRows16)") == [1, 1, 1, 0, 0, 0]
 
 
 def test_rotary_workgroups(routes):
