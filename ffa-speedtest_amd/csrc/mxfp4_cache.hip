@@ -250,6 +250,18 @@ __global__ __launch_bounds__(256) void mxfp4_append_tiles_kernel(const MxAppendP
   tl.hi = min(kPage, p.T - tl.n0);
   if (tl.lo >= tl.hi) return;
   tl.page = append_page(p.bt, p.bt_stride, p.num_pages, tl.b, P0);
+  uint32_t *lds = (uint32_t *)words[wv];
+  int part = blockIdx.y, parts = gridDim.y;
+  if (TURN != kTurnNone && p.v && parts >= 3) {
+    // V, which does not turn, by the first workgroup alone, beside the others' angles
+    if (part == 0) {
+      for (int u = wv; u < 4 * p.HKV; u += 4) tile_v<DT>(p, tl, u >> 2, u & 3, lds);
+      return;
+    }
+    --part;
+    --parts;
+  }
+  const bool v = p.v && parts == (int)gridDim.y;
   if constexpr (TURN != kTurnNone) {
     for (int i = threadIdx.x; i < 64 * 64; i += 256) {
       const int t = i >> 6;
@@ -258,13 +270,13 @@ __global__ __launch_bounds__(256) void mxfp4_append_tiles_kernel(const MxAppendP
     __syncthreads();
   }
   // units: two a head of K, four of V, two of q, the waves of the tile's workgroups in turn; q, which only turns, last (a 16K
-  // prompt's append 93 -> 89 us)
-  const int nk = 2 * p.HKV, kv = nk + (p.v ? 4 * p.HKV : 0), units = kv + (TURN == kTurnNone ? 0 : 2 * p.HQ);
-  for (int u = blockIdx.y * 4 + wv; u < units; u += 4 * gridDim.y) {
+  // prompt's append 4 % less)
+  const int nk = 2 * p.HKV, kv = nk + (v ? 4 * p.HKV : 0), units = kv + (TURN == kTurnNone ? 0 : 2 * p.HQ);
+  for (int u = part * 4 + wv; u < units; u += 4 * parts) {
     if (u < nk) {
       tile_k<DT, TURN>(p, tl, u >> 1, u & 1, cs);
     } else if (u < kv) {
-      tile_v<DT>(p, tl, (u - nk) >> 2, (u - nk) & 3, (uint32_t *)words[wv]);
+      tile_v<DT>(p, tl, (u - nk) >> 2, (u - nk) & 3, lds);
     } else {
       if constexpr (TURN != kTurnNone) tile_q<DT, TURN>(p, tl, (u - kv) >> 1, (u - kv) & 1, cs);
     }

@@ -177,11 +177,12 @@ inline bool mx_by_tiles(int B, int Tn, int units, bool rotary) {
   if (rotary) return Tn >= 64 && (long)B * Tn * units >= 160000;
   return Tn >= 32 || (long)B * units <= 512;
 }
-// workgroups that share a tile's units (each computes the tile's angles), of n fours of them: one round, four a CU.  us of a
-// 16K prompt, 32 + 8 heads, at 1, 2, 3, 4, 8 and 16 workgroups a tile  - / 99 / 95 / 94 / 107 / 109; 4 x 1500 tokens at 6, 8,
-// 11 and 22  38.0 / 37.4 / 39.0 / 41.1
+// Workgroups that share a tile's units, of n fours of them: five a CU.  With positions and three or more, one takes V alone, which
+// does not turn, and the others compute the tile's angles each.  us for four / five / six a CU, 32 + 8 heads: 16K tokens
+// 93 / 88 / 88.5 (with V among the others' units 91), 4 x 1500 27.2 / 26.6 / 26.9 (29.0), 4 x 4096 62 / 61 / 59 (65), 111 x 147 76 / 76 / 73
+// (78); 8 + 1 heads, 16K 17.8 / 18.5 / 19.8 (18.2), 111 x 147 23 / 23 / 24 (26).
 inline long mx_tile_splits(long tiles, long n, int cus) {
-  const long want = (4l * cus + tiles - 1) / tiles;
+  const long want = (5l * cus + tiles - 1) / tiles;
   return want < n ? want : n;
 }
 

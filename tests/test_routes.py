@@ -130,9 +130,9 @@ def test_mxfp4_appends(routes):
              (16, 128, 48, "true"), (64, 1, 16, "false"), (64, 16, 16, "false"), (256, 16, 16, "false")]
     got = routes(*(f"mx_by_tiles({B}, {Tn}, {units}, {rotary})" for B, Tn, units, rotary in tiles + pairs))
     assert got == [1] * len(tiles) + [0] * len(pairs)
-    # one round of four workgroups a CU, but no workgroup without a unit
+    # five workgroups a CU, but no workgroup without a unit
     assert routes("mx_tile_splits(256, 24, 256)", "mx_tile_splits(1, 24, 256)", "mx_tile_splits(94, 24, 256)",
-                  "mx_tile_splits(5000, 24, 256)") == [4, 24, 11, 1]
+                  "mx_tile_splits(5000, 24, 256)") == [5, 24, 14, 1]
 
 
 def test_mxfp4_page_ranges(routes):
