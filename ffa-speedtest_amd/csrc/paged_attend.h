@@ -55,6 +55,7 @@ struct AttendParams {
   int shared_blocks, shared_wgs;  // of the launch of both kinds
   const uint8_t *vs;              // mxfp4 pages: V's scales
   int even;                       // even ranges over the batch's pages, this many of one round; 0: ranges by sequence
+  int fold;                       // mxfp4: workgroups of a KV head among the first ones of all CUs, for pairs of them; 0: none
   int even_grow;                  // up to which multiple of the first their pages are looked for
   float even_share;               // fours of pages a range, as a share of all
 };
@@ -727,6 +728,19 @@ struct ManyLds {
   float2 nf4[FMT == kFmtNf4 ? 256 : 1];
   int hi[W], lo[W], bad;
 };
+// The row block of a set's nth workgroup (of n; `before` come before them) where CUs take two workgroups: the first of each
+// CU, `fold` a head, get the set's last blocks, the last first; the second ones its first blocks, the first first; and so on.
+__device__ __forceinline__ int folded(int nth, int n, int before, int fold) {
+  if (n > fold && before > 0) return n - 1 - nth;
+  if (n > fold) {
+    const int c = nth / fold, r = nth - c * fold;
+    return c & 1 ? c / 2 * fold + r : n - 1 - (c / 2 * fold + r);
+  }
+  const int c = before / fold, k = (c + 1) * fold - before;  // the first k are of the same kind
+  if ((c & 1) == 0) return nth < k ? n - 1 - nth : nth - k;
+  return nth < k ? nth : n - 1 - (nth - k);
+}
+
 template <int FMT, int RES, int VT, int NT, int W>
 __device__ __forceinline__ void many_rows(const AttendParams &p, int split, int hkv, int nth, int z, ManyLds<FMT, W> &s) {
   constexpr int kUnits = 8 / W, kVPieces = 16 / W;  // of a page, per wave
@@ -743,7 +757,7 @@ __device__ __forceinline__ void many_rows(const AttendParams &p, int split, int 
   if (set.n == 1) {
     const int ql = p.q_lens ? min(max(p.q_lens[set.b0], 0), p.L) : p.L;
     const int live = ((ql * p.G + 15) / 16 + per - 1) / per;
-    if (nth < live) rb = live - 1 - nth;
+    if (nth < live) rb = FMT == kFmtMxfp4 && p.fold ? folded(nth, live, z * (int)(gridDim.x / p.HKV), p.fold) : live - 1 - nth;
   }
   const int tile0 = rb * per + wv, tile_end = min((rb + 1) * per, tiles);
   const int pa = set.p0;

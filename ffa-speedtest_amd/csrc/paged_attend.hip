@@ -218,6 +218,7 @@ static int attend_run(const ffa_paged_attend_args *a, const uint8_t *v_scale, vo
   p.part_o = (float *)a->scratch;
   p.part_ml = p.part_o + parts * kD;
   p.even = pl.even;
+  p.fold = v_scale && a->ngroups == 0 && pl.own_slots == 1 ? mx_fold(pl.own_kind, a->B, a->HKV, pl.own_blocks, device_cus()) : 0;
   p.even_grow = mx_even_search(pl.even, a->B, pl.own_kind) ? 2 : 1;
   const int aim = p.even_grow == 2 ? pl.even : (pl.even - a->B > pl.even / 2 ? pl.even - a->B : pl.even / 2);
   p.even_share = 0.25f / (float)(aim > 0 ? aim : 1);

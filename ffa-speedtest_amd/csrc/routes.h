@@ -144,6 +144,14 @@ inline bool mx_by_sixteens(long rows, long heads, int pages, int cus) {
 // of 32 sequences by the one for 64, 500 23 -> 16, 1000 30 -> 26, 2000 42 -> 46.
 inline bool mx_one_range(int kind, int pages) { return pages <= (kind == kRows16 ? 32 : 16) && kind <= kRows64; }
 
+// mxfp4 pages, chunks of rows by one range each: workgroups of a KV head among the first ones of all CUs, where all workgroups
+// are resident at a time, two a CU: the second ones then go from the least to the most work (`folded`).  2 prompts of 1000 tokens,
+// 32 + 8 heads, 45 -> 38 us, of 2000, 8 + 1 heads, 56 -> 47; one of 2000 59.1 -> 57.6.  Where CUs take further ones as they get
+// free, the most work goes first (4 of 1000 65, folded 74).
+inline int mx_fold(int kind, int B, int HKV, int blocks, int cus) {
+  return (kind == kRows64 || kind == kRows128) && (long)B * HKV * blocks <= 2l * cus ? cus / HKV : 0;
+}
+
 // Ranges of ppw pages so that `units` (pages over all sets, heads and row blocks) make about `want` workgroups
 inline void page_ranges(long units, int pages, long want, int &ppw, int &slots) {
   long w = (units + want - 1) / want;

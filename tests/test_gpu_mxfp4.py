@@ -701,6 +701,24 @@ def test_attend_among_copies(gpu, monkeypatch, copies, case):
     case[0](gpu, *case[1:])
 
 
+@pytest.mark.parametrize("lens,L,HQ,HKV", [([1000, 990], 990, 16, 4), ([1500], 1500, 16, 4), ([400, 700, 650, 64], 600, 8, 2)])
+def test_attend_prompts(gpu, lens, L, HQ, HKV):
+    """Prompts of many workgroups, two a CU: every row of every block is written, with the right keys (padded ones zeros)."""
+    cache, table, sl, q = _batch(lens, HQ, HKV, L, torch.bfloat16, 89, gpu)
+    ql = [min(n, L) for n in lens]
+    out = cache.attend(q, table, sl, q_lens=torch.tensor(ql, device=gpu))
+    for b, n in enumerate(ql):
+        assert (out[b, n:] == 0).all() and (out[b, :n] != 0).any(-1).all()
+        rows = sorted({0, 1, 63, 64, 127, n // 2, n - 65, n - 1} & set(range(n)))
+        k, v = R.logical_kv(cache, table[b, :-(-lens[b] // 64)].tolist())
+        o, bound = reference(q[b], k[:lens[b]], v[:lens[b]], lens[b], n, SCALE, rows)
+        assert_close(out[b][rows], o[rows], bound[rows], q.dtype, f"sequence {b}")
+        for i in range(0, n, 97):  # against short chunks of their own
+            m = min(i + 6, n)
+            part = cache.attend(q[b:b + 1, i:m].contiguous(), table[b:b + 1], torch.tensor([lens[b] - n + m], device=gpu))
+            assert torch.allclose(part[0].float(), out[b, i:m].float(), atol=2.0 ** -6, rtol=2.0 ** -7)
+
+
 @pytest.mark.parametrize("L,HQ", [(1, 4), (3, 16), (6, 16), (14, 16), (31, 16)])
 def test_attend_padded_ragged_batches(gpu, L, HQ):
     """Sequences of none to 52 pages with none to all of L query tokens, in kernels for 2 to 248 rows."""

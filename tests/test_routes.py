@@ -161,3 +161,9 @@ def test_mxfp4_rows_by_sixteens(routes):
     one = [("kRows16", 1), ("kRows16", 32), ("kRows32", 16), ("kRows64", 16)]
     several = [("kRows16", 33), ("kRows32", 17), ("kRows64", 17), ("kRows128", 1), ("kRows256", 1)]
     assert routes(*(f"mx_one_range({kind}, {pages})" for kind, pages in one + several)) == [1] * len(one) + [0] * len(several)
+
+
+def test_mxfp4_folded_chunks(routes):
+    """Chunks whose workgroups are all resident, and in one round only."""
+    assert routes("mx_fold(kRows64, 2, 8, 32, 256)", "mx_fold(kRows128, 1, 8, 63, 256)", "mx_fold(kRows64, 4, 8, 32, 256)",
+                  "mx_fold(kRows256, 1, 8, 16, 256)", "mx_fold(kRows16, 2, 8, 8, 256)") == [32, 32, 0, 0, 0]
