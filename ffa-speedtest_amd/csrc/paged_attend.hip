@@ -136,7 +136,7 @@ static AttendPlan attend_plan(const ffa_paged_attend_args *a, int cus, bool mxfp
     long want = attend_resident(pl.shared_kind, cus);
     pl.both = attend_both(pl.shared_kind, pl.own_kind, a->own_pages_host, a->B) && own > 0 &&
               heads * pl.own_slots < 1l << 30;
-    if (pl.both) want = attend_shared_wgs(units, a->own_pages_host * a->HKV, cus);
+    if (pl.both) want = attend_shared_wgs(units, a->own_pages_host * a->HKV, cus, mxfp4 ? kMxOwnPage : 1.2);
     page_ranges(units, most, want, pl.shared_ppw, pl.shared_slots);
     pl.both = pl.both && (long)a->HKV * pl.shared_blocks * pl.shared_slots * a->ngroups < 1l << 30;
   }

@@ -708,13 +708,14 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) void m
   many_rows_mx(p, blockIdx.y, blockIdx.x % p.HKV, blockIdx.x / p.HKV, blockIdx.z, s);  // order as paged_attend_wide_kernel's
 }
 
+// Ranges are the few-row grid's fast order, but where about as many of them may be none as not: a CU then got two while another
+// got none (one token of 32 sequences of 3000, 34 -> 28 us; of 3 of 9000, where few are none, 15.4 -> 16.3).
+__host__ __device__ __forceinline__ bool ranges_last(const AttendParams &p) { return p.even != 0 && p.even <= 2 * p.B; }
+
 template <int NT>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void mxfp4_attend_kernel(const AttendParams p) {
   __shared__ MxLds<NT, 4> s;
-  // Ranges are the grid's fast order, but where about as many of them may be none as not: a CU then got two while another got
-  // none (one token of 32 sequences of 3000, 34 -> 28 us; of 3 of 9000, where few are none, 15.4 -> 16.3).
-  const bool last = p.even && p.even <= 2 * p.B;
-  const int split = last ? blockIdx.y : blockIdx.x, u = last ? blockIdx.x : blockIdx.y;
+  const int split = ranges_last(p) ? blockIdx.y : blockIdx.x, u = ranges_last(p) ? blockIdx.x : blockIdx.y;
   few_rows_mx<NT, 4>(p, split, u % p.HKV, u / p.HKV, blockIdx.z, s);
 }
 
@@ -745,8 +746,7 @@ void attend_mxfp4(const AttendParams &p, const AttendLaunch &a) {
     return;
   }
   const unsigned slots = (unsigned)a.slots, units = (unsigned)(p.HKV * a.blocks);
-  const dim3 few = p.even && p.even <= 2 * p.B ? dim3(units, slots, (unsigned)a.sets) : dim3(slots, units, (unsigned)a.sets);
-  const dim3 wide((unsigned)(p.HKV * a.blocks), (unsigned)a.slots, (unsigned)a.sets);
+  const dim3 wide(units, slots, (unsigned)a.sets), few = ranges_last(p) ? wide : dim3(slots, units, (unsigned)a.sets);
   switch (a.kind) {
     case kRows16: hipLaunchKernelGGL(mxfp4_attend_kernel<1>, few, dim3(256), 0, a.st, p); break;
     case kRows32: hipLaunchKernelGGL(mxfp4_attend_kernel<2>, few, dim3(256), 0, a.st, p); break;

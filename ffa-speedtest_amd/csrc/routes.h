@@ -169,9 +169,12 @@ inline bool attend_both(int shared_kind, int own_kind, long own_pages, int B) {
 }
 // The shared pages' workgroups there: the share of the CUs that their work is of all, in us of a CU: a page of 256 rows
 // 2.15, and 14 a workgroup; an own page of a KV head 1.2.  (Fixed shares of 50 / 63 / 75 / 88 / 100 %: the first case above 86 /
-// 97 / 96 / 103 / 109 us, the groups 84 / 84 / 74 / 74 / 79, 16 x 5 drafts behind 64K tokens 278 / 230 / 199 / 176 / 169.)
-inline long attend_shared_wgs(long units, long own_head_pages, int cus) {
-  const double many = 2.15 * units + 14. * cus, few = 1.2 * own_head_pages, share = many / (many + few);
+// 97 / 96 / 103 / 109 us, the groups 84 / 84 / 74 / 74 / 79, 16 x 5 drafts behind 64K tokens 278 / 230 / 199 / 176 / 169.)  own_page:
+// kMxOwnPage for mxfp4's, which are smaller (at 1.2 / 0.9 / 0.6 / 0.4 us, 64 sequences behind 32K tokens 79 / 75 / 79 / 79; 66 of five
+// groups 94 / 83 / 83 / 83).
+constexpr double kMxOwnPage = 0.9;
+inline long attend_shared_wgs(long units, long own_head_pages, int cus, double own_page = 1.2) {
+  const double many = 2.15 * units + 14. * cus, few = own_page * own_head_pages, share = many / (many + few);
   return (long)(cus * (share < 0.4 ? 0.4 : share)) + 1;
 }
 
