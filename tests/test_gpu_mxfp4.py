@@ -932,6 +932,33 @@ def test_a_captured_decode_step(gpu):
         sl += 1
 
 
+@pytest.mark.parametrize("L", [1, 5, 12])
+def test_a_captured_step_of_growing_ranges(gpu, L):
+    """Attention captured at a capacity, replayed with lengths that move the page ranges, between none and all of it."""
+    full = [2600, 700, 6000] * 25
+    cache, table, sl, q = _batch(full[:3], 16, 2, L, torch.float16, 101, gpu)
+    table, q, sl = table.repeat(25, 1), q.repeat(25, 1, 1, 1), torch.zeros(75, dtype=torch.int32, device=gpu)
+    run = lambda: cache.attend(q, table, sl, T=6000)  # noqa: E731
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        run()
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run()
+    g = torch.Generator().manual_seed(103)
+    for share in (0.0, 0.01, 0.4, 1.0, 0.7):
+        lens = [int(n * share) if share in (0.0, 1.0) else int(torch.randint(0, int(n * share) + 1, (1,), generator=g)) for n in full]
+        sl.copy_(torch.tensor(lens, dtype=torch.int32))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, run())
+        some = [b for b in (0, 1, 2, 36, 74) if lens[b] >= L]
+        for b in some:
+            _check(cache, table[b:b + 1], [lens[b]], q[b:b + 1], out[b:b + 1], tokens=sorted({0, L - 1}))
+
+
 def test_long_offsets(gpu):
     """A pool whose offsets pass 32 bits: its last pages are written and read like its first."""
     HKV = 64
