@@ -59,7 +59,13 @@ __device__ __forceinline__ f16x8 mx_operand(uint32_t w, float s) {
            c = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, s, 2), d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, s, 3);
   return f16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
-// the same with a factor for each of the eight: bytes of `s`
+// the same with a factor for each of the eight besides: fp16 pairs, normal numbers, as are the eight times s; products within fp16
+__device__ __forceinline__ f16x8 mx_operand(uint32_t w, float s, const f16x2 *f) {
+  const f16x8 x = mx_operand(w, s);
+  const f16x2 a = f16x2{x[0], x[1]} * f[0], b = f16x2{x[2], x[3]} * f[1], c = f16x2{x[4], x[5]} * f[2], d = f16x2{x[6], x[7]} * f[3];
+  return f16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+// the same with the factors given as bytes of `s`
 __device__ __forceinline__ f16x8 mx_operand(uint32_t w, uint2 s) {
   float x[8];
   mx_values8(w, 1.f, x);

@@ -4,12 +4,14 @@
 // Few rows (16 sequences of 8K-64K, 32 + 8 heads: 120 us, 5.9 TB/s; five drafted tokens of 8: 74 us, 4.2) are bound by
 // the pages' bytes (136 a token and head) only while the vector unit keeps up: the bytes of a 16-bit cache's token bring
 // four tokens to convert.  K's codes become the fp16 operand by one conversion a pair, which applies the block's power of
-// two.  V's powers of two belong to tokens, of which a V^T operand holds eight, so they multiply the weights: for each
-// block of 32 columns the weights' operand is w_t 2^(e_t - R), R the largest e so far, and V's codes are converted as they
-// are.  In a page that every row sees whole, and whose e lie within 14 of R, that is a packed product of fp16 pairs, exact;
-// other pages, put off to the end of a run of 64, take it in fp32, with what a row does not see left out.  A NaN block
-// thereby reaches the rows that see it and no other.  The weights' sum is a product with ones, of the weights as they are
-// rounded.
+// two.  V's powers of two belong to tokens, of which a V^T operand holds eight: its codes are converted times 2^-8 and
+// multiplied, in pairs, by fp16 numbers 2^(e + 8), made of four scale bytes at a time.  With e within -22 .. 7 those are normal
+// numbers; pages with others (blocks beyond 896, blocks of NaN) or with keys that some row does not see are put off to the end of
+// a run of 64 and take V through fp32, with NaN taken out and given to the rows that see it.  Either way each operand is the
+// value held, exactly, and blocks of zeros (2^-22) stay among the usual ones.  (With the powers of two in the weights' operand,
+// relative to the largest so far, 1-7 % less time, a token of no weight whose V was 2^24 times the others' took 4 % of the
+// result below fp16's steps, one of 2^28 nearly all of it.)  The weights' sum is a product with ones, of the weights as they
+// are rounded.
 // (The block-scaled matrix instruction on the codes themselves needs neither conversion, but it sums the products of a
 // group of channels on a common 14-bit grid: 256 + 2^-6 = 256 there, where sums in 32 bits keep 2^-15.)
 #include "paged_attend.h"
@@ -100,17 +102,6 @@ __device__ __forceinline__ int row16_max(int x) {
   return __builtin_amdgcn_readfirstlane(x);
 }
 
-// The largest scale byte of a page's first `tokens` tokens (NaN blocks apart), wave-uniform
-__device__ __forceinline__ int page_scale(uint32_t every, int lane, int tokens) {
-  int best = 0;
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int byte = (every >> (8 * j)) & 0xffu;
-    if (byte != kMxNan && 4 * (lane & 15) + j < tokens) best = max(best, byte);
-  }
-  return __builtin_amdgcn_readfirstlane((int)wave_max((float)best));
-}
-
 template <int NT, int W>
 union MxLds {
   FewLds<kFmtMxfp4, NT, W> join;
@@ -176,7 +167,6 @@ __device__ __forceinline__ void few_rows_mx(const AttendParams &p, int split, in
   hi = row16_max(hi);
 
   const f16x8 one = {1, 1, 1, 1, 1, 1, 1, 1};
-  int vtop = kMxLow;  // R + 127
   f32x4 S[NT][4];
   auto scores = [&]() {
 #pragma unroll
@@ -219,35 +209,16 @@ __device__ __forceinline__ void few_rows_mx(const AttendParams &p, int split, in
       for (int kap = 0; kap < 2; ++kap) Ls[t] = mfma16(one, __builtin_bit_cast(f16x8, w16[t][kap]), Ls[t]);
     }
   };
-  // R up to the page's largest scale; whether all of its scales then lie within 14 below R
-  auto scales = [&](int t0) {
-    const u16x2 a = __builtin_bit_cast(u16x2, V.every & 0x00ff00ffu), b = __builtin_bit_cast(u16x2, (V.every >> 8) & 0x00ff00ffu);
-    const u16x2 most = __builtin_elementwise_max(a, b), least = __builtin_elementwise_min(a, b);
-    const int up = max((int)most[0], (int)most[1]), low = min((int)least[0], (int)least[1]);
-    if (__ballot(up > vtop) != 0) [[unlikely]] {
-      const int now = max(vtop, page_scale(V.every, lane, hi - t0));
-      const float f = now - vtop > 126 ? 0.f : mx_factor(127 + vtop - now);
-      vtop = now;
-#pragma unroll
-      for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int u = 0; u < 8; ++u) O[t][u] *= f;
-    }
-    return __ballot(up > vtop || low < vtop - 14) == 0;
-  };
-  auto values = [&](int cb, const f16x8 (*P)[2]) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-      for (int kap = 0; kap < 2; ++kap) {
-        const f16x8 a = mx_operand(V.code[cb][2 * h + kap], 1.0f);
-#pragma unroll
-        for (int t = 0; t < NT; ++t) O[t][2 * cb + h] = mfma16(a, P[t][kap], O[t][2 * cb + h]);
-      }
+  // whether all of the page's powers of two are within 2^-22 .. 2^7
+  auto usual = [&]() {
+    const u16x2 low = {kMxLow, kMxLow};
+    const u16x2 a = __builtin_bit_cast(u16x2, V.every & 0x00ff00ffu) - low, b = __builtin_bit_cast(u16x2, (V.every >> 8) & 0x00ff00ffu) - low;
+    const u16x2 off = __builtin_elementwise_max(a, b);  // those below are far above
+    return __ballot(max((int)off[0], (int)off[1]) > 29) == 0;
   };
 
   const int last = min(pe, (hi + kPage - 1) / kPage);  // no row sees a later page
-  // 64 pages of the wave at a time: those that every row sees whole and whose scales lie together, then the others
+  // 64 pages of the wave at a time: the usual ones that every row sees whole, then the others
 #pragma unroll 1
   for (int p0 = pa + wv; p0 < last; p0 += 64 * W) {
     uint64_t others = 0;
@@ -264,7 +235,7 @@ __device__ __forceinline__ void few_rows_mx(const AttendParams &p, int split, in
         await_page();
         read_keys(slot, lane, K, V.every);
       }
-      if (lo < (pg + 1) * kPage || !scales(pg * kPage)) [[unlikely]] {
+      if (lo < (pg + 1) * kPage || !usual()) [[unlikely]] {
         others |= 1ull << i;
         if constexpr (kRing) {
           find_next();
@@ -283,28 +254,24 @@ __device__ __forceinline__ void few_rows_mx(const AttendParams &p, int split, in
         find_next();  // (before the copies: await_page counts those alone)
         copy_page(p, next, lane, slot);
       }
-      const uint32_t base = (uint32_t)(vtop - 15) * 0x01010101u;
 #pragma unroll
-      for (int cb = 0; cb < 4; ++cb) {
-        f16x8 P[NT][2];
+      for (int cb = 0; cb < 4; ++cb)
 #pragma unroll
-        for (int kap = 0; kap < 2; ++kap)
+        for (int kap = 0; kap < 2; ++kap) {
+          f16x2 f[4];  // 2^(e + 8) of tokens 16 g + 8 kap + 2 i, + 1
 #pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            // four bytes 127 + e to the upper bytes of the fp16 numbers 2^(e - R)
-            const uint32_t x = (V.scale[cb][2 * kap + j] - base) << 2;
-            const f16x2 f[2] = {bits_f16x2(__builtin_amdgcn_perm(0, x, 0x010c000cu)), bits_f16x2(__builtin_amdgcn_perm(0, x, 0x030c020cu))};
-#pragma unroll
-            for (int e = 0; e < 2; ++e)
-#pragma unroll
-              for (int t = 0; t < NT; ++t) {
-                const f16x2 y = bits_f16x2(w16[t][kap][2 * j + e]) * f[e];
-                P[t][kap][4 * j + 2 * e] = y[0];
-                P[t][kap][4 * j + 2 * e + 1] = y[1];
-              }
+          for (int i = 0; i < 2; ++i) {
+            const uint32_t x = (V.scale[cb][2 * kap + i] - 0x68686868u) << 2;  // the upper bytes of four
+            f[2 * i] = bits_f16x2(__builtin_amdgcn_perm(0, x, 0x010c000cu));
+            f[2 * i + 1] = bits_f16x2(__builtin_amdgcn_perm(0, x, 0x030c020cu));
           }
-        values(cb, P);
-      }
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const f16x8 a = mx_operand(V.code[cb][2 * h + kap], 0x1p-8f, f);
+#pragma unroll
+            for (int t = 0; t < NT; ++t) O[t][2 * cb + h] = mfma16(a, __builtin_bit_cast(f16x8, w16[t][kap]), O[t][2 * cb + h]);
+          }
+        }
       if constexpr (!kRing) load_values(p, next, lane, V);
     }
     if (others == 0) [[likely]] continue;
@@ -314,7 +281,6 @@ __device__ __forceinline__ void few_rows_mx(const AttendParams &p, int split, in
       const size_t blk = block(page_id(pg));
       load_keys(p, blk, lane, K);
       load_values(p, blk, lane, V);
-      scales(t0);
       scores();
 #pragma unroll
       for (int t = 0; t < NT; ++t)
@@ -324,21 +290,24 @@ __device__ __forceinline__ void few_rows_mx(const AttendParams &p, int split, in
           for (int i = 0; i < 4; ++i)
             if (t0 + 16 * g + 4 * i + tau >= lim[t]) S[t][tau][i] = -INFINITY;
       weights();
+      u32x4 keep[2];
+      uint32_t bad = 0;
+      partial_page_masks(g, hi - t0, keep);  // slots that no row sees are not data
 #pragma unroll
-      for (int cb = 0; cb < 4; ++cb) {
-        f16x8 P[NT][2];
+      for (int cb = 0; cb < 4; ++cb)
 #pragma unroll
-        for (int t = 0; t < NT; ++t)
+        for (int h = 0; h < 2; ++h)
 #pragma unroll
-          for (int k = 0; k < 16; ++k) {
-            const int byte = (V.scale[cb][k >> 2] >> (8 * (k & 3))) & 0xffu;
-            // byte - vtop <= 0 for what a row sees, but for NaN blocks
-            const float f = byte == kMxNan ? NAN : mx_factor(max(127 + min(byte - vtop, 0), 0));
-            const float w = (float)__builtin_bit_cast(f16x8, w16[t][k >> 3])[k & 7];
-            P[t][k >> 3][k & 7] = (_Float16)(t0 + 16 * g + k < lim[t] ? w * f : 0.f);
+          for (int kap = 0; kap < 2; ++kap) {
+            const uint2 vs = make_uint2(V.scale[cb][2 * kap], V.scale[cb][2 * kap + 1]);
+            const u32x4 v = __builtin_bit_cast(u32x4, mx_operand(V.code[cb][2 * h + kap], vs)) & keep[kap];
+            const f16x8 a = __builtin_bit_cast(f16x8, finite8(v, bad));
+#pragma unroll
+            for (int t = 0; t < NT; ++t) O[t][2 * cb + h] = mfma16(a, __builtin_bit_cast(f16x8, w16[t][kap]), O[t][2 * cb + h]);
           }
-        values(cb, P);
-      }
+      if (__ballot(bad != 0) != 0)
+#pragma unroll
+        for (int t = 0; t < NT; ++t) add_nan_blocks(p.vs + blk * kMxScales, lim[t] - t0, O[t]);
     }
     if (!kRing && p0 + 64 * W < last) {
       load_keys(p, block(page_id(p0 + 64 * W)), lane, K);
@@ -347,11 +316,7 @@ __device__ __forceinline__ void few_rows_mx(const AttendParams &p, int split, in
   }
   float l[NT];
 #pragma unroll
-  for (int t = 0; t < NT; ++t) {
-    l[t] = g == 0 ? Ls[t][0] : 0.f;  // join_waves sums over g
-#pragma unroll
-    for (int u = 0; u < 8; ++u) O[t][u] *= mx_factor(vtop);
-  }
+  for (int t = 0; t < NT; ++t) l[t] = g == 0 ? Ls[t][0] : 0.f;  // join_waves sums over g
   if constexpr (kRing) {  // the waves' copies, used or not, have arrived: their place is the join's
     __builtin_amdgcn_s_waitcnt(0x0f70);
     __syncthreads();

@@ -602,7 +602,7 @@ int ffa_mxfp4_dequant(const uint8_t *k_pages, const uint8_t *k_scale, const uint
 /*
  * ffa_paged_attend over mxfp4 pages: args as there with format FFA_PAGES_MXFP4, v the V codes, v_dtype and
  * res_dtype FFA_DT_NONE, k_zero and k_residual NULL; v_scale beside them.  Keys and values enter the products
- * exactly; the weights, times V's powers of two where rows are few, are rounded to fp16.
+ * exactly, whatever their powers of two; the weights are rounded to fp16.
  */
 size_t ffa_mxfp4_attend_scratch(const ffa_paged_attend_args *args, const uint8_t *v_scale);
 int ffa_mxfp4_attend(const ffa_paged_attend_args *args, const uint8_t *v_scale, void *stream);
