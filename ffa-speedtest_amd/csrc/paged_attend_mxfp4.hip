@@ -154,9 +154,11 @@ __device__ __forceinline__ void few_rows_mx(const AttendParams &p, int split, in
     const bool ok = r < R;
     const int bi = ok ? r / LG : 0, j = ok ? r - bi * LG : 0, i = j / p.G;
     const size_t row = ((size_t)(set.b0 + bi) * p.L + i) * p.HQ + hkv * p.G + (j - i * p.G);
-    load_q(p, row, ok, g, Q[t], cs[t]);
     lim[t] = ok ? row_limit(p, set.b0 + bi, i) : 0x7fffffff;  // rows past the last are computed, and not stored
-    lo = min(lo, lim[t]);
+    // rows that see nothing are zeros whatever is computed (of zeros, so that the others' maxima move without regard to them):
+    // with them, a padded batch would put every page off (five drafted tokens of 8 sequences, some padded, 239 us)
+    load_q(p, row, ok && lim[t] > 0, g, Q[t], cs[t]);
+    lo = min(lo, lim[t] > 0 ? lim[t] : 0x7fffffff);
     hi = max(hi, ok ? lim[t] : 0);
     m[t] = kNoMax;
     Ls[t] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -420,9 +422,9 @@ __device__ __forceinline__ void many_rows_mx(const AttendParams &p, int split, i
     const bool ok = tile0 + W * t < tile_end && r < R;
     const int bi = ok ? r / LG : 0, j = ok ? r - bi * LG : 0, i = j / p.G;
     const size_t row = ((size_t)(set.b0 + bi) * p.L + i) * p.HQ + hkv * p.G + (j - i * p.G);
-    load_q(p, row, ok, g, Q[t], cs[t]);
     lim[t] = ok ? row_limit(p, set.b0 + bi, i) : 0x7fffffff;
-    lo = min(lo, lim[t]);
+    load_q(p, row, ok && lim[t] > 0, g, Q[t], cs[t]);  // as in few_rows_mx
+    lo = min(lo, lim[t] > 0 ? lim[t] : 0x7fffffff);
     hi = max(hi, ok ? lim[t] : 0);
     m[t] = kNoMax;
     Ls[t] = f32x4{0.f, 0.f, 0.f, 0.f};
