@@ -27,19 +27,21 @@ def _launch(fn, args: ctypes.Structure, device: torch.device) -> int:
         return fn(ctypes.byref(args), N.stream_of(device))
 
 
+def _strides(x: torch.Tensor) -> tuple[int, int, int]:
+    """Strides of [B, T, H] (elements), 0 where a dimension has one entry: torch keeps any number there, contiguous or not."""
+    (b, t, h, _), (sb, st, sh, _) = x.shape, x.stride()
+    return (sb if b > 1 else 0, st if t > 1 else 0, sh if h > 1 else 0)
+
+
 def strided_rows(x: torch.Tensor) -> tuple[torch.Tensor, tuple[int, int, int]]:
     """x [B, T, H, 128] and its strides (elements; 0 where a dimension has one entry) as the kernels take rows: 128
     contiguous channels, every address a multiple of 16 bytes.  Others are copied."""
-    if not x.is_contiguous():
-        step = 16 // x.element_size()
-        strides = tuple([s if n > 1 else 0 for s, n in zip(x.stride()[:3], x.shape[:3])])
-        if x.stride(3) == 1 and not (strides[0] % step or strides[1] % step or strides[2] % step or x.data_ptr() % 16):
-            return x, strides
-        x = x.contiguous()
-    if x.data_ptr() % 16:
-        x = x.clone(memory_format=torch.contiguous_format)
-    b, t, h, _ = x.stride()
-    return x, (b, t, h)
+    step = 16 // x.element_size()
+    strides = _strides(x)
+    if x.stride(3) == 1 and not (strides[0] % step or strides[1] % step or strides[2] % step or x.data_ptr() % 16):
+        return x, strides
+    x = x.clone(memory_format=torch.contiguous_format)
+    return x, _strides(x)
 
 
 def rows_like(x: torch.Tensor) -> torch.Tensor:
@@ -127,8 +129,7 @@ class AxisRope:
         src, st = strided_rows(x)
         if not inplace:
             out = rows_like(x)
-            b, t, h, _ = out.stride()
-            return src, st, out, (b, t, h)
+            return src, st, out, _strides(out)
         if src is not x:
             raise ValueError("rows turned in place must have contiguous channels and 16-byte aligned strides")
         if any(n > 1 and s == 0 for n, s in zip(x.shape, x.stride())):
