@@ -30,3 +30,24 @@ def test_one_sequence_of_a_batch_at_an_odd_stride(gpu, dtype):
     assert all(torch.equal(a, b) for a, b in zip(*pages))
     a, b = rope.rotate(pos, q, k, inplace=True)
     assert a is q and b is k and torch.equal(q, want[0]) and torch.equal(k, want[1])
+
+
+def test_in_place_where_rows_overlap(gpu):
+    """Refused, and nothing is turned; rows side by side in one projection are turned."""
+    rope, pos = AxisRope((64,), device=gpu), torch.arange(5, device=gpu)[None]
+    joined = torch.randn(2, 5, 10, 128, device=gpu)
+    before = joined.clone()
+    wide = torch.as_strided(joined, (1, 9, 1, 128), (0, 64, 0, 1))
+    for q, k in ((joined[:, :, :8], joined[:, :, 6:]), (joined[:, :, 6:], joined[:, :, :8]), (joined[:, :, :4], joined[:, :, :4]),
+                 (joined[:, :, :1].expand(2, 5, 4, 128), None), (joined[:, :1].expand(2, 5, 10, 128), None)):
+        with pytest.raises(ValueError):
+            rope.rotate(pos, q, k, inplace=True)
+    with pytest.raises(ValueError):
+        rope.rotate(torch.arange(9, device=gpu)[None], wide, inplace=True)
+    assert torch.equal(joined, before)
+    want = rope.rotate(pos, joined[:, :, :6].clone(), joined[:, :, 6:8].clone())
+    rope.rotate(pos, joined[:, :, :6], joined[:, :, 6:8], inplace=True)
+    assert torch.equal(joined[:, :, :6], want[0]) and torch.equal(joined[:, :, 6:8], want[1])
+    assert torch.equal(joined[:, :, 8:], before[:, :, 8:])
+    rope.rotate(pos, joined[:, :, 1::2], joined[:, :, ::2], inplace=True)  # every other head
+    assert torch.equal(joined[:, :, 9], rope.rotate(pos, before[:, :, 9:])[:, :, 0])
