@@ -51,7 +51,7 @@ class PagedMXFP4Cache:
         """Quantize k and v [B, Tn, HKV, 128] (fp16, bf16, fp32) and write them at positions pos[b] + n.  ragged: rows
         of the table hold no pages past their own last position (as PagePool leaves them).  values: return
         (k, v) [B, Tn, HKV, 128] as the cache holds them, in k's type.  check=False leaves out the bounds check, which
-        reads the table on the host: tokens outside it are then not written.  Results carry no gradients."""
+        reads the table on the host: tokens outside it are then not written.  Results carry no gradients or tangents."""
         got = self._append(None, k, v, pos, block_table, None, None, ragged, values, check)
         return tuple(got[1:]) if values else None
 
@@ -60,7 +60,7 @@ class PagedMXFP4Cache:
                       ragged: bool = False, *, values: bool = False, check: bool = True):
         """append of k turned by `rope` (in fp32: k is not rounded between), with q [B, Tn, HQ, 128] turned beside it.
         positions [axes, B, Tn] (or [axes, Tn]): by default pos[b] + n on every axis.  Returns q turned (None without
-        q), or with values (q, k, v)."""
+        q), or with values (q, k, v), none of them with gradients or tangents: `rope.rotate` gives a q that has them."""
         got = self._append(q, k, v, pos, block_table, rope, positions, ragged, values, check)
         return tuple(got) if values else got[0]
 

@@ -10,6 +10,7 @@ import ctypes
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _native as N
 from .attend import _on
@@ -33,15 +34,22 @@ def _strides(x: torch.Tensor) -> tuple[int, int, int]:
     return (sb if b > 1 else 0, st if t > 1 else 0, sh if h > 1 else 0)
 
 
+def _dense(shape) -> tuple[int, int, int]:
+    """The same of contiguous rows."""
+    b, t, h, _ = shape
+    return (HEAD_DIM * h * t if b > 1 else 0, HEAD_DIM * h if t > 1 else 0, HEAD_DIM if h > 1 else 0)
+
+
 def strided_rows(x: torch.Tensor) -> tuple[torch.Tensor, tuple[int, int, int]]:
     """x [B, T, H, 128] and its strides (elements; 0 where a dimension has one entry) as the kernels take rows: 128
     contiguous channels, every address a multiple of 16 bytes.  Others are copied."""
+    if x.is_contiguous() and x.data_ptr() % 16 == 0:
+        return x, _dense(x.shape)
     step = 16 // x.element_size()
     strides = _strides(x)
     if x.stride(3) == 1 and not (strides[0] % step or strides[1] % step or strides[2] % step or x.data_ptr() % 16):
         return x, strides
-    x = x.clone(memory_format=torch.contiguous_format)
-    return x, _strides(x)
+    return x.clone(memory_format=torch.contiguous_format), _dense(x.shape)
 
 
 def rows_like(x: torch.Tensor) -> torch.Tensor:
@@ -182,8 +190,7 @@ class AxisRope:
         """What the kernel reads and writes for x: input, strides, output, strides."""
         src, st = strided_rows(x)
         if not inplace:
-            out = rows_like(x)
-            return src, st, out, _strides(out)
+            return src, st, rows_like(x), _dense(x.shape)
         if src is not x:
             raise ValueError("rows turned in place must have contiguous channels and 16-byte aligned strides")
         if not x.is_inference():
@@ -215,7 +222,7 @@ class AxisRope:
                inplace: bool = False):
         """q [B, T, H, 128] (and k, with heads of its own) turned by positions [axes, B, T] (or [axes, T] for every
         sequence; int32 or int64), angles in 64 bits, one rounding to the rows' type.  inverse: turned back, which is
-        also the gradient; `rotate` records it where q or k needs one.  inplace: into q and k themselves, no two rows of
+        also the gradient; `rotate` records it where q or k needs one, and turns tangents of forward mode with them.  inplace: into q and k themselves, no two rows of
         which may overlap.
         Returns q, or (q, k) where k is given."""
         B, T, _, _ = self._check(q, "q")
@@ -225,7 +232,7 @@ class AxisRope:
                 raise ValueError("q and k must have the same sequences, tokens and type")
         if inplace and (rows_overlap(q) if k is None else not _side_by_side(q, k) and rows_overlap(q, k)):
             raise ValueError("rows turned in place must not overlap (expanded ones, or q and k in each other's memory)")
-        if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+        if _differentiated(q) or (k is not None and _differentiated(k)):
             if inplace:
                 raise ValueError("rows that need gradients are not turned in place")
             got = _Rotate.apply(self, positions, inverse, q, k)
@@ -234,13 +241,23 @@ class AxisRope:
         return got[0] if k is None else got
 
 
+def _differentiated(x: torch.Tensor) -> bool:
+    """Whether x's gradient is recorded, or x has a tangent (forward mode)."""
+    if x.requires_grad and torch.is_grad_enabled():
+        return True
+    # (asked outside of forward mode's levels, which torch keeps to itself, unpack_dual costs half a us and says the same)
+    return getattr(forward_ad, "_current_level", 0) >= 0 and forward_ad.unpack_dual(x).tangent is not None
+
+
 class _Rotate(torch.autograd.Function):
-    """rotate with its gradient: the rotation back (linear, so the gradient's own is the rotation again)."""
+    """rotate with its derivatives: of its gradient the rotation back (linear, so the gradient's own is the rotation again), of
+    tangents the rotation."""
 
     @staticmethod
     def forward(ctx, rope, positions, inverse, q, k):
         ctx.rope, ctx.inverse, ctx.two = rope, inverse, k is not None
         ctx.save_for_backward(positions)
+        ctx.save_for_forward(positions)
         return rope._run(positions, q, k, inverse, False)
 
     @staticmethod
@@ -248,3 +265,8 @@ class _Rotate(torch.autograd.Function):
         (positions,) = ctx.saved_tensors
         got = _Rotate.apply(ctx.rope, positions, not ctx.inverse, gq, gk)
         return None, None, None, got[0], got[1] if ctx.two else None
+
+    @staticmethod
+    def jvp(ctx, _rope, _positions, _inverse, tq, tk=None):
+        (positions,) = ctx.saved_tensors
+        return _Rotate.apply(ctx.rope, positions, ctx.inverse, tq, tk if ctx.two else None)
