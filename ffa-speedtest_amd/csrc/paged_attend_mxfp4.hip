@@ -338,7 +338,8 @@ __device__ __forceinline__ void few_rows_mx(const AttendParams &p, int split, in
 //   steps 4-7   S_(j+1) = K_(j+1) Q      beside the other quarters: step 4 + tau takes S_(j+1)'s tile tau into the registers
 //                                        of S_j's, whose weights are done a step before
 // A weight's word holds two tokens of one tile, so V's operands are in that order in LDS: of a lane's sixteen tokens 0, 4,
-// 8, 12, 1, 5, ... .  Maxima are powers of two, which makes weights not yet multiplied scale exactly when one moves.
+// 8, 12, 1, 5, ... .  Maxima are powers of two, so that weights not yet multiplied scale without a rounding of
+// their own when one moves (but below fp16's normal numbers, by steps of 2^-24 beside weights of 2^8 and more).
 //
 // 2048 rows of 32 heads over 16K keys of 8: 445 us, 1.16 PFLOP/s of products where a large library product in fp16 reaches
 // 1.17 (a page at a time, scores, weights and values one after the other: 485; two groups of waves half a page apart: 461;

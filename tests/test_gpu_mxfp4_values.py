@@ -12,6 +12,7 @@ import torch
 import mxfp4_ref as R
 from attend_ref import U, assert_close, reference
 from ffa_mi355x.attend import SharedPrefix
+from ffa_mi355x.paged_mxfp4 import PagedMXFP4Cache
 
 pytestmark = pytest.mark.gpu
 LN2 = math.log(2)
@@ -194,3 +195,23 @@ def test_large_values_behind_shared_pages(gpu, HQ):
     for b in (0, 1, 20, B - 1):
         kk, vv = (x[:, 0] for x in R.logical_kv(cache, table[b].tolist()))
         _close(out[b, 0, HQ - 1], kk, u.double().numpy(), vv, shared + own, torch.bfloat16, LN2)
+
+
+@pytest.mark.parametrize("L,HQ,copies", KERNELS)
+def test_pages_without_values(gpu, L, HQ, copies):
+    """Keys appended alone to a new cache: its V is zeros, whose bytes are below the format's powers of two."""
+    g = torch.Generator().manual_seed(13)
+    n = 3300
+    cache = PagedMXFP4Cache(54, 1, gpu)
+    table = torch.randperm(54, generator=g)[:52].to(torch.int32)[None].to(gpu)
+    cache.append(_signs(g, 1, n, 1, 128).to(gpu), None, torch.zeros(1, dtype=torch.int32, device=gpu), table)
+    q = torch.randn(1, L, HQ, 128, generator=g).half().to(gpu).repeat(copies, 1, 1, 1)
+    lens = torch.full((copies,), n, dtype=torch.int32, device=gpu)
+    assert (cache.attend(q, table.repeat(copies, 1), lens) == 0).all()
+    v = torch.ones(1, 64, 1, 128, device=gpu)  # one page of values: what it weighs
+    cache.append(v, v, torch.full((1,), 128, dtype=torch.int32, device=gpu), table)
+    out = cache.attend(q, table.repeat(copies, 1), lens)
+    kk, vv = R.logical_kv(cache, table[0].tolist())
+    some = sorted({0, L // 2, L - 1})
+    o, bound = reference(q[0], kk, vv, n, L, 1 / math.sqrt(128), some)
+    assert_close(out[copies // 2][some], o[some], bound[some], q.dtype)
