@@ -830,9 +830,12 @@ __device__ __forceinline__ void many_rows(const AttendParams &p, int split, int 
     const bool ok = tile0 + W * t < tile_end && r < R;
     const int bi = ok ? r / LG : 0, j = ok ? r - bi * LG : 0, i = j / p.G;
     const size_t row = ((size_t)(set.b0 + bi) * p.L + i) * p.HQ + hkv * p.G + (j - i * p.G);
-    load_q(p, row, ok, g, Q[t], cs[t]);
     lim[t] = ok ? row_limit(p, set.b0 + bi, i) : 0x7fffffff;
-    lo = min(lo, lim[t]);
+    // mxfp4: rows that see nothing, which are zeros whatever is computed, hide no page from the others (26 sequences of up to
+    // 12000, 10 tokens each, some padded, 32 + 4 heads: 118 us with them)
+    const bool none = FMT == kFmtMxfp4 && lim[t] == 0;
+    load_q(p, row, ok && !none, g, Q[t], cs[t]);
+    lo = min(lo, none ? 0x7fffffff : lim[t]);
     hi = max(hi, ok ? lim[t] : 0);
     m[t] = kNoMax;
     Ls[t] = f32x4{0.f, 0.f, 0.f, 0.f};
