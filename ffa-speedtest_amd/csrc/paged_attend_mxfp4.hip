@@ -1,7 +1,7 @@
 // Exact attention over mxfp4 pages (keys and values in 4 bits): the kernel for few rows, the one for the most, and the
 // builds of paged_attend.h between them.
 //
-// Few rows (16 sequences of 8K-64K, 32 + 8 heads: 120 us, 5.9 TB/s; five drafted tokens of 8: 74 us, 4.2) are bound by
+// Few rows (16 sequences of 8K-64K, 32 + 8 heads: 122 us, 5.8 TB/s; five drafted tokens of 8: 78 us, 4.0) are bound by
 // the pages' bytes (136 a token and head) only while the vector unit keeps up: the bytes of a 16-bit cache's token bring
 // four tokens to convert.  K's codes become the fp16 operand by one conversion a pair, which applies the block's power of
 // two.  V's powers of two belong to tokens, of which a V^T operand holds eight: its codes are converted times 2^-8 and
@@ -46,9 +46,9 @@ __device__ __forceinline__ void load_values(const AttendParams &p, size_t blk, i
 }
 
 // With two row tiles a page's registers are short: the wave's pages then come through LDS, two ahead of use and in no
-// registers (five drafted tokens of 8 sequences 88 -> 74 us, of 2 35 -> 29; with one tile, 120.9 -> 121.6, one token after 2000
-// 12.6 -> 14.5).  The copies are buffer loads, for whose data the compiler waits nowhere: the waits below are all there are.
-// (Global loads into LDS make each wait of the kernel one for every load under way, those of the next page too: 77 us.)
+// registers (with V's powers of two in the weights still, five drafted tokens of 8 sequences 88 -> 74 us, of 2 35 -> 29; with one
+// tile, 120.9 -> 121.6, one token after 2000 12.6 -> 14.5).  The copies are buffer loads, for whose data the compiler waits nowhere: the waits below are all there are.
+// (Global loads into LDS make each wait of the kernel one for every load under way, those of the next page too: 77 us for 74.)
 struct MxSlot {
   u32x4 k[4][64], v[4][64];
   uint32_t ks[64], vs[64];
@@ -341,10 +341,10 @@ __device__ __forceinline__ void few_rows_mx(const AttendParams &p, int split, in
 // 8, 12, 1, 5, ... .  Maxima are powers of two, so that weights not yet multiplied scale without a rounding of
 // their own when one moves (but below fp16's normal numbers, by steps of 2^-24 beside weights of 2^8 and more).
 //
-// 2048 rows of 32 heads over 16K keys of 8: 445 us, 1.16 PFLOP/s of products where a large library product in fp16 reaches
-// 1.17 (a page at a time, scores, weights and values one after the other: 485; two groups of waves half a page apart: 461;
+// 2048 rows of 32 heads over 16K keys of 8: 450 us at the clock that holds (534 in the first launches), 1.15 PFLOP/s of products
+// where a large library product in fp16 reaches 1.17 (a page at a time, scores, weights and values one after the other: 485; two groups of waves half a page apart: 461;
 // 32x32x16 products, six instructions beside each: 491; 64 rows a wave, half of the LDS reads: 558).  The matrix cores are
-// busy 51 % of the cycles, vector issue 56 %.
+// busy 49 % of the cycles, vector issue 55 %.
 // ---------------------------------------------------------------------------
 struct WideLds {
   u32x4 k[2][16 * 64], v[3][16 * 64];
