@@ -9,7 +9,7 @@
 // numbers; pages with others (blocks beyond 896, blocks of NaN) or with keys that some row does not see are put off to the end of
 // a run of 64 and take V through fp32, with NaN taken out and given to the rows that see it.  Either way each operand is the
 // value held, exactly, and blocks of zeros (2^-22) stay among the usual ones.  (With the powers of two in the weights' operand,
-// relative to the largest so far, 1-7 % less time, a token of no weight whose V was 2^24 times the others' took 4 % of the
+// relative to the largest so far, which took 1-7 % less time, a token of no weight whose V was 2^24 times the others' took 4 % of the
 // result below fp16's steps, one of 2^28 nearly all of it.)  The weights' sum is a product with ones, of the weights as they
 // are rounded.
 // (The block-scaled matrix instruction on the codes themselves needs neither conversion, but it sums the products of a
@@ -47,7 +47,8 @@ __device__ __forceinline__ void load_values(const AttendParams &p, size_t blk, i
 
 // With two row tiles a page's registers are short: the wave's pages then come through LDS, two ahead of use and in no
 // registers (with V's powers of two in the weights still, five drafted tokens of 8 sequences 88 -> 74 us, of 2 35 -> 29; with one
-// tile, 120.9 -> 121.6, one token after 2000 12.6 -> 14.5).  The copies are buffer loads, for whose data the compiler waits nowhere: the waits below are all there are.
+// tile, 120.9 -> 121.6, one token after 2000 12.6 -> 14.5).  The copies are buffer loads, for whose data the compiler waits
+// nowhere: the waits below are all there are.
 // (Global loads into LDS make each wait of the kernel one for every load under way, those of the next page too: 77 us for 74.)
 struct MxSlot {
   u32x4 k[4][64], v[4][64];
@@ -342,9 +343,9 @@ __device__ __forceinline__ void few_rows_mx(const AttendParams &p, int split, in
 // their own when one moves (but below fp16's normal numbers, by steps of 2^-24 beside weights of 2^8 and more).
 //
 // 2048 rows of 32 heads over 16K keys of 8: 450 us at the clock that holds (534 in the first launches), 1.15 PFLOP/s of products
-// where a large library product in fp16 reaches 1.17 (a page at a time, scores, weights and values one after the other: 485; two groups of waves half a page apart: 461;
-// 32x32x16 products, six instructions beside each: 491; 64 rows a wave, half of the LDS reads: 558).  The matrix cores are
-// busy 49 % of the cycles, vector issue 55 %.
+// where a large library product in fp16 reaches 1.17 (a page at a time, scores, weights and values one after the other: 485; two
+// groups of waves half a page apart: 461; 32x32x16 products, six instructions beside each: 491; 64 rows a wave, half of the LDS
+// reads: 558).  The matrix cores are busy 49 % of the cycles, vector issue 55 %.
 // ---------------------------------------------------------------------------
 struct WideLds {
   u32x4 k[2][16 * 64], v[3][16 * 64];
